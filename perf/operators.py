@@ -172,9 +172,9 @@ def _cache(gen, lengths, kv_heads, dim, page):
     pages = sum(blocks) + 3
     codes = []
     for shape in ((pages, kv_heads, page, dim), (pages, kv_heads, dim, page)):
-        c = torch.empty(shape, dtype=torch.uint8, device="cuda")
+        c = torch.empty(shape, dtype=torch.int8, device="cuda")
         for part in c.split(max(1, (1 << 28) // (kv_heads * page * dim))):
-            part.copy_(_randn(gen, *part.shape).mul_(36).round_().clamp_(-127, 127).add_(128))
+            part.copy_(_randn(gen, *part.shape).mul_(36).round_().clamp_(-127, 127))
         codes.append(c)
     scales = [0.02 + 0.03 * torch.rand((pages, kv_heads), device="cuda", generator=gen)
               for _ in range(2)]
@@ -321,7 +321,7 @@ def _plain_prompt(s, c):
 
 
 def _plain_values(codes, scale):
-    return (codes.float() - 128.0) * scale[:, :, None, None]
+    return codes.float() * scale[:, :, None, None]
 
 
 def _plain_cached(s, c):
@@ -354,13 +354,13 @@ def _plain_append(s, c):
         s1 = torch.maximum(s0, x.abs().amax((1, 3)) / 127.0)
         over = s1.masked_fill(s1 == 0, 1.0)[:, None, :, None]
         was = codes[at].transpose(2, 3) if turned else codes[at]
-        was = was.transpose(1, 2).float() - 128.0
+        was = was.transpose(1, 2).float()
         again = torch.where(s1 > s0, 1.0, 0.0)[:, None, :, None]
         kept = torch.where(again > 0, (was * s0[:, None, :, None] / over).round(), was)
         put = (x / over).round().clamp(-127.0, 127.0)
         now = torch.where(fresh[:, :, None, None], put,
                           torch.where(old[:, :, None, None], kept, was))
-        now = (now + 128.0).to(torch.uint8).transpose(1, 2)
+        now = now.to(torch.int8).transpose(1, 2)
         codes[at] = now.transpose(2, 3) if turned else now
         scale[at] = s1
     first, count = _touched(c)
@@ -456,7 +456,7 @@ def _exact_append(s, c):
             for name in "kv":
                 x = s["new_" + name][cu[b] + lo - a:cu[b] + hi - a].double()
                 was = s[name][pid] if name == "k" else s[name][pid].transpose(1, 2)
-                was = was[:, :kept].transpose(0, 1).double() - 128
+                was = was[:, :kept].transpose(0, 1).double()
                 s0 = scales[name][pid] if kept else torch.zeros_like(scales[name][pid])
                 s1 = torch.maximum(s0, f32(x.abs().amax((0, 2)) / 127))
                 per = torch.where(s1 > 0, s1, 1.0)[:, None]
@@ -485,8 +485,8 @@ def exact(case, seed):
         at = s["table"][b, :-(-n // c["page"])].long()
 
         def held(g, at=at, n=n):
-            k = (s["k"][at, g].double() - 128) * s["k_scale"][at, g].double()[:, None, None]
-            v = (s["v"][at, g].double() - 128) * s["v_scale"][at, g].double()[:, None, None]
+            k = s["k"][at, g].double() * s["k_scale"][at, g].double()[:, None, None]
+            v = s["v"][at, g].double() * s["v_scale"][at, g].double()[:, None, None]
             return k.flatten(0, 1)[:n], v.transpose(1, 2).flatten(0, 1)[:n]
 
         spans.append((slice(b * c["queries"], (b + 1) * c["queries"]), held))

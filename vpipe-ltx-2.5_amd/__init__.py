@@ -77,6 +77,37 @@ class RouteC(ctypes.Structure):
     ]
 
 
+class AttnC(ctypes.Structure):
+    """ltx25_attn: how an attention call's heads lie in its tensors."""
+
+    _fields_ = [
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("q_stride", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64),
+        ("v_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+    ]
+
+
+class KVCacheC(ctypes.Structure):
+    """ltx25_kv_cache: a paged cache of 8-bit keys and values."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int),
+        ("page_tokens", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+    ]
+
+
 class Ltx25Error(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"ltx25 error {code}: {msg}")
@@ -142,6 +173,15 @@ SIGNATURES = {
     "ltx25_pack_bind_qlinear": (_i, [_vp, _vp, ctypes.c_char_p, _i, ctypes.POINTER(_i),
                                      ctypes.POINTER(QWeightC), ctypes.c_char_p, _sz]),
     "ltx25_pack_quantizable": (_i, [ctypes.c_char_p, ctypes.c_char_p, _i]),
+    "ltx25_attention": (_i, [_vp, ctypes.POINTER(AttnC), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i,
+                             _i]),
+    "ltx25_kv_append": (_i, [_vp, ctypes.POINTER(KVCacheC), _vp, _i, _vp, _vp, ctypes.c_int64,
+                             ctypes.c_int64, _vp, _vp, _i, _i]),
+    "ltx25_kv_read": (_i, [_vp, ctypes.POINTER(KVCacheC), _vp, _i, _vp, _vp, ctypes.c_int64,
+                           ctypes.c_int64, _vp, _vp, _i, _i]),
+    "ltx25_attention_cached": (_i, [_vp, ctypes.POINTER(AttnC), ctypes.POINTER(KVCacheC), _vp, _i,
+                                    _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _sz]),
+    "ltx25_attention_cached_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
 }
 
 _lib = None
@@ -288,6 +328,160 @@ def gelu_tanh(x, y, stream=None) -> None:
 def gate_heads(y, logits, heads: int, tokens: int, head_dim: int, stream=None) -> None:
     check(load().ltx25_gate_heads(_stream(stream), _ptr(y), _ptr(logits), heads, tokens,
                                   head_dim))
+
+
+# ---- attention (include/ltx25_attention.h) ------------------------------------------
+
+
+def _tokens(name: str, t) -> tuple[int, int, int, int]:
+    """(tokens, heads, head width, elements from a token to the next) of a bf16 tensor
+    [tokens][heads][head_dim] whose tokens lie in one piece each (a part of a fused
+    projection's output does)."""
+    torch = _torch or _import_torch()
+    if t.dtype != torch.bfloat16 or t.dim() != 3:
+        raise TypeError(f"{name} must be bf16 [tokens][heads][head_dim], got {t.dtype} "
+                        f"{tuple(t.shape)}")
+    n, heads, dim = t.shape
+    stride, head, one = t.stride()
+    if n > 0 and ((one != 1 and dim > 1) or (head != dim and heads > 1)):
+        raise ValueError(f"{name}: a token's heads must lie side by side, got strides {t.stride()}")
+    return n, heads, dim, stride if n > 1 else max(stride, heads * dim)
+
+
+def _int32(name: str, t, *shape) -> None:
+    torch = _torch or _import_torch()
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise TypeError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} "
+                        f"{tuple(t.shape)}")
+
+
+def _lse(t, tokens: int, heads: int) -> None:
+    torch = _torch or _import_torch()
+    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (tokens, heads)
+                          or not t.is_contiguous()):
+        raise TypeError(f"lse must be contiguous float32 [{tokens}][{heads}], got {t.dtype} "
+                        f"{tuple(t.shape)}")
+
+
+def attention(q, k, v, out, cu_q=None, cu_k=None, *, causal: bool, scale: float = 0.0, lse=None,
+              stream=None) -> None:
+    """Attention of packed sequences (ltx25_attention): q, out [total_q][heads][head_dim], k, v
+    [total_k][kv_heads][head_dim] bf16, cu_q, cu_k int32 [batch + 1] (both None: one sequence),
+    lse float32 [total_q][heads] or None. scale 0 is 1 / sqrt(head_dim)."""
+    nq, heads, dim, qs = _tokens("q", q)
+    nk, kv_heads, kdim, ks = _tokens("k", k)
+    if k.shape != v.shape or q.shape != out.shape or kdim != dim:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, out "
+                         f"{tuple(out.shape)} do not fit each other")
+    vs, os_ = _tokens("v", v)[3], _tokens("out", out)[3]
+    batch = 1
+    if cu_q is not None or cu_k is not None:
+        if cu_q is None or cu_k is None:
+            raise ValueError("cu_q and cu_k go together")
+        batch = cu_q.numel() - 1
+        _int32("cu_q", cu_q, batch + 1)
+        _int32("cu_k", cu_k, batch + 1)
+    _lse(lse, nq, heads)
+    a = AttnC(heads, kv_heads, dim, 1 if causal else 0, scale, qs, ks, vs, os_)
+    check(load().ltx25_attention(_stream(stream), ctypes.byref(a), _ptr(q), _ptr(k), _ptr(v),
+                                 _ptr(out), _ptr(lse), _ptr(cu_q), _ptr(cu_k), batch, nq, nk))
+
+
+class KVCache:
+    """A paged 8-bit cache held in torch device tensors (ltx25_kv_cache).
+
+    k: int8 [pages][kv_heads][page_tokens][head_dim], v: int8
+    [pages][kv_heads][head_dim][page_tokens], k_scale / v_scale: float32 [pages][kv_heads].
+    """
+
+    def __init__(self, k, v, k_scale, v_scale):
+        torch = _torch or _import_torch()
+        pages, heads, page, dim = k.shape
+        if (k.dtype != torch.int8 or v.dtype != torch.int8
+                or tuple(v.shape) != (pages, heads, dim, page)
+                or not (k.is_contiguous() and v.is_contiguous())):
+            raise TypeError(f"k and v must be contiguous int8 [pages][kv_heads][tokens][width] and "
+                            f"[pages][kv_heads][width][tokens], got {k.dtype} {tuple(k.shape)}, "
+                            f"{v.dtype} {tuple(v.shape)}")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) or not t.is_contiguous():
+                raise TypeError(f"{name} must be contiguous float32 [{pages}][{heads}], got "
+                                f"{t.dtype} {tuple(t.shape)}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, page, dim
+
+    @classmethod
+    def empty(cls, pages: int, page_tokens: int, kv_heads: int, head_dim: int, device="cuda"):
+        torch = _torch or _import_torch()
+        k = torch.empty((pages, kv_heads, page_tokens, head_dim), dtype=torch.int8, device=device)
+        v = torch.empty((pages, kv_heads, head_dim, page_tokens), dtype=torch.int8, device=device)
+        scales = [torch.empty((pages, kv_heads), dtype=torch.float32, device=device)
+                  for _ in range(2)]
+        return cls(k, v, *scales)
+
+    def c(self) -> KVCacheC:
+        return KVCacheC(_ptr(self.k), _ptr(self.v), _ptr(self.k_scale), _ptr(self.v_scale),
+                        self.pages, self.page_tokens, self.kv_heads, self.head_dim)
+
+
+def _moved(cache: KVCache, table, k, v, cu, start):
+    total, heads, dim, ks = _tokens("k", k)
+    vs = _tokens("v", v)[3]
+    if k.shape != v.shape or (heads, dim) != (cache.kv_heads, cache.head_dim):
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit the cache's "
+                         f"{cache.kv_heads} heads of width {cache.head_dim}")
+    batch = start.numel()
+    _int32("table", table, batch, table.shape[-1])
+    _int32("cu", cu, batch + 1)
+    _int32("start", start, batch)
+    return cache.c(), ks, vs, batch, total
+
+
+def kv_append(cache: KVCache, table, k, v, cu, start, stream=None) -> None:
+    """Quantize new keys and values [total][kv_heads][head_dim] into the cache
+    (ltx25_kv_append): sequence b's tokens cu[b] .. cu[b + 1] - 1 become tokens start[b] ... of
+    its pages table[b]."""
+    c, ks, vs, batch, total = _moved(cache, table, k, v, cu, start)
+    check(load().ltx25_kv_append(_stream(stream), ctypes.byref(c), _ptr(table), table.shape[1],
+                                 _ptr(k), _ptr(v), ks, vs, _ptr(cu), _ptr(start), batch, total))
+
+
+def kv_read(cache: KVCache, table, k, v, cu, start, stream=None) -> None:
+    """Read tokens start[b] ... of each sequence back into k, v [total][kv_heads][head_dim] at
+    cu[b] ... (ltx25_kv_read)."""
+    c, ks, vs, batch, total = _moved(cache, table, k, v, cu, start)
+    check(load().ltx25_kv_read(_stream(stream), ctypes.byref(c), _ptr(table), table.shape[1],
+                               _ptr(k), _ptr(v), ks, vs, _ptr(cu), _ptr(start), batch, total))
+
+
+def attention_cached_workspace(batch: int, q_len: int, heads: int, kv_heads: int, head_dim: int,
+                               max_len: int) -> int:
+    """Bytes of workspace that attention_cached needs (ltx25_attention_cached_workspace)."""
+    return int(load().ltx25_attention_cached_workspace(batch, q_len, heads, kv_heads, head_dim,
+                                                       max_len))
+
+
+def attention_cached(cache: KVCache, table, lens, q, out, q_len: int, max_len: int, workspace=None,
+                     *, causal: bool = True, scale: float = 0.0, lse=None, stream=None) -> None:
+    """Attention of each sequence's q_len newest tokens over its cache (ltx25_attention_cached):
+    q, out [batch * q_len][heads][head_dim] bf16, lens int32 [batch] with the queries' own tokens
+    counted, workspace a uint8 tensor of attention_cached_workspace() bytes."""
+    nq, heads, dim, qs = _tokens("q", q)
+    batch = lens.numel()
+    if q.shape != out.shape or nq != batch * q_len:
+        raise ValueError(f"q {tuple(q.shape)} and out {tuple(out.shape)} are not {batch} x {q_len} "
+                         f"tokens")
+    os_ = _tokens("out", out)[3]
+    _int32("table", table, batch, table.shape[-1])
+    _int32("lens", lens, batch)
+    _lse(lse, nq, heads)
+    a = AttnC(heads, cache.kv_heads, dim, 1 if causal else 0, scale, qs, 0, 0, os_)
+    c = cache.c()
+    held = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    check(load().ltx25_attention_cached(_stream(stream), ctypes.byref(a), ctypes.byref(c),
+                                        _ptr(table), table.shape[1], _ptr(lens), _ptr(q),
+                                        _ptr(out), _ptr(lse), batch, q_len, max_len,
+                                        _ptr(workspace), held))
 
 
 def probe_read(src, nbytes: int, sink, blocks: int, stream=None) -> None:

@@ -1,0 +1,133 @@
+// Device helpers and launchers of the attention kernels (attention.hip,
+// kv_cache.hip), and the launcher interface their C ABI layer
+// (capi_attention.cpp) calls.
+#pragma once
+
+#include "common.h"
+
+#include <cmath>
+
+namespace ltx25 {
+
+typedef __attribute__((address_space(3))) uint32_t lds_word;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+__device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
+
+// A buffer resource over `bytes` bytes at p: loads past them return zeros
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint32_t bytes)
+{
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
+}
+
+__device__ __forceinline__ float xor32_max(float v)
+{
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float xor32_sum(float v)
+{
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// A list of units, count(b) for each sequence b in order: the sequence and the
+// place within it of unit u. Every lane of a wave takes part and all get the
+// same answer; false when there are fewer units. The counts come from device
+// memory that the caller has not checked: each is cut to [0, 2^24] and the sum
+// kept in 64 bits.
+template <typename Count>
+__device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& seq, int& place)
+{
+  const int lane = threadIdx.x & 63;
+  long base = 0;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    const int n = b0 + lane < batch ? clampi(count(b0 + lane), 0, 1 << 24) : 0;
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(sum, d);
+      if (lane >= d) { sum += o; }
+    }
+    const unsigned long long past = __ballot(base + sum > (long)u);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      seq = __builtin_amdgcn_readfirstlane(b0 + at);
+      const int before = __shfl(sum - n, at);
+      place = __builtin_amdgcn_readfirstlane((int)(u - base) - before);
+      return true;
+    }
+    base += __shfl(sum, 63);
+  }
+  return false;
+}
+
+// ---- launchers --------------------------------------------------------------
+
+struct AttentionArgs {
+  const uint16_t* q = nullptr;
+  const uint16_t* k = nullptr;
+  const uint16_t* v = nullptr;
+  uint16_t* out = nullptr;
+  float* lse = nullptr;
+  const int* cu_q = nullptr;
+  const int* cu_k = nullptr;
+  int64_t qs = 0, ks = 0, vs = 0, os = 0;
+  int heads = 0, kv_heads = 0, head_dim = 0;
+  int causal = 0;
+  float scale = 0.0f;
+  int batch = 0, total_q = 0, total_k = 0;
+};
+hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream);
+
+struct CacheArgs {
+  int8_t* k = nullptr;
+  int8_t* v = nullptr;
+  float* ks = nullptr;
+  float* vs = nullptr;
+  int pages = 0, page_log2 = 0, kv_heads = 0, head_dim = 0;
+  const int* table = nullptr;
+  int table_stride = 0;
+};
+hipError_t launch_kv_append(const CacheArgs& c, const uint16_t* k, const uint16_t* v, int64_t ks,
+                            int64_t vs, const int* cu, const int* start, int batch, int total,
+                            hipStream_t stream);
+hipError_t launch_kv_read(const CacheArgs& c, uint16_t* k, uint16_t* v, int64_t ks, int64_t vs,
+                          const int* cu, const int* start, int batch, int total,
+                          hipStream_t stream);
+
+struct CachedArgs {
+  CacheArgs c;
+  const int* lens = nullptr;
+  const uint16_t* q = nullptr;
+  uint16_t* out = nullptr;
+  float* lse = nullptr;
+  float* workspace = nullptr;
+  int64_t qs = 0, os = 0;
+  int heads = 0, causal = 0;
+  float scale = 0.0f;
+  int batch = 0, q_len = 0, max_len = 0;
+};
+// How the cached attention's tokens are split; a function of the sizes alone,
+// so that the workspace can be asked for ahead.
+struct CachedPlan {
+  int row_tiles = 1;    // 16-row tiles of a workgroup
+  int row_blocks = 1;   // workgroups over a kv head's rows
+  int splits = 1;
+  int chunk = 0;        // tokens of a split
+  size_t workspace_bytes = 0;
+};
+CachedPlan plan_cached(int batch, int q_len, int heads, int kv_heads, int head_dim, int max_len);
+hipError_t launch_attention_cached(const CachedArgs& a, hipStream_t stream);
+
+// The current device is one that the kernels are built for (LTX25_OK, or the
+// code of the error that was set); capi.cpp.
+int check_device();
+
+}  // namespace ltx25

@@ -8,6 +8,7 @@
 // leaves the message in ltx25_last_error().
 #include "ltx25_qlinear.h"
 
+#include "attention.h"
 #include "common.h"
 
 #include <hip/hip_runtime.h>
@@ -138,6 +139,20 @@ int current_device(DeviceState** out)
   *out = &s;
   return LTX25_OK;
 }
+
+}  // namespace
+
+namespace ltx25 {
+
+int check_device()
+{
+  DeviceState* ds = nullptr;
+  return current_device(&ds);
+}
+
+}  // namespace ltx25
+
+namespace {
 
 // Grow `*buf` to at least `need` bytes. The old buffer may still be read by
 // work queued earlier, so the device is drained before it is released.

@@ -1,0 +1,705 @@
+// The paged cache of 8-bit keys and values: appending to it, reading it back,
+// and attention over it (ltx25_kv_append, ltx25_kv_read,
+// ltx25_attention_cached).
+#include "attention.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace ltx25 {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct CacheView {
+  int8_t* k;
+  int8_t* v;
+  float* ks;
+  float* vs;
+  const int* table;
+  int pages, pl, kv_heads, table_stride;   // pl: log2 of a page's tokens
+};
+
+// 8 codes -> 8 bf16, exactly
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t a, uint32_t b)
+{
+  auto f = [](uint32_t w, int i) { return (float)(int8_t)((w >> (8 * i)) & 0xffu); };
+  uint4 r;
+  r.x = pack_bf16x2(f(a, 0), f(a, 1));
+  r.y = pack_bf16x2(f(a, 2), f(a, 3));
+  r.z = pack_bf16x2(f(b, 0), f(b, 1));
+  r.w = pack_bf16x2(f(b, 2), f(b, 3));
+  return as_bf16x8(r);
+}
+
+// rint(x / s) within +-127; 0 for s = 0 and for a NaN
+__device__ __forceinline__ int quantize(float x, float s)
+{
+  const float r = rintf(x / s);
+  return s > 0.0f && r == r ? (int)fminf(fmaxf(r, -127.0f), 127.0f) : 0;
+}
+
+// ---- append, read -----------------------------------------------------------
+
+struct MoveParams {
+  CacheView c;
+  const uint16_t* k_in;
+  const uint16_t* v_in;
+  uint16_t* k_out;
+  uint16_t* v_out;
+  long kstride, vstride;
+  const int* cu;
+  const int* start;
+  int batch, total;
+};
+
+// One page of one sequence that a call touches: tokens lo .. hi - 1 of it are
+// packed tokens first + lo ...
+struct Span {
+  int pid;       // -1: no such page
+  int lo, hi;
+  long first;
+};
+
+// The unit blockIdx.x of all sequences' touched pages; false past the last.
+__device__ __forceinline__ bool find_span(const MoveParams& p, Span& s)
+{
+  constexpr int kFar = 1 << 30;
+  auto range = [&](int b, int& c0, int& n, int& at) {
+    c0 = clampi(p.cu[b], 0, p.total);
+    n = clampi(p.cu[b + 1], c0, p.total) - c0;
+    at = clampi(p.start[b], 0, kFar);
+  };
+  auto count = [&](int b) {
+    int c0, n, at;
+    range(b, c0, n, at);
+    return n > 0 ? ((at + (n - 1)) >> p.c.pl) - (at >> p.c.pl) + 1 : 0;
+  };
+  int seq = 0, place = 0;
+  if (!find_unit((int)blockIdx.x, p.batch, count, seq, place)) { return false; }
+  int c0, n, at;
+  range(seq, c0, n, at);
+  const int page = (at >> p.c.pl) + place;
+  const long t0 = (long)page << p.c.pl;   // the page's first token
+  s.lo = (int)(max((long)at, t0) - t0);
+  s.hi = (int)(min((long)at + n, t0 + (1 << p.c.pl)) - t0);
+  s.first = c0 + (t0 - at);
+  s.pid = -1;
+  if (page < p.c.table_stride) {
+    const int id = p.c.table[(long)seq * p.c.table_stride + page];
+    if (id >= 0 && id < p.c.pages) { s.pid = id; }
+  }
+  return true;
+}
+
+// A workgroup quantizes one page's new tokens of one kv head: their keys
+// (blockIdx.z 0) or their values (1).
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
+{
+  constexpr int kMaxP = 128;
+  constexpr int kPer = D / 8;   // 16-byte pieces of a token
+  constexpr int kHeld = kMaxP * kPer / kThreads;
+  __shared__ uint32_t wave_top[kThreads / 64];
+  __shared__ __attribute__((aligned(16))) uint8_t turned[D * (kMaxP + 4)];
+
+  Span sp;
+  if (!find_span(p, sp) || sp.pid < 0) { return; }
+  const int tid = threadIdx.x;
+  const int g = blockIdx.y;
+  const bool values = blockIdx.z != 0;
+  const int P = 1 << p.c.pl;
+  const uint16_t* const x = (values ? p.v_in : p.k_in) + g * D;
+  const long stride = values ? p.vstride : p.kstride;
+  int8_t* const codes = (values ? p.c.v : p.c.k) + (((long)sp.pid * p.c.kv_heads + g) << p.c.pl) * D;
+  float* const scale = (values ? p.c.vs : p.c.ks) + (long)sp.pid * p.c.kv_heads + g;
+
+  // the largest finite magnitude, as the bits of a bf16
+  const int pieces = (sp.hi - sp.lo) * kPer;
+  uint4 held[kHeld];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int at = tid + i * kThreads;
+    if (at < pieces) {
+      held[i] = *(const uint4*)(x + (sp.first + sp.lo + at / kPer) * stride + (at % kPer) * 8);
+      const uint32_t w[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = (w[j >> 1] >> (16 * (j & 1))) & 0x7fffu;
+        top = a < 0x7f80u ? max(top, a) : top;
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) { top = max(top, (uint32_t)__shfl_xor((int)top, d)); }
+  if ((tid & 63) == 0) { wave_top[tid >> 6] = top; }
+  const float s0 = sp.lo > 0 ? *scale : 0.0f;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) { top = max(top, wave_top[w]); }
+  const float s1 = fmaxf(s0, bf16_to_f32((uint16_t)top) / 127.0f);
+  const bool again = sp.lo > 0 && s1 > s0;   // the tokens before these: new codes
+  if (tid == 0) { *scale = s1; }
+
+  auto requantize = [&](uint32_t w) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float v = (float)(int8_t)((w >> (8 * j)) & 0xffu) * s0;
+      r |= ((uint32_t)quantize(v, s1) & 0xffu) << (8 * j);
+    }
+    return r;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int at = tid + i * kThreads;
+    if (at < pieces) {
+      const int tok = sp.lo + at / kPer, d0 = (at % kPer) * 8;
+      const uint32_t w[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+      uint32_t c[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = bf16_to_f32((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+        c[j >> 2] |= ((uint32_t)quantize(v, s1) & 0xffu) << (8 * (j & 3));
+      }
+      if (values) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          turned[(d0 + j) * (P + 4) + tok] = (uint8_t)(c[j >> 2] >> (8 * (j & 3)));
+        }
+      } else {
+        *(uint2*)(codes + tok * D + d0) = make_uint2(c[0], c[1]);
+      }
+    }
+  }
+  if (!values) {
+    if (again) {
+      for (int at = tid; at < sp.lo * D / 16; at += kThreads) {
+        uint4 w = *(const uint4*)(codes + at * 16);
+        w = make_uint4(requantize(w.x), requantize(w.y), requantize(w.z), requantize(w.w));
+        *(uint4*)(codes + at * 16) = w;
+      }
+    }
+    return;
+  }
+  __syncthreads();
+  // values: a channel's 16 tokens at a time, from the first that changes
+  const int t0 = again ? 0 : sp.lo & ~15;
+  const int runs = (sp.hi - t0 + 15) / 16;
+  for (int at = tid; at < D * runs; at += kThreads) {
+    const int d = at / runs, tok = t0 + (at % runs) * 16;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (tok < sp.lo) {
+      w = *(const uint4*)(codes + d * P + tok);
+      if (again) {
+        w = make_uint4(requantize(w.x), requantize(w.y), requantize(w.z), requantize(w.w));
+      }
+    }
+    uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int first = tok + 4 * j;
+      if (first + 3 >= sp.lo && first < sp.hi) {
+        const uint32_t n = *(const uint32_t*)(turned + d * (P + 4) + first);
+        // bytes of tokens lo .. hi - 1 are the new ones
+        const int skip = max(sp.lo - first, 0), end = min(sp.hi - first, 4);
+        const uint32_t mask = (0xffffffffu << (8 * skip)) & (0xffffffffu >> (8 * (4 - end)));
+        r[j] = (r[j] & ~mask) | (n & mask);
+      }
+    }
+    *(uint4*)(codes + d * P + tok) = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
+
+// A workgroup reads one page's span of one kv head back as bf16.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(MoveParams p)
+{
+  constexpr int kMaxP = 128;
+  constexpr int kPer = D / 8;
+  __shared__ __attribute__((aligned(16))) uint8_t turned[kMaxP * (D + 4)];
+  Span sp;
+  if (!find_span(p, sp)) { return; }
+  const int tid = threadIdx.x;
+  const int g = blockIdx.y;
+  const bool values = blockIdx.z != 0;
+  const int P = 1 << p.c.pl;
+  uint16_t* const y = (values ? p.v_out : p.k_out) + g * D;
+  const long stride = values ? p.vstride : p.kstride;
+  const long block = (long)(sp.pid < 0 ? 0 : sp.pid) * p.c.kv_heads + g;
+  const int8_t* const codes = (values ? p.c.v : p.c.k) + (block << p.c.pl) * D;
+  const float s = sp.pid < 0 ? 0.0f : (values ? p.c.vs : p.c.ks)[block];
+  if (values && sp.pid >= 0) {
+    const int t0 = sp.lo & ~15;
+    const int runs = (sp.hi - t0 + 15) / 16;
+    for (int at = tid; at < D * runs; at += kThreads) {
+      const int d = at / runs, tok = t0 + (at % runs) * 16;
+      const uint4 q = *(const uint4*)(codes + d * P + tok);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        turned[(tok + j) * (D + 4) + d] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+      }
+    }
+  }
+  __syncthreads();
+  for (int at = tid; at < (sp.hi - sp.lo) * kPer; at += kThreads) {
+    const int tok = sp.lo + at / kPer, d0 = (at % kPer) * 8;
+    uint2 q = make_uint2(0, 0);
+    if (sp.pid >= 0) {
+      if (values) {
+        const uint32_t* const w = (const uint32_t*)(turned + tok * (D + 4) + d0);
+        q = make_uint2(w[0], w[1]);
+      } else {
+        q = *(const uint2*)(codes + tok * D + d0);
+      }
+    }
+    auto value = [&](uint32_t w, int i) { return (float)(int8_t)((w >> (8 * i)) & 0xffu) * s; };
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (sp.pid >= 0) {
+      r.x = pack_bf16x2(value(q.x, 0), value(q.x, 1));
+      r.y = pack_bf16x2(value(q.x, 2), value(q.x, 3));
+      r.z = pack_bf16x2(value(q.y, 0), value(q.y, 1));
+      r.w = pack_bf16x2(value(q.y, 2), value(q.y, 3));
+    }
+    *(uint4*)(y + (sp.first + tok) * stride + d0) = r;
+  }
+}
+
+// ---- attention over the cache -------------------------------------------------
+
+struct CachedParams {
+  CacheView c;
+  const int* lens;
+  const uint16_t* q;
+  uint16_t* out;
+  float* lse;
+  float* part;       // [rows][splits][D] sums, then [rows][splits][2] maximum and sum
+  long qs, os;
+  int heads, share, causal;
+  float scale2;      // scale log2(e)
+  int batch, q_len, max_len;
+  int row_blocks, splits, chunk;
+};
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c)
+{
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float xor16_max(float v)
+{
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_sum(float v)
+{
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ int visible_len(const CachedParams& p, int b)
+{
+  const long most = min((long)p.max_len, (long)p.c.table_stride << p.c.pl);
+  return (int)min((long)max(p.lens[b], 0), most);
+}
+
+// A workgroup takes 16 RT rows (query token x head of the kv head) of one
+// sequence and kv head over one split of the tokens; its four waves take tiles
+// of 64 tokens in turn and join at the end.
+//
+// A wave multiplies S^T = K Q^T with v_mfma_f32_16x16x32_bf16. Row r of the
+// tile's 16-token block t is token 16 (r / 4) + 4 t + r % 4, so that the lanes
+// 16 j .. 16 j + 15 end up with the logits of tokens 16 j .. 16 j + 15: in
+// order, they are the right operand of O^T = V^T P^T, whose left one is 16 bytes
+// of a channel's tokens. Keys and values so go from memory to the matrix
+// instructions through registers alone.
+template <int D, int RT>
+__global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedParams p)
+{
+  constexpr int kL = D / 64;    // 16-byte loads of a token's key for each lane
+  constexpr int kDT = D / 16;   // 16-channel tiles
+  constexpr int kRows = 16 * RT;
+  __shared__ __attribute__((aligned(16))) float join[2][RT][64][kDT * 4 + 2];
+
+  int id = blockIdx.x;
+  const int rb = id % p.row_blocks;
+  id /= p.row_blocks;
+  const int split = id % p.splits;
+  id /= p.splits;
+  const int g = id % p.c.kv_heads;
+  const int b = id / p.c.kv_heads;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, kg = lane >> 4;
+  const int len = __builtin_amdgcn_readfirstlane(visible_len(p, b));
+  const int first = split * p.chunk;
+  if (first >= len && split > 0) { return; }
+  const int end = min(len, first + p.chunk);
+
+  // rows of the lane's column of each row tile
+  int limit[RT];
+  bf16x8 qf[RT][2 * kL];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = min(rb * kRows + rt * 16 + n, p.q_len * p.share - 1);
+    const int qi = r / p.share;
+    limit[rt] = p.causal ? len - p.q_len + qi : len - 1;
+    const uint16_t* const qp = p.q + ((long)b * p.q_len + qi) * p.qs +
+                               (long)(g * p.share + r % p.share) * D + kg * 16;
+#pragma unroll
+    for (int i = 0; i < 2 * kL; ++i) {
+      qf[rt][i] = as_bf16x8(*(const uint4*)(qp + (i >> 1) * 64 + (i & 1) * 8));
+    }
+  }
+  f32x4 o[RT][kDT];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) { o[rt][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+  }
+  const int* const table = p.c.table + (long)b * p.c.table_stride;
+  const int pmask = (1 << p.c.pl) - 1;
+
+  for (int t0 = first + wave * 64; t0 < end; t0 += 256) {
+    // pages of the tokens that the lane loads keys of (16 (n / 4) ..) and of
+    // those that it loads values of and holds the logits of (16 kg ..)
+    const int tk = t0 + 16 * (n >> 2), tv = t0 + 16 * kg;
+    const int last_page = p.c.table_stride - 1;
+    const int pk = clampi(table[min(tk >> p.c.pl, last_page)], 0, p.c.pages - 1);
+    const int pv_id = table[min(tv >> p.c.pl, last_page)];
+    const int pv = clampi(pv_id, 0, p.c.pages - 1);
+    const long bk = (long)pk * p.c.kv_heads + g, bv = (long)pv * p.c.kv_heads + g;
+    const int8_t* const kp = p.c.k + ((bk << p.c.pl) + (tk & pmask) + (n & 3)) * D + kg * 16;
+    const int8_t* const vp = p.c.v + (bv << p.c.pl) * D + ((long)n << p.c.pl) + (tv & pmask);
+    uint4 kc[4][kL], vc[kDT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int i = 0; i < kL; ++i) { kc[t][i] = *(const uint4*)(kp + t * 4 * D + i * 64); }
+    }
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) { vc[d] = *(const uint4*)(vp + ((long)d << (p.c.pl + 4))); }
+    const float sk = p.c.ks[bv] * p.scale2, sv = p.c.vs[bv];
+    const bool held = pv_id == pv;
+
+    f32x4 s[RT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) { s[rt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+#pragma unroll
+      for (int i = 0; i < kL; ++i) {
+        const bf16x8 a = codes_bf16(kc[t][i].x, kc[t][i].y);
+        const bf16x8 c = codes_bf16(kc[t][i].z, kc[t][i].w);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          s[rt][t] = mfma16(a, qf[rt][2 * i], s[rt][t]);
+          s[rt][t] = mfma16(c, qf[rt][2 * i + 1], s[rt][t]);
+        }
+      }
+    }
+    bf16x8 pf[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int lim = held ? min(limit[rt], end - 1) : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = s[rt][t][i] * sk;
+          s[rt][t][i] = tv + 4 * t + i <= lim ? v : -INFINITY;
+          top = fmaxf(top, s[rt][t][i]);
+        }
+      }
+      top = xor32_max(xor16_max(top));
+      const float m_new = fmaxf(m[rt], top);
+      const float ms = m_new == -INFINITY ? 0.0f : m_new;
+      const float keep = __builtin_amdgcn_exp2f(m[rt] - ms);
+      m[rt] = m_new;
+      float sum = 0.0f;
+      float w[16];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(s[rt][t][i] - ms);
+          sum += e;
+          // a masked token's scale may be anything
+          w[4 * t + i] = tv + 4 * t + i <= lim ? e * sv : 0.0f;
+        }
+      }
+      l[rt] = fmaf(l[rt], keep, sum);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint4 pw;
+        pw.x = pack_bf16x2(w[8 * j + 0], w[8 * j + 1]);
+        pw.y = pack_bf16x2(w[8 * j + 2], w[8 * j + 3]);
+        pw.z = pack_bf16x2(w[8 * j + 4], w[8 * j + 5]);
+        pw.w = pack_bf16x2(w[8 * j + 6], w[8 * j + 7]);
+        pf[rt][j] = as_bf16x8(pw);
+      }
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { o[rt][d][i] *= keep; }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) {
+      const bf16x8 a = codes_bf16(vc[d].x, vc[d].y);
+      const bf16x8 c = codes_bf16(vc[d].z, vc[d].w);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        o[rt][d] = mfma16(a, pf[rt][0], o[rt][d]);
+        o[rt][d] = mfma16(c, pf[rt][1], o[rt][d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) { l[rt] = xor32_sum(xor16_sum(l[rt])); }
+
+  // ---- the waves join: 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+  for (int step = 2; step >= 1; step /= 2) {
+    if (wave >= step && wave < 2 * step) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float* const at = join[wave - step][rt][lane];
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { at[4 * d + i] = o[rt][d][i]; }
+        }
+        at[4 * kDT] = m[rt];
+        at[4 * kDT + 1] = l[rt];
+      }
+    }
+    __syncthreads();
+    if (wave < step) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float* const at = join[wave][rt][lane];
+        const float m2 = at[4 * kDT], l2 = at[4 * kDT + 1];
+        const float mn = fmaxf(m[rt], m2);
+        const float ms = mn == -INFINITY ? 0.0f : mn;
+        const float a = __builtin_amdgcn_exp2f(m[rt] - ms), c = __builtin_amdgcn_exp2f(m2 - ms);
+        m[rt] = mn;
+        l[rt] = l[rt] * a + l2 * c;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { o[rt][d][i] = o[rt][d][i] * a + at[4 * d + i] * c; }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (wave != 0) { return; }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rb * kRows + rt * 16 + n;
+    if (r >= p.q_len * p.share) { continue; }
+    const long token = (long)b * p.q_len + r / p.share;
+    const int head = g * p.share + r % p.share;
+    const long at = token * p.heads + head;
+    if (p.splits > 1) {
+      const long rows = (long)p.batch * p.q_len * p.heads;
+      float* const op = p.part + (at * p.splits + split) * D + 4 * kg;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) { *(f32x4*)(op + 16 * d) = o[rt][d]; }
+      if (kg == 0) {
+        *(float2*)(p.part + rows * p.splits * D + (at * p.splits + split) * 2) =
+            make_float2(m[rt], l[rt]);
+      }
+    } else {
+      const float inv = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
+      uint16_t* const op = p.out + token * p.os + (long)head * D + 4 * kg;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) {
+        *(uint2*)(op + 16 * d) = make_uint2(pack_bf16x2(o[rt][d][0] * inv, o[rt][d][1] * inv),
+                                            pack_bf16x2(o[rt][d][2] * inv, o[rt][d][3] * inv));
+      }
+      if (p.lse != nullptr && kg == 0) {
+        p.lse[at] = l[rt] == 0.0f ? -INFINITY : (m[rt] + log2f(l[rt])) * 0.69314718055994531f;
+      }
+    }
+  }
+}
+
+// The splits of a row joined, in order; a wave for each row.
+template <int D>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(CachedParams p)
+{
+  constexpr int kPer = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long rows = (long)p.batch * p.q_len * p.heads;
+  const long at = (long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (at >= rows) { return; }
+  const long token = at / p.heads;
+  const int head = (int)(at % p.heads);
+  const int len = visible_len(p, (int)(token / p.q_len));
+  const int used = min((len + p.chunk - 1) / p.chunk, p.splits);
+  const float2* const ml = (const float2*)(p.part + rows * p.splits * D) + at * p.splits;
+  float top = -INFINITY;
+  for (int s = lane; s < used; s += 64) { top = fmaxf(top, ml[s].x); }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) { top = fmaxf(top, __shfl_xor(top, d)); }
+  const float ms = top == -INFINITY ? 0.0f : top;
+  const float* const op = p.part + at * p.splits * D + lane * kPer;
+  float l = 0.0f, acc[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) { acc[i] = 0.0f; }
+  for (int s = 0; s < used; ++s) {
+    const float2 x = ml[s];
+    const float w = __builtin_amdgcn_exp2f(x.x - ms);
+    l = fmaf(w, x.y, l);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) { acc[i] = fmaf(w, op[(long)s * D + i], acc[i]); }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* const y = p.out + token * p.os + (long)head * D + lane * kPer;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) { y[i] = f32_to_bf16(acc[i] * inv); }
+  if (p.lse != nullptr && lane == 0) {
+    p.lse[at] = l == 0.0f ? -INFINITY : (ms + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+CacheView view_of(const CacheArgs& c)
+{
+  CacheView v;
+  v.k = c.k;
+  v.v = c.v;
+  v.ks = c.ks;
+  v.vs = c.vs;
+  v.table = c.table;
+  v.pages = c.pages;
+  v.pl = c.page_log2;
+  v.kv_heads = c.kv_heads;
+  v.table_stride = c.table_stride;
+  return v;
+}
+
+// Pages that `total` tokens of `batch` sequences can touch: a sequence's n
+// tokens lie in at most n / P + 2.
+bool move_grid(const MoveParams& p, dim3& grid)
+{
+  const long units = ((long)p.total >> p.c.pl) + 2L * p.batch;
+  if (units > INT_MAX || p.c.kv_heads > 65535) { return false; }
+  grid = dim3((unsigned)units, (unsigned)p.c.kv_heads, 2);
+  return true;
+}
+
+template <int D, int RT>
+hipError_t run_cached(const CachedParams& p, hipStream_t stream)
+{
+  const long grid = (long)p.batch * p.c.kv_heads * p.splits * p.row_blocks;
+  const long rows = (long)p.batch * p.q_len * p.heads;
+  if (grid > INT_MAX || rows > INT_MAX) { return hipErrorInvalidConfiguration; }
+  attention_cached_kernel<D, RT><<<(int)grid, kThreads, 0, stream>>>(p);
+  if (p.splits > 1) {
+    constexpr int kWaves = kThreads / 64;
+    attention_join_kernel<D><<<(int)((rows + kWaves - 1) / kWaves), kThreads, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t run_cached(const CachedParams& p, int row_tiles, hipStream_t stream)
+{
+  if (row_tiles == 1) { return run_cached<D, 1>(p, stream); }
+  if (row_tiles == 2) { return run_cached<D, 2>(p, stream); }
+  return run_cached<D, 4>(p, stream);
+}
+
+}  // namespace
+
+hipError_t launch_kv_append(const CacheArgs& c, const uint16_t* k, const uint16_t* v, int64_t ks,
+                            int64_t vs, const int* cu, const int* start, int batch, int total,
+                            hipStream_t stream)
+{
+  const MoveParams p = {view_of(c), k, v, nullptr, nullptr, (long)ks, (long)vs, cu, start, batch,
+                        total};
+  dim3 grid;
+  if (!move_grid(p, grid)) { return hipErrorInvalidConfiguration; }
+  if (c.head_dim == 128) {
+    kv_append_kernel<128><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    kv_append_kernel<64><<<grid, kThreads, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_read(const CacheArgs& c, uint16_t* k, uint16_t* v, int64_t ks, int64_t vs,
+                          const int* cu, const int* start, int batch, int total,
+                          hipStream_t stream)
+{
+  const MoveParams p = {view_of(c), nullptr, nullptr, k, v, (long)ks, (long)vs, cu, start, batch,
+                        total};
+  dim3 grid;
+  if (!move_grid(p, grid)) { return hipErrorInvalidConfiguration; }
+  if (c.head_dim == 128) {
+    kv_read_kernel<128><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    kv_read_kernel<64><<<grid, kThreads, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+
+CachedPlan plan_cached(int batch, int q_len, int heads, int kv_heads, int head_dim, int max_len)
+{
+  CachedPlan r;
+  const long rows = (long)q_len * (heads / kv_heads);
+  r.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  r.row_blocks = (int)((rows + 16 * r.row_tiles - 1) / (16 * r.row_tiles));
+  // splits of whole rounds of the four waves (256 tokens), as many as fill the
+  // GPU four times over
+  const long units = (long)batch * kv_heads * r.row_blocks;
+  const long rounds = ((long)max_len + 255) / 256;
+  const long want = std::max(1L, std::min(rounds, (1024 + units - 1) / units));
+  const long per = std::max(1L, (rounds + want - 1) / want);
+  r.chunk = (int)std::min(per * 256, (long)(INT_MAX & ~255));
+  r.splits = (int)std::max(1L, (rounds + per - 1) / per);
+  if (r.splits > 1) {
+    r.workspace_bytes = (size_t)batch * q_len * heads * r.splits * (head_dim + 2) * sizeof(float);
+  }
+  return r;
+}
+
+hipError_t launch_attention_cached(const CachedArgs& a, hipStream_t stream)
+{
+  const CachedPlan plan =
+      plan_cached(a.batch, a.q_len, a.heads, a.c.kv_heads, a.c.head_dim, a.max_len);
+  CachedParams p;
+  p.c = view_of(a.c);
+  p.lens = a.lens;
+  p.q = a.q;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.part = a.workspace;
+  p.qs = (long)a.qs;
+  p.os = (long)a.os;
+  p.heads = a.heads;
+  p.share = a.heads / a.c.kv_heads;
+  p.causal = a.causal;
+  p.scale2 = a.scale * 1.4426950408889634f;
+  p.batch = a.batch;
+  p.q_len = a.q_len;
+  p.max_len = a.max_len;
+  p.row_blocks = plan.row_blocks;
+  p.splits = plan.splits;
+  p.chunk = plan.chunk;
+  return a.c.head_dim == 128 ? run_cached<128>(p, plan.row_tiles, stream)
+                             : run_cached<64>(p, plan.row_tiles, stream);
+}
+
+}  // namespace ltx25

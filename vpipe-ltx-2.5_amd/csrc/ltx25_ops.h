@@ -15,6 +15,7 @@
 // Header-only: everything below compiles into the caller.
 #pragma once
 
+#include "ltx25_attention.h"
 #include "ltx25_qlinear.h"
 
 #include <hip/hip_runtime.h>
@@ -125,6 +126,44 @@ public:
     note(ltx25_linear_q_lora(enc, x, &cw, bias, bias != nullptr ? LTX25_DT_BF16 : LTX25_DT_NONE,
                              a, b, rank, y, M, K, N,
                              gelu ? LTX25_EPI_GELU_TANH : LTX25_EPI_NONE));
+  }
+
+  // Attention between the projections and gate_heads: packed sequences, or one
+  // (cu_q and cu_k null, batch 1). Sizes and strides as ltx25_attn has them.
+  void attention(hipStream_t enc, const ltx25_attn& a, const void* q, const void* k, const void* v,
+                 void* out, float* lse, const int* cu_q, const int* cu_k, int batch, int total_q,
+                 int total_k) const
+  {
+    note(ltx25_attention(enc, &a, q, k, v, out, lse, cu_q, cu_k, batch, total_q, total_k));
+  }
+
+  // The 8-bit cache: new tokens in, tokens out as bf16, attention over it. k and
+  // v lie at a.k_stride and a.v_stride.
+  void kv_append(hipStream_t enc, const ltx25_attn& a, const ltx25_kv_cache& cache,
+                 const int* table, int table_stride, const void* k, const void* v, const int* cu,
+                 const int* start, int batch, int total) const
+  {
+    note(ltx25_kv_append(enc, &cache, table, table_stride, k, v, a.k_stride, a.v_stride, cu, start,
+                         batch, total));
+  }
+  void kv_read(hipStream_t enc, const ltx25_attn& a, const ltx25_kv_cache& cache, const int* table,
+               int table_stride, void* k, void* v, const int* cu, const int* start, int batch,
+               int total) const
+  {
+    note(ltx25_kv_read(enc, &cache, table, table_stride, k, v, a.k_stride, a.v_stride, cu, start,
+                       batch, total));
+  }
+  void attention_cached(hipStream_t enc, const ltx25_attn& a, const ltx25_kv_cache& cache,
+                        const int* table, int table_stride, const int* lens, const void* q,
+                        void* out, float* lse, int batch, int q_len, int max_len, void* workspace,
+                        size_t workspace_bytes) const
+  {
+    note(ltx25_attention_cached(enc, &a, &cache, table, table_stride, lens, q, out, lse, batch,
+                                q_len, max_len, workspace, workspace_bytes));
+  }
+  static size_t attention_cached_workspace(const ltx25_attn& a, int batch, int q_len, int max_len)
+  {
+    return ltx25_attention_cached_workspace(batch, q_len, a.heads, a.kv_heads, a.head_dim, max_len);
   }
 
   // The dequant-once arm (src/ltx25-metal-ops.cc:467-502): LTX25_DEQUANT_ONCE_*.

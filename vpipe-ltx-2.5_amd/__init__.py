@@ -333,32 +333,42 @@ def gate_heads(y, logits, heads: int, tokens: int, head_dim: int, stream=None) -
 # ---- attention (include/ltx25_attention.h) ------------------------------------------
 
 
-def _tokens(name: str, t) -> tuple[int, int, int, int]:
-    """(tokens, heads, head width, elements from a token to the next) of a bf16 tensor
-    [tokens][heads][head_dim] whose tokens lie in one piece each (a part of a fused
-    projection's output does)."""
-    torch = _torch or _import_torch()
-    if t.dtype != torch.bfloat16 or t.dim() != 3:
+def _tokens(name: str, t, shape) -> int:
+    """The elements from a token to the next of a bf16 tensor [tokens][heads][head_dim] (its
+    `shape`) whose tokens lie in one piece each, as a part of a fused projection's output does.
+    A decode step can take as long on the host as on the GPU, hence the one test of what is
+    usual."""
+    stride = t.stride()
+    if (len(shape) == 3 and stride[2] == 1 and stride[1] == shape[2] and shape[0] > 1
+            and t.dtype is _torch.bfloat16):
+        return stride[0]
+    if len(shape) != 3 or t.dtype is not _torch.bfloat16:
         raise TypeError(f"{name} must be bf16 [tokens][heads][head_dim], got {t.dtype} "
-                        f"{tuple(t.shape)}")
-    n, heads, dim = t.shape
-    stride, head, one = t.stride()
-    if n > 0 and ((one != 1 and dim > 1) or (head != dim and heads > 1)):
-        raise ValueError(f"{name}: a token's heads must lie side by side, got strides {t.stride()}")
-    return n, heads, dim, stride if n > 1 else max(stride, heads * dim)
+                        f"{tuple(shape)}")
+    n, heads, dim = shape
+    if n > 0 and ((stride[2] != 1 and dim > 1) or (stride[1] != dim and heads > 1)):
+        raise ValueError(f"{name}: a token's heads must lie side by side, got strides {stride}")
+    return stride[0] if n > 1 else max(stride[0], heads * dim)
 
 
-def _int32(name: str, t, *shape) -> None:
-    torch = _torch or _import_torch()
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise TypeError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} "
+def _int32(name: str, t, count: int) -> None:
+    if t.dtype is not _torch.int32 or t.numel() != count or not t.is_contiguous():
+        raise TypeError(f"{name} must be contiguous int32 with {count} elements, got {t.dtype} "
                         f"{tuple(t.shape)}")
+
+
+def _table(t, batch: int) -> int:
+    shape = t.shape
+    if (t.dtype is not _torch.int32 or len(shape) != 2 or shape[0] != batch
+            or not t.is_contiguous()):
+        raise TypeError(f"table must be contiguous int32 [{batch}][pages], got {t.dtype} "
+                        f"{tuple(shape)}")
+    return shape[1]
 
 
 def _lse(t, tokens: int, heads: int) -> None:
-    torch = _torch or _import_torch()
-    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (tokens, heads)
-                          or not t.is_contiguous()):
+    if (t.dtype is not _torch.float32 or tuple(t.shape) != (tokens, heads)
+            or not t.is_contiguous()):
         raise TypeError(f"lse must be contiguous float32 [{tokens}][{heads}], got {t.dtype} "
                         f"{tuple(t.shape)}")
 
@@ -368,23 +378,29 @@ def attention(q, k, v, out, cu_q=None, cu_k=None, *, causal: bool, scale: float 
     """Attention of packed sequences (ltx25_attention): q, out [total_q][heads][head_dim], k, v
     [total_k][kv_heads][head_dim] bf16, cu_q, cu_k int32 [batch + 1] (both None: one sequence),
     lse float32 [total_q][heads] or None. scale 0 is 1 / sqrt(head_dim)."""
-    nq, heads, dim, qs = _tokens("q", q)
-    nk, kv_heads, kdim, ks = _tokens("k", k)
-    if k.shape != v.shape or q.shape != out.shape or kdim != dim:
+    if _torch is None:
+        _import_torch()
+    q_shape, k_shape = q.shape, k.shape
+    qs, ks = _tokens("q", q, q_shape), _tokens("k", k, k_shape)
+    vs, os_ = _tokens("v", v, v.shape), _tokens("out", out, out.shape)
+    nq, heads, dim = q_shape
+    nk, kv_heads, kdim = k_shape
+    if k_shape != v.shape or q_shape != out.shape or kdim != dim:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, out "
                          f"{tuple(out.shape)} do not fit each other")
-    vs, os_ = _tokens("v", v)[3], _tokens("out", out)[3]
-    batch = 1
+    batch, pq, pk = 1, None, None
     if cu_q is not None or cu_k is not None:
         if cu_q is None or cu_k is None:
             raise ValueError("cu_q and cu_k go together")
         batch = cu_q.numel() - 1
         _int32("cu_q", cu_q, batch + 1)
         _int32("cu_k", cu_k, batch + 1)
-    _lse(lse, nq, heads)
+        pq, pk = cu_q.data_ptr(), cu_k.data_ptr()
+    if lse is not None:
+        _lse(lse, nq, heads)
     a = AttnC(heads, kv_heads, dim, 1 if causal else 0, scale, qs, ks, vs, os_)
-    check(load().ltx25_attention(_stream(stream), ctypes.byref(a), _ptr(q), _ptr(k), _ptr(v),
-                                 _ptr(out), _ptr(lse), _ptr(cu_q), _ptr(cu_k), batch, nq, nk))
+    check(load().ltx25_attention(_stream(stream), ctypes.byref(a), q.data_ptr(), k.data_ptr(),
+                                 v.data_ptr(), out.data_ptr(), _ptr(lse), pq, pk, batch, nq, nk))
 
 
 class KVCache:
@@ -409,6 +425,7 @@ class KVCache:
                                 f"{t.dtype} {tuple(t.shape)}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, page, dim
+        self._c = KVCacheC(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), pages, page, heads, dim)
 
     @classmethod
     def empty(cls, pages: int, page_tokens: int, kv_heads: int, head_dim: int, device="cuda"):
@@ -420,38 +437,37 @@ class KVCache:
         return cls(k, v, *scales)
 
     def c(self) -> KVCacheC:
-        return KVCacheC(_ptr(self.k), _ptr(self.v), _ptr(self.k_scale), _ptr(self.v_scale),
-                        self.pages, self.page_tokens, self.kv_heads, self.head_dim)
+        return self._c
 
 
 def _moved(cache: KVCache, table, k, v, cu, start):
-    total, heads, dim, ks = _tokens("k", k)
-    vs = _tokens("v", v)[3]
-    if k.shape != v.shape or (heads, dim) != (cache.kv_heads, cache.head_dim):
+    shape = k.shape
+    ks, vs = _tokens("k", k, shape), _tokens("v", v, v.shape)
+    total, heads, dim = shape
+    if shape != v.shape or heads != cache.kv_heads or dim != cache.head_dim:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit the cache's "
                          f"{cache.kv_heads} heads of width {cache.head_dim}")
     batch = start.numel()
-    _int32("table", table, batch, table.shape[-1])
+    stride = _table(table, batch)
     _int32("cu", cu, batch + 1)
     _int32("start", start, batch)
-    return cache.c(), ks, vs, batch, total
+    return (ctypes.byref(cache.c()), table.data_ptr(), stride, k.data_ptr(), v.data_ptr(), ks, vs,
+            cu.data_ptr(), start.data_ptr(), batch, total)
 
 
 def kv_append(cache: KVCache, table, k, v, cu, start, stream=None) -> None:
     """Quantize new keys and values [total][kv_heads][head_dim] into the cache
     (ltx25_kv_append): sequence b's tokens cu[b] .. cu[b + 1] - 1 become tokens start[b] ... of
     its pages table[b]."""
-    c, ks, vs, batch, total = _moved(cache, table, k, v, cu, start)
-    check(load().ltx25_kv_append(_stream(stream), ctypes.byref(c), _ptr(table), table.shape[1],
-                                 _ptr(k), _ptr(v), ks, vs, _ptr(cu), _ptr(start), batch, total))
+    args = _moved(cache, table, k, v, cu, start)
+    check(load().ltx25_kv_append(_stream(stream), *args))
 
 
 def kv_read(cache: KVCache, table, k, v, cu, start, stream=None) -> None:
     """Read tokens start[b] ... of each sequence back into k, v [total][kv_heads][head_dim] at
     cu[b] ... (ltx25_kv_read)."""
-    c, ks, vs, batch, total = _moved(cache, table, k, v, cu, start)
-    check(load().ltx25_kv_read(_stream(stream), ctypes.byref(c), _ptr(table), table.shape[1],
-                               _ptr(k), _ptr(v), ks, vs, _ptr(cu), _ptr(start), batch, total))
+    args = _moved(cache, table, k, v, cu, start)
+    check(load().ltx25_kv_read(_stream(stream), *args))
 
 
 def attention_cached_workspace(batch: int, q_len: int, heads: int, kv_heads: int, head_dim: int,
@@ -466,22 +482,25 @@ def attention_cached(cache: KVCache, table, lens, q, out, q_len: int, max_len: i
     """Attention of each sequence's q_len newest tokens over its cache (ltx25_attention_cached):
     q, out [batch * q_len][heads][head_dim] bf16, lens int32 [batch] with the queries' own tokens
     counted, workspace a uint8 tensor of attention_cached_workspace() bytes."""
-    nq, heads, dim, qs = _tokens("q", q)
+    shape = q.shape
+    qs, os_ = _tokens("q", q, shape), _tokens("out", out, out.shape)
+    nq, heads, dim = shape
     batch = lens.numel()
-    if q.shape != out.shape or nq != batch * q_len:
+    if shape != out.shape or nq != batch * q_len:
         raise ValueError(f"q {tuple(q.shape)} and out {tuple(out.shape)} are not {batch} x {q_len} "
                          f"tokens")
-    os_ = _tokens("out", out)[3]
-    _int32("table", table, batch, table.shape[-1])
+    pages = _table(table, batch)
     _int32("lens", lens, batch)
-    _lse(lse, nq, heads)
+    if lse is not None:
+        _lse(lse, nq, heads)
     a = AttnC(heads, cache.kv_heads, dim, 1 if causal else 0, scale, qs, 0, 0, os_)
-    c = cache.c()
-    held = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    check(load().ltx25_attention_cached(_stream(stream), ctypes.byref(a), ctypes.byref(c),
-                                        _ptr(table), table.shape[1], _ptr(lens), _ptr(q),
-                                        _ptr(out), _ptr(lse), batch, q_len, max_len,
-                                        _ptr(workspace), held))
+    at, held = None, 0
+    if workspace is not None:
+        at, held = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    check(load().ltx25_attention_cached(_stream(stream), ctypes.byref(a), ctypes.byref(cache.c()),
+                                        table.data_ptr(), pages, lens.data_ptr(), q.data_ptr(),
+                                        out.data_ptr(), _ptr(lse), batch, q_len, max_len, at,
+                                        held))
 
 
 def probe_read(src, nbytes: int, sink, blocks: int, stream=None) -> None:

@@ -37,13 +37,15 @@ __device__ __forceinline__ float xor32_sum(float v)
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// A list of units, count(b) for each sequence b in order: the sequence and the
-// place within it of unit u. Every lane of a wave takes part and all get the
+// A list of units, count(b) for each sequence b in order: the sequence, the
+// place within it of unit u, and the lane whose count(b) was the sequence's (what
+// else that call read is there). Every lane of a wave takes part and all get the
 // same answer; false when there are fewer units. The counts come from device
 // memory that the caller has not checked: each is cut to [0, 2^24] and the sum
 // kept in 64 bits.
 template <typename Count>
-__device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& seq, int& place)
+__device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& seq, int& place,
+                                          int& from)
 {
   const int lane = threadIdx.x & 63;
   long base = 0;
@@ -57,13 +59,12 @@ __device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& 
     }
     const unsigned long long past = __ballot(base + sum > (long)u);
     if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      seq = __builtin_amdgcn_readfirstlane(b0 + at);
-      const int before = __shfl(sum - n, at);
-      place = __builtin_amdgcn_readfirstlane((int)(u - base) - before);
+      from = __builtin_ctzll(past);
+      seq = b0 + from;
+      place = (int)(u - base) - __builtin_amdgcn_readlane(sum - n, from);
       return true;
     }
-    base += __shfl(sum, 63);
+    base += __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
 }

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(NW * 64) attention_kernel(PromptParams p)
     hg = blockIdx.x % p.head_groups;
     u = blockIdx.x / p.head_groups;
   }
-  int seq = 0, place = 0;
+  int seq = 0, place = 0, from = 0;
   auto len_q = [&](int b, int& q0) {
     if (p.cu_q == nullptr) { q0 = 0; return p.total_q; }
     q0 = clampi(p.cu_q[b], 0, p.total_q);
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(NW * 64) attention_kernel(PromptParams p)
     int q0;
     return (len_q(b, q0) + tb - 1) >> p.tb_log2;
   };
-  if (!find_unit(u, p.batch, tiles, seq, place)) { return; }
+  if (!find_unit(u, p.batch, tiles, seq, place, from)) { return; }
   int q0, k0;
   const int lq = __builtin_amdgcn_readfirstlane(len_q(seq, q0));
   q0 = __builtin_amdgcn_readfirstlane(q0);

@@ -39,6 +39,46 @@ __device__ __forceinline__ int quantize(float x, float s)
   return s > 0.0f && r == r ? (int)fminf(fmaxf(r, -127.0f), 127.0f) : 0;
 }
 
+// Four codes as bytes. `rs` > 0 is 1 / s, correctly rounded, for s well inside the
+// normal range and |x| at most 127 s: the quotient is x rs made better twice by its
+// exact remainder, after which it is the correctly rounded one (after the first
+// step it is off by less than a unit of its last place, from where the second is
+// Markstein's), in five operations for the division's ten; quotients too small for
+// an exact remainder are far below 1/2. Adding 3 * 2^22 rounds to even with the
+// code in the low byte. rs 0: any s and x.
+__device__ __forceinline__ uint32_t quantize4(const float (&x)[4], float s, float rs)
+{
+  uint32_t c[4];
+  if (rs > 0.0f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float q = x[i] * rs;
+      q = fmaf(fmaf(-q, s, x[i]), rs, q);
+      q = fmaf(fmaf(-q, s, x[i]), rs, q);
+      c[i] = __float_as_uint(q + 12582912.0f);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { c[i] = (uint32_t)quantize(x[i], s); }
+  }
+  const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+  return lo | hi;
+}
+
+// Four words of four bytes each, turned: word i of the result is byte i of the four
+__device__ __forceinline__ void turn4(uint32_t (&w)[4])
+{
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);   // 0.0 1.0 0.1 1.1
+  const uint32_t b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);   // 0.2 1.2 0.3 1.3
+  const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
 // ---- append, read -----------------------------------------------------------
 
 struct MoveParams {
@@ -56,7 +96,7 @@ struct MoveParams {
 // One page of one sequence that a call touches: tokens lo .. hi - 1 of it are
 // packed tokens first + lo ...
 struct Span {
-  int pid;       // -1: no such page
+  const int* id;   // where the page's id is; null past the table
   int lo, hi;
   long first;
 };
@@ -65,111 +105,152 @@ struct Span {
 __device__ __forceinline__ bool find_span(const MoveParams& p, Span& s)
 {
   constexpr int kFar = 1 << 30;
-  auto range = [&](int b, int& c0, int& n, int& at) {
+  int c0 = 0, n = 0, at = 0;
+  auto count = [&](int b) {
     c0 = clampi(p.cu[b], 0, p.total);
     n = clampi(p.cu[b + 1], c0, p.total) - c0;
     at = clampi(p.start[b], 0, kFar);
-  };
-  auto count = [&](int b) {
-    int c0, n, at;
-    range(b, c0, n, at);
     return n > 0 ? ((at + (n - 1)) >> p.c.pl) - (at >> p.c.pl) + 1 : 0;
   };
-  int seq = 0, place = 0;
-  if (!find_unit((int)blockIdx.x, p.batch, count, seq, place)) { return false; }
-  int c0, n, at;
-  range(seq, c0, n, at);
+  int seq = 0, place = 0, from = 0;
+  if (!find_unit((int)blockIdx.x, p.batch, count, seq, place, from)) { return false; }
+  c0 = __builtin_amdgcn_readlane(c0, from);
+  n = __builtin_amdgcn_readlane(n, from);
+  at = __builtin_amdgcn_readlane(at, from);
   const int page = (at >> p.c.pl) + place;
   const long t0 = (long)page << p.c.pl;   // the page's first token
   s.lo = (int)(max((long)at, t0) - t0);
   s.hi = (int)(min((long)at + n, t0 + (1 << p.c.pl)) - t0);
   s.first = c0 + (t0 - at);
-  s.pid = -1;
-  if (page < p.c.table_stride) {
-    const int id = p.c.table[(long)seq * p.c.table_stride + page];
-    if (id >= 0 && id < p.c.pages) { s.pid = id; }
-  }
+  s.id = page < p.c.table_stride ? p.c.table + (long)seq * p.c.table_stride + page : nullptr;
   return true;
 }
 
 // A workgroup quantizes one page's new tokens of one kv head: their keys
-// (blockIdx.z 0) or their values (1).
+// (blockIdx.z 0) or their values (1). A thread holds four tokens of 8 channels, so
+// that its codes are whole words both by token and, turned, by channel.
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
 {
   constexpr int kMaxP = 128;
   constexpr int kPer = D / 8;   // 16-byte pieces of a token
-  constexpr int kHeld = kMaxP * kPer / kThreads;
+  constexpr int kHeld = kMaxP / 4 * kPer / kThreads;
   __shared__ uint32_t wave_top[kThreads / 64];
   __shared__ __attribute__((aligned(16))) uint8_t turned[D * (kMaxP + 4)];
 
   Span sp;
-  if (!find_span(p, sp) || sp.pid < 0) { return; }
+  if (!find_span(p, sp) || sp.id == nullptr) { return; }
   const int tid = threadIdx.x;
   const int g = blockIdx.y;
   const bool values = blockIdx.z != 0;
   const int P = 1 << p.c.pl;
   const uint16_t* const x = (values ? p.v_in : p.k_in) + g * D;
   const long stride = values ? p.vstride : p.kstride;
-  int8_t* const codes = (values ? p.c.v : p.c.k) + (((long)sp.pid * p.c.kv_heads + g) << p.c.pl) * D;
-  float* const scale = (values ? p.c.vs : p.c.ks) + (long)sp.pid * p.c.kv_heads + g;
 
-  // the largest finite magnitude, as the bits of a bf16
-  const int pieces = (sp.hi - sp.lo) * kPer;
-  uint4 held[kHeld];
-  uint32_t top = 0;
+  // the tokens are asked for beside the page's id; the largest magnitude of what
+  // is finite, as the bits of a bf16
+  const int pid = *sp.id;
+  const int quad0 = sp.lo >> 2;
+  const int pieces = (((sp.hi + 3) >> 2) - quad0) * kPer;
+  uint4 held[kHeld][4];
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int at = tid + i * kThreads;
-    if (at < pieces) {
-      held[i] = *(const uint4*)(x + (sp.first + sp.lo + at / kPer) * stride + (at % kPer) * 8);
-      const uint32_t w[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t a = (w[j >> 1] >> (16 * (j & 1))) & 0x7fffu;
-        top = a < 0x7f80u ? max(top, a) : top;
+    for (int j = 0; j < 4; ++j) {
+      const int tok = (quad0 + at / kPer) * 4 + j;
+      held[i][j] = make_uint4(0, 0, 0, 0);
+      if (at < pieces && tok >= sp.lo && tok < sp.hi) {
+        held[i][j] = *(const uint4*)(x + (sp.first + tok) * stride + (at % kPer) * 8);
+      }
+    }
+  }
+  if (pid < 0 || pid >= p.c.pages) { return; }
+  int8_t* const codes = (values ? p.c.v : p.c.k) + (((long)pid * p.c.kv_heads + g) << p.c.pl) * D;
+  float* const scale = (values ? p.c.vs : p.c.ks) + (long)pid * p.c.kv_heads + g;
+  const float s0 = sp.lo > 0 ? *scale : 0.0f;
+
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  auto magnitudes = [](uint32_t w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); };
+  u16x2 tops = {0, 0};
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w[4] = {held[i][j].x, held[i][j].y, held[i][j].z, held[i][j].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { tops = __builtin_elementwise_max(tops, magnitudes(w[k])); }
+    }
+  }
+  uint32_t top = max((uint32_t)tops[0], (uint32_t)tops[1]);
+  bool odd = top >= 0x7f80u;   // an infinity or a NaN among the lane's values
+  if (odd) {
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w[4] = {held[i][j].x, held[i][j].y, held[i][j].z, held[i][j].w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t a = (w[k >> 1] >> (16 * (k & 1))) & 0x7fffu;
+          top = a < 0x7f80u ? max(top, a) : top;
+        }
       }
     }
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) { top = max(top, (uint32_t)__shfl_xor((int)top, d)); }
   if ((tid & 63) == 0) { wave_top[tid >> 6] = top; }
-  const float s0 = sp.lo > 0 ? *scale : 0.0f;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) { top = max(top, wave_top[w]); }
   const float s1 = fmaxf(s0, bf16_to_f32((uint16_t)top) / 127.0f);
   const bool again = sp.lo > 0 && s1 > s0;   // the tokens before these: new codes
   if (tid == 0) { *scale = s1; }
+  const bool easy = s1 >= 0x1p-90f && s1 <= 0x1p90f;
+  const float rs = easy ? 1.0f / s1 : 0.0f;
 
+  // an old code's value is at most 127 s0, so quantize4's bound holds for it too
   auto requantize = [&](uint32_t w) {
-    uint32_t r = 0;
+    float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float v = (float)(int8_t)((w >> (8 * j)) & 0xffu) * s0;
-      r |= ((uint32_t)quantize(v, s1) & 0xffu) << (8 * j);
-    }
-    return r;
+    for (int j = 0; j < 4; ++j) { v[j] = (float)(int8_t)((w >> (8 * j)) & 0xffu) * s0; }
+    return quantize4(v, s1, rs);
   };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int at = tid + i * kThreads;
     if (at < pieces) {
-      const int tok = sp.lo + at / kPer, d0 = (at % kPer) * 8;
-      const uint32_t w[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
-      uint32_t c[2] = {0, 0};
+      const int tok0 = (quad0 + at / kPer) * 4, d0 = (at % kPer) * 8;
+      uint32_t c[2][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = bf16_to_f32((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
-        c[j >> 2] |= ((uint32_t)quantize(v, s1) & 0xffu) << (8 * (j & 3));
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w[4] = {held[i][j].x, held[i][j].y, held[i][j].z, held[i][j].w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[k] = bf16_to_f32((uint16_t)(w[2 * h + (k >> 1)] >> (16 * (k & 1))));
+          }
+          c[h][j] = quantize4(v, s1, odd ? 0.0f : rs);
+        }
       }
       if (values) {
+        turn4(c[0]);
+        turn4(c[1]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          turned[(d0 + j) * (P + 4) + tok] = (uint8_t)(c[j >> 2] >> (8 * (j & 3)));
+        for (int k = 0; k < 8; ++k) {
+          *(uint32_t*)(turned + (d0 + k) * (P + 4) + tok0) = c[k >> 2][k & 3];
         }
       } else {
-        *(uint2*)(codes + tok * D + d0) = make_uint2(c[0], c[1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (tok0 + j >= sp.lo && tok0 + j < sp.hi) {
+            *(uint2*)(codes + (tok0 + j) * D + d0) = make_uint2(c[0][j], c[1][j]);
+          }
+        }
       }
     }
   }
@@ -221,16 +302,18 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(MoveParams p)
   __shared__ __attribute__((aligned(16))) uint8_t turned[kMaxP * (D + 4)];
   Span sp;
   if (!find_span(p, sp)) { return; }
+  int pid = sp.id == nullptr ? -1 : *sp.id;
+  if (pid >= p.c.pages) { pid = -1; }
   const int tid = threadIdx.x;
   const int g = blockIdx.y;
   const bool values = blockIdx.z != 0;
   const int P = 1 << p.c.pl;
   uint16_t* const y = (values ? p.v_out : p.k_out) + g * D;
   const long stride = values ? p.vstride : p.kstride;
-  const long block = (long)(sp.pid < 0 ? 0 : sp.pid) * p.c.kv_heads + g;
+  const long block = (long)(pid < 0 ? 0 : pid) * p.c.kv_heads + g;
   const int8_t* const codes = (values ? p.c.v : p.c.k) + (block << p.c.pl) * D;
-  const float s = sp.pid < 0 ? 0.0f : (values ? p.c.vs : p.c.ks)[block];
-  if (values && sp.pid >= 0) {
+  const float s = pid < 0 ? 0.0f : (values ? p.c.vs : p.c.ks)[block];
+  if (values && pid >= 0) {
     const int t0 = sp.lo & ~15;
     const int runs = (sp.hi - t0 + 15) / 16;
     for (int at = tid; at < D * runs; at += kThreads) {
@@ -247,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(MoveParams p)
   for (int at = tid; at < (sp.hi - sp.lo) * kPer; at += kThreads) {
     const int tok = sp.lo + at / kPer, d0 = (at % kPer) * 8;
     uint2 q = make_uint2(0, 0);
-    if (sp.pid >= 0) {
+    if (pid >= 0) {
       if (values) {
         const uint32_t* const w = (const uint32_t*)(turned + tok * (D + 4) + d0);
         q = make_uint2(w[0], w[1]);
@@ -257,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(MoveParams p)
     }
     auto value = [&](uint32_t w, int i) { return (float)(int8_t)((w >> (8 * i)) & 0xffu) * s; };
     uint4 r = make_uint4(0, 0, 0, 0);
-    if (sp.pid >= 0) {
+    if (pid >= 0) {
       r.x = pack_bf16x2(value(q.x, 0), value(q.x, 1));
       r.y = pack_bf16x2(value(q.x, 2), value(q.x, 3));
       r.z = pack_bf16x2(value(q.y, 0), value(q.y, 1));
@@ -317,27 +400,46 @@ __device__ __forceinline__ int visible_len(const CachedParams& p, int b)
 // order, they are the right operand of O^T = V^T P^T, whose left one is 16 bytes
 // of a channel's tokens. Keys and values so go from memory to the matrix
 // instructions through registers alone.
-template <int D, int RT>
-__global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedParams p)
+template <int D, int RT, int NW>
+__global__ void __launch_bounds__(NW * 64) attention_cached_kernel(CachedParams p)
 {
   constexpr int kL = D / 64;    // 16-byte loads of a token's key for each lane
   constexpr int kDT = D / 16;   // 16-channel tiles
   constexpr int kRows = 16 * RT;
-  __shared__ __attribute__((aligned(16))) float join[2][RT][64][kDT * 4 + 2];
+  __shared__ __attribute__((aligned(16))) float join[NW][16][D + 4];
+  __shared__ float2 stat[NW][16];
 
-  int id = blockIdx.x;
-  const int rb = id % p.row_blocks;
-  id /= p.row_blocks;
-  const int split = id % p.splits;
-  id /= p.splits;
-  const int g = id % p.c.kv_heads;
-  const int b = id / p.c.kv_heads;
+  // Workgroups go round-robin to the 8 XCDs. The kv heads are innermost, so that
+  // every XCD gets its share of each sequence, however long; the blocks of rows
+  // of one part of the tokens stay on one XCD, side by side.
+  const int units = p.splits * p.batch * p.c.kv_heads, whole = units & ~7;
+  int u, rb;
+  if ((int)blockIdx.x < whole * p.row_blocks) {
+    const int at = blockIdx.x % (8 * p.row_blocks);
+    u = blockIdx.x / (8 * p.row_blocks) * 8 + at % 8;
+    rb = at / 8;
+  } else {
+    const int at = blockIdx.x - whole * p.row_blocks;
+    u = whole + at % (units - whole);
+    rb = at / (units - whole);
+  }
+  const int g = u % p.c.kv_heads;
+  const int b = u / p.c.kv_heads % p.batch;
+  const int split = u / p.c.kv_heads / p.batch;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, kg = lane >> 4;
-  const int len = __builtin_amdgcn_readfirstlane(visible_len(p, b));
   const int first = split * p.chunk;
+  const int* const table = p.c.table + (long)b * p.c.table_stride;
+  // pages of the tokens of which the lane loads the keys (16 (n / 4) ..), and of
+  // those of which it loads the values and holds the logits (16 kg ..); the first
+  // ones are asked for together with the length
+  const int last_page = p.c.table_stride - 1;
+  auto page_of = [&](int t) { return table[min(t >> p.c.pl, last_page)]; };
+  int t0 = first + wave * 64;
+  int id_k = page_of(t0 + 16 * (n >> 2)), id_v = page_of(t0 + 16 * kg);
+  const int len = __builtin_amdgcn_readfirstlane(visible_len(p, b));
   if (first >= len && split > 0) { return; }
   const int end = min(len, first + p.chunk);
 
@@ -365,30 +467,36 @@ __global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedParams
 #pragma unroll
     for (int d = 0; d < kDT; ++d) { o[rt][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
   }
-  const int* const table = p.c.table + (long)b * p.c.table_stride;
   const int pmask = (1 << p.c.pl) - 1;
 
-  for (int t0 = first + wave * 64; t0 < end; t0 += 256) {
-    // pages of the tokens that the lane loads keys of (16 (n / 4) ..) and of
-    // those that it loads values of and holds the logits of (16 kg ..)
-    const int tk = t0 + 16 * (n >> 2), tv = t0 + 16 * kg;
-    const int last_page = p.c.table_stride - 1;
-    const int pk = clampi(table[min(tk >> p.c.pl, last_page)], 0, p.c.pages - 1);
-    const int pv_id = table[min(tv >> p.c.pl, last_page)];
-    const int pv = clampi(pv_id, 0, p.c.pages - 1);
-    const long bk = (long)pk * p.c.kv_heads + g, bv = (long)pv * p.c.kv_heads + g;
+  uint4 kc[4][kL];
+  auto load_keys = [&](int t0, int id) {
+    const int tk = t0 + 16 * (n >> 2);
+    const long bk = (long)clampi(id, 0, p.c.pages - 1) * p.c.kv_heads + g;
     const int8_t* const kp = p.c.k + ((bk << p.c.pl) + (tk & pmask) + (n & 3)) * D + kg * 16;
-    const int8_t* const vp = p.c.v + (bv << p.c.pl) * D + ((long)n << p.c.pl) + (tv & pmask);
-    uint4 kc[4][kL], vc[kDT];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int i = 0; i < kL; ++i) { kc[t][i] = *(const uint4*)(kp + t * 4 * D + i * 64); }
     }
+  };
+  if (t0 < end) { load_keys(t0, id_k); }
+  for (; t0 < end; t0 += 64 * NW) {
+    const int tv = t0 + 16 * kg;
+    const int pv = clampi(id_v, 0, p.c.pages - 1);
+    const bool held = id_v == pv;
+    const long bv = (long)pv * p.c.kv_heads + g;
+    const int8_t* const vp = p.c.v + (bv << p.c.pl) * D + ((long)n << p.c.pl) + (tv & pmask);
+    uint4 vc[kDT];
 #pragma unroll
     for (int d = 0; d < kDT; ++d) { vc[d] = *(const uint4*)(vp + ((long)d << (p.c.pl + 4))); }
     const float sk = p.c.ks[bv] * p.scale2, sv = p.c.vs[bv];
-    const bool held = pv_id == pv;
+    // the next tile's pages; its keys are asked for as soon as this one's are used
+    const int t1 = t0 + 64 * NW;
+    if (t1 < end) {
+      id_k = page_of(t1 + 16 * (n >> 2));
+      id_v = page_of(t1 + 16 * kg);
+    }
 
     f32x4 s[RT][4];
 #pragma unroll
@@ -406,6 +514,7 @@ __global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedParams
         }
       }
     }
+    if (t1 < end) { load_keys(t1, id_k); }
     bf16x8 pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -467,80 +576,70 @@ __global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedParams
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) { l[rt] = xor32_sum(xor16_sum(l[rt])); }
 
-  // ---- the waves join: 2 and 3 into 0 and 1, then 1 into 0
-#pragma unroll
-  for (int step = 2; step >= 1; step /= 2) {
-    if (wave >= step && wave < 2 * step) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float* const at = join[wave - step][rt][lane];
-#pragma unroll
-        for (int d = 0; d < kDT; ++d) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { at[4 * d + i] = o[rt][d][i]; }
-        }
-        at[4 * kDT] = m[rt];
-        at[4 * kDT + 1] = l[rt];
-      }
-    }
-    __syncthreads();
-    if (wave < step) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float* const at = join[wave][rt][lane];
-        const float m2 = at[4 * kDT], l2 = at[4 * kDT + 1];
-        const float mn = fmaxf(m[rt], m2);
-        const float ms = mn == -INFINITY ? 0.0f : mn;
-        const float a = __builtin_amdgcn_exp2f(m[rt] - ms), c = __builtin_amdgcn_exp2f(m2 - ms);
-        m[rt] = mn;
-        l[rt] = l[rt] * a + l2 * c;
-#pragma unroll
-        for (int d = 0; d < kDT; ++d) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { o[rt][d][i] = o[rt][d][i] * a + at[4 * d + i] * c; }
-        }
-      }
-    }
-    __syncthreads();
-  }
-  if (wave != 0) { return; }
+  // ---- the waves join through LDS, 16 rows at a time: a thread takes D / 16
+  // channels of one row
+  constexpr int kPer = D / 16;
+  static_assert(NW * 64 == kThreads, "16 rows x 16 threads");
+  const int jr = threadIdx.x >> 4, jd = (threadIdx.x & 15) * kPer;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = rb * kRows + rt * 16 + n;
+    if (rt > 0) { __syncthreads(); }
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) { *(f32x4*)&join[wave][n][16 * d + 4 * kg] = o[rt][d]; }
+    if (kg == 0) { stat[wave][n] = make_float2(m[rt], l[rt]); }
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { top = fmaxf(top, stat[w][jr].x); }
+    const float ms = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) { acc[i] = 0.0f; }
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float2 x = stat[w][jr];
+      const float f = __builtin_amdgcn_exp2f(x.x - ms);
+      sum = fmaf(f, x.y, sum);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) { acc[i] = fmaf(f, join[w][jr][jd + i], acc[i]); }
+    }
+    const int r = rb * kRows + rt * 16 + jr;
     if (r >= p.q_len * p.share) { continue; }
     const long token = (long)b * p.q_len + r / p.share;
     const int head = g * p.share + r % p.share;
     const long at = token * p.heads + head;
     if (p.splits > 1) {
       const long rows = (long)p.batch * p.q_len * p.heads;
-      float* const op = p.part + (at * p.splits + split) * D + 4 * kg;
+      float* const op = p.part + (at * p.splits + split) * D + jd;
 #pragma unroll
-      for (int d = 0; d < kDT; ++d) { *(f32x4*)(op + 16 * d) = o[rt][d]; }
-      if (kg == 0) {
+      for (int i = 0; i < kPer; i += 4) {
+        *(f32x4*)(op + i) = f32x4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
+      }
+      if (jd == 0) {
         *(float2*)(p.part + rows * p.splits * D + (at * p.splits + split) * 2) =
-            make_float2(m[rt], l[rt]);
+            make_float2(top, sum);
       }
     } else {
-      const float inv = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
-      uint16_t* const op = p.out + token * p.os + (long)head * D + 4 * kg;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint32_t* const op = (uint32_t*)(p.out + token * p.os + (long)head * D + jd);
 #pragma unroll
-      for (int d = 0; d < kDT; ++d) {
-        *(uint2*)(op + 16 * d) = make_uint2(pack_bf16x2(o[rt][d][0] * inv, o[rt][d][1] * inv),
-                                            pack_bf16x2(o[rt][d][2] * inv, o[rt][d][3] * inv));
-      }
-      if (p.lse != nullptr && kg == 0) {
-        p.lse[at] = l[rt] == 0.0f ? -INFINITY : (m[rt] + log2f(l[rt])) * 0.69314718055994531f;
+      for (int i = 0; i < kPer; i += 2) { op[i / 2] = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv); }
+      if (p.lse != nullptr && jd == 0) {
+        p.lse[at] = sum == 0.0f ? -INFINITY : (ms + log2f(sum)) * 0.69314718055994531f;
       }
     }
   }
 }
 
-// The splits of a row joined, in order; a wave for each row.
+// The splits of a row joined; a wave for each row. D / 4 lanes take 4 channels
+// each of one split, so that 64 / (D / 4) splits are read side by side, and four
+// of those in flight; always added in the same order.
 template <int D>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(CachedParams p)
 {
-  constexpr int kPer = D / 64;
+  constexpr int kLanes = D / 4, kSide = 64 / kLanes;
   const int lane = threadIdx.x & 63;
+  const int part = lane / kLanes, d = (lane % kLanes) * 4;
   const long rows = (long)p.batch * p.q_len * p.heads;
   const long at = (long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (at >= rows) { return; }
@@ -552,24 +651,39 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(CachedParams p
   float top = -INFINITY;
   for (int s = lane; s < used; s += 64) { top = fmaxf(top, ml[s].x); }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) { top = fmaxf(top, __shfl_xor(top, d)); }
+  for (int i = 1; i < 64; i *= 2) { top = fmaxf(top, __shfl_xor(top, i)); }
   const float ms = top == -INFINITY ? 0.0f : top;
-  const float* const op = p.part + at * p.splits * D + lane * kPer;
-  float l = 0.0f, acc[kPer];
+  const float* const op = p.part + at * p.splits * D + d;
+  float l = 0.0f;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = part; s0 < used; s0 += 4 * kSide) {
+    f32x4 x[4];
+    float2 st[4];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) { acc[i] = 0.0f; }
-  for (int s = 0; s < used; ++s) {
-    const float2 x = ml[s];
-    const float w = __builtin_amdgcn_exp2f(x.x - ms);
-    l = fmaf(w, x.y, l);
+    for (int j = 0; j < 4; ++j) {
+      const int s = min(s0 + j * kSide, used - 1);
+      x[j] = *(const f32x4*)(op + (long)s * D);
+      st[j] = ml[s];
+    }
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) { acc[i] = fmaf(w, op[(long)s * D + i], acc[i]); }
+    for (int j = 0; j < 4; ++j) {
+      const float w = s0 + j * kSide < used ? __builtin_amdgcn_exp2f(st[j].x - ms) : 0.0f;
+      l = fmaf(w, st[j].y, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { acc[i] = fmaf(w, x[j][i], acc[i]); }
+    }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* const y = p.out + token * p.os + (long)head * D + lane * kPer;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) { y[i] = f32_to_bf16(acc[i] * inv); }
-  if (p.lse != nullptr && lane == 0) {
+  for (int i = kLanes; i < 64; i *= 2) {
+    l += __shfl_xor(l, i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { acc[j] += __shfl_xor(acc[j], i); }
+  }
+  if (part != 0) { return; }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *(uint2*)(p.out + token * p.os + (long)head * D + d) =
+      make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  if (p.lse != nullptr && d == 0) {
     p.lse[at] = l == 0.0f ? -INFINITY : (ms + log2f(l)) * 0.69314718055994531f;
   }
 }
@@ -599,13 +713,13 @@ bool move_grid(const MoveParams& p, dim3& grid)
   return true;
 }
 
-template <int D, int RT>
+template <int D, int RT, int NW>
 hipError_t run_cached(const CachedParams& p, hipStream_t stream)
 {
   const long grid = (long)p.batch * p.c.kv_heads * p.splits * p.row_blocks;
   const long rows = (long)p.batch * p.q_len * p.heads;
   if (grid > INT_MAX || rows > INT_MAX) { return hipErrorInvalidConfiguration; }
-  attention_cached_kernel<D, RT><<<(int)grid, kThreads, 0, stream>>>(p);
+  attention_cached_kernel<D, RT, NW><<<(int)grid, NW * 64, 0, stream>>>(p);
   if (p.splits > 1) {
     constexpr int kWaves = kThreads / 64;
     attention_join_kernel<D><<<(int)((rows + kWaves - 1) / kWaves), kThreads, 0, stream>>>(p);
@@ -614,11 +728,13 @@ hipError_t run_cached(const CachedParams& p, hipStream_t stream)
 }
 
 template <int D>
-hipError_t run_cached(const CachedParams& p, int row_tiles, hipStream_t stream)
+hipError_t run_cached(const CachedParams& p, const CachedPlan& plan, hipStream_t stream)
 {
-  if (row_tiles == 1) { return run_cached<D, 1>(p, stream); }
-  if (row_tiles == 2) { return run_cached<D, 2>(p, stream); }
-  return run_cached<D, 4>(p, stream);
+  if (plan.row_tiles == 1) {
+    return run_cached<D, 1, 4>(p, stream);
+  }
+  if (plan.row_tiles == 2) { return run_cached<D, 2, 4>(p, stream); }
+  return run_cached<D, 4, 4>(p, stream);
 }
 
 }  // namespace
@@ -661,12 +777,21 @@ CachedPlan plan_cached(int batch, int q_len, int heads, int kv_heads, int head_d
   const long rows = (long)q_len * (heads / kv_heads);
   r.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   r.row_blocks = (int)((rows + 16 * r.row_tiles - 1) / (16 * r.row_tiles));
-  // splits of whole rounds of the four waves (256 tokens), as many as fill the
-  // GPU four times over
+  // Parts of whole rounds of the four waves (256 tokens). Up to 4 rounds: one part,
+  // since a round takes about 1.2 us where the GPU is not full and the join's own
+  // launch 5 (700 tokens, 8 kv heads: 9.7 us for 11.4 in 3 parts). Else two
+  // workgroups for each CU, which hold enough loads in flight (32 rows of 131072
+  // tokens: 175 us, 180 with four workgroups, 185 with eight) -- but no part longer
+  // than 8 rounds or a 16th of the tokens, since the lengths may be very uneven and
+  // only the longest is known here.
   const long units = (long)batch * kv_heads * r.row_blocks;
   const long rounds = ((long)max_len + 255) / 256;
-  const long want = std::max(1L, std::min(rounds, (1024 + units - 1) / units));
-  const long per = std::max(1L, (rounds + want - 1) / want);
+  long per = std::max(rounds, 1L);
+  if (rounds > 4) {
+    const long want = (512 + units - 1) / units;
+    per = std::min((rounds + want - 1) / want, std::max(8L, rounds / 16));
+    per = (rounds + (rounds + per - 1) / per - 1) / ((rounds + per - 1) / per);
+  }
   r.chunk = (int)std::min(per * 256, (long)(INT_MAX & ~255));
   r.splits = (int)std::max(1L, (rounds + per - 1) / per);
   if (r.splits > 1) {
@@ -698,8 +823,8 @@ hipError_t launch_attention_cached(const CachedArgs& a, hipStream_t stream)
   p.row_blocks = plan.row_blocks;
   p.splits = plan.splits;
   p.chunk = plan.chunk;
-  return a.c.head_dim == 128 ? run_cached<128>(p, plan.row_tiles, stream)
-                             : run_cached<64>(p, plan.row_tiles, stream);
+  return a.c.head_dim == 128 ? run_cached<128>(p, plan, stream)
+                             : run_cached<64>(p, plan, stream);
 }
 
 }  // namespace ltx25

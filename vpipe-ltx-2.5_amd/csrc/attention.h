@@ -37,6 +37,39 @@ __device__ __forceinline__ float xor32_sum(float v)
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
+// v of the lane that the DPP control names, 0 where there is none or the row is
+// masked off
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int dpp_or_zero(int v)
+{
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+
+// The sum over the lanes up to the lane's own: within rows of 16, then the rows'
+// last lanes on (DPP moves take a VALU operation's time, a shuffle an LDS access's)
+__device__ __forceinline__ int scan_sum(int v)
+{
+  v += dpp_or_zero<0x111>(v);
+  v += dpp_or_zero<0x112>(v);
+  v += dpp_or_zero<0x114>(v);
+  v += dpp_or_zero<0x118>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);
+  v += dpp_or_zero<0x143, 0xc>(v);
+  return v;
+}
+
+// The largest over the wave
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+  v = max(v, (uint32_t)dpp_or_zero<0x111>((int)v));
+  v = max(v, (uint32_t)dpp_or_zero<0x112>((int)v));
+  v = max(v, (uint32_t)dpp_or_zero<0x114>((int)v));
+  v = max(v, (uint32_t)dpp_or_zero<0x118>((int)v));
+  v = max(v, (uint32_t)dpp_or_zero<0x142, 0xa>((int)v));
+  v = max(v, (uint32_t)dpp_or_zero<0x143, 0xc>((int)v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // A list of units, count(b) for each sequence b in order: the sequence, the
 // place within it of unit u, and the lane whose count(b) was the sequence's (what
 // else that call read is there). Every lane of a wave takes part and all get the
@@ -51,12 +84,7 @@ __device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& 
   long base = 0;
   for (int b0 = 0; b0 < batch; b0 += 64) {
     const int n = b0 + lane < batch ? clampi(count(b0 + lane), 0, 1 << 24) : 0;
-    int sum = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int o = __shfl_up(sum, d);
-      if (lane >= d) { sum += o; }
-    }
+    const int sum = scan_sum(n);
     const unsigned long long past = __ballot(base + sum > (long)u);
     if (past != 0) {
       from = __builtin_ctzll(past);

@@ -126,15 +126,59 @@ __device__ __forceinline__ bool find_span(const MoveParams& p, Span& s)
   return true;
 }
 
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ u16x2 max_magnitudes(u16x2 top, uint4 v)
+{
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  }
+  return top;
+}
+
+// The largest finite magnitude of 8 values, as the bits of a bf16
+__device__ __forceinline__ uint32_t max_finite(uint32_t top, uint4 v)
+{
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = (w[i >> 1] >> (16 * (i & 1))) & 0x7fffu;
+    top = a < 0x7f80u ? max(top, a) : top;
+  }
+  return top;
+}
+
+// 8 values' codes
+__device__ __forceinline__ uint2 quantize8(uint4 x, float s, float rs)
+{
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t c[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = bf16_to_f32((uint16_t)(w[2 * h + (k >> 1)] >> (16 * (k & 1))));
+    }
+    c[h] = quantize4(v, s, rs);
+  }
+  return make_uint2(c[0], c[1]);
+}
+
 // A workgroup quantizes one page's new tokens of one kv head: their keys
 // (blockIdx.z 0) or their values (1). A thread holds four tokens of 8 channels, so
-// that its codes are whole words both by token and, turned, by channel.
+// that its codes are whole words both by token and, turned, by channel; of a few
+// tokens (a decode step's one) it holds one token's 8 channels, since a quarter or
+// less of that work is then there to do.
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
 {
   constexpr int kMaxP = 128;
   constexpr int kPer = D / 8;   // 16-byte pieces of a token
   constexpr int kHeld = kMaxP / 4 * kPer / kThreads;
+  constexpr int kFew = kThreads / kPer;
   __shared__ uint32_t wave_top[kThreads / 64];
   __shared__ __attribute__((aligned(16))) uint8_t turned[D * (kMaxP + 4)];
 
@@ -146,22 +190,51 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
   const int P = 1 << p.c.pl;
   const uint16_t* const x = (values ? p.v_in : p.k_in) + g * D;
   const long stride = values ? p.vstride : p.kstride;
+  const bool few = sp.hi - sp.lo <= kFew;
 
-  // the tokens are asked for beside the page's id; the largest magnitude of what
-  // is finite, as the bits of a bf16
+  // the tokens are asked for beside the page's id
   const int pid = *sp.id;
   const int quad0 = sp.lo >> 2;
-  const int pieces = (((sp.hi + 3) >> 2) - quad0) * kPer;
+  const int pieces = few ? (sp.hi - sp.lo) * kPer : (((sp.hi + 3) >> 2) - quad0) * kPer;
   uint4 held[kHeld][4];
+  uint32_t top = 0;
+  bool odd = false;   // an infinity or a NaN among the lane's values
+  if (few) {
+    held[0][0] = make_uint4(0, 0, 0, 0);
+    if (tid < pieces) {
+      held[0][0] = *(const uint4*)(x + (sp.first + sp.lo + tid / kPer) * stride + (tid % kPer) * 8);
+    }
+    const u16x2 tops = max_magnitudes(u16x2{0, 0}, held[0][0]);
+    top = max((uint32_t)tops[0], (uint32_t)tops[1]);
+    odd = top >= 0x7f80u;
+    if (odd) { top = max_finite(0, held[0][0]); }
+  } else {
+    u16x2 tops = {0, 0};
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const int at = tid + i * kThreads;
+    for (int i = 0; i < kHeld; ++i) {
+      const int at = tid + i * kThreads;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int tok = (quad0 + at / kPer) * 4 + j;
-      held[i][j] = make_uint4(0, 0, 0, 0);
-      if (at < pieces && tok >= sp.lo && tok < sp.hi) {
-        held[i][j] = *(const uint4*)(x + (sp.first + tok) * stride + (at % kPer) * 8);
+      for (int j = 0; j < 4; ++j) {
+        const int tok = (quad0 + at / kPer) * 4 + j;
+        held[i][j] = make_uint4(0, 0, 0, 0);
+        if (at < pieces && tok >= sp.lo && tok < sp.hi) {
+          held[i][j] = *(const uint4*)(x + (sp.first + tok) * stride + (at % kPer) * 8);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { tops = max_magnitudes(tops, held[i][j]); }
+    }
+    top = max((uint32_t)tops[0], (uint32_t)tops[1]);
+    odd = top >= 0x7f80u;
+    if (odd) {
+      top = 0;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { top = max_finite(top, held[i][j]); }
       }
     }
   }
@@ -169,38 +242,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
   int8_t* const codes = (values ? p.c.v : p.c.k) + (((long)pid * p.c.kv_heads + g) << p.c.pl) * D;
   float* const scale = (values ? p.c.vs : p.c.ks) + (long)pid * p.c.kv_heads + g;
   const float s0 = sp.lo > 0 ? *scale : 0.0f;
-
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  auto magnitudes = [](uint32_t w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); };
-  u16x2 tops = {0, 0};
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w[4] = {held[i][j].x, held[i][j].y, held[i][j].z, held[i][j].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) { tops = __builtin_elementwise_max(tops, magnitudes(w[k])); }
-    }
-  }
-  uint32_t top = max((uint32_t)tops[0], (uint32_t)tops[1]);
-  bool odd = top >= 0x7f80u;   // an infinity or a NaN among the lane's values
-  if (odd) {
-    top = 0;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w[4] = {held[i][j].x, held[i][j].y, held[i][j].z, held[i][j].w};
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t a = (w[k >> 1] >> (16 * (k & 1))) & 0x7fffu;
-          top = a < 0x7f80u ? max(top, a) : top;
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) { top = max(top, (uint32_t)__shfl_xor((int)top, d)); }
+  top = wave_max(top);
   if ((tid & 63) == 0) { wave_top[tid >> 6] = top; }
   __syncthreads();
 #pragma unroll
@@ -210,6 +252,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
   if (tid == 0) { *scale = s1; }
   const bool easy = s1 >= 0x1p-90f && s1 <= 0x1p90f;
   const float rs = easy ? 1.0f / s1 : 0.0f;
+  const float my_rs = odd ? 0.0f : rs;
 
   // an old code's value is at most 127 s0, so quantize4's bound holds for it too
   auto requantize = [&](uint32_t w) {
@@ -218,37 +261,45 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
     for (int j = 0; j < 4; ++j) { v[j] = (float)(int8_t)((w >> (8 * j)) & 0xffu) * s0; }
     return quantize4(v, s1, rs);
   };
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const int at = tid + i * kThreads;
-    if (at < pieces) {
-      const int tok0 = (quad0 + at / kPer) * 4, d0 = (at % kPer) * 8;
-      uint32_t c[2][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w[4] = {held[i][j].x, held[i][j].y, held[i][j].z, held[i][j].w};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            v[k] = bf16_to_f32((uint16_t)(w[2 * h + (k >> 1)] >> (16 * (k & 1))));
-          }
-          c[h][j] = quantize4(v, s1, odd ? 0.0f : rs);
-        }
-      }
+  if (few) {
+    if (tid < pieces) {
+      const int tok = sp.lo + tid / kPer, d0 = (tid % kPer) * 8;
+      const uint2 c = quantize8(held[0][0], s1, my_rs);
       if (values) {
-        turn4(c[0]);
-        turn4(c[1]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          *(uint32_t*)(turned + (d0 + k) * (P + 4) + tok0) = c[k >> 2][k & 3];
+          turned[(d0 + k) * (P + 4) + tok] = (uint8_t)((k < 4 ? c.x : c.y) >> (8 * (k & 3)));
         }
       } else {
+        *(uint2*)(codes + tok * D + d0) = c;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int at = tid + i * kThreads;
+      if (at < pieces) {
+        const int tok0 = (quad0 + at / kPer) * 4, d0 = (at % kPer) * 8;
+        uint32_t c[2][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (tok0 + j >= sp.lo && tok0 + j < sp.hi) {
-            *(uint2*)(codes + (tok0 + j) * D + d0) = make_uint2(c[0][j], c[1][j]);
+          const uint2 q = quantize8(held[i][j], s1, my_rs);
+          c[0][j] = q.x;
+          c[1][j] = q.y;
+        }
+        if (values) {
+          turn4(c[0]);
+          turn4(c[1]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            *(uint32_t*)(turned + (d0 + k) * (P + 4) + tok0) = c[k >> 2][k & 3];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (tok0 + j >= sp.lo && tok0 + j < sp.hi) {
+              *(uint2*)(codes + (tok0 + j) * D + d0) = make_uint2(c[0][j], c[1][j]);
+            }
           }
         }
       }
@@ -648,23 +699,27 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(CachedParams p
   const int len = visible_len(p, (int)(token / p.q_len));
   const int used = min((len + p.chunk - 1) / p.chunk, p.splits);
   const float2* const ml = (const float2*)(p.part + rows * p.splits * D) + at * p.splits;
+  const float* const op = p.part + at * p.splits * D + d;
+  f32x4 x[4];
+  float2 st[4];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int s = max(min(s0 + j * kSide, used - 1), 0);
+      x[j] = *(const f32x4*)(op + (long)s * D);
+      st[j] = ml[s];
+    }
+  };
+  fetch(part);   // beside the maxima
   float top = -INFINITY;
   for (int s = lane; s < used; s += 64) { top = fmaxf(top, ml[s].x); }
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) { top = fmaxf(top, __shfl_xor(top, i)); }
   const float ms = top == -INFINITY ? 0.0f : top;
-  const float* const op = p.part + at * p.splits * D + d;
   float l = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s0 = part; s0 < used; s0 += 4 * kSide) {
-    f32x4 x[4];
-    float2 st[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int s = min(s0 + j * kSide, used - 1);
-      x[j] = *(const f32x4*)(op + (long)s * D);
-      st[j] = ml[s];
-    }
+    if (s0 != part) { fetch(s0); }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float w = s0 + j * kSide < used ? __builtin_amdgcn_exp2f(st[j].x - ms) : 0.0f;
@@ -782,14 +837,14 @@ CachedPlan plan_cached(int batch, int q_len, int heads, int kv_heads, int head_d
   // launch 5 (700 tokens, 8 kv heads: 9.7 us for 11.4 in 3 parts). Else two
   // workgroups for each CU, which hold enough loads in flight (32 rows of 131072
   // tokens: 175 us, 180 with four workgroups, 185 with eight) -- but no part longer
-  // than 8 rounds or a 16th of the tokens, since the lengths may be very uneven and
+  // than 20 rounds or a 16th of the tokens, since the lengths may be very uneven and
   // only the longest is known here.
   const long units = (long)batch * kv_heads * r.row_blocks;
   const long rounds = ((long)max_len + 255) / 256;
   long per = std::max(rounds, 1L);
   if (rounds > 4) {
     const long want = (512 + units - 1) / units;
-    per = std::min((rounds + want - 1) / want, std::max(8L, rounds / 16));
+    per = std::min((rounds + want - 1) / want, std::max(20L, rounds / 16));
     per = (rounds + (rounds + per - 1) / per - 1) / ((rounds + per - 1) / per);
   }
   r.chunk = (int)std::min(per * 256, (long)(INT_MAX & ~255));

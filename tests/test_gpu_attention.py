@@ -203,3 +203,85 @@ def test_attention_empty_calls_do_nothing(pkg, dev):
     pkg.attention(k[:2], e, e, out, causal=False, lse=z)     # no keys: zeros, -inf
     torch.cuda.synchronize()
     assert bool((out == 0).all()) and bool((z == -float("inf")).all())
+
+
+# long enough for the form whose waves take turns (from 2048 keys a sequence and 512 of its
+# workgroups on): queries, keys, heads, kv heads, causal
+LONG = [
+    ([4097], [4097], 32, 8, True),
+    ([4200], [4200], 32, 32, False),
+    ([2600], [3000], 56, 8, True),                    # 2^3 heads of 7 do not divide: one at a time
+    ([1, 2500, 3900], [2100, 2500, 4100], 24, 3, True),
+    ([3000, 2000], [1500, 2700], 32, 8, True),        # queries that see nothing
+    ([8200], [2048], 16, 16, False),
+]
+
+
+@pytest.mark.parametrize("lens_q,lens_k,heads,kv_heads,causal", LONG)
+def test_attention_long_against_64_bits(pkg, dev, lens_q, lens_k, heads, kv_heads, causal):
+    """Rows at the ends, on both sides of tile and workgroup edges, and spread between."""
+    say(f"attention long {lens_q} {lens_k} heads {heads}/{kv_heads} causal={causal}")
+    q = _randn(31, sum(lens_q), heads, 128, std=1.5)
+    k, v = (_randn(s, sum(lens_k), kv_heads, 128) for s in (32, 33))
+    out, z = _run(pkg, q, k, v, lens_q, lens_k, causal)
+    again, _ = _run(pkg, q, k, v, lens_q, lens_k, causal)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+    assert not bool(torch.isnan(out).any()) and not bool(torch.isnan(z).any())
+    kc, vc = k.cpu(), v.cpu()
+    a = b = 0
+    for n, m in zip(lens_q, lens_k):
+        edges = [0, 1, 31, 32, 63, 64, 65, 255, 256, 1000, n // 2, n - 257, n - 65, n - 2, n - 1]
+        for i in sorted({e for e in edges if 0 <= e < n}):
+            see = max(0, min(m, i + 1 + m - n)) if causal else m
+            row = slice(a + i, a + i + 1)
+            want = attn_ref.attend(q[row], kc[b:b + see], vc[b:b + see], 128 ** -0.5, False)
+            attn_ref.check(out[row], z[row], want, f"row {i} of {n}")
+        a, b = a + n, b + m
+
+
+def test_attention_long_unseen_values_have_no_influence(pkg, dev):
+    n = 4200
+    q, k, v = _randn(34, n, 32, 128), _randn(35, n, 8, 128), _randn(36, n, 8, 128)
+    clean, _ = _run(pkg, q, k, v, [n], [n], True)
+    k[3001, 2], v[3001, 2, 7], v[4150, 5] = float("nan"), float("inf"), float("nan")
+    say("attention long unseen")
+    out, _ = _run(pkg, q, k, v, [n], [n], True)
+    same = torch.ones(n, 32, dtype=torch.bool)
+    same[3001:, 8:12], same[4150:, 20:24] = False, False
+    # rows beside a bad value in a tile are computed again, one key at a time: within the bounds
+    # of the clean ones, not the same bits
+    near = torch.zeros_like(same)
+    near[2944:3001, 8:12], near[4096:4150, 20:24] = True, True
+    bits = (out.view(torch.int16) == clean.view(torch.int16)).all(2).cpu()
+    assert bool(bits[same & ~near].all())
+    for i, h in ((2990, 8), (3000, 11), (4149, 20), (4097, 23)):
+        want = attn_ref.attend(q[i:i + 1, h:h + 1], k[:i + 1, h // 4:h // 4 + 1],
+                               v[:i + 1, h // 4:h // 4 + 1], 128 ** -0.5, False)
+        attn_ref.check(out[i:i + 1, h:h + 1], None, want, f"row {i} head {h}")
+    assert not bool(torch.isfinite(out[3001:, 8:12]).any())
+    assert not bool(torch.isfinite(out[4150:, 20:24]).any())
+
+
+def test_attention_rising_logits_over_many_tiles(pkg, dev):
+    """A maximum that rises by more than 2^12 in the weights again and again, in both forms."""
+    for n, heads in ((900, 2), (4100, 32)):
+        q = torch.ones(n, heads, 128, dtype=torch.bfloat16, device="cuda")
+        ramp = torch.arange(n, device="cuda").float() * 0.4
+        k = (ramp[:, None, None] * torch.ones(1, 2, 128, device="cuda") / 128).to(torch.bfloat16)
+        v = _randn(37, n, 2, 128)
+        say(f"attention rising {n}")
+        out, z = _run(pkg, q, k, v, [n], [n], True, 1.0)
+        for i in (0, 5, 64, 200, 777, n - 1):
+            want = attn_ref.attend(q[i:i + 1], k[:i + 1], v[:i + 1], 1.0, False)
+            attn_ref.check(out[i:i + 1], z[i:i + 1], want, f"row {i} of {n}")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_several_hundred_sequences(pkg, dev, dim):
+    rng = np.random.default_rng(38)
+    lens = [int(n) for n in rng.integers(0, 6, 600)]
+    lens[300], lens[577] = 70, 40
+    q, k, v = _randn(39, sum(lens), 2, dim), _randn(40, sum(lens), 1, dim), _randn(41, sum(lens), 1, dim)
+    say(f"attention of 600 sequences x {dim}")
+    out, z = _run(pkg, q, k, v, lens, lens, True)
+    _verify(q, k, v, out, z, lens, lens, True)

@@ -90,6 +90,7 @@ APPENDS = [  # tokens held, new tokens, kv heads, width, page
     ([1, 100, 127], [127, 300, 2], 2, 64, 128),
     ([50, 3, 0], [0, 20, 0], 2, 128, 64),
     ([i % 37 for i in range(70)], [1 + i % 3 for i in range(70)], 1, 64, 16),
+    ([i % 23 for i in range(300)], [i % 4 for i in range(300)], 1, 64, 16),
 ]
 
 

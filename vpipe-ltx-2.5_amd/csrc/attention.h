@@ -71,28 +71,48 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v)
 }
 
 // A list of units, count(b) for each sequence b in order: the sequence, the
-// place within it of unit u, and the lane whose count(b) was the sequence's (what
-// else that call read is there). Every lane of a wave takes part and all get the
-// same answer; false when there are fewer units. The counts come from device
-// memory that the caller has not checked: each is cut to [0, 2^24] and the sum
+// place within it of unit u, and the lane whose last count(b) was the sequence's
+// (what else that call read is there). Every lane of a wave takes part and all get
+// the same answer; false when there are fewer units. The counts come from device
+// memory that the caller has not checked: each is cut to [0, 2^24] and the sums
 // kept in 64 bits.
+//
+// More than 64 sequences are looked at 256 at a time, whose reads are then in
+// flight together, and the unit's own is read again at the end.
 template <typename Count>
 __device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& seq, int& place,
                                           int& from)
 {
   const int lane = threadIdx.x & 63;
-  long base = 0;
-  for (int b0 = 0; b0 < batch; b0 += 64) {
-    const int n = b0 + lane < batch ? clampi(count(b0 + lane), 0, 1 << 24) : 0;
+  auto count_of = [&](int b) { return b < batch ? clampi(count(b), 0, 1 << 24) : 0; };
+  if (batch <= 64) {
+    const int n = count_of(lane);
     const int sum = scan_sum(n);
-    const unsigned long long past = __ballot(base + sum > (long)u);
-    if (past != 0) {
-      from = __builtin_ctzll(past);
-      seq = b0 + from;
-      place = (int)(u - base) - __builtin_amdgcn_readlane(sum - n, from);
-      return true;
+    const unsigned long long past = __ballot(sum > u);
+    if (past == 0) { return false; }
+    from = seq = __builtin_ctzll(past);
+    place = u - __builtin_amdgcn_readlane(sum - n, from);
+    return true;
+  }
+  long base = 0;
+  for (int b0 = 0; b0 < batch; b0 += 256) {
+    int n[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { n[j] = count_of(b0 + 64 * j + lane); }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int sum = scan_sum(n[j]);
+      const unsigned long long past = __ballot(base + sum > (long)u);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        seq = b0 + 64 * j + at;
+        place = (int)(u - base) - __builtin_amdgcn_readlane(sum - n[j], at);
+        (void)count(seq);   // in every lane
+        from = 0;
+        return true;
+      }
+      base += __builtin_amdgcn_readlane(sum, 63);
     }
-    base += __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
 }

@@ -11,10 +11,27 @@
 // registers hold them, and V^T's fragments are read from LDS in that order by
 // the transposing LDS read (4 tokens x 16 channels for each 16 lanes).
 //
-// K and V tiles go from global memory straight into LDS (16 bytes a lane), two
-// stages. Their rows' 16-byte pieces are swizzled on the way in (the source
-// address is permuted, the LDS side of such a load is linear) so that the
-// fragment reads meet no bank twice.
+// K and V tiles go from global memory straight into LDS (16 bytes a lane), the
+// loads in flight counted by hand. Their rows' 16-byte pieces are swizzled on the
+// way in (the source address is permuted, the LDS side of such a load is linear)
+// so that the fragment reads meet no bank twice (SQ_LDS_BANK_CONFLICT is 0 in the
+// loop).
+//
+// What bounds it: a tile takes a wave 32 products of 32 cycles on the matrix
+// cores and about 140 operations for the weights, 33 of them exponentials at 9
+// cycles and the rest at 5 each: as much time as the products, which two waves a
+// SIMD overlap only in part. The instructions' energy counts as well: 17% fewer
+// cycles (attention_turns_kernel against attention_kernel) came at 10% less clock.
+// Two forms:
+//   attention_kernel: 4 waves, 128 rows; two to four such workgroups share a CU
+//   and one computes while another waits. 333-token prompts 19 us where 8 waves
+//   took 25, 48 prompts of 40 to 200 tokens 13 against 16.
+//   attention_turns_kernel (head width 128): 8 waves, 256 rows, in two groups
+//   that take turns with the matrix cores. 16384 causal tokens, 32 / 8 heads: 1850
+//   us (1190 TFLOP/s) against 2045; 8160 tokens that all see each other, 32 heads:
+//   917 us (1190 TFLOP/s) against 1037; where less than about two rounds of
+//   workgroups fill the GPU, or the sequences are short, it is the slower one (2048
+//   tokens: 52.6 us against 49.7; eight of 1024: 91 against 91.5).
 #include "attention.h"
 
 #include <climits>
@@ -22,8 +39,7 @@
 namespace ltx25 {
 namespace {
 
-constexpr int kBN = 64;     // tokens of a tile
-constexpr int kWaves = 8;   // of a workgroup
+constexpr int kBN = 64;   // tokens of a tile
 
 struct PromptParams {
   const uint16_t* q;
@@ -61,25 +77,154 @@ __device__ __forceinline__ int v_piece(int row, int c)
   return D == 128 ? c ^ ((row & 3) << 2) : c ^ (((row >> 1) & 1) << 2);
 }
 
-template <int D, int NW>
-__global__ void __launch_bounds__(NW * 64) attention_kernel(PromptParams p)
-{
-  constexpr int kRow = D * 2;             // bytes of a row
-  constexpr int kTile = kBN * kRow;       // bytes of a stage of K or V
-  constexpr int kPieces = kRow / 16;
-  constexpr int kRowsPer = 64 / kPieces;  // rows of one load instruction
-  constexpr int kLoads = kBN / kRowsPer / NW;   // of K, and of V, per wave
-  constexpr int kKC = D / 16;             // k chunks of the first product
-  constexpr int kDT = D / 32;             // 32-channel tiles of the second
-  static_assert(kLoads >= 1 && kLoads * NW * kRowsPer == kBN, "the waves load whole tiles");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ bool any_lane(bool b) { return __any(b) != 0; }
 
+// 16 bytes a lane from the buffer straight into LDS, lane after lane from the LDS
+// address `to`. In asm, so that the compiler does not make every LDS read wait for
+// it; the kernel counts the loads in flight itself.
+__device__ __forceinline__ void load_lds(i32x4 from, uint32_t to, int offset)
+{
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(to), "v"(offset), "s"(from)
+               : "memory");
+}
+
+// A buffer over `bytes` bytes at p, as the asm takes it
+__device__ __forceinline__ i32x4 words_of(const void* p, uint32_t bytes)
+{
+  const uint64_t a = (uint64_t)p;
+  return i32x4{(int)(uint32_t)a, (int)((uint32_t)(a >> 32) & 0xffffu), (int)bytes, 0x00020000};
+}
+
+// A barrier that the scheduler moves nothing across
+__device__ __forceinline__ void meet()
+{
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <int P>
+__device__ __forceinline__ void prio() { __builtin_amdgcn_s_setprio(P); }
+
+// At most N of the wave's loads are still in flight, and every wave has come here
+template <int N>
+__device__ __forceinline__ void landed()
+{
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+  __syncthreads();
+}
+
+// V^T's fragment: 4 tokens at a, 4 at b, of the lane's channel
+__device__ __forceinline__ bf16x8 turned(const uint8_t* a, const uint8_t* b)
+{
+  union { s16x4 h[2]; bf16x8 f; } r;
+  r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
+  r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)b);
+  return r.f;
+}
+
+// The compiler's scheduler moves nothing across: the order of the steps below is
+// the one that overlaps the two products with the weights' arithmetic
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// The order of a block: AHEAD fragments (READS reads each) first, then product
+// after product with the reads of the fragment AHEAD on
+template <int N, int AHEAD, int READS>
+__device__ __forceinline__ void ahead()
+{
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if (i + AHEAD < N) { __builtin_amdgcn_sched_group_barrier(0x100, READS, 0); }
+  }
+}
+
+// What a workgroup works on: sequence `seq`, its unit of rows counted from the
+// sequence's end, and the sequence's place in the tensors.
+struct Unit {
+  int from_end;
+  int q0, lq, k0, lk;
+};
+
+// Unit u of all sequences' units of 2^tb queries; false past the last. One
+// sequence: the last unit first, which under a causal mask has the most keys. Up
+// to 64 sequences: in the order of their keys, most first, so that the longest
+// work does not start last; a lane holds a sequence, and the key count L where
+// unit u lies is found by halving (6 DPP additions a step). More sequences: one
+// after another.
+__device__ __forceinline__ bool find_rows(const PromptParams& p, int u, Unit& r)
+{
+  const int lane = threadIdx.x & 63;
+  const int tb = 1 << p.tb_log2;
+  if (p.cu_q == nullptr) {
+    r = {u, 0, p.total_q, 0, p.total_k};
+    return u < (p.total_q + tb - 1) >> p.tb_log2;
+  }
+  int q0 = 0, lq = 0, k0 = 0, lk = 0;
+  auto read = [&](int b) {
+    const int qa = p.cu_q[b], qb = p.cu_q[b + 1], ka = p.cu_k[b], kb = p.cu_k[b + 1];
+    q0 = clampi(qa, 0, p.total_q);
+    lq = clampi(qb, q0, p.total_q) - q0;
+    k0 = clampi(ka, 0, p.total_k);
+    lk = clampi(kb, k0, p.total_k) - k0;
+    return (lq + tb - 1) >> p.tb_log2;
+  };
+  int at = 0;
+  if (p.batch > 64) {
+    int seq;
+    if (!find_unit(u, p.batch, read, seq, r.from_end, at)) { return false; }
+  } else {
+    const int n = lane < p.batch ? read(lane) : 0;
+    const int most = (lk + tb - 1) >> p.tb_log2;   // the last unit's keys, in units
+    // units of the lane's sequence with at least L keys
+    auto with = [&](int L) { return p.causal ? clampi(most - L + 1, 0, n) : most >= L ? n : 0; };
+    auto total = [&](int v) { return __builtin_amdgcn_readlane(scan_sum(v), 63); };
+    // units that see no key count as having none or less: they come last
+    const int floor = -(p.total_q >> p.tb_log2) - 1;
+    int lo = floor, hi = (int)wave_max((uint32_t)most) + 1;
+    if (total(n) <= u) { return false; }
+    while (hi - lo > 1) {   // with(lo) > u >= with(hi)
+      const int mid = lo + (hi - lo) / 2;
+      if (total(with(mid)) > u) { lo = mid; } else { hi = mid; }
+    }
+    const int before = with(lo + 1);
+    const int here = with(lo) - before;
+    const int place = u - total(before);
+    const int sum = scan_sum(here);
+    at = __builtin_ctzll(__ballot(sum > place));
+    r.from_end = __builtin_amdgcn_readlane(before, at) + place -
+                 __builtin_amdgcn_readlane(sum - here, at);
+  }
+  r.q0 = __builtin_amdgcn_readlane(q0, at);
+  r.lq = __builtin_amdgcn_readlane(lq, at);
+  r.k0 = __builtin_amdgcn_readlane(k0, at);
+  r.lk = __builtin_amdgcn_readlane(lk, at);
+  return true;
+}
+
+// A wave's rows and the workgroup's tiles.
+template <int D, int NW>
+struct Rows {
+  int q0, lq, k0, lk;   // the sequence
+  int tok0, head0, g;   // first token and head of the workgroup, kv head
+  int tok, head;        // of the lane's row
+  bool valid;
+  int limit;            // the last key that the lane's row sees
+  int wave_lo, wave_hi; // and that the wave's first and last rows see
+  int n_tiles;
+};
+
+template <int D, int NW>
+__device__ __forceinline__ bool find(const PromptParams& p, Rows<D, NW>& r)
+{
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = lane >> 5;
   const int tb = 1 << p.tb_log2;
-
-  // ---- this workgroup's rows
   int hg, u;
   if (p.head_groups % 8 == 0) {
     // workgroups go round-robin to the 8 XCDs: a kv head's stay on one, in
@@ -92,225 +237,204 @@ __global__ void __launch_bounds__(NW * 64) attention_kernel(PromptParams p)
     hg = blockIdx.x % p.head_groups;
     u = blockIdx.x / p.head_groups;
   }
-  int seq = 0, place = 0, from = 0;
-  auto len_q = [&](int b, int& q0) {
-    if (p.cu_q == nullptr) { q0 = 0; return p.total_q; }
-    q0 = clampi(p.cu_q[b], 0, p.total_q);
-    return clampi(p.cu_q[b + 1], q0, p.total_q) - q0;
-  };
-  auto tiles = [&](int b) {
-    int q0;
-    return (len_q(b, q0) + tb - 1) >> p.tb_log2;
-  };
-  if (!find_unit(u, p.batch, tiles, seq, place, from)) { return; }
-  int q0, k0;
-  const int lq = __builtin_amdgcn_readfirstlane(len_q(seq, q0));
-  q0 = __builtin_amdgcn_readfirstlane(q0);
-  int lk = p.total_k;
-  k0 = 0;
-  if (p.cu_k != nullptr) {
-    k0 = clampi(p.cu_k[seq], 0, p.total_k);
-    lk = clampi(p.cu_k[seq + 1], k0, p.total_k) - k0;
-    k0 = __builtin_amdgcn_readfirstlane(k0);
-    lk = __builtin_amdgcn_readfirstlane(lk);
-  }
-  // a causal sequence's long tiles first
-  const int n_units = (lq + tb - 1) >> p.tb_log2;
-  const int tok0 = (n_units - 1 - place) << p.tb_log2;
-  const int head0 = hg << p.hp_log2;
-  const int g = head0 / p.share;
-
+  Unit un;
+  if (!find_rows(p, u, un)) { return false; }
+  r.q0 = un.q0;
+  r.lq = un.lq;
+  r.k0 = un.k0;
+  r.lk = un.lk;
+  r.tok0 = (((un.lq + tb - 1) >> p.tb_log2) - 1 - un.from_end) << p.tb_log2;
+  r.head0 = hg << p.hp_log2;
+  r.g = r.head0 / p.share;
   const int row = wave * 32 + (lane & 31);
-  const int head = head0 + (row >> p.tb_log2);
-  const int tok = tok0 + (row & (tb - 1));
-  const bool valid = tok < lq;
-  // the first and last token of the wave's rows; the last key that a query sees
-  const int wlo = tok0 + (p.tb_log2 >= 5 ? (wave * 32) & (tb - 1) : 0);
-  const int whi = min(wlo + min(tb, 32), lq) - 1;
-  const int shift = p.causal ? lk - lq : 0;
-  auto last_key = [&](int t) { return p.causal ? min(t + shift, lk - 1) : lk - 1; };
-  const int limit = last_key(min(tok, lq - 1));
-  const int wave_lo = wlo < lq ? last_key(wlo) : -1;
-  const int wave_hi = wlo < lq ? last_key(whi) : -1;
-  const int wg_hi = last_key(min(tok0 + tb, lq) - 1);
-  const int n_tiles = wg_hi < 0 ? 0 : wg_hi / kBN + 1;
+  r.head = r.head0 + (row >> p.tb_log2);
+  r.tok = r.tok0 + (row & (tb - 1));
+  r.valid = r.tok < r.lq;
+  const int shift = p.causal ? r.lk - r.lq : 0;
+  auto last_key = [&](int t) { return p.causal ? min(t + shift, un.lk - 1) : un.lk - 1; };
+  const int lo = r.tok0 + (p.tb_log2 >= 5 ? (wave * 32) & (tb - 1) : 0);
+  const int hi = min(lo + min(tb, 32), r.lq) - 1;
+  r.limit = last_key(min(r.tok, r.lq - 1));
+  r.wave_lo = lo < r.lq ? last_key(lo) : -1;
+  r.wave_hi = lo < r.lq ? last_key(hi) : -1;
+  const int last = last_key(min(r.tok0 + tb, r.lq) - 1);
+  r.n_tiles = last < 0 ? 0 : last / kBN + 1;
+  return true;
+}
 
-  // ---- queries: lane's row, 8 channels of each 16
-  bf16x8 qf[kKC];
+// The lane's row's queries, 8 channels of each 16
+template <int D, int NW>
+__device__ __forceinline__ void load_queries(const PromptParams& p, const Rows<D, NW>& r,
+                                             bf16x8 (&qf)[D / 16])
+{
+  const int half = (threadIdx.x >> 5) & 1;
+  const uint16_t* const qp =
+      p.q + (long)(r.q0 + min(r.tok, r.lq - 1)) * p.qs + r.head * D + half * 8;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) { qf[i] = as_bf16x8(*(const uint4*)(qp + i * 16)); }
+}
+
+// The loads of K and V into LDS, tile after tile: instruction i of a wave fills 1
+// KB, kRowsPer rows. Every tile is asked for by the same number of instructions,
+// past the last one too (of no bytes), so that the counts of loads in flight hold
+// everywhere.
+template <int D, int NW>
+struct Loader {
+  static constexpr int kRow = D * 2;             // bytes of a row
+  static constexpr int kTile = kBN * kRow;       // bytes of a stage
+  static constexpr int kPieces = kRow / 16;
+  static constexpr int kRowsPer = 64 / kPieces;  // rows of one instruction
+  static constexpr int kLoads = kBN / kRowsPer / NW;   // of K, and of V, per wave
+  static_assert(kLoads >= 1 && kLoads * NW * kRowsPer == kBN, "the waves load whole tiles");
+
+  uint32_t lds0, k_bytes, v_bytes;
+  int koff[kLoads], voff[kLoads];
+  const uint16_t* kp;   // the next tile of K, the next of V, and the rows left
+  const uint16_t* vp;
+  long k_step, v_step;
+  int k_left, v_left;
+
+  __device__ __forceinline__ Loader(const PromptParams& p, const Rows<D, NW>& r, uint8_t* lds)
   {
-    const uint16_t* const qp = p.q + (long)(q0 + min(tok, lq - 1)) * p.qs + head * D + half * 8;
-#pragma unroll
-    for (int i = 0; i < kKC; ++i) { qf[i] = as_bf16x8(*(const uint4*)(qp + i * 16)); }
-  }
-
-  // ---- loads into LDS: instruction i of a wave fills 1 KB, kRowsPer rows
-  const int lrow = lane / kPieces;
-  const uint32_t ks_bytes = (uint32_t)p.ks * 2u, vs_bytes = (uint32_t)p.vs * 2u;
-  auto load_tile = [&](int t, int st) {
-    const int rows = min(lk - t * kBN, kBN);
-    const long at = (long)k0 + (long)t * kBN;
-    const __amdgpu_buffer_rsrc_t kr =
-        buffer_of(p.k + at * p.ks + g * D, (uint32_t)(rows - 1) * ks_bytes + kRow);
-    const __amdgpu_buffer_rsrc_t vr =
-        buffer_of(p.v + at * p.vs + g * D, (uint32_t)(rows - 1) * vs_bytes + kRow);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    k_bytes = (uint32_t)p.ks * 2u;
+    v_bytes = (uint32_t)p.vs * 2u;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = (wave * kLoads + i) * kRowsPer + lrow;
-      const int piece = k_piece<D>(r, lane % kPieces);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          kr, (lds_word*)(lds + st * kTile + (wave * kLoads + i) * 1024), 16,
-          (int)(r * ks_bytes + piece * 16), 0, 0, 0);
+      const int row = (wave * kLoads + i) * kRowsPer + lane / kPieces;
+      koff[i] = (int)(row * k_bytes + k_piece<D>(row, lane % kPieces) * 16);
+      voff[i] = (int)(row * v_bytes + v_piece<D>(row, lane % kPieces) * 16);
     }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int r = (wave * kLoads + i) * kRowsPer + lrow;
-      const int piece = v_piece<D>(r, lane % kPieces);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          vr, (lds_word*)(lds + (2 + st) * kTile + (wave * kLoads + i) * 1024), 16,
-          (int)(r * vs_bytes + piece * 16), 0, 0, 0);
-    }
-  };
-
-  f32x16 o[kDT];
-#pragma unroll
-  for (int d = 0; d < kDT; ++d) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) { o[d][i] = 0.0f; }
+    lds0 = (uint32_t)(uintptr_t)(lds_word*)lds + wave * kLoads * 1024;
+    kp = p.k + (long)r.k0 * p.ks + r.g * D;
+    vp = p.v + (long)r.k0 * p.vs + r.g * D;
+    k_step = (long)kBN * p.ks;
+    v_step = (long)kBN * p.vs;
+    k_left = v_left = min(r.n_tiles * kBN, r.lk);
   }
-  float m = -INFINITY, l = 0.0f;
+  // the next tile into stage `st`, of the stages of K, then those of V
+  __device__ __forceinline__ void keys(int st)
+  {
+    const int rows = min(k_left, kBN);
+    const i32x4 from = words_of(kp, rows > 0 ? (uint32_t)(rows - 1) * k_bytes + kRow : 0u);
+    kp += k_step;
+    k_left -= kBN;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) { load_lds(from, lds0 + st * kTile + i * 1024, koff[i]); }
+  }
+  __device__ __forceinline__ void values(int st)
+  {
+    const int rows = min(v_left, kBN);
+    const i32x4 from = words_of(vp, rows > 0 ? (uint32_t)(rows - 1) * v_bytes + kRow : 0u);
+    vp += v_step;
+    v_left -= kBN;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) { load_lds(from, lds0 + st * kTile + i * 1024, voff[i]); }
+  }
+};
 
-  if (n_tiles > 0) { load_tile(0, 0); }
-  for (int t = 0; t < n_tiles; ++t) {
-    // this tile has landed (every wave's share), and no wave reads the other stage
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the loads into LDS are counted by hand
-    __syncthreads();
-    const int st = t & 1;
-    if (t + 1 < n_tiles) { load_tile(t + 1, st ^ 1); }
-    if (t * kBN > wave_hi) { continue; }
+// Fragments, by the order in which the products take them: the first product's
+// step i is k chunk i / 2 of tokens 32 (i % 2) .., the second's 16 tokens i / (D /
+// 32) of channels 32 (i % (D / 32)) ..
+template <int D>
+__device__ __forceinline__ bf16x8 k_frag(const uint8_t* kt, int i)
+{
+  const int lane = threadIdx.x & 63;
+  const int r = (i & 1) * 32 + (lane & 31);
+  return as_bf16x8(*(const uint4*)(kt + r * D * 2 + k_piece<D>(r, (i & ~1) + (lane >> 5)) * 16));
+}
+template <int D>
+__device__ __forceinline__ bf16x8 v_frag(const uint8_t* vt, int i)
+{
+  const int lane = threadIdx.x & 63;
+  const int r = i / (D / 32) * 16 + (lane >> 5) * 4 + ((lane & 15) >> 2);
+  const int piece = i % (D / 32) * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+  const int low = (lane & 1) * 8;
+  return turned(vt + r * D * 2 + v_piece<D>(r, piece) * 16 + low,
+                vt + (r + 8) * D * 2 + v_piece<D>(r + 8, piece) * 16 + low);
+}
 
-    // ---- logits: s[b] holds tokens 32 b + (i & 3) + 8 (i >> 2) + 4 half
-    const uint8_t* const kt = lds + st * kTile;
-    f32x16 s[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { s[b][i] = 0.0f; }
-      const int r = b * 32 + (lane & 31);
-#pragma unroll
-      for (int i = 0; i < kKC; ++i) {
-        const uint4 kf = *(const uint4*)(kt + r * kRow + k_piece<D>(r, 2 * i + half) * 16);
-        s[b] = mfma32(as_bf16x8(kf), qf[i], s[b]);
-      }
-    }
-    if (t * kBN + kBN - 1 > wave_lo) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int token = t * kBN + b * 32 + (i & 3) + 8 * (i >> 2) + 4 * half;
-          if (token > limit) { s[b][i] = -INFINITY; }
-        }
-      }
-    }
-    // ---- running maximum and sum
-    float top = s[0][0];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { top = fmaxf(top, s[b][i]); }
-    }
-    const float m_new = fmaxf(m, xor32_max(top));
-    const float mc = m_new == -INFINITY ? 0.0f : m_new * p.c;   // nothing seen yet
-    const float keep = __builtin_amdgcn_exp2f(fmaf(m, p.c, -mc));
-    m = m_new;
-    float sum = 0.0f;
+// -infinity for what a row does not see of tile t, of which s[b][i] is token
+// 32 b + (i & 3) + 8 (i >> 2) + 4 half
+template <int D, int NW>
+__device__ __forceinline__ void mask(const Rows<D, NW>& r, int t, f32x16 (&s)[2])
+{
+  if (t * kBN + kBN - 1 > r.wave_lo) {
+    const int lim = r.limit - t * kBN - 4 * (int)((threadIdx.x >> 5) & 1);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.c, -mc));
-        sum += s[b][i];
-      }
-    }
-    l = fmaf(l, keep, sum);
-#pragma unroll
-    for (int d = 0; d < kDT; ++d) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { o[d][i] *= keep; }
-    }
-    // ---- O^T += V^T P^T, 16 tokens a step
-    const uint8_t* const vt = lds + (2 + st) * kTile;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint4 pw;
-      const f32x16& sc = s[c >> 1];
-      const int e = (c & 1) * 8;
-      pw.x = pack_bf16x2(sc[e + 0], sc[e + 1]);
-      pw.y = pack_bf16x2(sc[e + 2], sc[e + 3]);
-      pw.z = pack_bf16x2(sc[e + 4], sc[e + 5]);
-      pw.w = pack_bf16x2(sc[e + 6], sc[e + 7]);
-      const bf16x8 pf = as_bf16x8(pw);
-      const int r = c * 16 + half * 4 + ((lane & 15) >> 2);
-#pragma unroll
-      for (int d = 0; d < kDT; ++d) {
-        const int piece = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-        const uint8_t* const a = vt + r * kRow + v_piece<D>(r, piece) * 16 + (lane & 1) * 8;
-        const uint8_t* const b = vt + (r + 8) * kRow + v_piece<D>(r + 8, piece) * 16 + (lane & 1) * 8;
-        union { s16x4 h[2]; bf16x8 f; } vf;
-        vf.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
-        vf.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)b);
-        o[d] = mfma32(vf.f, pf, o[d]);
+        s[b][i] = b * 32 + (i & 3) + 8 * (i >> 2) > lim ? -INFINITY : s[b][i];
       }
     }
   }
+}
 
-  // ---- out, lse
+// The sums and statistics of the wave's rows out: through LDS, each wave its own
+// part of it, so that a store has whole rows' pieces side by side.
+template <int D, int NW>
+__device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>& r, uint8_t* lds,
+                                       f32x16 (&o)[D / 32], float m, float l)
+{
+  constexpr int kRow = D * 2, kPieces = kRow / 16, kRowsPer = 64 / kPieces, kDT = D / 32;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5;
+  const int tb = 1 << p.tb_log2;
   l = xor32_sum(l);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  bool bad = false;
+  landed<0>();
+  uint8_t* const mine = lds + wave * 32 * kRow;
+  float nans[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // a NaN stays one in a sum
 #pragma unroll
   for (int d = 0; d < kDT; ++d) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      o[d][i] *= inv;
-      bad = bad || __builtin_isnan(o[d][i]);
-    }
-  }
-  if (valid) {
-    uint16_t* const op = p.out + (long)(q0 + tok) * p.os + head * D + half * 4;
+    for (int i = 0; i < 4; ++i) {
+      float x[4];
 #pragma unroll
-    for (int d = 0; d < kDT; ++d) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint2 w;
-        w.x = pack_bf16x2(o[d][4 * i], o[d][4 * i + 1]);
-        w.y = pack_bf16x2(o[d][4 * i + 2], o[d][4 * i + 3]);
-        *(uint2*)(op + d * 32 + i * 8) = w;
+      for (int j = 0; j < 4; ++j) {
+        x[j] = o[d][4 * i + j] * inv;
+        nans[j] += x[j];
       }
-    }
-    if (p.lse != nullptr && half == 0) {
-      p.lse[(long)(q0 + tok) * p.heads + head] =
-          l == 0.0f ? -INFINITY : fmaf(m, p.c, __builtin_log2f(l)) * 0.69314718055994531f;
+      *(uint2*)(mine + (lane & 31) * kRow + k_piece<D>(lane & 31, d * 4 + i) * 16 + half * 8) =
+          make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
     }
   }
+#pragma unroll
+  for (int i = 0; i < 32 / kRowsPer; ++i) {
+    const int at = i * kRowsPer + lane / kPieces, wr = wave * 32 + at;
+    const int t = r.tok0 + (wr & (tb - 1)), c = lane % kPieces;
+    const uint4 v = *(const uint4*)(mine + at * kRow + k_piece<D>(at, c) * 16);
+    if (t < r.lq) {
+      *(uint4*)(p.out + (long)(r.q0 + t) * p.os + (r.head0 + (wr >> p.tb_log2)) * D + c * 8) = v;
+    }
+  }
+  if (p.lse != nullptr && half == 0 && r.valid) {
+    p.lse[(long)(r.q0 + r.tok) * p.heads + r.head] =
+        l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l)) * 0.69314718055994531f;
+  }
+  const float sum = (nans[0] + nans[1]) + (nans[2] + nans[3]);
+  const bool bad = sum != sum;
   // A NaN in a row: a weight of zero times an infinite or NaN value that the
   // row does not see (a tile's masked tokens take part in the second product)
   // gives one too. Such rows are computed again over the tokens they see alone,
   // one at a time, by the whole wave: a rare case whose speed does not matter.
-  unsigned long long again = __ballot(bad && valid);
+  unsigned long long again = __ballot(bad && r.valid);
   again = (again | (again >> 32)) & 0xffffffffull;
   while (again != 0) {
-    const int r = __builtin_ctzll(again);
+    const int at = __builtin_ctzll(again);
     again &= again - 1;
-    const int rtok = __shfl(tok, r), rhead = __shfl(head, r), rlimit = __shfl(limit, r);
+    const int rtok = __shfl(r.tok, at), rhead = __shfl(r.head, at), rlimit = __shfl(r.limit, at);
     constexpr int kPer = D / 64;
-    const uint16_t* const qp = p.q + (long)(q0 + rtok) * p.qs + rhead * D + lane * kPer;
+    const uint16_t* const qp = p.q + (long)(r.q0 + rtok) * p.qs + rhead * D + lane * kPer;
     float qv[kPer], acc[kPer], rm = -INFINITY, rl = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) { qv[i] = bf16_to_f32(qp[i]); acc[i] = 0.0f; }
     for (int j = 0; j <= rlimit; ++j) {
-      const uint16_t* const kp = p.k + (long)(k0 + j) * p.ks + g * D + lane * kPer;
-      const uint16_t* const vp = p.v + (long)(k0 + j) * p.vs + g * D + lane * kPer;
+      const uint16_t* const kp = p.k + (long)(r.k0 + j) * p.ks + r.g * D + lane * kPer;
+      const uint16_t* const vp = p.v + (long)(r.k0 + j) * p.vs + r.g * D + lane * kPer;
       float x = 0.0f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) { x = fmaf(qv[i], bf16_to_f32(kp[i]), x); }
@@ -326,16 +450,293 @@ __global__ void __launch_bounds__(NW * 64) attention_kernel(PromptParams p)
       for (int i = 0; i < kPer; ++i) { acc[i] = fmaf(acc[i], kept, w * bf16_to_f32(vp[i])); }
     }
     const float rinv = rl == 0.0f ? 0.0f : 1.0f / rl;
-    uint16_t* const op = p.out + (long)(q0 + rtok) * p.os + rhead * D + lane * kPer;
+    uint16_t* const op = p.out + (long)(r.q0 + rtok) * p.os + rhead * D + lane * kPer;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) { op[i] = f32_to_bf16(acc[i] * rinv); }
   }
 }
 
+// 4 waves, two stages of tiles: the next tile lands while this one is multiplied.
 template <int D>
-hipError_t run(const PromptParams& p, int grid, hipStream_t st)
+__global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptParams p)
 {
-  attention_kernel<D, kWaves><<<grid, kWaves * 64, 0, st>>>(p);
+  constexpr int kNW = 4;
+  using Load = Loader<D, kNW>;
+  constexpr int kTile = Load::kTile;
+  constexpr int kKC = D / 16;   // k chunks of the first product
+  constexpr int kDT = D / 32;   // 32-channel tiles of the second
+  static_assert(kNW * 32 * Load::kRow <= 4 * kTile, "the staged output fits the stages");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];   // K 0, 1, V 0, 1
+
+  Rows<D, kNW> r;
+  if (!find(p, r)) { return; }
+  Load load(p, r, lds);
+  bf16x8 qf[kKC];
+  load_queries(p, r, qf);
+  load.keys(0);
+  load.values(2);
+  // the queries are waited for here: inside the loop the compiler's wait for them
+  // would be one for the tiles under way, in every round
+#pragma unroll
+  for (int i = 0; i < kKC; ++i) { asm volatile("" : "+v"(qf[i])); }
+
+  f32x16 o[kDT];
+#pragma unroll
+  for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { o[d][i] = 0.0f; }
+  }
+  float m = -INFINITY, l = 0.0f;
+
+  for (int t = 0; t < r.n_tiles; ++t) {
+    // this tile is there, every wave's share of it, and no wave reads tile t - 1,
+    // whose stage the next one takes
+    const int st = t & 1;
+    landed<0>();
+    load.keys(st ^ 1);
+    load.values(2 + (st ^ 1));
+    if (t * kBN > r.wave_hi) { continue; }
+    const uint8_t* const kt = lds + st * kTile;
+    const uint8_t* const vt = lds + (2 + st) * kTile;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { s[b][i] = 0.0f; }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kKC; ++i) { s[i & 1] = mfma32(k_frag<D>(kt, i), qf[i >> 1], s[i & 1]); }
+    ahead<2 * kKC, 8, 1>();
+    mask(r, t, s);
+    // ---- the row's maximum, in four chains side by side (an operation that waits
+    // for the one before it takes 9 cycles, else 5). It is let lag behind the
+    // largest logit by up to 2^8 in the weights, whose sum then stays far inside
+    // f32: most tiles leave the sums as they are.
+    float tops[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x16& x = s[j >> 1];
+      const int e = (j & 1) * 8;
+      tops[j] = fmaxf(fmaxf(x[e], x[e + 1]), x[e + 2]);
+      tops[j] = fmaxf(fmaxf(x[e + 3], x[e + 4]), tops[j]);
+      tops[j] = fmaxf(fmaxf(x[e + 5], x[e + 6]), tops[j]);
+      tops[j] = fmaxf(x[e + 7], tops[j]);
+    }
+    const float top = xor32_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+    if (any_lane((top - m) * p.c > 8.0f || m == -INFINITY)) {
+      const float m_new = fmaxf(m, top);
+      const float mz = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet
+      const float keep = exp2_of((m - mz) * p.c);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { o[d][i] *= keep; }
+      }
+    }
+    // ---- weights, and O^T += V^T P^T, 16 tokens a step
+    const float mc = m == -INFINITY ? 0.0f : m * p.c;
+    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      f32x16& sc = s[c >> 1];
+      const int e = (c & 1) * 8;
+#pragma unroll
+      for (int i = e; i < e + 8; ++i) {
+        sc[i] = exp2_of(fmaf(sc[i], p.c, -mc));
+        sums[i & 3] += sc[i];
+      }
+      uint4 pw;
+      pw.x = pack_bf16x2(sc[e + 0], sc[e + 1]);
+      pw.y = pack_bf16x2(sc[e + 2], sc[e + 3]);
+      pw.z = pack_bf16x2(sc[e + 4], sc[e + 5]);
+      pw.w = pack_bf16x2(sc[e + 6], sc[e + 7]);
+      const bf16x8 pf = as_bf16x8(pw);
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) { o[d] = mfma32(v_frag<D>(vt, c * kDT + d), pf, o[d]); }
+    }
+    l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
+  finish(p, r, lds, o, m, l);
+}
+
+// 8 waves in two groups of four, one wave of each on every SIMD, that take turns:
+// while one group multiplies (its tile's logits, and the weights of the tile before
+// with their values), the other takes its tile's weights; a barrier ends each turn,
+// and the second group runs a turn behind. What a wave asks for in its weights' turn
+// -- keys two tiles on, values one on -- has the turns until the end of its next
+// products to land, and goes where no group reads any more: three stages.
+__global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
+{
+  constexpr int D = 128, kNW = 8;
+  using Load = Loader<D, kNW>;
+  constexpr int kTile = Load::kTile;
+  constexpr int kKC = D / 16;   // k chunks of the first product
+  constexpr int kDT = D / 32;   // 32-channel tiles of the second
+  constexpr int kStages = 3;
+  constexpr int kAhead = 6;     // fragments read ahead
+  static_assert(kNW * 32 * Load::kRow <= 2 * kStages * kTile, "the staged output fits");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStages * kTile];
+
+  Rows<D, kNW> r;
+  if (!find(p, r)) { return; }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Load load(p, r, lds);
+  bf16x8 qf[kKC];
+  load_queries(p, r, qf);
+  load.keys(0);
+  load.keys(1);
+  load.values(kStages);
+  // as in attention_kernel
+#pragma unroll
+  for (int i = 0; i < kKC; ++i) { asm volatile("" : "+v"(qf[i])); }
+
+  const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f,
+                       0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  f32x16 o[kDT];
+#pragma unroll
+  for (int d = 0; d < kDT; ++d) { o[d] = zero; }
+  // the row's maximum so far and its product with c; -infinity: nothing seen yet
+  float m = -INFINITY, mc = -INFINITY, l = 0.0f;
+
+  constexpr int kQK = 2 * kKC, kPV = 4 * kDT;   // products of a tile
+
+  // s[b] holds the logits of tokens 32 b + (i & 3) + 8 (i >> 2) + 4 half of a tile,
+  // pw the weights of the tile before
+  f32x16 s[2];
+  uint32_t pw[16];
+  auto part = [&](int c) {
+    return as_bf16x8(make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]));
+  };
+  auto first_product = [&](const uint8_t* kt) {
+    bf16x8 f[kQK];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) { f[i] = k_frag<D>(kt, i); }
+    fence();
+#pragma unroll
+    for (int i = 0; i < kQK; ++i) {
+      s[i & 1] = mfma32(f[i], qf[i >> 1], i < 2 ? zero : s[i & 1]);
+      if (i + kAhead < kQK) { f[i + kAhead] = k_frag<D>(kt, i + kAhead); }
+      fence();
+    }
+  };
+  auto second_product = [&](const uint8_t* vt) {
+    bf16x8 f[kPV];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) { f[i] = v_frag<D>(vt, i); }
+    fence();
+#pragma unroll
+    for (int i = 0; i < kPV; ++i) {
+      o[i % kDT] = mfma32(f[i], part(i / kDT), o[i % kDT]);
+      if (i + kAhead < kPV) { f[i + kAhead] = v_frag<D>(vt, i + kAhead); }
+      fence();
+    }
+  };
+  auto both_products = [&](const uint8_t* vt, const uint8_t* kt) {
+    bf16x8 f[kPV + kQK];
+    auto frag = [&](int i) { return i < kPV ? v_frag<D>(vt, i) : k_frag<D>(kt, i - kPV); };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) { f[i] = frag(i); }
+    fence();
+#pragma unroll
+    for (int i = 0; i < kPV + kQK; ++i) {
+      if (i < kPV) {
+        o[i % kDT] = mfma32(f[i], part(i / kDT), o[i % kDT]);
+      } else {
+        const int j = i - kPV;
+        s[j & 1] = mfma32(f[i], qf[j >> 1], j < 2 ? zero : s[j & 1]);
+      }
+      if (i + kAhead < kPV + kQK) { f[i + kAhead] = frag(i + kAhead); }
+      fence();
+    }
+  };
+  auto softmax = [&](int t) {
+    mask(r, t, s);
+    float sums[4];
+    auto weigh = [&]() {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { sums[j] = 0.0f; }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float a = exp2_of(fmaf(s[i >> 3][2 * (i & 7)], p.c, -mc));
+        const float b = exp2_of(fmaf(s[i >> 3][2 * (i & 7) + 1], p.c, -mc));
+        sums[2 * (i & 1)] += a;
+        sums[2 * (i & 1) + 1] += b;
+        pw[i] = pack_bf16x2(a, b);
+      }
+      return (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    };
+    // The weights are taken from the maximum so far, and only if a lane's sum of 32
+    // passes 2^12 -- a logit that much above the maximum, a first look at any key, a
+    // NaN -- the maximum is brought up to date, the sums with it, and the weights are
+    // taken again: most tiles need no maximum at all, and weights up to 2^12 are as
+    // exact as others in floating point.
+    float sum = weigh();
+    if (any_lane(!(sum <= 4096.0f))) {
+      float top = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i) { top = fmaxf(top, s[i >> 4][i & 15]); }
+      const float m_new = fmaxf(m, xor32_max(top));
+      const float mz = m_new == -INFINITY ? 0.0f : m_new;
+      const float keep = exp2_of((m - mz) * p.c);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { o[d][i] *= keep; }
+      }
+      mc = mz * p.c;
+      sum = weigh();
+      mc = m == -INFINITY ? -INFINITY : mc;
+    }
+    l += sum;
+  };
+
+  if (r.n_tiles > 0) {
+    landed<2 * Load::kLoads>();
+    if (wave >= kNW / 2) { meet(); }
+    int at = 0, prev = 2;   // stages of tile t, and of tile t - 1
+    for (int t = 0; t < r.n_tiles; ++t) {
+      const uint8_t* const kt = lds + at * kTile;
+      const uint8_t* const vt = lds + (kStages + prev) * kTile;
+      const int next = at == 2 ? 0 : at + 1;
+      prio<1>();
+      // past its last tile a wave's next logits are not used: a path without them would
+      // cost registers that the loop does not have
+      if (t == 0) {
+        first_product(kt);
+      } else if ((t - 1) * kBN <= r.wave_hi) {
+        both_products(vt, kt);
+      }
+      prio<0>();
+      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+      meet();
+      load.keys(prev);                // of tile t + 2
+      load.values(kStages + next);    // of tile t + 1
+      if (t * kBN <= r.wave_hi) { softmax(t); }
+      meet();
+      prev = at;
+      at = next;
+    }
+    if (wave < kNW / 2) { meet(); }
+    if ((r.n_tiles - 1) * kBN <= r.wave_hi) { second_product(lds + (kStages + prev) * kTile); }
+  }
+
+  finish(p, r, lds, o, m, l);
+}
+
+hipError_t run(const PromptParams& p, int head_dim, bool turns, int grid, hipStream_t st)
+{
+  if (turns) {
+    attention_turns_kernel<<<grid, 512, 0, st>>>(p);
+  } else if (head_dim == 128) {
+    attention_kernel<128><<<grid, 256, 0, st>>>(p);
+  } else {
+    attention_kernel<64><<<grid, 256, 0, st>>>(p);
+  }
   return hipGetLastError();
 }
 
@@ -362,17 +763,21 @@ hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream)
   p.total_k = a.total_k;
   p.causal = a.causal;
   p.c = a.scale * 1.4426950408889634f;
-  // rows: heads of one kv head side by side first, so that a tile spans few
-  // tokens and little of it is masked
+  // The form that takes turns, from two rounds of its workgroups on and for long
+  // sequences (the figures at the top of this file).
+  const bool turns = a.head_dim == 128 && (long)a.total_q * a.heads >= 2L * 256 * 256 &&
+                     a.total_k / a.batch >= 2048;
+  // rows: heads of one kv head side by side first, so that a workgroup spans few
+  // tokens and little of its last tile is masked, 32 tokens of a head at least
+  const int rows_log2 = turns ? 8 : 7;
   p.hp_log2 = 0;
-  while (p.share % (2 << p.hp_log2) == 0 && p.hp_log2 < 3) { ++p.hp_log2; }
-  p.tb_log2 = 8 - p.hp_log2;
+  while (p.share % (2 << p.hp_log2) == 0 && p.hp_log2 < rows_log2 - 5) { ++p.hp_log2; }
+  p.tb_log2 = rows_log2 - p.hp_log2;
   p.head_groups = a.heads >> p.hp_log2;
   const long units = (long)(a.total_q >> p.tb_log2) + a.batch;
   const long grid = units * p.head_groups;
   if (grid > INT_MAX) { return hipErrorInvalidConfiguration; }
-  return a.head_dim == 128 ? run<128>(p, (int)grid, stream)
-                           : run<64>(p, (int)grid, stream);
+  return run(p, a.head_dim, turns, (int)grid, stream);
 }
 
 }  // namespace ltx25

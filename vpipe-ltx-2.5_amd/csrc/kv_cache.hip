@@ -451,9 +451,10 @@ __device__ __forceinline__ int visible_len(const CachedParams& p, int b)
 // order, they are the right operand of O^T = V^T P^T, whose left one is 16 bytes
 // of a channel's tokens. Keys and values so go from memory to the matrix
 // instructions through registers alone.
-template <int D, int RT, int NW>
-__global__ void __launch_bounds__(NW * 64) attention_cached_kernel(CachedParams p)
+template <int D, int RT>
+__global__ void __launch_bounds__(kThreads) attention_cached_kernel(CachedParams p)
 {
+  constexpr int NW = kThreads / 64;
   constexpr int kL = D / 64;    // 16-byte loads of a token's key for each lane
   constexpr int kDT = D / 16;   // 16-channel tiles
   constexpr int kRows = 16 * RT;
@@ -531,23 +532,39 @@ __global__ void __launch_bounds__(NW * 64) attention_cached_kernel(CachedParams 
       for (int i = 0; i < kL; ++i) { kc[t][i] = *(const uint4*)(kp + t * 4 * D + i * 64); }
     }
   };
-  if (t0 < end) { load_keys(t0, id_k); }
-  for (; t0 < end; t0 += 64 * NW) {
-    const int tv = t0 + 16 * kg;
-    const int pv = clampi(id_v, 0, p.c.pages - 1);
-    const bool held = id_v == pv;
-    const long bv = (long)pv * p.c.kv_heads + g;
-    const int8_t* const vp = p.c.v + (bv << p.c.pl) * D + ((long)n << p.c.pl) + (tv & pmask);
-    uint4 vc[kDT];
+  // A tile's keys are asked for as soon as the keys of the tile before have been
+  // used, its scales and the next pages' ids behind them, its values as soon as those
+  // of the tile before have been: one tile of each in registers, and always loads in
+  // flight.
+  uint4 vc[kDT];
+  auto load_values = [&](int t0, int id) {
+    const long bv = (long)clampi(id, 0, p.c.pages - 1) * p.c.kv_heads + g;
+    const int8_t* const vp =
+        p.c.v + (bv << p.c.pl) * D + ((long)n << p.c.pl) + ((t0 + 16 * kg) & pmask);
 #pragma unroll
     for (int d = 0; d < kDT; ++d) { vc[d] = *(const uint4*)(vp + ((long)d << (p.c.pl + 4))); }
-    const float sk = p.c.ks[bv] * p.scale2, sv = p.c.vs[bv];
-    // the next tile's pages; its keys are asked for as soon as this one's are used
+  };
+  float next_k = 0.0f, next_v = 0.0f;
+  auto load_scales = [&](int id) {
+    const long bv = (long)clampi(id, 0, p.c.pages - 1) * p.c.kv_heads + g;
+    next_k = p.c.ks[bv];
+    next_v = p.c.vs[bv];
+  };
+  int id_v1 = id_v;
+  if (t0 < end) {
+    load_keys(t0, id_k);
+    load_scales(id_v);
     const int t1 = t0 + 64 * NW;
     if (t1 < end) {
       id_k = page_of(t1 + 16 * (n >> 2));
-      id_v = page_of(t1 + 16 * kg);
+      id_v1 = page_of(t1 + 16 * kg);
     }
+    load_values(t0, id_v);
+  }
+  for (; t0 < end; t0 += 64 * NW) {
+    const int tv = t0 + 16 * kg;
+    const bool held = id_v >= 0 && id_v < p.c.pages;
+    const int t1 = t0 + 64 * NW;
 
     f32x4 s[RT][4];
 #pragma unroll
@@ -565,7 +582,17 @@ __global__ void __launch_bounds__(NW * 64) attention_cached_kernel(CachedParams 
         }
       }
     }
-    if (t1 < end) { load_keys(t1, id_k); }
+    const float sk = next_k * p.scale2, sv = next_v;
+    id_v = id_v1;
+    if (t1 < end) {
+      load_keys(t1, id_k);
+      load_scales(id_v);
+      const int t2 = t1 + 64 * NW;
+      if (t2 < end) {
+        id_k = page_of(t2 + 16 * (n >> 2));
+        id_v1 = page_of(t2 + 16 * kg);
+      }
+    }
     bf16x8 pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -623,15 +650,16 @@ __global__ void __launch_bounds__(NW * 64) attention_cached_kernel(CachedParams 
         o[rt][d] = mfma16(c, pf[rt][1], o[rt][d]);
       }
     }
+    if (t1 < end) { load_values(t1, id_v); }
   }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) { l[rt] = xor32_sum(xor16_sum(l[rt])); }
 
-  // ---- the waves join through LDS, 16 rows at a time: a thread takes D / 16
+  // ---- the waves join through LDS, 16 rows at a time: a thread takes kPer
   // channels of one row
-  constexpr int kPer = D / 16;
-  static_assert(NW * 64 == kThreads, "16 rows x 16 threads");
-  const int jr = threadIdx.x >> 4, jd = (threadIdx.x & 15) * kPer;
+  constexpr int kPer = D * 16 / (NW * 64);
+  static_assert(kPer % 4 == 0, "a thread's channels are whole stores");
+  const int jr = threadIdx.x / (4 * NW), jd = threadIdx.x % (4 * NW) * kPer;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     if (rt > 0) { __syncthreads(); }
@@ -768,13 +796,13 @@ bool move_grid(const MoveParams& p, dim3& grid)
   return true;
 }
 
-template <int D, int RT, int NW>
+template <int D, int RT>
 hipError_t run_cached(const CachedParams& p, hipStream_t stream)
 {
   const long grid = (long)p.batch * p.c.kv_heads * p.splits * p.row_blocks;
   const long rows = (long)p.batch * p.q_len * p.heads;
   if (grid > INT_MAX || rows > INT_MAX) { return hipErrorInvalidConfiguration; }
-  attention_cached_kernel<D, RT, NW><<<(int)grid, NW * 64, 0, stream>>>(p);
+  attention_cached_kernel<D, RT><<<(int)grid, kThreads, 0, stream>>>(p);
   if (p.splits > 1) {
     constexpr int kWaves = kThreads / 64;
     attention_join_kernel<D><<<(int)((rows + kWaves - 1) / kWaves), kThreads, 0, stream>>>(p);
@@ -785,11 +813,9 @@ hipError_t run_cached(const CachedParams& p, hipStream_t stream)
 template <int D>
 hipError_t run_cached(const CachedParams& p, const CachedPlan& plan, hipStream_t stream)
 {
-  if (plan.row_tiles == 1) {
-    return run_cached<D, 1, 4>(p, stream);
-  }
-  if (plan.row_tiles == 2) { return run_cached<D, 2, 4>(p, stream); }
-  return run_cached<D, 4, 4>(p, stream);
+  if (plan.row_tiles == 1) { return run_cached<D, 1>(p, stream); }
+  if (plan.row_tiles == 2) { return run_cached<D, 2>(p, stream); }
+  return run_cached<D, 4>(p, stream);
 }
 
 }  // namespace
@@ -832,17 +858,17 @@ CachedPlan plan_cached(int batch, int q_len, int heads, int kv_heads, int head_d
   const long rows = (long)q_len * (heads / kv_heads);
   r.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   r.row_blocks = (int)((rows + 16 * r.row_tiles - 1) / (16 * r.row_tiles));
-  // Parts of whole rounds of the four waves (256 tokens). Up to 4 rounds: one part,
-  // since a round takes about 1.2 us where the GPU is not full and the join's own
-  // launch 5 (700 tokens, 8 kv heads: 9.7 us for 11.4 in 3 parts). Else two
-  // workgroups for each CU, which hold enough loads in flight (32 rows of 131072
-  // tokens: 175 us, 180 with four workgroups, 185 with eight) -- but no part longer
-  // than 20 rounds or a 16th of the tokens, since the lengths may be very uneven and
-  // only the longest is known here.
+  // Parts of whole rounds of the four waves (256 tokens). Up to 3 rounds: one part. A
+  // round more takes 2 us where the GPU is not full, the join's launch 3 on the GPU and
+  // 3 on the host (700 tokens, 8 kv heads: 9.1 us a call, 11.4 in 3 parts; replayed in a
+  // graph 8.6 and 7.7). Else two workgroups for each CU, which hold enough loads in
+  // flight (32 kv heads of 131072 tokens: 175 us, 180 with four workgroups, 185 with
+  // eight) -- but no part longer than 20 rounds or a 16th of the tokens, since the
+  // lengths may be very uneven and only the longest is known here.
   const long units = (long)batch * kv_heads * r.row_blocks;
   const long rounds = ((long)max_len + 255) / 256;
   long per = std::max(rounds, 1L);
-  if (rounds > 4) {
+  if (rounds > 3) {
     const long want = (512 + units - 1) / units;
     per = std::min((rounds + want - 1) / want, std::max(20L, rounds / 16));
     per = (rounds + (rounds + per - 1) / per - 1) / ((rounds + per - 1) / per);

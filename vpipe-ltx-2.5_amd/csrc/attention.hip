@@ -175,7 +175,10 @@ __device__ __forceinline__ bool find_rows(const PromptParams& p, int u, Unit& r)
     return (lq + tb - 1) >> p.tb_log2;
   };
   int at = 0;
-  if (p.batch > 64) {
+  if (p.batch == 1) {
+    if (u >= read(0)) { return false; }
+    r.from_end = u;
+  } else if (p.batch > 64) {
     int seq;
     if (!find_unit(u, p.batch, read, seq, r.from_end, at)) { return false; }
   } else {

@@ -121,7 +121,8 @@ int ltx25_kv_read(void* stream, const ltx25_kv_cache* cache, const int* table, i
  *   bytes, 16-byte aligned, any contents, in use until the call has run (NULL
  *   where that is 0).
  * Keys and values enter both products as their exact codes; a page's scales
- * multiply the logits and the weights in f32. The tokens are split over
+ * multiply the logits and the weights in f32, and these are rounded to f16 (under
+ * a power of two) for the second product. The tokens are split over
  * workgroups and the parts joined in one fixed order: the same call gives the
  * same bits. */
 int ltx25_attention_cached(void* stream, const ltx25_attn* a, const ltx25_kv_cache* cache,

@@ -301,6 +301,53 @@ def test_attention_cached_block_scales_far_apart(pkg, dev):
     _verify(c, table, lens, q, 1, True, out, z)
 
 
+def _verify_close(c, table, lens, q, q_len, out, z):
+    """The weights keep 11 bits for the second product, and what is done in f32 adds at most 2^-12 at
+    these logits (130 products of f32 each): beside the output's own rounding to bf16, 2^-8 of it."""
+    ref = attn_ref.Cache(c.k, c.v, c.k_scale, c.v_scale)
+    for b, n in enumerate(lens):
+        rows = slice(b * q_len, (b + 1) * q_len)
+        k, v = (torch.from_numpy(ref.values(w, table[b], 0, n)) for w in (0, 1))
+        want = attn_ref.attend(q[rows], k, v, c.head_dim ** -0.5, True)
+        attn_ref.check(out[rows], z[rows], want, f"sequence {b}")
+        exact, mag = want[0], want[2]
+        err = (out[rows].cpu().double() - exact).abs()
+        err -= 2.0 ** -8 * 1.001 * exact.abs() + (2.0 ** -11 + 2.0 ** -12) * mag
+        assert float(err.max()) <= 0, f"sequence {b}: {float(err.max()):.3e} past the bound"
+
+
+@pytest.mark.parametrize("lens,q_len,heads,kv_heads,dim,page", [
+    ([16], 16, 16, 2, 64, 32), ([700], 1, 32, 8, 128, 64), ([1, 2, 3, 2000], 3, 8, 2, 128, 16),
+    ([1100], 24, 2, 1, 128, 64), ([5000], 1, 4, 1, 64, 128)])
+def test_attention_cached_rounds_the_output_alone(pkg, dev, lens, q_len, heads, kv_heads, dim, page):
+    say(f"attention_cached close {lens} q_len {q_len} heads {heads}/{kv_heads} x {dim} page {page}")
+    table, pages = _table(68, lens, page)
+    c = _cache(pkg, 69, pages, page, kv_heads, dim)
+    q = _randn(70, len(lens) * q_len, heads, dim)
+    out, z = _attend(pkg, c, table, lens, q, q_len, True)
+    _verify_close(c, table, lens, q, q_len, out, z)
+
+
+@pytest.mark.parametrize("loud", [2.0 ** 10, 2.0 ** 24])
+@pytest.mark.parametrize("q_len,heads", [(1, 4), (8, 4), (12, 4)])
+def test_attention_cached_loud_blocks_that_no_query_looks_at(pkg, dev, loud, q_len, heads):
+    """Blocks of values that are much larger than the others', before and after them, whose keys
+    have logits so low that they do not count; a block of zeros that does."""
+    lens, page, dim = [640], 64, 64
+    table, pages = _table(71, lens, page)
+    c = _cache(pkg, 72, pages, page, 1, dim)
+    q = _randn(73, q_len, heads, dim).abs()
+    for at in (0, 4, 9):
+        c.k[table[0, at]] = -127
+        c.k_scale[table[0, at], 0] = 0.2
+        c.v_scale[table[0, at], 0] *= loud
+    c.v_scale[table[0, 2], 0] = 0.0
+    say(f"attention_cached loud {loud} q_len {q_len}")
+    # the last tokens lie in a loud block: the queries see it, and none of it counts
+    out, z = _attend(pkg, c, table, lens, q, q_len, True)
+    _verify_close(c, table, lens, q, q_len, out, z)
+
+
 def test_attention_cached_far_pages(pkg, dev):
     """Pages past 2^31 bytes of the cache."""
     page, heads, dim, pages = 64, 8, 128, 33000

@@ -78,7 +78,6 @@ __device__ __forceinline__ int v_piece(int row, int c)
 }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ bool any_lane(bool b) { return __any(b) != 0; }
 
 // 16 bytes a lane from the buffer straight into LDS, lane after lane from the LDS
 // address `to`. In asm, so that the compiler does not make every LDS read wait for

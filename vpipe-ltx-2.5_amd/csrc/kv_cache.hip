@@ -32,6 +32,27 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t a, uint32_t b)
   return as_bf16x8(r);
 }
 
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f16x8 as_f16x8(uint4 v) { return __builtin_bit_cast(f16x8, v); }
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
+{
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+}
+
+// 8 codes -> 8 f16, exactly: 0x64 before a byte u makes 1024 + u
+__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b)
+{
+  auto two = [](uint32_t w, uint32_t bytes) {
+    const uint32_t x = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, bytes);
+    const f16x2 y = __builtin_bit_cast(f16x2, x) - f16x2{1152, 1152};
+    return __builtin_bit_cast(uint32_t, y);
+  };
+  return as_f16x8(make_uint4(two(a, 0x04010400u), two(a, 0x04030402u), two(b, 0x04010400u),
+                             two(b, 0x04030402u)));
+}
+
 // rint(x / s) within +-127; 0 for s = 0 and for a NaN
 __device__ __forceinline__ int quantize(float x, float s)
 {
@@ -422,6 +443,11 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c)
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c)
+{
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
 __device__ __forceinline__ float xor16_max(float v)
 {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
@@ -452,15 +478,28 @@ __device__ __forceinline__ int visible_len(const CachedParams& p, int b)
 // of a channel's tokens. Keys and values so go from memory to the matrix
 // instructions through registers alone.
 //
-// Two row tiles are held to two waves a SIMD (256 registers): 8 queries of 16
-// sequences of 4000 tokens 37.7 us, 42.6 with the registers it would take.
+// The second product's weights w = exp(s - m) times the page's scale lie in f16
+// under a running power of two of their own, 2^mw: the largest has 2^13 to 2^15, so
+// that weights 2^27 times smaller keep all their 11 bits, and the output's own
+// rounding is all of its error (0.00166 of its norm; with weights in bf16 0.0024,
+// 0.0030 where few keys count). The sums stay as they are while no row's largest
+// weight grows four times over, which pays for the second maximum: 64 sequences of
+// 200 to 4000 tokens 64.1 us, 65 with bf16 weights and sums rescaled for every tile.
+// (The weights as two bf16 each are as exact and took 66; 57 us for 52 at head width
+// 64, 16 sequences of 8000 tokens.)
+//
+// Held to registers: two row tiles to two waves a SIMD (8 queries of 16 sequences of
+// 4000 tokens 37.7 us, 42.6 with the registers it would take), one of head width 64
+// to four (16 sequences of 8000 tokens 52.3 us, 55.2 with three).
 template <int D, int RT>
-__global__ void __launch_bounds__(kThreads, RT == 2 ? 2 : 1) attention_cached_kernel(CachedParams p)
+__global__ void __launch_bounds__(kThreads, RT == 2 ? 2 : D == 64 && RT == 1 ? 4 : 1)
+attention_cached_kernel(CachedParams p)
 {
   constexpr int NW = kThreads / 64;
   constexpr int kL = D / 64;    // 16-byte loads of a token's key for each lane
   constexpr int kDT = D / 16;   // 16-channel tiles
   constexpr int kRows = 16 * RT;
+  constexpr float kRoom = 13.0f, kLag = 2.0f;   // of w, log2
   __shared__ __attribute__((aligned(16))) float join[NW][16][D + 4];
   __shared__ float2 stat[NW][16];
 
@@ -515,9 +554,10 @@ __global__ void __launch_bounds__(kThreads, RT == 2 ? 2 : 1) attention_cached_ke
   }
   f32x4 o[RT][kDT];
   float m[RT], l[RT];
+  float mw[RT];   // log2 of what w is counted in, over 2^m
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY;
+    m[rt] = mw[rt] = -INFINITY;
     l[rt] = 0.0f;
 #pragma unroll
     for (int d = 0; d < kDT; ++d) { o[rt][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
@@ -596,25 +636,51 @@ __global__ void __launch_bounds__(kThreads, RT == 2 ? 2 : 1) attention_cached_ke
         id_v1 = page_of(t2 + 16 * kg);
       }
     }
-    bf16x8 pf[RT][2];
+    const float lsv = __builtin_amdgcn_logf(fabsf(sv));
+    f16x8 pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int lim = held ? min(limit[rt], end - 1) : -1;
+      // the scale of a page without a token that the row sees may be anything
+      const float sv_seen = tv <= lim ? sv : 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { s[rt][t][i] *= sk; }
+      }
+      if (any_lane(lim < tv + 15)) {   // else the tile is seen whole
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[rt][t][i] = tv + 4 * t + i <= lim ? s[rt][t][i] : -INFINITY;
+          }
+        }
+      }
       float top = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = s[rt][t][i] * sk;
-          s[rt][t][i] = tv + 4 * t + i <= lim ? v : -INFINITY;
-          top = fmaxf(top, s[rt][t][i]);
+        for (int i = 0; i < 4; ++i) { top = fmaxf(top, s[rt][t][i]); }
+      }
+      const float m_new = fmaxf(m[rt], xor32_max(xor16_max(top)));
+      const float ms = m_new == -INFINITY ? 0.0f : m_new;
+      const float lag = m[rt] - ms, keep = __builtin_amdgcn_exp2f(lag);
+      m[rt] = m_new;
+      // the row's largest w: the 16 tokens of a lane are of one page
+      const float top_w = xor32_max(xor16_max(top - ms + lsv)) - kRoom;
+      mw[rt] += lag;
+      if (any_lane(top_w > mw[rt] + kLag)) {
+        const float mw_new = fmaxf(mw[rt], top_w);
+        const float keep_o = mw_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw[rt] - mw_new);
+        mw[rt] = mw_new;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { o[rt][d][i] *= keep_o; }
         }
       }
-      top = xor32_max(xor16_max(top));
-      const float m_new = fmaxf(m[rt], top);
-      const float ms = m_new == -INFINITY ? 0.0f : m_new;
-      const float keep = __builtin_amdgcn_exp2f(m[rt] - ms);
-      m[rt] = m_new;
+      const float f = sv_seen * __builtin_amdgcn_exp2f(fminf(-mw[rt], 127.0f));
       float sum = 0.0f;
       float w[16];
 #pragma unroll
@@ -623,30 +689,24 @@ __global__ void __launch_bounds__(kThreads, RT == 2 ? 2 : 1) attention_cached_ke
         for (int i = 0; i < 4; ++i) {
           const float e = __builtin_amdgcn_exp2f(s[rt][t][i] - ms);
           sum += e;
-          // a masked token's scale may be anything
-          w[4 * t + i] = tv + 4 * t + i <= lim ? e * sv : 0.0f;
+          w[4 * t + i] = e * f;
         }
       }
       l[rt] = fmaf(l[rt], keep, sum);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint4 pw;
-        pw.x = pack_bf16x2(w[8 * j + 0], w[8 * j + 1]);
-        pw.y = pack_bf16x2(w[8 * j + 2], w[8 * j + 3]);
-        pw.z = pack_bf16x2(w[8 * j + 4], w[8 * j + 5]);
-        pw.w = pack_bf16x2(w[8 * j + 6], w[8 * j + 7]);
-        pf[rt][j] = as_bf16x8(pw);
-      }
-#pragma unroll
-      for (int d = 0; d < kDT; ++d) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { o[rt][d][i] *= keep; }
+        pw.x = pack_f16x2(w[8 * j + 0], w[8 * j + 1]);
+        pw.y = pack_f16x2(w[8 * j + 2], w[8 * j + 3]);
+        pw.z = pack_f16x2(w[8 * j + 4], w[8 * j + 5]);
+        pw.w = pack_f16x2(w[8 * j + 6], w[8 * j + 7]);
+        pf[rt][j] = as_f16x8(pw);
       }
     }
 #pragma unroll
     for (int d = 0; d < kDT; ++d) {
-      const bf16x8 a = codes_bf16(vc[d].x, vc[d].y);
-      const bf16x8 c = codes_bf16(vc[d].z, vc[d].w);
+      const f16x8 a = codes_f16(vc[d].x, vc[d].y);
+      const f16x8 c = codes_f16(vc[d].z, vc[d].w);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         o[rt][d] = mfma16(a, pf[rt][0], o[rt][d]);
@@ -656,7 +716,16 @@ __global__ void __launch_bounds__(kThreads, RT == 2 ? 2 : 1) attention_cached_ke
     if (t1 < end) { load_values(t1, id_v); }
   }
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) { l[rt] = xor32_sum(xor16_sum(l[rt])); }
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] = xor32_sum(xor16_sum(l[rt]));
+    // the sums, in 2^m from here on
+    const float f = __builtin_amdgcn_exp2f(mw[rt]);
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { o[rt][d][i] *= f; }
+    }
+  }
 
   // ---- the waves join through LDS, 16 rows at a time: a thread takes kPer
   // channels of one row

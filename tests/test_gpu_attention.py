@@ -285,3 +285,20 @@ def test_attention_of_several_hundred_sequences(pkg, dev, dim):
     say(f"attention of 600 sequences x {dim}")
     out, z = _run(pkg, q, k, v, lens, lens, True)
     _verify(q, k, v, out, z, lens, lens, True)
+
+
+@pytest.mark.parametrize("n,heads,kv_heads,dim", [(300, 2, 1, 64), (300, 2, 2, 128), (4200, 32, 8, 128)])
+def test_attention_values_near_the_end_of_f32(pkg, dev, n, heads, kv_heads, dim):
+    """Values up to 2^126 under logits that rise slowly: each row's mean is finite, though its sums
+    under a maximum that lags are not."""
+    q = torch.ones(n, heads, dim, dtype=torch.bfloat16, device="cuda")
+    k = torch.linspace(0, 5, n, device="cuda")[:, None, None].expand(n, kv_heads, dim) / dim
+    k, v = k.to(torch.bfloat16), _randn(38, n, kv_heads, dim)
+    v[:, 0] = (v[:, 0].float().clamp(-2, 2) * 2.0 ** 125).to(torch.bfloat16)
+    say(f"attention large values {n}")
+    out, z = _run(pkg, q, k, v, [n], [n], False, 1.0)
+    for i in (0, n - 1):
+        for h in (0, heads - 1):
+            g = h // (heads // kv_heads)
+            want = attn_ref.attend(q[i:i + 1, h:h + 1], k[:, g:g + 1], v[:, g:g + 1], 1.0, False)
+            attn_ref.check(out[i:i + 1, h:h + 1], z[i:i + 1, h:h + 1], want, f"row {i} head {h}")

@@ -348,6 +348,19 @@ def test_attention_cached_loud_blocks_that_no_query_looks_at(pkg, dev, loud, q_l
     _verify_close(c, table, lens, q, q_len, out, z)
 
 
+@pytest.mark.parametrize("n,heads,dim", [(300, 4, 64), (700, 40, 128), (5000, 4, 128), (5000, 4, 64)])
+def test_attention_cached_values_near_the_end_of_f32(pkg, dev, n, heads, dim):
+    """Values up to 2^126 under flat logits: the means are finite, though the sums are not, in one
+    part and in several."""
+    table, pages = _table(74, [n], 64)
+    c = _cache(pkg, 75, pages, 64, 1, dim)
+    c.v_scale.fill_(2.0 ** 119)
+    q = _randn(76, 1, heads, dim, std=0.1)
+    say(f"attention_cached large values {n}")
+    out, z = _attend(pkg, c, table, [n], q, 1, True)
+    _verify(c, table, [n], q, 1, True, out, z)
+
+
 def test_attention_cached_far_pages(pkg, dev):
     """Pages past 2^31 bytes of the cache."""
     page, heads, dim, pages = 64, 8, 128, 33000

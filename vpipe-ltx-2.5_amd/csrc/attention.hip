@@ -81,7 +81,8 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 
 // 16 bytes a lane from the buffer straight into LDS, lane after lane from the LDS
 // address `to`. In asm, so that the compiler does not make every LDS read wait for
-// it; the kernel counts the loads in flight itself.
+// it; the kernel counts the loads in flight itself. Nothing else in these kernels
+// uses m0.
 __device__ __forceinline__ void load_lds(i32x4 from, uint32_t to, int offset)
 {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
@@ -392,7 +393,7 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   landed<0>();
   uint8_t* const mine = lds + wave * 32 * kRow;
-  float nans[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // a NaN stays one in a sum
+  float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // a NaN or an infinity stays in a sum
 #pragma unroll
   for (int d = 0; d < kDT; ++d) {
 #pragma unroll
@@ -401,7 +402,7 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j] = o[d][4 * i + j] * inv;
-        nans[j] += x[j];
+        odd[j] += x[j];
       }
       *(uint2*)(mine + (lane & 31) * kRow + k_piece<D>(lane & 31, d * 4 + i) * 16 + half * 8) =
           make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
@@ -420,12 +421,13 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
     p.lse[(long)(r.q0 + r.tok) * p.heads + r.head] =
         l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l)) * 0.69314718055994531f;
   }
-  const float sum = (nans[0] + nans[1]) + (nans[2] + nans[3]);
-  const bool bad = sum != sum;
+  const bool bad = !(fabsf((odd[0] + odd[1]) + (odd[2] + odd[3])) < INFINITY);
   // A NaN in a row: a weight of zero times an infinite or NaN value that the
   // row does not see (a tile's masked tokens take part in the second product)
-  // gives one too. Such rows are computed again over the tokens they see alone,
-  // one at a time, by the whole wave: a rare case whose speed does not matter.
+  // gives one too. An infinity: weights above a maximum that lags took the sums of
+  // values near f32's end past it. Such rows are computed again over the tokens they
+  // see alone, one at a time, by the whole wave, as a mean that each token moves: a
+  // rare case whose speed does not matter.
   unsigned long long again = __ballot(bad && r.valid);
   again = (again | (again >> 32)) & 0xffffffffull;
   while (again != 0) {
@@ -450,14 +452,17 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
       const float kept = __builtin_amdgcn_exp2f(fmaf(rm, p.c, -nc));
       const float w = __builtin_amdgcn_exp2f(fmaf(x, p.c, -nc));
       rm = n;
-      rl = fmaf(rl, kept, w);
+      const float before = rl * kept;
+      rl = before + w;
+      const float inv_l = rl == 0.0f ? 0.0f : 1.0f / rl;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) { acc[i] = fmaf(acc[i], kept, w * bf16_to_f32(vp[i])); }
+      for (int i = 0; i < kPer; ++i) {
+        acc[i] = fmaf(acc[i], before * inv_l, w * inv_l * bf16_to_f32(vp[i]));
+      }
     }
-    const float rinv = rl == 0.0f ? 0.0f : 1.0f / rl;
     uint16_t* const op = p.out + (long)(r.q0 + rtok) * p.os + rhead * D + lane * kPer;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) { op[i] = f32_to_bf16(acc[i] * rinv); }
+    for (int i = 0; i < kPer; ++i) { op[i] = f32_to_bf16(acc[i]); }
   }
 }
 

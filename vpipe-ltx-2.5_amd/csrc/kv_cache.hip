@@ -430,7 +430,7 @@ struct CachedParams {
   const uint16_t* q;
   uint16_t* out;
   float* lse;
-  float* part;       // [rows][splits][D] sums, then [rows][splits][2] maximum and sum
+  float* part;       // [rows][splits][D] means, then [rows][splits][2] maximum and sum
   long qs, os;
   int heads, share, causal;
   float scale2;      // scale log2(e)
@@ -718,8 +718,8 @@ attention_cached_kernel(CachedParams p)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] = xor32_sum(xor16_sum(l[rt]));
-    // the sums, in 2^m from here on
-    const float f = __builtin_amdgcn_exp2f(mw[rt]);
+    // means from here on: they stay in range where sums of large values would not
+    const float f = l[rt] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mw[rt]) / l[rt];
 #pragma unroll
     for (int d = 0; d < kDT; ++d) {
 #pragma unroll
@@ -743,16 +743,20 @@ attention_cached_kernel(CachedParams p)
 #pragma unroll
     for (int w = 0; w < NW; ++w) { top = fmaxf(top, stat[w][jr].x); }
     const float ms = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, acc[kPer];
+    float part[NW], sum = 0.0f, acc[kPer];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float2 x = stat[w][jr];
+      part[w] = __builtin_amdgcn_exp2f(x.x - ms) * x.y;
+      sum += part[w];
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) { acc[i] = 0.0f; }
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float2 x = stat[w][jr];
-      const float f = __builtin_amdgcn_exp2f(x.x - ms);
-      sum = fmaf(f, x.y, sum);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) { acc[i] = fmaf(f, join[w][jr][jd + i], acc[i]); }
+      for (int i = 0; i < kPer; ++i) { acc[i] = fmaf(part[w] * inv, join[w][jr][jd + i], acc[i]); }
     }
     const int r = rb * kRows + rt * 16 + jr;
     if (r >= p.q_len * p.share) { continue; }
@@ -771,10 +775,9 @@ attention_cached_kernel(CachedParams p)
             make_float2(top, sum);
       }
     } else {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       uint32_t* const op = (uint32_t*)(p.out + token * p.os + (long)head * D + jd);
 #pragma unroll
-      for (int i = 0; i < kPer; i += 2) { op[i / 2] = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv); }
+      for (int i = 0; i < kPer; i += 2) { op[i / 2] = pack_bf16x2(acc[i], acc[i + 1]); }
       if (p.lse != nullptr && jd == 0) {
         p.lse[at] = sum == 0.0f ? -INFINITY : (ms + log2f(sum)) * 0.69314718055994531f;
       }
@@ -817,27 +820,29 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(CachedParams p
   for (int i = 1; i < 64; i *= 2) { top = fmaxf(top, __shfl_xor(top, i)); }
   const float ms = top == -INFINITY ? 0.0f : top;
   float l = 0.0f;
+  for (int s = lane; s < used; s += 64) { l = fmaf(__builtin_amdgcn_exp2f(ml[s].x - ms), ml[s].y, l); }
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) { l += __shfl_xor(l, i); }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s0 = part; s0 < used; s0 += 4 * kSide) {
     if (s0 != part) { fetch(s0); }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float w = s0 + j * kSide < used ? __builtin_amdgcn_exp2f(st[j].x - ms) : 0.0f;
-      l = fmaf(w, st[j].y, l);
+      const float w =
+          s0 + j * kSide < used ? __builtin_amdgcn_exp2f(st[j].x - ms) * st[j].y * inv : 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) { acc[i] = fmaf(w, x[j][i], acc[i]); }
     }
   }
 #pragma unroll
   for (int i = kLanes; i < 64; i *= 2) {
-    l += __shfl_xor(l, i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) { acc[j] += __shfl_xor(acc[j], i); }
   }
   if (part != 0) { return; }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   *(uint2*)(p.out + token * p.os + (long)head * D + d) =
-      make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+      make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
   if (p.lse != nullptr && d == 0) {
     p.lse[at] = l == 0.0f ? -INFINITY : (ms + log2f(l)) * 0.69314718055994531f;
   }

@@ -11,6 +11,9 @@
  * its tensors is the caller's `workspace`, so calls on different streams may
  * overlap and a call may be captured into a HIP graph.
  *
+ * A call takes at most 2^27 packed tokens (queries, keys or new cache tokens), and
+ * sequences of a cache at most 2^30.
+ *
  * Lengths, cumulative lengths and page tables are device memory, so that a
  * serving loop can keep them on the GPU; they are read when the kernels run.
  * The kernels keep every access inside the sizes given by the host whatever
@@ -131,7 +134,9 @@ int ltx25_attention_cached(void* stream, const ltx25_attn* a, const ltx25_kv_cac
                            void* workspace, size_t workspace_bytes);
 
 /* Bytes of workspace that ltx25_attention_cached needs; 0 for sizes it refuses
- * and where it needs none. Grows with batch, q_len, heads and max_len. */
+ * and where it needs none. Not monotone: a smaller batch or fewer queries may be
+ * split into more parts and need more. A program that makes calls of several sizes
+ * with one workspace takes the largest of theirs. */
 size_t ltx25_attention_cached_workspace(int batch, int q_len, int heads, int kv_heads, int head_dim,
                                         int max_len);
 

@@ -172,3 +172,22 @@ def test_binding_checks_tensors(pkg):
         pkg.kv_append(c, table, k, k, i32(0, 4, 4), i32(0))
     with pytest.raises(ValueError):
         pkg.attention_cached(c, table, i32(10), t(3, 8, 128), t(3, 8, 128), 2, 100)
+
+
+def test_more_packed_tokens_than_a_call_takes(pkg, lib):
+    many = (1 << 27) + 1
+    assert _attention(pkg, lib, total_q=many) == pkg.E_INVAL
+    assert "total_q" in pkg.last_error()
+    assert _attention(pkg, lib, total_k=many) == pkg.E_INVAL
+    for name in ("ltx25_kv_append", "ltx25_kv_read"):
+        assert _append(pkg, lib, total=many, name=name) == pkg.E_INVAL
+        assert "total" in pkg.last_error()
+    assert _cached(pkg, lib, batch=1 << 14, q_len=(1 << 13) + 1) == pkg.E_INVAL
+
+
+def test_workspace_of_each_size_is_asked_for(pkg, lib):
+    """More sequences may need less workspace: a call is held to its own need."""
+    one, few = (pkg.attention_cached_workspace(b, 1, 8, 8, 128, 5120) for b in (64, 60))
+    assert one == 0 and few > 0
+    c, a = _cache(pkg, kv_heads=8), _attn(pkg, kv_heads=8)
+    assert _cached(pkg, lib, a, c, batch=60, max_len=5120, ws_bytes=few - 1) == pkg.E_INVAL

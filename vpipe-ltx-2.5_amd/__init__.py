@@ -472,7 +472,8 @@ def kv_read(cache: KVCache, table, k, v, cu, start, stream=None) -> None:
 
 def attention_cached_workspace(batch: int, q_len: int, heads: int, kv_heads: int, head_dim: int,
                                max_len: int) -> int:
-    """Bytes of workspace that attention_cached needs (ltx25_attention_cached_workspace)."""
+    """Bytes of workspace that attention_cached needs (ltx25_attention_cached_workspace); not monotone
+    in the sizes."""
     return int(load().ltx25_attention_cached_workspace(batch, q_len, heads, kv_heads, head_dim,
                                                        max_len))
 

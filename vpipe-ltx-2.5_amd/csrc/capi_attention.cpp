@@ -31,9 +31,12 @@ int check_pointer(const char* name, const void* p, uintptr_t align)
 
 // The kernels form a 64-token tile's offsets in 32 bits.
 constexpr int64_t kStrideMax = (int64_t)1 << 23;
-// Tokens of a sequence and of a call; positions past them would not fit the
-// kernels' 32-bit token numbers.
+// Tokens of a cached sequence; positions past them would not fit the kernels' 32-bit
+// token numbers.
 constexpr int kTokensMax = 1 << 30;
+// Packed tokens of a call: no sequence then has more than 2^24 units of work
+// (find_unit's bound), nor 64 sequences' units more than 32 bits hold.
+constexpr int kPackedMax = 1 << 27;
 
 int check_stride(const char* name, int64_t stride, int heads, int head_dim)
 {
@@ -109,10 +112,10 @@ int check_cache(const ltx25_kv_cache* c, const int* table, int table_stride, int
   return LTX25_OK;
 }
 
-int check_tokens(const char* name, long tokens)
+int check_tokens(const char* name, long tokens, int most)
 {
-  if (tokens < 0 || tokens > kTokensMax) {
-    return set_error(LTX25_E_INVAL, "%s=%ld is not in 0 .. %d", name, tokens, kTokensMax);
+  if (tokens < 0 || tokens > most) {
+    return set_error(LTX25_E_INVAL, "%s=%ld is not in 0 .. %d", name, tokens, most);
   }
   return LTX25_OK;
 }
@@ -124,7 +127,7 @@ int check_move(const ltx25_kv_cache* cache, const int* table, int table_stride, 
 {
   int rc = check_cache(cache, table, table_stride, batch, c);
   if (rc != LTX25_OK) { return rc; }
-  if ((rc = check_tokens("total", total)) != LTX25_OK ||
+  if ((rc = check_tokens("total", total, kPackedMax)) != LTX25_OK ||
       (rc = check_stride("k_stride", k_stride, c->kv_heads, c->head_dim)) != LTX25_OK ||
       (rc = check_stride("v_stride", v_stride, c->kv_heads, c->head_dim)) != LTX25_OK) {
     return rc;
@@ -152,8 +155,8 @@ int ltx25_attention(void* stream, const ltx25_attn* a, const void* q, const void
   if (rc != LTX25_OK) { return rc; }
   if ((rc = check_stride("k_stride", a->k_stride, a->kv_heads, a->head_dim)) != LTX25_OK ||
       (rc = check_stride("v_stride", a->v_stride, a->kv_heads, a->head_dim)) != LTX25_OK ||
-      (rc = check_tokens("total_q", total_q)) != LTX25_OK ||
-      (rc = check_tokens("total_k", total_k)) != LTX25_OK) {
+      (rc = check_tokens("total_q", total_q, kPackedMax)) != LTX25_OK ||
+      (rc = check_tokens("total_k", total_k, kPackedMax)) != LTX25_OK) {
     return rc;
   }
   if (batch < 0) { return set_error(LTX25_E_INVAL, "batch=%d is negative", batch); }
@@ -230,7 +233,7 @@ size_t ltx25_attention_cached_workspace(int batch, int q_len, int heads, int kv_
 {
   if (batch <= 0 || q_len <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128) || max_len <= 0 || max_len > kTokensMax ||
-      (long)batch * q_len > kTokensMax) {
+      (long)batch * q_len > kPackedMax) {
     return 0;
   }
   return ltx25::plan_cached(batch, q_len, heads, kv_heads, head_dim, max_len).workspace_bytes;
@@ -255,8 +258,8 @@ int ltx25_attention_cached(void* stream, const ltx25_attn* a, const ltx25_kv_cac
   if (q_len < 0 || max_len < 0) {
     return set_error(LTX25_E_INVAL, "q_len=%d max_len=%d must not be negative", q_len, max_len);
   }
-  if ((rc = check_tokens("max_len", max_len)) != LTX25_OK ||
-      (rc = check_tokens("batch * q_len", (long)batch * q_len)) != LTX25_OK) {
+  if ((rc = check_tokens("max_len", max_len, kTokensMax)) != LTX25_OK ||
+      (rc = check_tokens("batch * q_len", (long)batch * q_len, kPackedMax)) != LTX25_OK) {
     return rc;
   }
   if (batch == 0 || q_len == 0) { return LTX25_OK; }

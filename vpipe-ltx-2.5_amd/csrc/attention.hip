@@ -14,24 +14,31 @@
 // K and V tiles go from global memory straight into LDS (16 bytes a lane), the
 // loads in flight counted by hand. Their rows' 16-byte pieces are swizzled on the
 // way in (the source address is permuted, the LDS side of such a load is linear)
-// so that the fragment reads meet no bank twice (SQ_LDS_BANK_CONFLICT is 0 in the
-// loop).
+// so that the fragment reads meet no bank twice (the conflicts counted, 250 cycles a
+// workgroup however many its tiles, are the output's on its way through LDS).
 //
 // What bounds it: a tile takes a wave 32 products of 32 cycles on the matrix
 // cores and about 140 operations for the weights, 33 of them exponentials at 9
 // cycles and the rest at 5 each: as much time as the products, which two waves a
-// SIMD overlap only in part. The instructions' energy counts as well: 17% fewer
-// cycles (attention_turns_kernel against attention_kernel) came at 10% less clock.
+// SIMD overlap only in part (matrix cores busy 66% of the cycles on long prompts).
+// The instructions' energy counts as well: 17% fewer cycles (attention_turns_kernel
+// against attention_kernel) came at 10% less clock. The weights are rounded to bf16
+// as the values are; the sums and statistics are f32.
 // Two forms:
 //   attention_kernel: 4 waves, 128 rows; two to four such workgroups share a CU
-//   and one computes while another waits. 333-token prompts 19 us where 8 waves
-//   took 25, 48 prompts of 40 to 200 tokens 13 against 16.
+//   and one computes while another waits.
 //   attention_turns_kernel (head width 128): 8 waves, 256 rows, in two groups
-//   that take turns with the matrix cores. 16384 causal tokens, 32 / 8 heads: 1850
-//   us (1190 TFLOP/s) against 2045; 8160 tokens that all see each other, 32 heads:
-//   917 us (1190 TFLOP/s) against 1037; where less than about two rounds of
-//   workgroups fill the GPU, or the sequences are short, it is the slower one (2048
-//   tokens: 52.6 us against 49.7; eight of 1024: 91 against 91.5).
+//   that take turns with the matrix cores.
+// The second is the faster one from two rounds of workgroups on and for sequences
+// that are long on average; whole calls of 32 heads (8 of keys), first and second form:
+//   one causal prompt of 333 tokens      11.7 us   14.0
+//                        2048            49.5      53.8
+//                        4096             144       126
+//                       16384            2006      1830 (1200 TFLOP/s)
+//   eight of 1024                          95        98
+//   four of 2048                          156       149
+//   8000 tokens beside 200, 100 and 60    496       459
+//   8160 that all see each other, 32 heads of keys  1024  893 (1222 TFLOP/s)
 #include "attention.h"
 
 #include <climits>
@@ -773,8 +780,8 @@ hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream)
   p.total_k = a.total_k;
   p.causal = a.causal;
   p.c = a.scale * 1.4426950408889634f;
-  // The form that takes turns, from two rounds of its workgroups on and for long
-  // sequences (the figures at the top of this file).
+  // The form that takes turns, from two rounds of its workgroups on and for sequences
+  // that are long on average (the figures at the top of this file).
   const bool turns = a.head_dim == 128 && (long)a.total_q * a.heads >= 2L * 256 * 256 &&
                      a.total_k / a.batch >= 2048;
   // rows: heads of one kv head side by side first, so that a workgroup spans few

@@ -192,7 +192,11 @@ __device__ __forceinline__ uint2 quantize8(uint4 x, float s, float rs)
 // (blockIdx.z 0) or their values (1). A thread holds four tokens of 8 channels, so
 // that its codes are whole words both by token and, turned, by channel; of a few
 // tokens (a decode step's one) it holds one token's 8 channels, since a quarter or
-// less of that work is then there to do.
+// less of that work is then there to do (one token each of 64 sequences, 8 heads of
+// 128: 5.7 us, 8.4 by fours).
+//
+// Bound by memory where there is much to do: 8192 tokens of 8 heads of 128, 50 MB read
+// and written, 14.9 us (3.4 TB/s; a page's first code waits for all its values).
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
 {
@@ -365,7 +369,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
   }
 }
 
-// A workgroup reads one page's span of one kv head back as bf16.
+// A workgroup reads one page's span of one kv head back as bf16; values are turned in
+// LDS. Bound by memory: 8192 tokens of 8 heads of 128, 50 MB, 11 us (4.6 TB/s).
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(MoveParams p)
 {
@@ -487,6 +492,9 @@ __device__ __forceinline__ int visible_len(const CachedParams& p, int b)
 // 200 to 4000 tokens 64.1 us, 65 with bf16 weights and sums rescaled for every tile.
 // (The weights as two bf16 each are as exact and took 66; 57 us for 52 at head width
 // 64, 16 sequences of 8000 tokens.)
+//
+// Bound by memory: 4 x 8 kv heads of 99991 to 131072 tokens, 988 MB, 171 us (5.8 TB/s); 64
+// sequences of 200 to 4000 tokens, 275 MB, 55 us (5.0 TB/s).
 //
 // Held to registers: two row tiles to two waves a SIMD (8 queries of 16 sequences of
 // 4000 tokens 37.7 us, 42.6 with the registers it would take), one of head width 64
@@ -787,7 +795,8 @@ attention_cached_kernel(CachedParams p)
 
 // The splits of a row joined; a wave for each row. D / 4 lanes take 4 channels
 // each of one split, so that 64 / (D / 4) splits are read side by side, and four
-// of those in flight; always added in the same order.
+// of those in flight; always added in the same order. Bound by the latency of its
+// loads, one after another: 4.8 us.
 template <int D>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(CachedParams p)
 {
@@ -939,7 +948,7 @@ CachedPlan plan_cached(int batch, int q_len, int heads, int kv_heads, int head_d
   // round more takes 2 us where the GPU is not full, the join's launch 3 on the GPU and
   // 3 on the host (700 tokens, 8 kv heads: 9.1 us a call, 11.4 in 3 parts; replayed in a
   // graph 8.6 and 7.7). Else two workgroups for each CU, which hold enough loads in
-  // flight (32 kv heads of 131072 tokens: 175 us, 180 with four workgroups, 185 with
+  // flight (4 x 8 kv heads of 99991 to 131072 tokens: 175 us, 180 with four workgroups, 185 with
   // eight) -- but past 20 rounds no part longer than 8 rounds or a 16th of the tokens,
   // since the lengths may be very uneven and only the longest is known here (63
   // sequences of 200 tokens beside one of 30000: 52 us for 78 in parts of 20 rounds).

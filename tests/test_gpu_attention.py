@@ -302,3 +302,50 @@ def test_attention_values_near_the_end_of_f32(pkg, dev, n, heads, kv_heads, dim)
             g = h // (heads // kv_heads)
             want = attn_ref.attend(q[i:i + 1, h:h + 1], k[:, g:g + 1], v[:, g:g + 1], 1.0, False)
             attn_ref.check(out[i:i + 1, h:h + 1], z[i:i + 1, h:h + 1], want, f"row {i} head {h}")
+
+
+@pytest.mark.parametrize("n,heads,kv_heads,dim", [(200, 4, 2, 64), (200, 4, 2, 128), (4200, 32, 8, 128)])
+def test_attention_nan_channels_that_are_seen_and_unseen(pkg, dev, n, heads, kv_heads, dim):
+    """Channels of the values that are NaN from a seen token, from an unseen one of the same tile, or
+    from both: the seen ones show, the others do not, and what is beside them keeps its bits."""
+    q, k, v = _randn(39, n, heads, dim), _randn(40, n, kv_heads, dim), _randn(41, n, kv_heads, dim)
+    clean, _ = _run(pkg, q, k, v, [n], [n], True)
+    nan, at = float("nan"), n - n % 64 - 30     # `at` lies inside a tile
+    v[10, :, 3], v[at, :, 3], v[at, :, 5], v[at + 2, 0, 7] = nan, nan, nan, float("inf")
+    say(f"attention nan channels {n} x {dim}")
+    out, z = _run(pkg, q, k, v, [n], [n], True)
+    assert bool(torch.isfinite(z).all())
+    bad = torch.isnan(out)
+    assert not bool(bad[:10].any()) and bool(bad[10:, :, 3].all())
+    assert bool(bad[at:, :, 5].all()) and not bool(bad[:at, :, 5].any())
+    share = heads // kv_heads
+    assert bool(torch.isinf(out[at + 2:, :share, 7]).all())
+    assert bool(torch.isfinite(out[:at + 2, :share, 7]).all())
+    untouched = torch.ones(dim, dtype=torch.bool)
+    untouched[[3, 5, 7]] = False
+    assert torch.equal(out[..., untouched].view(torch.int16), clean[..., untouched].view(torch.int16))
+    for i in (at - 1, at):
+        want = attn_ref.attend(q[i:i + 1], k[:i + 1], v[:i + 1], dim ** -0.5, False)
+        ok = ~torch.isnan(want[0])
+        err = (out[i:i + 1].cpu().double() - want[0]).abs()[ok] - attn_ref.OUT_BOUND * want[2][ok]
+        assert float(err.max()) <= 0, f"row {i}"
+
+
+def test_attention_nan_everywhere_ends_soon(pkg, dev):
+    """Tensors full of NaN: NaN out, and in about the time of any others."""
+    n = 6000
+    q, k, v = _randn(42, n, 32, 128), _randn(43, n, 8, 128), _randn(44, n, 8, 128)
+    times = []
+    for bad in (None, q, v, k):
+        t = [x if x is not bad else torch.full_like(x, float("nan")) for x in (q, k, v)]
+        out = torch.empty_like(q)
+        say("attention full of NaN")
+        pkg.attention(*t, out, causal=True)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        pkg.attention(*t, out, causal=True)
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+        assert bool(torch.isnan(out).all()) == (bad is not None)
+    assert max(times[1:]) < 20 * times[0] + 1.0, times

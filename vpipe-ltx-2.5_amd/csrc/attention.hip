@@ -47,6 +47,12 @@ namespace ltx25 {
 namespace {
 
 constexpr int kBN = 64;   // tokens of a tile
+// The weights are 2^(logit - maximum - kShift), so that under a maximum that lags by
+// up to 2^12 sums of values near f32's end stay in range; weights 2^94 below the
+// largest are still normal numbers. 32, because the exponents of most weights then
+// differ in as few bits as without a shift: with 28 they lie on both sides of a power of
+// two, and the power that this costs the matrix cores makes a long prompt 1% slower.
+constexpr float kShift = 32.0f;
 
 struct PromptParams {
   const uint16_t* q;
@@ -385,6 +391,18 @@ __device__ __forceinline__ void mask(const Rows<D, NW>& r, int t, f32x16 (&s)[2]
   }
 }
 
+// Whether one of 8 bf16 is an infinity or a NaN
+__device__ __forceinline__ bool not_finite(uint4 v)
+{
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    any = any || (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+  }
+  return any;
+}
+
 // The sums and statistics of the wave's rows out: through LDS, each wave its own
 // part of it, so that a store has whole rows' pieces side by side.
 template <int D, int NW>
@@ -400,7 +418,7 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   landed<0>();
   uint8_t* const mine = lds + wave * 32 * kRow;
-  float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // a NaN or an infinity stays in a sum
+  float nans[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // a NaN stays one in a sum
 #pragma unroll
   for (int d = 0; d < kDT; ++d) {
 #pragma unroll
@@ -409,7 +427,7 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j] = o[d][4 * i + j] * inv;
-        odd[j] += x[j];
+        nans[j] += x[j];
       }
       *(uint2*)(mine + (lane & 31) * kRow + k_piece<D>(lane & 31, d * 4 + i) * 16 + half * 8) =
           make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
@@ -426,29 +444,48 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
   }
   if (p.lse != nullptr && half == 0 && r.valid) {
     p.lse[(long)(r.q0 + r.tok) * p.heads + r.head] =
-        l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l)) * 0.69314718055994531f;
+        l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l * 0x1p32f)) * 0.69314718055994531f;
   }
-  const bool bad = !(fabsf((odd[0] + odd[1]) + (odd[2] + odd[3])) < INFINITY);
-  // A NaN in a row: a weight of zero times an infinite or NaN value that the
-  // row does not see (a tile's masked tokens take part in the second product)
-  // gives one too. An infinity: weights above a maximum that lags took the sums of
-  // values near f32's end past it. Such rows are computed again over the tokens they
-  // see alone, one at a time, by the whole wave, as a mean that each token moves: a
-  // rare case whose speed does not matter.
-  unsigned long long again = __ballot(bad && r.valid);
+  const float sum = (nans[0] + nans[1]) + (nans[2] + nans[3]);
+  // A NaN in a row: a weight of zero times an infinite or NaN value that the row does
+  // not see (a causal tile's masked tokens take part in the second product) gives one
+  // too. If there is such a value among these tokens, the row's NaN channels are
+  // computed again over the tokens that it sees alone, one at a time, by the whole wave,
+  // as a mean that each token moves, until they are NaN from what it does see: a rare
+  // case, but one that tensors full of NaN must not make endless. A sum of weights that
+  // is a NaN has seen one itself.
+  unsigned long long again = __ballot(sum != sum && l == l && r.valid);
   again = (again | (again >> 32)) & 0xffffffffull;
   while (again != 0) {
     const int at = __builtin_ctzll(again);
     again &= again - 1;
     const int rtok = __shfl(r.tok, at), rhead = __shfl(r.head, at), rlimit = __shfl(r.limit, at);
     constexpr int kPer = D / 64;
-    const uint16_t* const qp = p.q + (long)(r.q0 + rtok) * p.qs + rhead * D + lane * kPer;
+    bool unseen = false;   // a value that is not finite among the masked tokens
+    const int end = min(r.n_tiles * kBN, r.lk);
+    for (int j = max(rlimit + 1, 0) + (lane >> 3); j < end; j += 8) {
+      const uint16_t* const vp = p.v + (long)(r.k0 + j) * p.vs + r.g * D + (lane & 7) * (D / 8);
+#pragma unroll
+      for (int i = 0; i < D / 8; i += 8) { unseen = unseen || not_finite(*(const uint4*)(vp + i)); }
+    }
+    if (!any_lane(unseen)) { continue; }
+    const int d0 = lane * kPer;
+    const uint16_t* const staged =
+        (const uint16_t*)(mine + at * kRow + k_piece<D>(at, d0 / 8) * 16) + d0 % 8;
+    bool nan_at[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) { nan_at[i] = (staged[i] & 0x7fff) > 0x7f80; }
+    const uint16_t* const qp = p.q + (long)(r.q0 + rtok) * p.qs + rhead * D + d0;
     float qv[kPer], acc[kPer], rm = -INFINITY, rl = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) { qv[i] = bf16_to_f32(qp[i]); acc[i] = 0.0f; }
     for (int j = 0; j <= rlimit; ++j) {
-      const uint16_t* const kp = p.k + (long)(r.k0 + j) * p.ks + r.g * D + lane * kPer;
-      const uint16_t* const vp = p.v + (long)(r.k0 + j) * p.vs + r.g * D + lane * kPer;
+      bool open = false;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) { open = open || (nan_at[i] && acc[i] == acc[i]); }
+      if (!any_lane(open)) { break; }
+      const uint16_t* const kp = p.k + (long)(r.k0 + j) * p.ks + r.g * D + d0;
+      const uint16_t* const vp = p.v + (long)(r.k0 + j) * p.vs + r.g * D + d0;
       float x = 0.0f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) { x = fmaf(qv[i], bf16_to_f32(kp[i]), x); }
@@ -467,9 +504,11 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
         acc[i] = fmaf(acc[i], before * inv_l, w * inv_l * bf16_to_f32(vp[i]));
       }
     }
-    uint16_t* const op = p.out + (long)(r.q0 + rtok) * p.os + rhead * D + lane * kPer;
+    uint16_t* const op = p.out + (long)(r.q0 + rtok) * p.os + rhead * D + d0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) { op[i] = f32_to_bf16(acc[i]); }
+    for (int i = 0; i < kPer; ++i) {
+      if (nan_at[i]) { op[i] = f32_to_bf16(acc[i]); }
+    }
   }
 }
 
@@ -554,7 +593,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
       }
     }
     // ---- weights, and O^T += V^T P^T, 16 tokens a step
-    const float mc = m == -INFINITY ? 0.0f : m * p.c;
+    const float mc = m == -INFINITY ? 0.0f : fmaf(m, p.c, kShift);
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -615,7 +654,8 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
   f32x16 o[kDT];
 #pragma unroll
   for (int d = 0; d < kDT; ++d) { o[d] = zero; }
-  // the row's maximum so far and its product with c; -infinity: nothing seen yet
+  // the row's maximum so far and, with c and shifted, what the weights are taken from;
+  // -infinity: nothing seen yet
   float m = -INFINITY, mc = -INFINITY, l = 0.0f;
 
   constexpr int kQK = 2 * kKC, kPV = 4 * kDT;   // products of a tile
@@ -691,7 +731,7 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
     // taken again: most tiles need no maximum at all, and weights up to 2^12 are as
     // exact as others in floating point.
     float sum = weigh();
-    if (any_lane(!(sum <= 4096.0f))) {
+    if (any_lane(!(sum <= 0x1p-20f))) {   // 2^12, shifted
       float top = s[0][0];
 #pragma unroll
       for (int i = 1; i < 32; ++i) { top = fmaxf(top, s[i >> 4][i & 15]); }
@@ -705,7 +745,7 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
 #pragma unroll
         for (int i = 0; i < 16; ++i) { o[d][i] *= keep; }
       }
-      mc = mz * p.c;
+      mc = fmaf(mz, p.c, kShift);
       sum = weigh();
       mc = m == -INFINITY ? -INFINITY : mc;
     }

@@ -18,10 +18,11 @@
 // workgroup however many its tiles, are the output's on its way through LDS).
 //
 // What bounds it: a tile takes a wave 32 products of 32 cycles on the matrix
-// cores and about 140 operations for the weights, 33 of them exponentials at 9
-// cycles and the rest at 5 each: as much time as the products, which two waves a
+// cores and about 120 operations for the weights, 32 of them exponentials at 9
+// cycles and the rest at 4 to 5 each: as much time as the products, which two waves a
 // SIMD overlap only in part (matrix cores busy 66% of the cycles on long prompts).
-// The instructions' energy counts as well: 17% fewer cycles (attention_turns_kernel
+// At head width 64 the weights' operations alone do (80% of the cycles, and the matrix
+// cores 48%, before the maximum went). The instructions' energy counts as well: 17% fewer cycles (attention_turns_kernel
 // against attention_kernel) came at 10% less clock. The weights are rounded to bf16
 // as the values are; the sums and statistics are f32.
 // Two forms:
@@ -542,7 +543,9 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
 #pragma unroll
     for (int i = 0; i < 16; ++i) { o[d][i] = 0.0f; }
   }
-  float m = -INFINITY, l = 0.0f;
+  // the row's maximum so far and, with c and shifted, what the weights are taken from;
+  // -infinity: nothing seen yet
+  float m = -INFINITY, mc = -INFINITY, l = 0.0f;
 
   for (int t = 0; t < r.n_tiles; ++t) {
     // this tile is there, every wave's share of it, and no wave reads tile t - 1,
@@ -556,33 +559,50 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
     const uint8_t* const vt = lds + (2 + st) * kTile;
 
     f32x16 s[2];
+    auto logits = [&]() {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { s[b][i] = 0.0f; }
+        for (int i = 0; i < 16; ++i) { s[b][i] = 0.0f; }
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * kKC; ++i) { s[i & 1] = mfma32(k_frag<D>(kt, i), qf[i >> 1], s[i & 1]); }
+      ahead<2 * kKC, 8, 1>();
+      mask(r, t, s);
+    };
+    uint32_t pw[16];
+    auto weigh = [&]() {
+      float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float a = exp2_of(fmaf(s[i >> 3][2 * (i & 7)], p.c, -mc));
+        const float b = exp2_of(fmaf(s[i >> 3][2 * (i & 7) + 1], p.c, -mc));
+        sums[2 * (i & 1)] += a;
+        sums[2 * (i & 1) + 1] += b;
+        pw[i] = pack_bf16x2(a, b);
+      }
+      return (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    };
+    // The weights are taken from the maximum so far, and only if a lane's sum of 32
+    // passes 2^12 -- a logit that much above the maximum, a first look at any key, a
+    // NaN -- the maximum is brought up to date, the sums with it, and the weights are
+    // taken again, of logits multiplied again, since the registers have room for one of
+    // the two: most tiles need no maximum at all (5% of the time at head width 64), and
+    // weights up to 2^12 are as exact as others in floating point.
+    logits();
+    float sum = 0.0f;
+    bool settle = t == 0;
+    if (t > 0) {
+      sum = weigh();
+      settle = any_lane(!(sum <= 0x1p-20f));
+      if (settle) { logits(); }
     }
+    if (settle) {
+      float top = s[0][0];
 #pragma unroll
-    for (int i = 0; i < 2 * kKC; ++i) { s[i & 1] = mfma32(k_frag<D>(kt, i), qf[i >> 1], s[i & 1]); }
-    ahead<2 * kKC, 8, 1>();
-    mask(r, t, s);
-    // ---- the row's maximum, in four chains side by side (an operation that waits
-    // for the one before it takes 9 cycles, else 5). It is let lag behind the
-    // largest logit by up to 2^8 in the weights, whose sum then stays far inside
-    // f32: most tiles leave the sums as they are.
-    float tops[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x16& x = s[j >> 1];
-      const int e = (j & 1) * 8;
-      tops[j] = fmaxf(fmaxf(x[e], x[e + 1]), x[e + 2]);
-      tops[j] = fmaxf(fmaxf(x[e + 3], x[e + 4]), tops[j]);
-      tops[j] = fmaxf(fmaxf(x[e + 5], x[e + 6]), tops[j]);
-      tops[j] = fmaxf(x[e + 7], tops[j]);
-    }
-    const float top = xor32_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-    if (any_lane((top - m) * p.c > 8.0f || m == -INFINITY)) {
-      const float m_new = fmaxf(m, top);
-      const float mz = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen yet
+      for (int i = 1; i < 32; ++i) { top = fmaxf(top, s[i >> 4][i & 15]); }
+      const float m_new = fmaxf(m, xor32_max(top));
+      const float mz = m_new == -INFINITY ? 0.0f : m_new;
       const float keep = exp2_of((m - mz) * p.c);
       m = m_new;
       l *= keep;
@@ -591,29 +611,17 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
 #pragma unroll
         for (int i = 0; i < 16; ++i) { o[d][i] *= keep; }
       }
+      mc = fmaf(mz, p.c, kShift);
+      sum = weigh();
+      mc = m == -INFINITY ? -INFINITY : mc;
     }
-    // ---- weights, and O^T += V^T P^T, 16 tokens a step
-    const float mc = m == -INFINITY ? 0.0f : fmaf(m, p.c, kShift);
-    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    l += sum;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      f32x16& sc = s[c >> 1];
-      const int e = (c & 1) * 8;
-#pragma unroll
-      for (int i = e; i < e + 8; ++i) {
-        sc[i] = exp2_of(fmaf(sc[i], p.c, -mc));
-        sums[i & 3] += sc[i];
-      }
-      uint4 pw;
-      pw.x = pack_bf16x2(sc[e + 0], sc[e + 1]);
-      pw.y = pack_bf16x2(sc[e + 2], sc[e + 3]);
-      pw.z = pack_bf16x2(sc[e + 4], sc[e + 5]);
-      pw.w = pack_bf16x2(sc[e + 6], sc[e + 7]);
-      const bf16x8 pf = as_bf16x8(pw);
+      const bf16x8 pf = as_bf16x8(make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]));
 #pragma unroll
       for (int d = 0; d < kDT; ++d) { o[d] = mfma32(v_frag<D>(vt, c * kDT + d), pf, o[d]); }
     }
-    l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
   }
   finish(p, r, lds, o, m, l);
 }
@@ -654,9 +662,7 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
   f32x16 o[kDT];
 #pragma unroll
   for (int d = 0; d < kDT; ++d) { o[d] = zero; }
-  // the row's maximum so far and, with c and shifted, what the weights are taken from;
-  // -infinity: nothing seen yet
-  float m = -INFINITY, mc = -INFINITY, l = 0.0f;
+  float m = -INFINITY, mc = -INFINITY, l = 0.0f;   // as in attention_kernel
 
   constexpr int kQK = 2 * kKC, kPV = 4 * kDT;   // products of a tile
 
@@ -725,11 +731,7 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
       }
       return (sums[0] + sums[1]) + (sums[2] + sums[3]);
     };
-    // The weights are taken from the maximum so far, and only if a lane's sum of 32
-    // passes 2^12 -- a logit that much above the maximum, a first look at any key, a
-    // NaN -- the maximum is brought up to date, the sums with it, and the weights are
-    // taken again: most tiles need no maximum at all, and weights up to 2^12 are as
-    // exact as others in floating point.
+    // as in attention_kernel, with the logits still there
     float sum = weigh();
     if (any_lane(!(sum <= 0x1p-20f))) {   // 2^12, shifted
       float top = s[0][0];

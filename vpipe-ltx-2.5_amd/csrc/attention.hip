@@ -32,14 +32,15 @@
 //   that take turns with the matrix cores.
 // The second is the faster one from two rounds of workgroups on and for sequences
 // that are long on average; whole calls of 32 heads (8 of keys), first and second form:
-//   one causal prompt of 333 tokens      11.7 us   14.0
-//                        2048            49.5      53.8
-//                        4096             144       126
-//                       16384            2006      1830 (1200 TFLOP/s)
+//   one causal prompt of 333 tokens      12.6 us   14.7
+//                        2048              52        56
+//                        4096             148       130
+//                       16384            2032      1890 (1163 TFLOP/s)
 //   eight of 1024                          95        98
 //   four of 2048                          156       149
-//   8000 tokens beside 200, 100 and 60    496       459
-//   8160 that all see each other, 32 heads of keys  1024  893 (1222 TFLOP/s)
+//   8000 tokens beside 200, 100 and 60    495       471
+//   8160 that all see each other, 32 heads of keys  1015  918 (1188 TFLOP/s)
+// on a card whose power allowed 3% less than another's.
 #include "attention.h"
 
 #include <climits>

@@ -67,6 +67,21 @@ int ltx25_attention(void* stream, const ltx25_attn* a, const void* q, const void
                     void* out, float* lse, const int* cu_q, const int* cu_k, int batch,
                     int total_q, int total_k);
 
+/* The same where few rows see many keys (a few queries behind a long prefix, few
+ * heads): the keys are split over more workgroups and the parts joined in one fixed
+ * order, in a workspace as ltx25_attention_cached's: device memory of at least
+ * ltx25_attention_workspace() bytes, 16-byte aligned, any contents, in use until the
+ * call has run. Where that is 0 there is nothing to split, no workspace is needed and
+ * the call is ltx25_attention's. */
+int ltx25_attention_split(void* stream, const ltx25_attn* a, const void* q, const void* k,
+                          const void* v, void* out, float* lse, const int* cu_q, const int* cu_k,
+                          int batch, int total_q, int total_k, void* workspace,
+                          size_t workspace_bytes);
+
+/* Bytes of workspace that ltx25_attention_split needs; 0 for sizes it refuses and where
+ * it splits nothing. Not monotone in the sizes. */
+size_t ltx25_attention_workspace(const ltx25_attn* a, int batch, int total_q, int total_k);
+
 /* A cache of keys and values in pages of page_tokens tokens, held as signed
  * bytes with one scale for each page and kv head: value = code * scale.
  *   k        int8 [pages][kv_heads][page_tokens][head_dim]

@@ -191,3 +191,30 @@ def test_workspace_of_each_size_is_asked_for(pkg, lib):
     assert one == 0 and few > 0
     c, a = _cache(pkg, kv_heads=8), _attn(pkg, kv_heads=8)
     assert _cached(pkg, lib, a, c, batch=60, max_len=5120, ws_bytes=few - 1) == pkg.E_INVAL
+
+
+def _split(pkg, lib, a=None, ws=FAKE, ws_bytes=1 << 30, total_q=4, total_k=4000, **kw):
+    a = a or _attn(pkg)
+    p = dict(q=FAKE, k=FAKE, v=FAKE, out=FAKE, batch=1)
+    p.update(kw)
+    return lib.ltx25_attention_split(None, ctypes.byref(a), p["q"], p["k"], p["v"], p["out"], None,
+                                     FAKE, FAKE, p["batch"], total_q, total_k, ws, ws_bytes)
+
+
+def test_split_refusals_and_workspace(pkg, lib):
+    need = pkg.attention_workspace(8, 2, 128, 1, 4, 4000)
+    assert need > 0 and need % (4 * 8 * (128 + 2) * 4) == 0
+    assert _split(pkg, lib, ws=None) == pkg.E_INVAL
+    assert _split(pkg, lib, ws=FAKE + 8) == pkg.E_INVAL
+    assert _split(pkg, lib, ws_bytes=need - 1) == pkg.E_INVAL
+    assert str(need) in pkg.last_error()
+    assert _split(pkg, lib, _attn(pkg, heads=7)) == pkg.E_INVAL
+    assert _split(pkg, lib, q=None) == pkg.E_INVAL
+    assert _split(pkg, lib, total_k=(1 << 27) + 1) == pkg.E_INVAL
+    assert _split(pkg, lib, total_q=0, ws=None) == pkg.OK
+    assert _split(pkg, lib, batch=0, ws=None) == pkg.OK
+    # many rows, short keys, no keys, sizes that are refused: nothing to split
+    for sizes in ((32, 8, 128, 1, 16384, 16384), (8, 2, 128, 1, 4, 200), (8, 2, 128, 1, 4, 0),
+                  (7, 2, 128, 1, 4, 4000), (8, 2, 96, 1, 4, 4000), (8, 2, 128, 0, 4, 4000),
+                  (8, 0, 128, 1, 4, 4000), (8, 2, 128, 1, 4, (1 << 27) + 1)):
+        assert pkg.attention_workspace(*sizes) == 0

@@ -349,3 +349,107 @@ def test_attention_nan_everywhere_ends_soon(pkg, dev):
         times.append(a.elapsed_time(b))
         assert bool(torch.isnan(out).all()) == (bad is not None)
     assert max(times[1:]) < 20 * times[0] + 1.0, times
+
+
+def _parts(pkg, heads, kv_heads, dim, batch, nq, nk):
+    return pkg.attention_workspace(heads, kv_heads, dim, batch, nq, nk) // max(
+        nq * heads * (dim + 2) * 4, 1)
+
+
+SPLIT = [  # queries, keys, heads, kv heads, width, causal
+    ([1], [1100], 1, 1, 128, True),
+    ([5], [4000], 8, 2, 128, True),
+    ([5], [4001], 8, 2, 64, True),
+    ([70], [3000], 4, 4, 128, False),
+    ([70], [3000], 4, 4, 64, False),
+    ([1300], [1300], 1, 1, 128, True),                     # parts past the first rows' last key
+    ([1300], [1300], 2, 1, 64, True),
+    ([3, 1, 9], [5000, 2, 4000], 4, 1, 128, True),         # a sequence with fewer tiles than parts
+    ([40, 0, 7], [3000, 100, 1500], 6, 2, 64, True),
+    ([2, 6], [0, 3000], 4, 2, 128, False),                 # queries without keys
+    ([20, 5], [10, 3000], 4, 2, 128, True),                # queries that see nothing
+]
+
+
+@pytest.mark.parametrize("lens_q,lens_k,heads,kv_heads,dim,causal", SPLIT)
+def test_attention_of_few_rows_in_parts(pkg, dev, lens_q, lens_k, heads, kv_heads, dim, causal):
+    nq, nk, batch = sum(lens_q), sum(lens_k), len(lens_q)
+    q, k, v = _randn(45, nq, heads, dim), _randn(46, nk, kv_heads, dim), _randn(47, nk, kv_heads, dim)
+    need = pkg.attention_workspace(heads, kv_heads, dim, batch, nq, nk)
+    assert _parts(pkg, heads, kv_heads, dim, batch, nq, nk) >= 2
+    # a byte pattern that is a NaN in every word, and a margin that has to stay
+    ws = torch.full((need + 256,), 0xff, dtype=torch.uint8, device="cuda")
+    out = torch.full((nq + 3, heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    z = torch.full((nq, heads), float("nan"), device="cuda")
+    say(f"attention in parts {lens_q} {lens_k} heads {heads}/{kv_heads} x {dim} causal {causal}")
+    pkg.attention(q, k, v, out[:nq], _cu(lens_q), _cu(lens_k), causal=causal, lse=z,
+                  workspace=ws[:need])
+    torch.cuda.synchronize()
+    assert bool((ws[need:] == 0xff).all()) and bool((out[nq:] == 7.0).all())
+    _verify(q, k, v, out[:nq], z, lens_q, lens_k, causal)
+    # the binding's own workspace, no statistics, and again: the same bits
+    for _ in range(2):
+        again = torch.full_like(out[:nq], float("nan"))
+        pkg.attention(q, k, v, again, _cu(lens_q), _cu(lens_k), causal=causal)
+        torch.cuda.synchronize()
+        assert torch.equal(again.view(torch.int16), out[:nq].view(torch.int16))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_in_parts_unseen_and_seen_nan(pkg, dev, dim):
+    """As without parts: what a row does not see has no influence, what it sees shows."""
+    n = 1400
+    q, k, v = _randn(48, n, 2, dim), _randn(49, n, 1, dim), _randn(50, n, 1, dim)
+    assert _parts(pkg, 2, 1, dim, 1, n, n) >= 2
+    clean, _ = _run(pkg, q, k, v, [n], [n], True)
+    nan = float("nan")
+    v[700, 0, 3], v[1300, 0, 5], k[1390], v[1395, 0, 9] = nan, float("inf"), nan, nan
+    say(f"attention in parts, NaN x {dim}")
+    out, z = _run(pkg, q, k, v, [n], [n], True)
+    assert bool(torch.isfinite(out[:700]).all()) and bool(torch.isfinite(z[:1390]).all())
+    assert bool(torch.isnan(out[700:, :, 3]).all())
+    assert bool(torch.isfinite(out[700:1300, :, 4:]).all())
+    assert not bool(torch.isfinite(out[1300:, :, 5]).any())
+    assert bool(torch.isnan(out[1390:]).all()) and bool(torch.isnan(z[1390:]).all())
+    rest = torch.ones(dim, dtype=torch.bool)
+    rest[[3, 5]] = False
+    # a NaN logit makes all rows of its wave take their maxima: beside it other bits
+    assert torch.equal(out[:1344][..., rest].view(torch.int16), clean[:1344][..., rest].view(torch.int16))
+    for i in (680, 699, 1350, 1380, 1389):
+        want = attn_ref.attend(q[i:i + 1], k[:i + 1], v[:i + 1], dim ** -0.5, False)
+        err = (out[i:i + 1].cpu().double() - want[0]).abs() - attn_ref.OUT_BOUND * want[2]
+        assert float((err if i < 700 else err[..., rest]).max()) <= 0, f"row {i}"
+
+
+def test_attention_in_parts_rows_of_no_sequence_stay(pkg, dev):
+    """Tokens before, between and after the sequences that cu_q names keep what they hold."""
+    q, k, v = _randn(51, 20, 4, 128), _randn(52, 4000, 2, 128), _randn(53, 4000, 2, 128)
+    out = torch.full_like(q, 7.0)
+    z = torch.full((20, 4), 7.0, device="cuda")
+    cu_q = torch.tensor([4, 12], dtype=torch.int32, device="cuda")
+    cu_k = torch.tensor([100, 3900], dtype=torch.int32, device="cuda")
+    say("attention in parts, tokens of no sequence")
+    pkg.attention(q, k, v, out, cu_q, cu_k, causal=True, lse=z)
+    torch.cuda.synchronize()
+    for t in (out, z):
+        assert bool((t[:4] == 7.0).all()) and bool((t[12:] == 7.0).all())
+    want = attn_ref.attend(q[4:12], k[100:3900], v[100:3900], 128 ** -0.5, True)
+    attn_ref.check(out[4:12], z[4:12], want)
+
+
+def test_attention_in_parts_in_a_graph(pkg, dev):
+    q, k, v = _randn(54, 9, 8, 128), _randn(55, 6000, 2, 128), _randn(56, 6000, 2, 128)
+    want, _ = _run(pkg, q, k, v, [9], [6000], True, lse=False)
+    out, cu_q, cu_k = torch.empty_like(q), _cu([9]), _cu([6000])
+    ws = torch.zeros(pkg.attention_workspace(8, 2, 128, 1, 9, 6000), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.attention(q, k, v, out, cu_q, cu_k, causal=True, workspace=ws)
+    for rep in range(3):
+        out.fill_(float("nan"))
+        ws.fill_(0xff)
+        torch.cuda.synchronize()
+        say(f"attention in parts, replay {rep}")
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16))

@@ -175,6 +175,9 @@ SIGNATURES = {
     "ltx25_pack_quantizable": (_i, [ctypes.c_char_p, ctypes.c_char_p, _i]),
     "ltx25_attention": (_i, [_vp, ctypes.POINTER(AttnC), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i,
                              _i]),
+    "ltx25_attention_split": (_i, [_vp, ctypes.POINTER(AttnC), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i,
+                                   _i, _i, _vp, _sz]),
+    "ltx25_attention_workspace": (_sz, [ctypes.POINTER(AttnC), _i, _i, _i]),
     "ltx25_kv_append": (_i, [_vp, ctypes.POINTER(KVCacheC), _vp, _i, _vp, _vp, ctypes.c_int64,
                              ctypes.c_int64, _vp, _vp, _i, _i]),
     "ltx25_kv_read": (_i, [_vp, ctypes.POINTER(KVCacheC), _vp, _i, _vp, _vp, ctypes.c_int64,
@@ -374,10 +377,13 @@ def _lse(t, tokens: int, heads: int) -> None:
 
 
 def attention(q, k, v, out, cu_q=None, cu_k=None, *, causal: bool, scale: float = 0.0, lse=None,
-              stream=None) -> None:
+              workspace=None, stream=None) -> None:
     """Attention of packed sequences (ltx25_attention): q, out [total_q][heads][head_dim], k, v
     [total_k][kv_heads][head_dim] bf16, cu_q, cu_k int32 [batch + 1] (both None: one sequence),
-    lse float32 [total_q][heads] or None. scale 0 is 1 / sqrt(head_dim)."""
+    lse float32 [total_q][heads] or None. scale 0 is 1 / sqrt(head_dim).
+
+    Few rows over many keys are split (ltx25_attention_split) in `workspace`, a uint8 tensor of
+    attention_workspace() bytes; on torch's current stream one is allocated where none is given."""
     if _torch is None:
         _import_torch()
     q_shape, k_shape = q.shape, k.shape
@@ -399,8 +405,27 @@ def attention(q, k, v, out, cu_q=None, cu_k=None, *, causal: bool, scale: float 
     if lse is not None:
         _lse(lse, nq, heads)
     a = AttnC(heads, kv_heads, dim, 1 if causal else 0, scale, qs, ks, vs, os_)
+    # only such sizes can have parts: 8 tiles of 64 keys, 256 workgroups of 128 rows at most
+    if nk > 448 * batch and nq * heads <= 65536 and (workspace is not None or stream is None):
+        need = load().ltx25_attention_workspace(ctypes.byref(a), batch, nq, nk)
+        if need > 0:
+            if workspace is None:
+                workspace = _torch.empty(need, dtype=_torch.uint8, device=q.device)
+            check(load().ltx25_attention_split(
+                _stream(stream), ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                out.data_ptr(), _ptr(lse), pq, pk, batch, nq, nk, workspace.data_ptr(),
+                workspace.numel() * workspace.element_size()))
+            return
     check(load().ltx25_attention(_stream(stream), ctypes.byref(a), q.data_ptr(), k.data_ptr(),
                                  v.data_ptr(), out.data_ptr(), _ptr(lse), pq, pk, batch, nq, nk))
+
+
+def attention_workspace(heads: int, kv_heads: int, head_dim: int, batch: int, total_q: int,
+                        total_k: int) -> int:
+    """Bytes of workspace in which attention splits the keys of few rows
+    (ltx25_attention_workspace); 0 where it does not."""
+    a = AttnC(heads, kv_heads, head_dim, 0, 0.0, 0, 0, 0, 0)
+    return int(load().ltx25_attention_workspace(ctypes.byref(a), batch, total_q, total_k))
 
 
 class KVCache:

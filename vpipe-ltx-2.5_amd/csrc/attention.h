@@ -112,6 +112,61 @@ __device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& 
   return false;
 }
 
+// One row's parts joined by a wave: `used` means of D channels at `means`, a maximum
+// (log2) and a sum each at `ml`. D / 4 lanes take 4 channels each of one part, so that
+// 64 / (D / 4) parts are read side by side, and four of those in flight; always added in
+// the same order. No parts at all, or none with a sum: zeros.
+template <int D>
+__device__ __forceinline__ void join_parts(const float* means, const float2* ml, int used,
+                                           uint16_t* out, float* lse)
+{
+  constexpr int kLanes = D / 4, kSide = 64 / kLanes;
+  const int lane = threadIdx.x & 63;
+  const int part = lane / kLanes, d = (lane % kLanes) * 4;
+  f32x4 x[4];
+  float2 st[4];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int s = max(min(s0 + j * kSide, used - 1), 0);
+      x[j] = *(const f32x4*)(means + (long)s * D + d);
+      st[j] = ml[s];
+    }
+  };
+  fetch(part);   // beside the maxima
+  float top = -INFINITY;
+  for (int s = lane; s < used; s += 64) { top = fmaxf(top, ml[s].x); }
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) { top = fmaxf(top, __shfl_xor(top, i)); }
+  const float ms = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;
+  for (int s = lane; s < used; s += 64) { l = fmaf(__builtin_amdgcn_exp2f(ml[s].x - ms), ml[s].y, l); }
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) { l += __shfl_xor(l, i); }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = part; s0 < used; s0 += 4 * kSide) {
+    if (s0 != part) { fetch(s0); }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float w =
+          s0 + j * kSide < used ? __builtin_amdgcn_exp2f(st[j].x - ms) * st[j].y * inv : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { acc[i] = fmaf(w, x[j][i], acc[i]); }
+    }
+  }
+#pragma unroll
+  for (int i = kLanes; i < 64; i *= 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { acc[j] += __shfl_xor(acc[j], i); }
+  }
+  if (part != 0) { return; }
+  *(uint2*)(out + d) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+  if (lse != nullptr && d == 0) {
+    *lse = l == 0.0f ? -INFINITY : (ms + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
 // ---- launchers --------------------------------------------------------------
 
 struct AttentionArgs {
@@ -127,7 +182,19 @@ struct AttentionArgs {
   int causal = 0;
   float scale = 0.0f;
   int batch = 0, total_q = 0, total_k = 0;
+  float* workspace = nullptr;   // null: every row in one part
 };
+// How a call's work is cut; a function of the sizes alone, so that the workspace can be
+// asked for ahead.
+struct PromptPlan {
+  bool turns = false;         // the form of 8 waves
+  int hp_log2 = 0, tb_log2 = 0;   // a workgroup's rows: 2^hp heads x 2^tb tokens
+  int head_groups = 1;
+  long units = 0;             // units of 2^tb tokens, at most
+  int splits = 1;             // parts of the keys, with a workspace
+  size_t workspace_bytes = 0;
+};
+PromptPlan plan_prompt(int heads, int kv_heads, int head_dim, int batch, int total_q, int total_k);
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream);
 
 struct CacheArgs {

@@ -43,6 +43,7 @@
 // on a card whose power allowed 3% less than another's.
 #include "attention.h"
 
+#include <algorithm>
 #include <climits>
 
 namespace ltx25 {
@@ -71,7 +72,9 @@ struct PromptParams {
   float c;                // scale log2(e): the softmax runs on powers of two
   int hp_log2, tb_log2;   // a workgroup's rows: 2^hp heads x 2^tb tokens
   int head_groups;
-};
+  int splits;             // parts of a row's keys
+  float* part;            // [total_q][heads][splits][D] means, then [total_q][heads][splits][2]
+};                        // maximum and sum
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c)
 {
@@ -237,11 +240,11 @@ struct Rows {
   bool valid;
   int limit;            // the last key that the lane's row sees
   int wave_lo, wave_hi; // and that the wave's first and last rows see
-  int n_tiles;
+  int first, end;       // the workgroup's tiles
 };
 
 template <int D, int NW>
-__device__ __forceinline__ bool find(const PromptParams& p, Rows<D, NW>& r)
+__device__ __forceinline__ bool find(const PromptParams& p, Rows<D, NW>& r, bool split)
 {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -279,7 +282,14 @@ __device__ __forceinline__ bool find(const PromptParams& p, Rows<D, NW>& r)
   r.wave_lo = lo < r.lq ? last_key(lo) : -1;
   r.wave_hi = lo < r.lq ? last_key(hi) : -1;
   const int last = last_key(min(r.tok0 + tb, r.lq) - 1);
-  r.n_tiles = last < 0 ? 0 : last / kBN + 1;
+  const int n_tiles = last < 0 ? 0 : last / kBN + 1;
+  r.first = 0;
+  r.end = n_tiles;
+  if (split) {
+    const int per = (n_tiles + p.splits - 1) / p.splits;
+    r.first = min((int)blockIdx.y * per, n_tiles);
+    r.end = min(r.first + per, n_tiles);
+  }
   return true;
 }
 
@@ -328,11 +338,11 @@ struct Loader {
       voff[i] = (int)(row * v_bytes + v_piece<D>(row, lane % kPieces) * 16);
     }
     lds0 = (uint32_t)(uintptr_t)(lds_word*)lds + wave * kLoads * 1024;
-    kp = p.k + (long)r.k0 * p.ks + r.g * D;
-    vp = p.v + (long)r.k0 * p.vs + r.g * D;
+    kp = p.k + (long)(r.k0 + r.first * kBN) * p.ks + r.g * D;
+    vp = p.v + (long)(r.k0 + r.first * kBN) * p.vs + r.g * D;
     k_step = (long)kBN * p.ks;
     v_step = (long)kBN * p.vs;
-    k_left = v_left = min(r.n_tiles * kBN, r.lk);
+    k_left = v_left = min(r.end * kBN, r.lk) - r.first * kBN;
   }
   // the next tile into stage `st`, of the stages of K, then those of V
   __device__ __forceinline__ void keys(int st)
@@ -406,8 +416,9 @@ __device__ __forceinline__ bool not_finite(uint4 v)
 }
 
 // The sums and statistics of the wave's rows out: through LDS, each wave its own
-// part of it, so that a store has whole rows' pieces side by side.
-template <int D, int NW>
+// part of it, so that a store has whole rows' pieces side by side. SPLIT: a part's means,
+// maximum (log2) and sum into the workspace instead.
+template <bool SPLIT, int D, int NW>
 __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>& r, uint8_t* lds,
                                        f32x16 (&o)[D / 32], float m, float l)
 {
@@ -440,11 +451,28 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
     const int at = i * kRowsPer + lane / kPieces, wr = wave * 32 + at;
     const int t = r.tok0 + (wr & (tb - 1)), c = lane % kPieces;
     const uint4 v = *(const uint4*)(mine + at * kRow + k_piece<D>(at, c) * 16);
-    if (t < r.lq) {
+    if (!SPLIT && t < r.lq) {
       *(uint4*)(p.out + (long)(r.q0 + t) * p.os + (r.head0 + (wr >> p.tb_log2)) * D + c * 8) = v;
     }
   }
-  if (p.lse != nullptr && half == 0 && r.valid) {
+  const long row = ((long)(r.q0 + r.tok) * p.heads + r.head) * p.splits + blockIdx.y;
+  if (SPLIT) {
+    if (r.valid) {
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          *(f32x4*)(p.part + row * D + d * 32 + i * 8 + half * 4) =
+              f32x4{o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv,
+                    o[d][4 * i + 3] * inv};
+        }
+      }
+      if (half == 0) {
+        *(float2*)(p.part + (long)p.total_q * p.heads * p.splits * D + row * 2) =
+            make_float2(l == 0.0f ? -INFINITY : m * p.c, l * 0x1p32f);
+      }
+    }
+  } else if (p.lse != nullptr && half == 0 && r.valid) {
     p.lse[(long)(r.q0 + r.tok) * p.heads + r.head] =
         l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l * 0x1p32f)) * 0.69314718055994531f;
   }
@@ -464,8 +492,8 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
     const int rtok = __shfl(r.tok, at), rhead = __shfl(r.head, at), rlimit = __shfl(r.limit, at);
     constexpr int kPer = D / 64;
     bool unseen = false;   // a value that is not finite among the masked tokens
-    const int end = min(r.n_tiles * kBN, r.lk);
-    for (int j = max(rlimit + 1, 0) + (lane >> 3); j < end; j += 8) {
+    const int begin = r.first * kBN, end = min(r.end * kBN, r.lk);
+    for (int j = max(rlimit + 1, begin) + (lane >> 3); j < end; j += 8) {
       const uint16_t* const vp = p.v + (long)(r.k0 + j) * p.vs + r.g * D + (lane & 7) * (D / 8);
 #pragma unroll
       for (int i = 0; i < D / 8; i += 8) { unseen = unseen || not_finite(*(const uint4*)(vp + i)); }
@@ -481,7 +509,7 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
     float qv[kPer], acc[kPer], rm = -INFINITY, rl = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) { qv[i] = bf16_to_f32(qp[i]); acc[i] = 0.0f; }
-    for (int j = 0; j <= rlimit; ++j) {
+    for (int j = begin; j < min(rlimit + 1, end); ++j) {
       bool open = false;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) { open = open || (nan_at[i] && acc[i] == acc[i]); }
@@ -507,16 +535,26 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
       }
     }
     uint16_t* const op = p.out + (long)(r.q0 + rtok) * p.os + rhead * D + d0;
+    float* const pp =
+        p.part + (((long)(r.q0 + rtok) * p.heads + rhead) * p.splits + blockIdx.y) * D + d0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (nan_at[i]) { op[i] = f32_to_bf16(acc[i]); }
+      if (nan_at[i]) {
+        if (SPLIT) {
+          pp[i] = acc[i];
+        } else {
+          op[i] = f32_to_bf16(acc[i]);
+        }
+      }
     }
   }
 }
 
 // 4 waves, two stages of tiles: the next tile lands while this one is multiplied.
-template <int D>
-__global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptParams p)
+// SPLIT: few rows see many keys; a workgroup takes part blockIdx.y of its rows' tiles, and
+// attention_parts_kernel joins the parts.
+template <int D, bool SPLIT>
+__global__ void __launch_bounds__(256, D == 64 && !SPLIT ? 4 : 2) attention_kernel(PromptParams p)
 {
   constexpr int kNW = 4;
   using Load = Loader<D, kNW>;
@@ -527,7 +565,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];   // K 0, 1, V 0, 1
 
   Rows<D, kNW> r;
-  if (!find(p, r)) { return; }
+  if (!find(p, r, SPLIT)) { return; }
   Load load(p, r, lds);
   bf16x8 qf[kKC];
   load_queries(p, r, qf);
@@ -548,10 +586,10 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
   // -infinity: nothing seen yet
   float m = -INFINITY, mc = -INFINITY, l = 0.0f;
 
-  for (int t = 0; t < r.n_tiles; ++t) {
+  for (int t = r.first; t < r.end; ++t) {
     // this tile is there, every wave's share of it, and no wave reads tile t - 1,
     // whose stage the next one takes
-    const int st = t & 1;
+    const int st = (t - r.first) & 1;
     landed<0>();
     load.keys(st ^ 1);
     load.values(2 + (st ^ 1));
@@ -592,8 +630,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
     // weights up to 2^12 are as exact as others in floating point.
     logits();
     float sum = 0.0f;
-    bool settle = t == 0;
-    if (t > 0) {
+    bool settle = t == r.first;
+    if (!settle) {
       sum = weigh();
       settle = any_lane(!(sum <= 0x1p-20f));
       if (settle) { logits(); }
@@ -624,7 +662,25 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) attention_kernel(PromptP
       for (int d = 0; d < kDT; ++d) { o[d] = mfma32(v_frag<D>(vt, c * kDT + d), pf, o[d]); }
     }
   }
-  finish(p, r, lds, o, m, l);
+  finish<SPLIT>(p, r, lds, o, m, l);
+}
+
+// The parts of attention_kernel's rows joined, a row a wave. The grid's x is the other
+// kernel's, so that rows of no sequence stay as they are.
+template <int D>
+__global__ void __launch_bounds__(256) attention_parts_kernel(PromptParams p)
+{
+  Rows<D, 4> r;
+  if (!find(p, r, false)) { return; }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int at = blockIdx.y * 4 + wave;
+  const int tok = r.tok0 + (at & ((1 << p.tb_log2) - 1)), head = r.head0 + (at >> p.tb_log2);
+  if (tok >= r.lq) { return; }
+  const long row = (long)(r.q0 + tok) * p.heads + head;
+  join_parts<D>(p.part + row * p.splits * D,
+                (const float2*)(p.part + (long)p.total_q * p.heads * p.splits * D) + row * p.splits,
+                p.splits, p.out + (long)(r.q0 + tok) * p.os + head * D,
+                p.lse == nullptr ? nullptr : p.lse + row);
 }
 
 // 8 waves in two groups of four, one wave of each on every SIMD, that take turns:
@@ -646,7 +702,7 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStages * kTile];
 
   Rows<D, kNW> r;
-  if (!find(p, r)) { return; }
+  if (!find(p, r, false)) { return; }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Load load(p, r, lds);
   bf16x8 qf[kKC];
@@ -755,11 +811,11 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
     l += sum;
   };
 
-  if (r.n_tiles > 0) {
+  if (r.end > 0) {
     landed<2 * Load::kLoads>();
     if (wave >= kNW / 2) { meet(); }
     int at = 0, prev = 2;   // stages of tile t, and of tile t - 1
-    for (int t = 0; t < r.n_tiles; ++t) {
+    for (int t = 0; t < r.end; ++t) {
       const uint8_t* const kt = lds + at * kTile;
       const uint8_t* const vt = lds + (kStages + prev) * kTile;
       const int next = at == 2 ? 0 : at + 1;
@@ -782,28 +838,70 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
       at = next;
     }
     if (wave < kNW / 2) { meet(); }
-    if ((r.n_tiles - 1) * kBN <= r.wave_hi) { second_product(lds + (kStages + prev) * kTile); }
+    if ((r.end - 1) * kBN <= r.wave_hi) { second_product(lds + (kStages + prev) * kTile); }
   }
 
-  finish(p, r, lds, o, m, l);
+  finish<false>(p, r, lds, o, m, l);
 }
 
-hipError_t run(const PromptParams& p, int head_dim, bool turns, int grid, hipStream_t st)
+template <int D>
+hipError_t run(const PromptParams& p, const PromptPlan& plan, int grid, hipStream_t st)
 {
-  if (turns) {
+  if (p.splits > 1) {
+    attention_kernel<D, true><<<dim3(grid, p.splits), 256, 0, st>>>(p);
+    attention_parts_kernel<D><<<dim3(grid, 32), 256, 0, st>>>(p);
+  } else if (D == 128 && plan.turns) {
     attention_turns_kernel<<<grid, 512, 0, st>>>(p);
-  } else if (head_dim == 128) {
-    attention_kernel<128><<<grid, 256, 0, st>>>(p);
   } else {
-    attention_kernel<64><<<grid, 256, 0, st>>>(p);
+    attention_kernel<D, false><<<grid, 256, 0, st>>>(p);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
+PromptPlan plan_prompt(int heads, int kv_heads, int head_dim, int batch, int total_q, int total_k)
+{
+  PromptPlan r;
+  const int share = heads / kv_heads;
+  // The form that takes turns, from two rounds of its workgroups on and for sequences
+  // that are long on average (the figures at the top of this file).
+  r.turns = head_dim == 128 && (long)total_q * heads >= 2L * 256 * 256 && total_k / batch >= 2048;
+  // rows: heads of one kv head side by side first, so that a workgroup spans few
+  // tokens and little of its last tile is masked, 32 tokens of a head at least
+  const int rows_log2 = r.turns ? 8 : 7;
+  while (share % (2 << r.hp_log2) == 0 && r.hp_log2 < rows_log2 - 5) { ++r.hp_log2; }
+  r.tb_log2 = rows_log2 - r.hp_log2;
+  r.head_groups = heads >> r.hp_log2;
+  r.units = (long)(total_q >> r.tb_log2) + batch;
+  // Parts of the keys, for few rows: as many as make the call's time least. A tile takes
+  // a workgroup 1.1 us (0.76 at head width 64), half as long again where two share a CU;
+  // the join 6 us, a tenth more for each part, and the means' bytes at 4 TB/s. Measured, in
+  // one part and in those chosen: 5 queries of 32 heads over 4000 keys 71 and 14 us, over
+  // 16000 269 and 22; 500 over 16000 277 and 143; 2048 causal tokens of 4 heads 40 and 26.
+  // Where it says one: 1200 causal tokens of 16 heads 26, 31 in two.
+  const long grid = r.units * r.head_groups, tiles = (total_k / batch + kBN - 1) / kBN;
+  const float rows = (float)total_q * heads, tile_us = head_dim == 128 ? 1.1f : 0.76f;
+  const long most = std::min({512 / std::max(grid, 1L), tiles / 2, 64L});
+  float best = tiles * tile_us;
+  for (int n = 2; n <= most; ++n) {
+    const float us = tiles * tile_us / n * (grid * n > 256 ? 1.55f : 1.0f) + 6.0f + 0.1f * n +
+                     rows * n * (head_dim + 2) * 8 / 4e6f;
+    if (us < best) {
+      best = us;
+      r.splits = n;
+    }
+  }
+  if (r.splits > 1) {
+    r.workspace_bytes = (size_t)total_q * heads * r.splits * (head_dim + 2) * sizeof(float);
+  }
+  return r;
+}
+
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream)
 {
+  const PromptPlan plan =
+      plan_prompt(a.heads, a.kv_heads, a.head_dim, a.batch, a.total_q, a.total_k);
   PromptParams p;
   p.q = a.q;
   p.k = a.k;
@@ -823,21 +921,15 @@ hipError_t launch_attention(const AttentionArgs& a, hipStream_t stream)
   p.total_k = a.total_k;
   p.causal = a.causal;
   p.c = a.scale * 1.4426950408889634f;
-  // The form that takes turns, from two rounds of its workgroups on and for sequences
-  // that are long on average (the figures at the top of this file).
-  const bool turns = a.head_dim == 128 && (long)a.total_q * a.heads >= 2L * 256 * 256 &&
-                     a.total_k / a.batch >= 2048;
-  // rows: heads of one kv head side by side first, so that a workgroup spans few
-  // tokens and little of its last tile is masked, 32 tokens of a head at least
-  const int rows_log2 = turns ? 8 : 7;
-  p.hp_log2 = 0;
-  while (p.share % (2 << p.hp_log2) == 0 && p.hp_log2 < rows_log2 - 5) { ++p.hp_log2; }
-  p.tb_log2 = rows_log2 - p.hp_log2;
-  p.head_groups = a.heads >> p.hp_log2;
-  const long units = (long)(a.total_q >> p.tb_log2) + a.batch;
-  const long grid = units * p.head_groups;
+  p.hp_log2 = plan.hp_log2;
+  p.tb_log2 = plan.tb_log2;
+  p.head_groups = plan.head_groups;
+  p.splits = a.workspace != nullptr ? plan.splits : 1;
+  p.part = a.workspace;
+  const long grid = plan.units * plan.head_groups;
   if (grid > INT_MAX) { return hipErrorInvalidConfiguration; }
-  return run(p, a.head_dim, turns, (int)grid, stream);
+  return a.head_dim == 128 ? run<128>(p, plan, (int)grid, stream)
+                           : run<64>(p, plan, (int)grid, stream);
 }
 
 }  // namespace ltx25

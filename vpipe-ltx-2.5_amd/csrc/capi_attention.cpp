@@ -120,6 +120,16 @@ int check_tokens(const char* name, long tokens, int most)
   return LTX25_OK;
 }
 
+int check_workspace(const void* workspace, size_t bytes, size_t need)
+{
+  const int rc = check_pointer("workspace", workspace, 16);
+  if (rc == LTX25_OK && bytes < need) {
+    return set_error(LTX25_E_INVAL, "the workspace has %zu bytes; this call needs %zu", bytes,
+                     need);
+  }
+  return rc;
+}
+
 // What append and read share.
 int check_move(const ltx25_kv_cache* cache, const int* table, int table_stride, const void* k,
                const void* v, int64_t k_stride, int64_t v_stride, const int* cu, const int* start,
@@ -144,11 +154,12 @@ int check_move(const ltx25_kv_cache* cache, const int* table, int table_stride, 
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-int ltx25_attention(void* stream, const ltx25_attn* a, const void* q, const void* k, const void* v,
-                    void* out, float* lse, const int* cu_q, const int* cu_k, int batch,
-                    int total_q, int total_k)
+// `split`: the workspace is asked for and used where the plan has parts.
+int attention(void* stream, const ltx25_attn* a, const void* q, const void* k, const void* v,
+              void* out, float* lse, const int* cu_q, const int* cu_k, int batch, int total_q,
+              int total_k, bool split, void* workspace, size_t workspace_bytes)
 {
   float scale = 0.0f;
   int rc = check_attn(a, &scale);
@@ -174,8 +185,13 @@ int ltx25_attention(void* stream, const ltx25_attn* a, const void* q, const void
   if (!aligned(lse, 4) || !aligned(cu_q, 4) || !aligned(cu_k, 4)) {
     return set_error(LTX25_E_INVAL, "lse, cu_q or cu_k is not 4-byte aligned");
   }
+  const size_t need = split ? ltx25_attention_workspace(a, batch, total_q, total_k) : 0;
+  if (need > 0 && (rc = check_workspace(workspace, workspace_bytes, need)) != LTX25_OK) {
+    return rc;
+  }
   if ((rc = ltx25::check_device()) != LTX25_OK) { return rc; }
   ltx25::AttentionArgs p;
+  p.workspace = need > 0 ? (float*)workspace : nullptr;
   p.q = (const uint16_t*)q;
   p.k = (const uint16_t*)k;
   p.v = (const uint16_t*)v;
@@ -197,6 +213,38 @@ int ltx25_attention(void* stream, const ltx25_attn* a, const void* q, const void
   p.total_k = total_k;
   const hipError_t e = ltx25::launch_attention(p, (hipStream_t)stream);
   return e == hipSuccess ? LTX25_OK : hip_error(e, "attention launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int ltx25_attention(void* stream, const ltx25_attn* a, const void* q, const void* k, const void* v,
+                    void* out, float* lse, const int* cu_q, const int* cu_k, int batch,
+                    int total_q, int total_k)
+{
+  return attention(stream, a, q, k, v, out, lse, cu_q, cu_k, batch, total_q, total_k, false,
+                   nullptr, 0);
+}
+
+size_t ltx25_attention_workspace(const ltx25_attn* a, int batch, int total_q, int total_k)
+{
+  if (a == nullptr || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads != 0 ||
+      (a->head_dim != 64 && a->head_dim != 128) || batch <= 0 || total_q <= 0 || total_k <= 0 ||
+      total_q > kPackedMax || total_k > kPackedMax) {
+    return 0;
+  }
+  return ltx25::plan_prompt(a->heads, a->kv_heads, a->head_dim, batch, total_q, total_k)
+      .workspace_bytes;
+}
+
+int ltx25_attention_split(void* stream, const ltx25_attn* a, const void* q, const void* k,
+                          const void* v, void* out, float* lse, const int* cu_q, const int* cu_k,
+                          int batch, int total_q, int total_k, void* workspace,
+                          size_t workspace_bytes)
+{
+  return attention(stream, a, q, k, v, out, lse, cu_q, cu_k, batch, total_q, total_k, true,
+                   workspace, workspace_bytes);
 }
 
 int ltx25_kv_append(void* stream, const ltx25_kv_cache* cache, const int* table, int table_stride,
@@ -271,12 +319,8 @@ int ltx25_attention_cached(void* stream, const ltx25_attn* a, const ltx25_kv_cac
   if (!aligned(lse, 4)) { return set_error(LTX25_E_INVAL, "lse is not 4-byte aligned"); }
   const size_t need = ltx25_attention_cached_workspace(batch, q_len, a->heads, a->kv_heads,
                                                        a->head_dim, max_len);
-  if (need > 0) {
-    if ((rc = check_pointer("workspace", workspace, 16)) != LTX25_OK) { return rc; }
-    if (workspace_bytes < need) {
-      return set_error(LTX25_E_INVAL, "the workspace has %zu bytes; this call needs %zu",
-                       workspace_bytes, need);
-    }
+  if (need > 0 && (rc = check_workspace(workspace, workspace_bytes, need)) != LTX25_OK) {
+    return rc;
   }
   if ((rc = ltx25::check_device()) != LTX25_OK) { return rc; }
   p.lens = lens;

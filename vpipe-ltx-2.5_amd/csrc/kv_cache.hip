@@ -793,68 +793,21 @@ attention_cached_kernel(CachedParams p)
   }
 }
 
-// The splits of a row joined; a wave for each row. D / 4 lanes take 4 channels
-// each of one split, so that 64 / (D / 4) splits are read side by side, and four
-// of those in flight; always added in the same order. Bound by the latency of its
-// loads, one after another: 4.8 us.
+// The parts of a row joined; a wave for each row. Bound by the latency of its loads,
+// one after another: 4.8 us.
 template <int D>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(CachedParams p)
 {
-  constexpr int kLanes = D / 4, kSide = 64 / kLanes;
-  const int lane = threadIdx.x & 63;
-  const int part = lane / kLanes, d = (lane % kLanes) * 4;
   const long rows = (long)p.batch * p.q_len * p.heads;
   const long at = (long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (at >= rows) { return; }
   const long token = at / p.heads;
   const int head = (int)(at % p.heads);
   const int len = visible_len(p, (int)(token / p.q_len));
-  const int used = min((len + p.chunk - 1) / p.chunk, p.splits);
-  const float2* const ml = (const float2*)(p.part + rows * p.splits * D) + at * p.splits;
-  const float* const op = p.part + at * p.splits * D + d;
-  f32x4 x[4];
-  float2 st[4];
-  auto fetch = [&](int s0) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int s = max(min(s0 + j * kSide, used - 1), 0);
-      x[j] = *(const f32x4*)(op + (long)s * D);
-      st[j] = ml[s];
-    }
-  };
-  fetch(part);   // beside the maxima
-  float top = -INFINITY;
-  for (int s = lane; s < used; s += 64) { top = fmaxf(top, ml[s].x); }
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) { top = fmaxf(top, __shfl_xor(top, i)); }
-  const float ms = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f;
-  for (int s = lane; s < used; s += 64) { l = fmaf(__builtin_amdgcn_exp2f(ml[s].x - ms), ml[s].y, l); }
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) { l += __shfl_xor(l, i); }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = part; s0 < used; s0 += 4 * kSide) {
-    if (s0 != part) { fetch(s0); }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float w =
-          s0 + j * kSide < used ? __builtin_amdgcn_exp2f(st[j].x - ms) * st[j].y * inv : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { acc[i] = fmaf(w, x[j][i], acc[i]); }
-    }
-  }
-#pragma unroll
-  for (int i = kLanes; i < 64; i *= 2) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { acc[j] += __shfl_xor(acc[j], i); }
-  }
-  if (part != 0) { return; }
-  *(uint2*)(p.out + token * p.os + (long)head * D + d) =
-      make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
-  if (p.lse != nullptr && d == 0) {
-    p.lse[at] = l == 0.0f ? -INFINITY : (ms + log2f(l)) * 0.69314718055994531f;
-  }
+  join_parts<D>(p.part + at * p.splits * D,
+                (const float2*)(p.part + rows * p.splits * D) + at * p.splits,
+                min((len + p.chunk - 1) / p.chunk, p.splits), p.out + token * p.os + (long)head * D,
+                p.lse == nullptr ? nullptr : p.lse + at);
 }
 
 CacheView view_of(const CacheArgs& c)

@@ -137,6 +137,21 @@ public:
     note(ltx25_attention(enc, &a, q, k, v, out, lse, cu_q, cu_k, batch, total_q, total_k));
   }
 
+  // The same with the keys of few rows split over more workgroups, in a workspace of
+  // attention_workspace bytes (0: nothing to split, none needed).
+  void attention_split(hipStream_t enc, const ltx25_attn& a, const void* q, const void* k,
+                       const void* v, void* out, float* lse, const int* cu_q, const int* cu_k,
+                       int batch, int total_q, int total_k, void* workspace,
+                       size_t workspace_bytes) const
+  {
+    note(ltx25_attention_split(enc, &a, q, k, v, out, lse, cu_q, cu_k, batch, total_q, total_k,
+                               workspace, workspace_bytes));
+  }
+  static size_t attention_workspace(const ltx25_attn& a, int batch, int total_q, int total_k)
+  {
+    return ltx25_attention_workspace(&a, batch, total_q, total_k);
+  }
+
   // The 8-bit cache: new tokens in, tokens out as bf16, attention over it. k and
   // v lie at a.k_stride and a.v_stride.
   void kv_append(hipStream_t enc, const ltx25_attn& a, const ltx25_kv_cache& cache,

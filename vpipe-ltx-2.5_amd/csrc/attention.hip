@@ -19,12 +19,12 @@
 //
 // What bounds it: a tile takes a wave 32 products of 32 cycles on the matrix
 // cores and about 120 operations for the weights, 32 of them exponentials at 9
-// cycles and the rest at 4 to 5 each: as much time as the products, which two waves a
-// SIMD overlap only in part (matrix cores busy 66% of the cycles on long prompts).
-// At head width 64 the weights' operations alone do (80% of the cycles, and the matrix
-// cores 48%, before the maximum went). The instructions' energy counts as well: 17% fewer cycles (attention_turns_kernel
-// against attention_kernel) came at 10% less clock. The weights are rounded to bf16
-// as the values are; the sums and statistics are f32.
+// cycles and the rest at 4 to 5 each. Two waves a SIMD overlap them only in part, since
+// a product also takes about 16 cycles of the other wave's issue: of long prompts'
+// cycles the matrix cores are busy in 66%, at head width 64 in 48%, where the weights'
+// operations take 80%. The instructions' energy counts as well: 17% fewer cycles
+// (attention_turns_kernel against attention_kernel) came at 10% less clock. The weights
+// are rounded to bf16 as the values are; the sums and statistics are f32.
 // Two forms:
 //   attention_kernel: 4 waves, 128 rows; two to four such workgroups share a CU
 //   and one computes while another waits.

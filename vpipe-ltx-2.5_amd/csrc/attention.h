@@ -115,7 +115,9 @@ __device__ __forceinline__ bool find_unit(int u, int batch, Count&& count, int& 
 // One row's parts joined by a wave: `used` means of D channels at `means`, a maximum
 // (log2) and a sum each at `ml`. D / 4 lanes take 4 channels each of one part, so that
 // 64 / (D / 4) parts are read side by side, and four of those in flight; always added in
-// the same order. No parts at all, or none with a sum: zeros.
+// the same order. No parts at all, or none with a sum: zeros. A mean that is not finite
+// comes from a token that the row sees, whose weight is positive however small: it counts
+// whole, where a weight below f32's range would make a NaN of an infinity.
 template <int D>
 __device__ __forceinline__ void join_parts(const float* means, const float2* ml, int used,
                                            uint16_t* out, float* lse)
@@ -149,10 +151,12 @@ __device__ __forceinline__ void join_parts(const float* means, const float2* ml,
     if (s0 != part) { fetch(s0); }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float w =
-          s0 + j * kSide < used ? __builtin_amdgcn_exp2f(st[j].x - ms) * st[j].y * inv : 0.0f;
+      if (s0 + j * kSide >= used) { break; }   // x is the last part's again
+      const float w = __builtin_amdgcn_exp2f(st[j].x - ms) * st[j].y * inv;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { acc[i] = fmaf(w, x[j][i], acc[i]); }
+      for (int i = 0; i < 4; ++i) {
+        acc[i] = fmaf(fabsf(x[j][i]) < INFINITY ? w : 1.0f, x[j][i], acc[i]);
+      }
     }
   }
 #pragma unroll

@@ -484,8 +484,8 @@ __device__ __forceinline__ int visible_len(const CachedParams& p, int b)
 // instructions through registers alone.
 //
 // The second product's weights w = exp(s - m) times the page's scale lie in f16
-// under a running power of two of their own, 2^mw: the largest has 2^13 to 2^15, so
-// that weights 2^27 times smaller keep all their 11 bits, and the output's own
+// under a running power of two of their own, 2^mw: the largest has 2^12 to 2^15, so
+// that weights 2^26 times smaller keep all their 11 bits, and the output's own
 // rounding is all of its error (0.00166 of its norm; with weights in bf16 0.0024,
 // 0.0030 where few keys count). The sums stay as they are while no row's largest
 // weight grows four times over, which pays for the second maximum: 64 sequences of
@@ -507,7 +507,9 @@ attention_cached_kernel(CachedParams p)
   constexpr int kL = D / 64;    // 16-byte loads of a token's key for each lane
   constexpr int kDT = D / 16;   // 16-channel tiles
   constexpr int kRows = 16 * RT;
-  constexpr float kRoom = 13.0f, kLag = 2.0f;   // of w, log2
+  // of w, log2; a lane's weights count as 2^kFaint times the row's largest one or more where
+  // mw is chosen, which keeps 2^-mw times any seen scale inside f32
+  constexpr float kRoom = 13.0f, kLag = 2.0f, kFaint = -110.0f;
   __shared__ __attribute__((aligned(16))) float join[NW][16][D + 4];
   __shared__ float2 stat[NW][16];
 
@@ -644,13 +646,16 @@ attention_cached_kernel(CachedParams p)
         id_v1 = page_of(t2 + 16 * kg);
       }
     }
-    const float lsv = __builtin_amdgcn_logf(fabsf(sv));
+    // the scale in two parts, since 1 / sv may be past f32's end: a logarithm and a reciprocal
+    // lose scales below 2^-113, which appending makes of values below 2^-106
+    const float sv_m = __builtin_amdgcn_frexp_mantf(sv);
+    const float sv_e = (float)__builtin_amdgcn_frexp_expf(sv);
     f16x8 pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int lim = held ? min(limit[rt], end - 1) : -1;
-      // the scale of a page without a token that the row sees may be anything
-      const float sv_seen = tv <= lim ? sv : 0.0f;
+      // the scale of a page without a token that the row sees may be anything: not counted
+      const bool seen = tv <= lim;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -676,7 +681,8 @@ attention_cached_kernel(CachedParams p)
       const float lag = m[rt] - ms, keep = __builtin_amdgcn_exp2f(lag);
       m[rt] = m_new;
       // the row's largest w: the 16 tokens of a lane are of one page
-      const float top_w = xor32_max(xor16_max(top - ms + lsv)) - kRoom;
+      const float lane_w = seen && sv != 0.0f ? fmaxf(top - ms, kFaint) + sv_e : -INFINITY;
+      const float top_w = xor32_max(xor16_max(lane_w)) - kRoom;
       mw[rt] += lag;
       if (any_lane(top_w > mw[rt] + kLag)) {
         const float mw_new = fmaxf(mw[rt], top_w);
@@ -688,7 +694,8 @@ attention_cached_kernel(CachedParams p)
           for (int i = 0; i < 4; ++i) { o[rt][d][i] *= keep_o; }
         }
       }
-      const float f = sv_seen * __builtin_amdgcn_exp2f(fminf(-mw[rt], 127.0f));
+      const float f =
+          (seen ? sv_m : 0.0f) * __builtin_amdgcn_exp2f(fminf(sv_e - mw[rt], 127.0f));
       float sum = 0.0f;
       float w[16];
 #pragma unroll
@@ -726,12 +733,14 @@ attention_cached_kernel(CachedParams p)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] = xor32_sum(xor16_sum(l[rt]));
-    // means from here on: they stay in range where sums of large values would not
-    const float f = l[rt] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mw[rt]) / l[rt];
+    // means from here on: they stay in range where sums of large values would not. 2^mw in
+    // two steps: it may be below f32's range where the mean is not
+    const float half = __builtin_amdgcn_exp2f(0.5f * mw[rt]);
+    const float f = l[rt] == 0.0f ? 0.0f : half / l[rt];
 #pragma unroll
     for (int d = 0; d < kDT; ++d) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { o[rt][d][i] *= f; }
+      for (int i = 0; i < 4; ++i) { o[rt][d][i] = o[rt][d][i] * half * f; }
     }
   }
 

@@ -80,3 +80,47 @@ def test_seen_infinity_in_a_part_that_hardly_counts(pkg, dev, dim):
     out, _ = _attend(pkg, q, k, v, False, True, 1.0)
     assert bool((out[..., 5] == INF).all()) and bool((out[..., 6] == -INF).all())
     assert bool(torch.isfinite(out[..., 7:]).all())
+
+
+# queries, heads, kv heads, width: the 8-wave form, the 4-wave form, and the keys in parts
+COSTS = [(8192, 32, 8, 128), (8192, 32, 8, 64), (2048, 1, 1, 128), (2048, 1, 1, 64)]
+
+
+@pytest.mark.parametrize("n,heads,kv_heads,dim", COSTS)
+def test_a_value_that_rows_do_not_see_costs_them_little(pkg, dev, n, heads, kv_heads, dim):
+    """One value that is not finite in the last token of a causal prompt: the rows that share its
+    tile and do not see it are right, and the call is not much slower (the rows of one tile of 64
+    walk their keys once more; 3 times a clean call and 3 ms leave room for a busy card)."""
+    q, k, v = _randn(5, n, heads, dim), _randn(6, n, kv_heads, dim), _randn(7, n, kv_heads, dim)
+    clean, zc = _attend(pkg, q, k, v, True)
+    assert bool(torch.isfinite(clean).all()) and bool(torch.isfinite(zc).all())
+
+    def took(value):
+        times = []
+        for _ in range(3):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            pkg.attention(q, k, value, out, causal=True)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    out = torch.empty_like(q)
+    before = took(v)
+    for bad in (NAN, INF):
+        w = v.clone()
+        w[n - 1, :, 3] = bad
+        say(f"attention one value {bad} in the last of {n} tokens, heads {heads}/{kv_heads} x {dim}")
+        after = took(w)
+        rest = torch.ones(dim, dtype=torch.bool)
+        rest[3] = False
+        assert torch.equal(_bits(out[:, :, rest]), _bits(clean[:, :, rest]))
+        assert bool(torch.isnan(out[n - 1, :, 3]).all() if bad != bad else (out[n - 1, :, 3] == bad).all())
+        for i in (n - 64, n - 33, n - 32, n - 2):
+            for h in (0, heads - 1):
+                g = h // (heads // kv_heads)
+                want = attn_ref.attend(q[i:i + 1, h:h + 1], k[:i + 1, g:g + 1],
+                                       w[:i + 1, g:g + 1], dim ** -0.5, False)
+                attn_ref.check(out[i:i + 1, h:h + 1], None, want, f"row {i} head {h}")
+        assert after < 3.0 * before + 3.0, (after, before)

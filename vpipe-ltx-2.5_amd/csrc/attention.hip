@@ -415,6 +415,211 @@ __device__ __forceinline__ bool not_finite(uint4 v)
   return any;
 }
 
+// 8 bf16, each as pick() makes it of its bits
+template <typename Pick>
+__device__ __forceinline__ bf16x8 each_bf16(bf16x8 f, Pick&& pick)
+{
+  const uint4 v = __builtin_bit_cast(uint4, f);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { x[i] = pick(w[i] & 0xffffu) | pick(w[i] >> 16) << 16; }
+  return as_bf16x8(make_uint4(x[0], x[1], x[2], x[3]));
+}
+
+// The wave's rows' means again, for the elements whose bits are set in `open`: those that
+// the sums left as a NaN (bit 16 d + i: register i of o[d]). A weight of zero times a value
+// that is not finite gives one too, and a causal tile's masked tokens take part in the second
+// product, so that a row can show what it does not see.
+//
+// First the values alone, 32 tokens at a time, for infinities and NaN that the rows do see: a
+// block that has any is multiplied as indicators of each kind. Weights are positive, so an
+// element that sees infinities of one sign is that infinity; one that sees a NaN, both signs,
+// or an infinity under a logit of -infinity, whose weight is zero, is a NaN. An element that has
+// shown itself a NaN is settled, and where all are, the wave is done. What is then left saw
+// finite values alone: its mean is taken over the keys once more, with every value that is not
+// finite as 0. It is kept as a mean, halved, that each block moves: no sum leaves f32's range.
+//
+// `mine`: the wave's own 32 rows of LDS. Rare, and no faster than that asks for: one value that
+// is not finite in the last of 8192 causal tokens, 32 / 8 heads of 128, makes the call 1.6 ms
+// for 0.5 (117 ms when the rows were taken one at a time), values that are all infinite 4.7 (239).
+template <bool SPLIT, int D, int NW>
+__device__ __forceinline__ void again(const PromptParams& p, const Rows<D, NW>& r, uint8_t* mine,
+                                      uint64_t open)
+{
+  constexpr int kRow = D * 2, kPieces = kRow / 16, kRowsPer = 64 / kPieces, kDT = D / 32;
+  constexpr int kKC = D / 16, kBlock = 32;
+  const int begin = r.first * kBN, end = min(r.end * kBN, r.wave_hi + 1);
+  // taken anew, so that the loops before this hold no registers for what follows from them
+  int tok = r.tok, head = r.head, limit = r.limit, at = threadIdx.x & 63;
+  asm volatile("" : "+v"(tok), "+v"(head), "+v"(limit), "+v"(at));
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int row0 = at / kPieces, piece = at % kPieces;   // of the values that the lane fetches
+
+  // s[i]: token t0 + (i & 3) + 8 (i >> 2) + 4 half
+  f32x16 s;
+  auto logits = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { s[i] = 0.0f; }
+    const uint16_t* const kp = p.k + (long)(r.k0 + min(t0 + (lane & 31), r.lk - 1)) * p.ks +
+                               r.g * D + half * 8;
+    const uint16_t* const qp =
+        p.q + (long)(r.q0 + min(tok, r.lq - 1)) * p.qs + head * D + half * 8;
+    fence();
+#pragma unroll
+    for (int c = 0; c < kKC; ++c) {
+      s = mfma32(as_bf16x8(*(const uint4*)(kp + c * 16)),
+                 as_bf16x8(*(const uint4*)(qp + c * 16)), s);
+    }
+    fence();
+  };
+  // the block's values into LDS, if any is not finite (which is the answer) or `all`
+  auto fetch = [&](int t0, bool all) {
+    uint4 v[kBlock / kRowsPer];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kBlock / kRowsPer; ++i) {
+      const int row = i * kRowsPer + row0;
+      v[i] = *(const uint4*)(p.v + (long)(r.k0 + min(t0 + row, r.lk - 1)) * p.vs + r.g * D +
+                             piece * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < kBlock / kRowsPer; ++i) { bad = bad || not_finite(v[i]); }
+    bad = any_lane(bad);
+    if (bad || all) {
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");   // the reads of the block before
+#pragma unroll
+      for (int i = 0; i < kBlock / kRowsPer; ++i) {
+        const int row = i * kRowsPer + row0;
+        *(uint4*)(mine + row * kRow + v_piece<D>(row, piece) * 16) = v[i];
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    }
+    return bad;
+  };
+  uint32_t pw[8];   // weights, two of bf16 each
+  auto part = [&](int c) {
+    return as_bf16x8(make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]));
+  };
+
+  uint64_t plus = 0, minus = 0, nans = 0;
+  for (int t0 = begin; t0 < end && any_lane((open & ~nans) != 0); t0 += kBlock) {
+    if (!fetch(t0, false)) { continue; }
+    logits(t0);
+    // 1 for a token that the row sees, 2^10 for one whose weight is zero
+    const int lim = limit - t0 - 4 * half;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      auto of = [&](int j) {
+        return (j & 3) + 8 * (j >> 2) > lim ? 0u : s[j] == -INFINITY ? 0x4480u : 0x3f80u;
+      };
+      pw[i] = of(2 * i) | of(2 * i + 1) << 16;
+    }
+#pragma unroll 1
+    for (int d = 0; d < kDT; ++d) {
+      // how often the row sees values whose bits under the mask lie in lo .. hi
+      auto count = [&](uint32_t mask, uint32_t lo, uint32_t hi, uint64_t& kind) {
+        f32x16 n;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { n[i] = 0.0f; }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          n = mfma32(each_bf16(v_frag<D>(mine, c * kDT + d),
+                               [&](uint32_t x) { return (x & mask) - lo <= hi - lo ? 0x3f80u : 0u; }),
+                     part(c), n);
+        }
+        uint32_t some = 0, none = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          some |= n[i] > 0.0f ? 1u << i : 0u;
+          none |= n[i] >= 1024.0f ? 1u << i : 0u;
+        }
+        kind |= (uint64_t)some << (16 * d);
+        nans |= (uint64_t)none << (16 * d);
+      };
+      count(0xffffu, 0x7f80u, 0x7f80u, plus);
+      count(0xffffu, 0xff80u, 0xff80u, minus);
+      count(0x7fffu, 0x7f81u, 0x7fffu, nans);
+    }
+    nans |= plus & minus;
+  }
+  open &= ~nans;
+
+  f32x16 o[kDT];
+#pragma unroll
+  for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { o[d][i] = 0.0f; }
+  }
+  if (any_lane((open & ~(plus | minus)) != 0)) {
+    float m = -INFINITY, l = 0.0f;
+    for (int t0 = begin; t0 < end; t0 += kBlock) {
+      (void)fetch(t0, true);
+      logits(t0);
+      const int lim = limit - t0 - 4 * half;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = (i & 3) + 8 * (i >> 2) > lim ? -INFINITY : s[i];
+        top = fmaxf(top, s[i]);
+      }
+      const float m_new = fmaxf(m, xor32_max(top));
+      const float mz = m_new == -INFINITY ? 0.0f : m_new;
+      const float before = l * exp2_of((m - mz) * p.c);
+      m = m_new;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = exp2_of((s[i] - mz) * p.c);
+        sum += s[i];
+      }
+      l = before + xor32_sum(sum);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l, keep = before * inv;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        pw[i] = pack_bf16x2(s[2 * i] * (0.5f * inv), s[2 * i + 1] * (0.5f * inv));
+      }
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { o[d][i] *= keep; }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          o[d] = mfma32(each_bf16(v_frag<D>(mine, c * kDT + d),
+                                  [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u ? 0u : x; }),
+                        part(c), o[d]);
+        }
+        fence();
+      }
+    }
+  }
+
+  // behind the wave's own stores of the same elements
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  const long token = r.q0 + tok;
+  uint16_t* const op = p.out + token * p.os + head * D + 4 * half;
+  float* const pp =
+      p.part + ((token * p.heads + head) * p.splits + blockIdx.y) * D + 4 * half;
+#pragma unroll
+  for (int d = 0; d < kDT; ++d) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t bit = 1ull << (16 * d + i);
+      if ((open & bit) != 0) {
+        // rounding may not make an infinity of a mean of finite values
+        const float mean = fminf(fmaxf(o[d][i] * 2.0f, -0x1.fep127f), 0x1.fep127f);
+        const float x = (plus & bit) != 0 ? INFINITY : (minus & bit) != 0 ? -INFINITY : mean;
+        const int channel = d * 32 + (i & 3) + 8 * (i >> 2);
+        if (SPLIT) {
+          pp[channel] = x;
+        } else {
+          op[channel] = f32_to_bf16(x);
+        }
+      }
+    }
+  }
+}
+
 // The sums and statistics of the wave's rows out: through LDS, each wave its own
 // part of it, so that a store has whole rows' pieces side by side. SPLIT: a part's means,
 // maximum (log2) and sum into the workspace instead.
@@ -477,76 +682,19 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
         l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l * 0x1p32f)) * 0.69314718055994531f;
   }
   const float sum = (nans[0] + nans[1]) + (nans[2] + nans[3]);
-  // A NaN in a row: a weight of zero times an infinite or NaN value that the row does
-  // not see (a causal tile's masked tokens take part in the second product) gives one
-  // too. If there is such a value among these tokens, the row's NaN channels are
-  // computed again over the tokens that it sees alone, one at a time, by the whole wave,
-  // as a mean that each token moves, until they are NaN from what it does see: a rare
-  // case, but one that tensors full of NaN must not make endless. A sum of weights that
-  // is a NaN has seen one itself.
-  unsigned long long again = __ballot(sum != sum && l == l && r.valid);
-  again = (again | (again >> 32)) & 0xffffffffull;
-  while (again != 0) {
-    const int at = __builtin_ctzll(again);
-    again &= again - 1;
-    const int rtok = __shfl(r.tok, at), rhead = __shfl(r.head, at), rlimit = __shfl(r.limit, at);
-    constexpr int kPer = D / 64;
-    bool unseen = false;   // a value that is not finite among the masked tokens
-    const int begin = r.first * kBN, end = min(r.end * kBN, r.lk);
-    for (int j = max(rlimit + 1, begin) + (lane >> 3); j < end; j += 8) {
-      const uint16_t* const vp = p.v + (long)(r.k0 + j) * p.vs + r.g * D + (lane & 7) * (D / 8);
+  // A sum of weights that is a NaN has seen one itself
+  const bool bad = r.valid && l == l && sum != sum;
+  if (__builtin_expect(any_lane(bad), 0)) {
+    uint64_t open = 0;
 #pragma unroll
-      for (int i = 0; i < D / 8; i += 8) { unseen = unseen || not_finite(*(const uint4*)(vp + i)); }
-    }
-    if (!any_lane(unseen)) { continue; }
-    const int d0 = lane * kPer;
-    const uint16_t* const staged =
-        (const uint16_t*)(mine + at * kRow + k_piece<D>(at, d0 / 8) * 16) + d0 % 8;
-    bool nan_at[kPer];
+    for (int d = 0; d < kDT; ++d) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) { nan_at[i] = (staged[i] & 0x7fff) > 0x7f80; }
-    const uint16_t* const qp = p.q + (long)(r.q0 + rtok) * p.qs + rhead * D + d0;
-    float qv[kPer], acc[kPer], rm = -INFINITY, rl = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) { qv[i] = bf16_to_f32(qp[i]); acc[i] = 0.0f; }
-    for (int j = begin; j < min(rlimit + 1, end); ++j) {
-      bool open = false;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) { open = open || (nan_at[i] && acc[i] == acc[i]); }
-      if (!any_lane(open)) { break; }
-      const uint16_t* const kp = p.k + (long)(r.k0 + j) * p.ks + r.g * D + d0;
-      const uint16_t* const vp = p.v + (long)(r.k0 + j) * p.vs + r.g * D + d0;
-      float x = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) { x = fmaf(qv[i], bf16_to_f32(kp[i]), x); }
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) { x += __shfl_xor(x, d); }
-      const float n = fmaxf(rm, x);
-      const float nc = n == -INFINITY ? 0.0f : n * p.c;
-      const float kept = __builtin_amdgcn_exp2f(fmaf(rm, p.c, -nc));
-      const float w = __builtin_amdgcn_exp2f(fmaf(x, p.c, -nc));
-      rm = n;
-      const float before = rl * kept;
-      rl = before + w;
-      const float inv_l = rl == 0.0f ? 0.0f : 1.0f / rl;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        acc[i] = fmaf(acc[i], before * inv_l, w * inv_l * bf16_to_f32(vp[i]));
+      for (int i = 0; i < 16; ++i) {
+        const float x = o[d][i] * inv;
+        open |= x != x ? 1ull << (16 * d + i) : 0ull;
       }
     }
-    uint16_t* const op = p.out + (long)(r.q0 + rtok) * p.os + rhead * D + d0;
-    float* const pp =
-        p.part + (((long)(r.q0 + rtok) * p.heads + rhead) * p.splits + blockIdx.y) * D + d0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (nan_at[i]) {
-        if (SPLIT) {
-          pp[i] = acc[i];
-        } else {
-          op[i] = f32_to_bf16(acc[i]);
-        }
-      }
-    }
+    again<SPLIT>(p, r, mine, bad ? open : 0ull);
   }
 }
 

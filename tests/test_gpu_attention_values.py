@@ -124,3 +124,63 @@ def test_a_value_that_rows_do_not_see_costs_them_little(pkg, dev, n, heads, kv_h
                                        w[:i + 1, g:g + 1], dim ** -0.5, False)
                 attn_ref.check(out[i:i + 1, h:h + 1], None, want, f"row {i} head {h}")
         assert after < 3.0 * before + 3.0, (after, before)
+
+
+def _even(seed, *shape):
+    """Values from 1 to 2 of one sign, so that a mean of them is of their size."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return 1.0 + torch.rand(shape, device="cuda", generator=g)
+
+
+def _check_small(q, k, v, out, rows, scale, what):
+    """attn_ref's bound for the roundings to 8 bits, and half a unit of bf16's smallest values (2^-133)
+    with as much again for f32's own."""
+    heads, kv_heads = q.shape[1], k.shape[1]
+    for i in rows:
+        for h in (0, heads - 1):
+            g = h // (heads // kv_heads)
+            ref, _, mag, _ = attn_ref.attend(q[i:i + 1, h:h + 1], k[:, g:g + 1], v[:, g:g + 1], scale,
+                                             False)
+            err = (out[i:i + 1, h:h + 1].cpu().double() - ref).abs()
+            assert bool((err <= attn_ref.OUT_BOUND * mag + 2.0 ** -133).all()), (what, i, h)
+
+
+# queries, keys, heads, kv heads: in parts, the 4-wave form, the 8-wave form
+SMALL = [(5, 1500, 2, 1), (300, 300, 2, 1), (4200, 4200, 32, 8)]
+
+
+@pytest.mark.parametrize("power", [-90, -100, -112, -120, -125])
+@pytest.mark.parametrize("nq,nk,heads,kv_heads", SMALL)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_values_keep_their_bits(pkg, dev, power, nq, nk, heads, kv_heads, dim):
+    """Values down to the smallest normal ones, under logits that rise so that the maximum lags."""
+    q = torch.ones(nq, heads, dim, dtype=torch.bfloat16, device="cuda")
+    k = torch.linspace(0, 5, nk, device="cuda")[:, None, None].expand(nk, kv_heads, dim) / dim
+    k = k.to(torch.bfloat16)
+    v = (_even(8, nk, kv_heads, dim) * 2.0 ** power).to(torch.bfloat16)
+    say(f"attention values of 2^{power}, {nq} x {nk} heads {heads}/{kv_heads} x {dim}")
+    out, z = _attend(pkg, q, k, v, False, True, 1.0)
+    _check_small(q, k, v, out, (0, nq // 2, nq - 1), 1.0, power)
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv_heads", SMALL)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_values_beside_the_largest_and_beside_unseen_ones(pkg, dev, nq, nk, heads, kv_heads, dim):
+    """One row's channels at both ends of the range, and a small channel whose last token holds an
+    infinity that only the last query sees."""
+    q, k = _randn(9, nq, heads, dim), _randn(10, nk, kv_heads, dim)
+    v = _even(11, nk, kv_heads, dim)
+    v[..., :8] *= 2.0 ** 126
+    v[..., 8:] *= 2.0 ** -122
+    v = v.to(torch.bfloat16)
+    say(f"attention values at both ends, {nq} x {nk} heads {heads}/{kv_heads} x {dim}")
+    out, _ = _attend(pkg, q, k, v, False)
+    assert bool(torch.isfinite(out).all())
+    _check_small(q, k, v, out, (0, nq // 2, nq - 1), dim ** -0.5, "both ends")
+    if nq == nk:
+        v[nk - 1, :, 9] = INF
+        out, _ = _attend(pkg, q, k, v, True)
+        assert bool((out[nq - 1, :, 9] == INF).all()) and bool(torch.isfinite(out[:nq - 1]).all())
+        for i in (nq - 40, nq - 2):
+            _check_small(q, k[:i + 1], v[:i + 1], out, (i,), dim ** -0.5, "beside an unseen infinity")

@@ -45,17 +45,23 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace ltx25 {
 namespace {
 
 constexpr int kBN = 64;   // tokens of a tile
-// The weights are 2^(logit - maximum - kShift), so that under a maximum that lags by
-// up to 2^12 sums of values near f32's end stay in range; weights 2^94 below the
-// largest are still normal numbers. 32, because the exponents of most weights then
-// differ in as few bits as without a shift: with 28 they lie on both sides of a power of
-// two, and the power that this costs the matrix cores makes a long prompt 1% slower.
-constexpr float kShift = 32.0f;
+
+// A bit for each of a lane's D / 2 elements
+template <int D>
+using Bits = std::conditional_t<D == 64, uint32_t, uint64_t>;
+
+// The weights are 2^(logit - maximum - kShift). With 8, 16 and 32 a long prompt takes 0.6 to
+// 1% less time than with 0, 4 and 12, at the same instructions (16384 causal tokens: 1771, 1768
+// and 1765 us for 1782, 1787 and 1789). 8, since a product with the smallest normal value,
+// 2^-126, then keeps 15 bits, and with 32 none.
+constexpr float kShift = 8.0f, kOne = 256.0f;
+constexpr float kMost = 4096.0f / kOne;   // what a lane's weights may sum to under an old maximum
 
 struct PromptParams {
   const uint16_t* q;
@@ -243,6 +249,18 @@ struct Rows {
   int first, end;       // the workgroup's tiles
 };
 
+// The row of the workgroup's rows that the lane holds
+template <int D, int NW>
+__device__ __forceinline__ void find_row(const PromptParams& p, Rows<D, NW>& r, int lane)
+{
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = wave * 32 + (lane & 31);
+  r.head = r.head0 + (row >> p.tb_log2);
+  r.tok = r.tok0 + (row & ((1 << p.tb_log2) - 1));
+  r.valid = r.tok < r.lq;
+  r.limit = p.causal ? min(min(r.tok, r.lq - 1) + r.lk - r.lq, r.lk - 1) : r.lk - 1;
+}
+
 template <int D, int NW>
 __device__ __forceinline__ bool find(const PromptParams& p, Rows<D, NW>& r, bool split)
 {
@@ -270,15 +288,11 @@ __device__ __forceinline__ bool find(const PromptParams& p, Rows<D, NW>& r, bool
   r.tok0 = (((un.lq + tb - 1) >> p.tb_log2) - 1 - un.from_end) << p.tb_log2;
   r.head0 = hg << p.hp_log2;
   r.g = r.head0 / p.share;
-  const int row = wave * 32 + (lane & 31);
-  r.head = r.head0 + (row >> p.tb_log2);
-  r.tok = r.tok0 + (row & (tb - 1));
-  r.valid = r.tok < r.lq;
+  find_row(p, r, lane);
   const int shift = p.causal ? r.lk - r.lq : 0;
   auto last_key = [&](int t) { return p.causal ? min(t + shift, un.lk - 1) : un.lk - 1; };
   const int lo = r.tok0 + (p.tb_log2 >= 5 ? (wave * 32) & (tb - 1) : 0);
   const int hi = min(lo + min(tb, 32), r.lq) - 1;
-  r.limit = last_key(min(r.tok, r.lq - 1));
   r.wave_lo = lo < r.lq ? last_key(lo) : -1;
   r.wave_hi = lo < r.lq ? last_key(hi) : -1;
   const int last = last_key(min(r.tok0 + tb, r.lq) - 1);
@@ -428,16 +442,17 @@ __device__ __forceinline__ bf16x8 each_bf16(bf16x8 f, Pick&& pick)
 }
 
 // The wave's rows' means again, for the elements whose bits are set in `open`: those that
-// the sums left as a NaN (bit 16 d + i: register i of o[d]). A weight of zero times a value
-// that is not finite gives one too, and a causal tile's masked tokens take part in the second
-// product, so that a row can show what it does not see.
+// the sums left not finite (bit 16 d + i: register i of o[d]), `was_nan` those that are a NaN.
+// A sum of weights up to 2^12 times values near f32's end passes it though the mean does not.
+// A weight of zero times a value that is not finite is a NaN, and a causal tile's masked
+// tokens take part in the second product, so that a row can show what it does not see.
 //
 // First the values alone, 32 tokens at a time, for infinities and NaN that the rows do see: a
 // block that has any is multiplied as indicators of each kind. Weights are positive, so an
 // element that sees infinities of one sign is that infinity; one that sees a NaN, both signs,
 // or an infinity under a logit of -infinity, whose weight is zero, is a NaN. An element that has
-// shown itself a NaN is settled, and where all are, the wave is done. What is then left saw
-// finite values alone: its mean is taken over the keys once more, with every value that is not
+// shown itself a NaN is settled, as is an infinity of one that was no NaN, and where all
+// are, the wave is done. What is then left saw finite values alone: its mean is taken over the keys once more, with every value that is not
 // finite as 0. It is kept as a mean, halved, that each block moves: no sum leaves f32's range.
 //
 // `mine`: the wave's own 32 rows of LDS. Rare, and no faster than that asks for: one value that
@@ -445,16 +460,19 @@ __device__ __forceinline__ bf16x8 each_bf16(bf16x8 f, Pick&& pick)
 // for 0.5 (117 ms when the rows were taken one at a time), values that are all infinite 4.7 (239).
 template <bool SPLIT, int D, int NW>
 __device__ __forceinline__ void again(const PromptParams& p, const Rows<D, NW>& r, uint8_t* mine,
-                                      uint64_t open)
+                                      Bits<D> open, Bits<D> was_nan)
 {
   constexpr int kRow = D * 2, kPieces = kRow / 16, kRowsPer = 64 / kPieces, kDT = D / 32;
   constexpr int kKC = D / 16, kBlock = 32;
   const int begin = r.first * kBN, end = min(r.end * kBN, r.wave_hi + 1);
-  // taken anew, so that the loops before this hold no registers for what follows from them
-  int tok = r.tok, head = r.head, limit = r.limit, at = threadIdx.x & 63;
-  asm volatile("" : "+v"(tok), "+v"(head), "+v"(limit), "+v"(at));
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int row0 = at / kPieces, piece = at % kPieces;   // of the values that the lane fetches
+  // the lane's row found anew, so that the loops before this hold no registers for it
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  const int half = lane >> 5;
+  Rows<D, NW> x = r;
+  find_row(p, x, lane);
+  const int tok = x.tok, head = x.head, limit = x.limit;
+  const int row0 = lane / kPieces, piece = lane % kPieces;   // of the values that the lane fetches
 
   // s[i]: token t0 + (i & 3) + 8 (i >> 2) + 4 half
   f32x16 s;
@@ -497,13 +515,21 @@ __device__ __forceinline__ void again(const PromptParams& p, const Rows<D, NW>& 
     }
     return bad;
   };
+  // v_frag of 16 tokens from 16 c on and channels from 32 d on, of the lane found anew
+  auto frag = [&](int c, int d) {
+    const int row = c * 16 + half * 4 + ((lane & 15) >> 2);
+    const int at = v_piece<D>(row, d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1));
+    const uint8_t* const x = mine + row * kRow + at * 16 + (lane & 1) * 8;
+    return turned(x, x + 8 * kRow);   // 8 rows on the pieces lie alike
+  };
   uint32_t pw[8];   // weights, two of bf16 each
   auto part = [&](int c) {
     return as_bf16x8(make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]));
   };
 
-  uint64_t plus = 0, minus = 0, nans = 0;
-  for (int t0 = begin; t0 < end && any_lane((open & ~nans) != 0); t0 += kBlock) {
+  Bits<D> plus = 0, minus = 0, nans = 0;
+  for (int t0 = begin; t0 < end; t0 += kBlock) {
+    if (!any_lane((open & ~(nans | (~was_nan & (plus | minus)))) != 0)) { break; }
     if (!fetch(t0, false)) { continue; }
     logits(t0);
     // 1 for a token that the row sees, 2^10 for one whose weight is zero
@@ -518,13 +544,13 @@ __device__ __forceinline__ void again(const PromptParams& p, const Rows<D, NW>& 
 #pragma unroll 1
     for (int d = 0; d < kDT; ++d) {
       // how often the row sees values whose bits under the mask lie in lo .. hi
-      auto count = [&](uint32_t mask, uint32_t lo, uint32_t hi, uint64_t& kind) {
+      auto count = [&](uint32_t mask, uint32_t lo, uint32_t hi, Bits<D>& kind) {
         f32x16 n;
 #pragma unroll
         for (int i = 0; i < 16; ++i) { n[i] = 0.0f; }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          n = mfma32(each_bf16(v_frag<D>(mine, c * kDT + d),
+          n = mfma32(each_bf16(frag(c, d),
                                [&](uint32_t x) { return (x & mask) - lo <= hi - lo ? 0x3f80u : 0u; }),
                      part(c), n);
         }
@@ -534,8 +560,8 @@ __device__ __forceinline__ void again(const PromptParams& p, const Rows<D, NW>& 
           some |= n[i] > 0.0f ? 1u << i : 0u;
           none |= n[i] >= 1024.0f ? 1u << i : 0u;
         }
-        kind |= (uint64_t)some << (16 * d);
-        nans |= (uint64_t)none << (16 * d);
+        kind |= (Bits<D>)some << (16 * d);
+        nans |= (Bits<D>)none << (16 * d);
       };
       count(0xffffu, 0x7f80u, 0x7f80u, plus);
       count(0xffffu, 0xff80u, 0xff80u, minus);
@@ -585,7 +611,7 @@ __device__ __forceinline__ void again(const PromptParams& p, const Rows<D, NW>& 
         for (int i = 0; i < 16; ++i) { o[d][i] *= keep; }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          o[d] = mfma32(each_bf16(v_frag<D>(mine, c * kDT + d),
+          o[d] = mfma32(each_bf16(frag(c, d),
                                   [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u ? 0u : x; }),
                         part(c), o[d]);
         }
@@ -604,7 +630,7 @@ __device__ __forceinline__ void again(const PromptParams& p, const Rows<D, NW>& 
   for (int d = 0; d < kDT; ++d) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const uint64_t bit = 1ull << (16 * d + i);
+      const Bits<D> bit = (Bits<D>)1 << (16 * d + i);
       if ((open & bit) != 0) {
         // rounding may not make an infinity of a mean of finite values
         const float mean = fminf(fmaxf(o[d][i] * 2.0f, -0x1.fep127f), 0x1.fep127f);
@@ -636,7 +662,7 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   landed<0>();
   uint8_t* const mine = lds + wave * 32 * kRow;
-  float nans[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // a NaN stays one in a sum
+  float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // a NaN where any is not finite
 #pragma unroll
   for (int d = 0; d < kDT; ++d) {
 #pragma unroll
@@ -645,7 +671,7 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j] = o[d][4 * i + j] * inv;
-        nans[j] += x[j];
+        odd[j] = fmaf(x[j], 0.0f, odd[j]);
       }
       *(uint2*)(mine + (lane & 31) * kRow + k_piece<D>(lane & 31, d * 4 + i) * 16 + half * 8) =
           make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
@@ -674,27 +700,29 @@ __device__ __forceinline__ void finish(const PromptParams& p, const Rows<D, NW>&
       }
       if (half == 0) {
         *(float2*)(p.part + (long)p.total_q * p.heads * p.splits * D + row * 2) =
-            make_float2(l == 0.0f ? -INFINITY : m * p.c, l * 0x1p32f);
+            make_float2(l == 0.0f ? -INFINITY : m * p.c, l * kOne);
       }
     }
   } else if (p.lse != nullptr && half == 0 && r.valid) {
     p.lse[(long)(r.q0 + r.tok) * p.heads + r.head] =
-        l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l * 0x1p32f)) * 0.69314718055994531f;
+        l == 0.0f ? -INFINITY : fmaf(m, p.c, log2f(l * kOne)) * 0.69314718055994531f;
   }
-  const float sum = (nans[0] + nans[1]) + (nans[2] + nans[3]);
   // A sum of weights that is a NaN has seen one itself
-  const bool bad = r.valid && l == l && sum != sum;
+  const float any = (odd[0] + odd[1]) + (odd[2] + odd[3]);
+  const bool bad = r.valid && l == l && any != any;
   if (__builtin_expect(any_lane(bad), 0)) {
-    uint64_t open = 0;
+    Bits<D> open = 0, nans = 0;
 #pragma unroll
     for (int d = 0; d < kDT; ++d) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float x = o[d][i] * inv;
-        open |= x != x ? 1ull << (16 * d + i) : 0ull;
+        const Bits<D> bit = (Bits<D>)1 << (16 * d + i);
+        open |= fabsf(x) < INFINITY ? 0 : bit;
+        nans |= x != x ? bit : 0;
       }
     }
-    again<SPLIT>(p, r, mine, bad ? open : 0ull);
+    again<SPLIT>(p, r, mine, bad ? open : 0, nans);
   }
 }
 
@@ -781,7 +809,7 @@ __global__ void __launch_bounds__(256, D == 64 && !SPLIT ? 4 : 2) attention_kern
     bool settle = t == r.first;
     if (!settle) {
       sum = weigh();
-      settle = any_lane(!(sum <= 0x1p-20f));
+      settle = any_lane(!(sum <= kMost));
       if (settle) { logits(); }
     }
     if (settle) {
@@ -938,7 +966,7 @@ __global__ void __launch_bounds__(512, 2) attention_turns_kernel(PromptParams p)
     };
     // as in attention_kernel, with the logits still there
     float sum = weigh();
-    if (any_lane(!(sum <= 0x1p-20f))) {   // 2^12, shifted
+    if (any_lane(!(sum <= kMost))) {
       float top = s[0][0];
 #pragma unroll
       for (int i = 1; i < 32; ++i) { top = fmaxf(top, s[i >> 4][i & 15]); }

@@ -69,3 +69,14 @@ def test_a_cache_in_host_memory_is_refused_by_every_call(pkg, name):
                 call(c, table, x, x, _i32(0, 4), _i32(0))
         with pytest.raises(ValueError, match="cache." + name):
             pkg.attention_cached(c, table, _i32(4), _bf16(1, 8, 128), _bf16(1, 8, 128), 1, 100)
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_scale", "v_scale"])
+def test_a_caches_tensors_stay_its_own(pkg, name):
+    """Calls go to the addresses that the cache was made with: another tensor in their place would
+    be ignored, and the old one's memory, freed, written to."""
+    c = _cache(pkg)
+    old, address = getattr(c, name), bytes(c.c())
+    with pytest.raises(AttributeError):
+        setattr(c, name, old.clone())
+    assert getattr(c, name) is old and bytes(c.c()) == address

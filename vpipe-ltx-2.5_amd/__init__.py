@@ -443,7 +443,16 @@ class KVCache:
 
     k: int8 [pages][kv_heads][page_tokens][head_dim], v: int8
     [pages][kv_heads][head_dim][page_tokens], k_scale / v_scale: float32 [pages][kv_heads].
+
+    Calls work on the tensors given here, whose contents may change at will; a cache in other
+    tensors is another KVCache (assigning to k, v, k_scale or v_scale is refused, since the calls
+    would go on with the old ones' memory).
     """
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
 
     def __init__(self, k, v, k_scale, v_scale):
         torch = _torch or _import_torch()
@@ -458,7 +467,7 @@ class KVCache:
             if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) or not t.is_contiguous():
                 raise TypeError(f"{name} must be contiguous float32 [{pages}][{heads}], got "
                                 f"{t.dtype} {tuple(t.shape)}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors = (k, v, k_scale, v_scale)
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, page, dim
         self._c = KVCacheC(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), pages, page, heads, dim)
         self._checked = False
@@ -478,8 +487,7 @@ class KVCache:
     def check(self) -> None:
         """Refuse a cache in host memory, which may be made but not given to a kernel."""
         if not self._checked:
-            _reachable("cache.k cache.v cache.k_scale cache.v_scale", self.k, self.v, self.k_scale,
-                       self.v_scale)
+            _reachable("cache.k cache.v cache.k_scale cache.v_scale", *self._tensors)
             self._checked = True
 
 

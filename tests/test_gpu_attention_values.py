@@ -184,3 +184,16 @@ def test_small_values_beside_the_largest_and_beside_unseen_ones(pkg, dev, nq, nk
         assert bool((out[nq - 1, :, 9] == INF).all()) and bool(torch.isfinite(out[:nq - 1]).all())
         for i in (nq - 40, nq - 2):
             _check_small(q, k[:i + 1], v[:i + 1], out, (i,), dim ** -0.5, "beside an unseen infinity")
+
+
+@pytest.mark.parametrize("stride", [513, 532, 1 << 23, 0])
+def test_one_token_of_any_stride(pkg, dev, stride):
+    """A tensor of one token has no next one: what its stride says does not matter."""
+    q, k, v = (_randn(s, 1, h, 64).as_strided((1, h, 64), (stride, 64, 1))
+               for s, h in ((12, 8), (13, 2), (14, 2)))
+    out = torch.full((1, 8, 64), NAN, dtype=torch.bfloat16, device="cuda")
+    z = torch.full((1, 8), NAN, device="cuda")
+    say(f"attention one token of stride {stride}")
+    pkg.attention(q, k, v, out.as_strided((1, 8, 64), (stride, 64, 1)), causal=True, lse=z)
+    torch.cuda.synchronize()
+    attn_ref.check(out, z, attn_ref.attend(q, k, v, 64 ** -0.5, True))

@@ -351,7 +351,7 @@ def _tokens(name: str, t, shape) -> int:
     n, heads, dim = shape
     if n > 0 and ((stride[2] != 1 and dim > 1) or (stride[1] != dim and heads > 1)):
         raise ValueError(f"{name}: a token's heads must lie side by side, got strides {stride}")
-    return stride[0] if n > 1 else max(stride[0], heads * dim)
+    return stride[0] if n > 1 else heads * dim   # one token: there is no next one
 
 
 def _int32(name: str, t, count: int) -> None:

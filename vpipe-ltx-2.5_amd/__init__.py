@@ -378,7 +378,8 @@ def _lse(t, tokens: int, heads: int) -> None:
 
 def _reachable(names: str, *tensors) -> None:
     """Refuse a tensor in host memory, whose address means nothing to the kernels (None, and
-    pinned memory, which they do reach, pass)."""
+    pinned memory, which they do reach, pass). Callers look at is_cuda themselves first: 0.2 us
+    less for a call whose tensors all lie there."""
     for i, t in enumerate(tensors):
         if t is not None and not t.is_cuda and not t.is_pinned():
             raise ValueError(f"{names.split()[i]} must lie in the GPU's memory, got a tensor on "
@@ -413,7 +414,10 @@ def attention(q, k, v, out, cu_q=None, cu_k=None, *, causal: bool, scale: float 
         pq, pk = cu_q.data_ptr(), cu_k.data_ptr()
     if lse is not None:
         _lse(lse, nq, heads)
-    _reachable("q k v out cu_q cu_k lse workspace", q, k, v, out, cu_q, cu_k, lse, workspace)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and out.is_cuda
+            and (cu_q is None or cu_q.is_cuda and cu_k.is_cuda)
+            and (lse is None or lse.is_cuda) and (workspace is None or workspace.is_cuda)):
+        _reachable("q k v out cu_q cu_k lse workspace", q, k, v, out, cu_q, cu_k, lse, workspace)
     a = AttnC(heads, kv_heads, dim, 1 if causal else 0, scale, qs, ks, vs, os_)
     # only such sizes can have parts: 8 tiles of 64 keys, 256 workgroups of 128 rows at most
     if nk > 448 * batch and nq * heads <= 65536 and (workspace is not None or stream is None):
@@ -470,7 +474,7 @@ class KVCache:
         self._tensors = (k, v, k_scale, v_scale)
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, page, dim
         self._c = KVCacheC(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), pages, page, heads, dim)
-        self._checked = False
+        self.checked = False
 
     @classmethod
     def empty(cls, pages: int, page_tokens: int, kv_heads: int, head_dim: int, device="cuda"):
@@ -486,9 +490,8 @@ class KVCache:
 
     def check(self) -> None:
         """Refuse a cache in host memory, which may be made but not given to a kernel."""
-        if not self._checked:
-            _reachable("cache.k cache.v cache.k_scale cache.v_scale", *self._tensors)
-            self._checked = True
+        _reachable("cache.k cache.v cache.k_scale cache.v_scale", *self._tensors)
+        self.checked = True
 
 
 def _moved(cache: KVCache, table, k, v, cu, start):
@@ -502,8 +505,10 @@ def _moved(cache: KVCache, table, k, v, cu, start):
     stride = _table(table, batch)
     _int32("cu", cu, batch + 1)
     _int32("start", start, batch)
-    cache.check()
-    _reachable("table k v cu start", table, k, v, cu, start)
+    if not cache.checked:
+        cache.check()
+    if not (table.is_cuda and k.is_cuda and v.is_cuda and cu.is_cuda and start.is_cuda):
+        _reachable("table k v cu start", table, k, v, cu, start)
     return (ctypes.byref(cache.c()), table.data_ptr(), stride, k.data_ptr(), v.data_ptr(), ks, vs,
             cu.data_ptr(), start.data_ptr(), batch, total)
 
@@ -547,8 +552,11 @@ def attention_cached(cache: KVCache, table, lens, q, out, q_len: int, max_len: i
     _int32("lens", lens, batch)
     if lse is not None:
         _lse(lse, nq, heads)
-    cache.check()
-    _reachable("table lens q out workspace lse", table, lens, q, out, workspace, lse)
+    if not cache.checked:
+        cache.check()
+    if not (table.is_cuda and lens.is_cuda and q.is_cuda and out.is_cuda
+            and (workspace is None or workspace.is_cuda) and (lse is None or lse.is_cuda)):
+        _reachable("table lens q out workspace lse", table, lens, q, out, workspace, lse)
     a = AttnC(heads, cache.kv_heads, dim, 1 if causal else 0, scale, qs, 0, 0, os_)
     at, held = None, 0
     if workspace is not None:

@@ -124,3 +124,37 @@ def test_appended_small_values_are_attended_to(pkg, dev):
     out, z, _ = _attend(pkg, c, table, [n], q, 1)
     _close(c, table, n, q, 0, 1, out, z)
     assert bool((out.float() > 2.0 ** -126).all())
+
+
+# keys, batch, heads, kv heads, width: both sides of 20 rounds of 256 tokens with every CU's work
+# there, and parts beyond a wave's lanes
+LONG = [([5120] * 2 + [300] * 62, 8, 8, 64), ([5121] * 2 + [300] * 62, 8, 8, 64),
+        ([17000], 2, 1, 128), ([131072], 1, 1, 128), ([131072], 2, 1, 64), ([40000, 131, 9000], 4, 2, 64)]
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,dim", LONG)
+def test_long_contexts_in_many_parts(pkg, dev, lens, heads, kv_heads, dim):
+    page = 64
+    table, pages = _table(12, lens, page)
+    c = _cache(pkg, 13, pages, page, kv_heads, dim)
+    q = _randn(14, len(lens), heads, dim)
+    say(f"attention_cached long {lens[:3]} heads {heads}/{kv_heads} x {dim}")
+    out, z, parts = _attend(pkg, c, table, lens, q, 1)
+    assert parts >= (65 if lens[0] >= 17000 and len(lens) == 1 else 0)
+    share = heads // kv_heads
+    for b in (0, 1, len(lens) - 1):
+        if b >= len(lens):
+            continue
+        ids = torch.from_numpy(table[b, :-(-lens[b] // page)]).cuda().long()
+        k = (c.k[ids].double() * c.k_scale[ids].double()[:, :, None, None]).transpose(1, 2)
+        v = (c.v[ids].double() * c.v_scale[ids].double()[:, :, None, None]).permute(0, 3, 1, 2)
+        k, v = (x.reshape(-1, kv_heads, dim)[:lens[b]] for x in (k, v))
+        for h in range(heads):
+            x = k[:, h // share] @ q[b, h].double() * dim ** -0.5
+            top = torch.logsumexp(x, 0)
+            w = torch.exp(x - top)
+            want, mag = w @ v[:, h // share], w @ v[:, h // share].abs()
+            err = (out[b, h].double() - want).abs() - attn_ref.OUT_BOUND * mag
+            assert float(err.max()) <= 0, (b, h)
+            size = (k[:, h // share].abs() @ q[b, h].double().abs()).max() * dim ** -0.5
+            assert abs(float(z[b, h] - top)) <= attn_ref.LSE_BOUND * (1 + float(size)), (b, h)

@@ -59,8 +59,13 @@ typedef struct ltx25_attn {
  *   NULL with batch 1: one sequence of total_q queries and total_k keys.
  *   lse: float [total_q][heads] or NULL: the natural logarithm of the sum of
  *   the exponentials, to merge with attention over other keys.
+ * out may not overlap q, k or v.
  * A query that sees no key gives zeros and an lse of -infinity. A key or value
- * that a query does not see has no influence on it, be it infinite or NaN.
+ * that a query does not see adds nothing to it, be it infinite or NaN; an infinite
+ * value that it does see shows in its channel, however small its weight. (Rows side
+ * by side take their maxima together: what one of them sees may change the last bits
+ * of another's rounding, within the errors below. A call with the same tensors gives
+ * the same bits.) Values count over f32's whole range of normal numbers.
  * Products of bf16, sums and softmax statistics in f32; the weights are rounded
  * to bf16 for the second product; one rounding to bf16 at the end. */
 int ltx25_attention(void* stream, const ltx25_attn* a, const void* q, const void* k, const void* v,

@@ -21,8 +21,8 @@
 // cores and about 120 operations for the weights, 32 of them exponentials at 9
 // cycles and the rest at 4 to 5 each. Two waves a SIMD overlap them only in part, since
 // a product also takes about 16 cycles of the other wave's issue: of long prompts'
-// cycles the matrix cores are busy in 66%, at head width 64 in 48%, where the weights'
-// operations take 80%. The instructions' energy counts as well: 17% fewer cycles
+// cycles the matrix cores are busy in 66%, at head width 64 in 50 to 55%, where vector
+// operations take 69 to 76%. The instructions' energy counts as well: 17% fewer cycles
 // (attention_turns_kernel against attention_kernel) came at 10% less clock. The weights
 // are rounded to bf16 as the values are; the sums and statistics are f32.
 // Two forms:

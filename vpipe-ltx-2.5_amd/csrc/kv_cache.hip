@@ -913,7 +913,8 @@ CachedPlan plan_cached(int batch, int q_len, int heads, int kv_heads, int head_d
   // flight (4 x 8 kv heads of 99991 to 131072 tokens: 175 us, 180 with four workgroups, 185 with
   // eight) -- but past 20 rounds no part longer than 8 rounds or a 16th of the tokens,
   // since the lengths may be very uneven and only the longest is known here (63
-  // sequences of 200 tokens beside one of 30000: 52 us for 78 in parts of 20 rounds).
+  // sequences of 200 tokens beside one of 30000: 52 us for 78 in parts of 20 rounds; from how
+  // many rounds on that pays has not been measured).
   const long units = (long)batch * kv_heads * r.row_blocks;
   const long rounds = ((long)max_len + 255) / 256;
   long per = std::max(rounds, 1L);

@@ -145,7 +145,9 @@ int ltx25_kv_read(void* stream, const ltx25_kv_cache* cache, const int* table, i
  *   where that is 0).
  * Keys and values enter both products as their exact codes; a page's scales
  * multiply the logits and the weights in f32, and these are rounded to f16 (under
- * a power of two) for the second product. The tokens are split over
+ * a power of two of the row's) for the second product: a weight times its scale that
+ * is 2^26 times smaller than the row's largest has fewer than 11 bits, and one 2^37
+ * times smaller counts as zero. The tokens are split over
  * workgroups and the parts joined in one fixed order: the same call gives the
  * same bits. */
 int ltx25_attention_cached(void* stream, const ltx25_attn* a, const ltx25_kv_cache* cache,

@@ -451,9 +451,10 @@ __device__ __forceinline__ bf16x8 each_bf16(bf16x8 f, Pick&& pick)
 // block that has any is multiplied as indicators of each kind. Weights are positive, so an
 // element that sees infinities of one sign is that infinity; one that sees a NaN, both signs,
 // or an infinity under a logit of -infinity, whose weight is zero, is a NaN. An element that has
-// shown itself a NaN is settled, as is an infinity of one that was no NaN, and where all
-// are, the wave is done. What is then left saw finite values alone: its mean is taken over the keys once more, with every value that is not
-// finite as 0. It is kept as a mean, halved, that each block moves: no sum leaves f32's range.
+// shown itself a NaN is settled, as is an infinity of one that was no NaN, and where all are,
+// the wave is done. What is then left saw finite values alone: its mean is taken over the keys
+// once more, with every value that is not finite as 0. It is kept as a mean, halved, that each
+// block moves: no sum leaves f32's range.
 //
 // `mine`: the wave's own 32 rows of LDS. Rare, and no faster than that asks for: one value that
 // is not finite in the last of 8192 causal tokens, 32 / 8 heads of 128, makes the call 1.6 ms

@@ -29,6 +29,7 @@ E_DECLINED = 5
 DT_NONE = 0
 DT_BF16 = 1
 DT_F32 = 2
+DT_I32 = 3
 
 EPI_NONE = 0
 EPI_GELU_TANH = 1
@@ -105,6 +106,53 @@ class KVCacheC(ctypes.Structure):
         ("page_tokens", ctypes.c_int),
         ("kv_heads", ctypes.c_int),
         ("head_dim", ctypes.c_int),
+    ]
+
+
+class Mx4C(ctypes.Structure):
+    """ltx25_mx4: rows in microscaled 4 bits."""
+
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("rows", ctypes.c_int),
+        ("K", ctypes.c_int),
+    ]
+
+
+class NormC(ctypes.Structure):
+    """ltx25_norm: sizes and types of a norm's tensors."""
+
+    _fields_ = [
+        ("width", ctypes.c_int),
+        ("layer", ctypes.c_int),
+        ("eps", ctypes.c_float),
+        ("residual_scale", ctypes.c_float),
+        ("x_dtype", ctypes.c_int),
+        ("mod_dtype", ctypes.c_int),
+        ("weight_dtype", ctypes.c_int),
+        ("mod_rows", ctypes.c_int),
+        ("x_stride", ctypes.c_int64),
+        ("x_out_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+        ("mod_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+    ]
+
+
+class RotationC(ctypes.Structure):
+    """ltx25_rotation: positions of one to four axes and their frequencies."""
+
+    _fields_ = [
+        ("head_dim", ctypes.c_int),
+        ("rot_dim", ctypes.c_int),
+        ("interleaved", ctypes.c_int),
+        ("n_axes", ctypes.c_int),
+        ("freq_heads", ctypes.c_int),
+        ("pos_dtype", ctypes.c_int),
+        ("freqs", ctypes.c_void_p),
+        ("axes", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
     ]
 
 
@@ -185,6 +233,25 @@ SIGNATURES = {
     "ltx25_attention_cached": (_i, [_vp, ctypes.POINTER(AttnC), ctypes.POINTER(KVCacheC), _vp, _i,
                                     _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _sz]),
     "ltx25_attention_cached_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "ltx25_mx4_scale_bytes": (_sz, [_i, _i]),
+    "ltx25_mx4_quantize_rows": (_i, [_vp, _vp, _i, ctypes.c_int64, ctypes.POINTER(Mx4C)]),
+    "ltx25_mx4_dequant": (_i, [_vp, ctypes.POINTER(Mx4C), _vp, ctypes.c_int64]),
+    "ltx25_mx4_pack_scales": (_i, [_vp, _vp, ctypes.POINTER(Mx4C)]),
+    "ltx25_mx4_unpack_scales": (_i, [_vp, ctypes.POINTER(Mx4C), _vp]),
+    "ltx25_mx4_gemm": (_i, [_vp, ctypes.POINTER(Mx4C), ctypes.POINTER(Mx4C), _vp, _i, _vp, _i, _vp,
+                            _sz]),
+    "ltx25_mx4_gemm_workspace": (_sz, [_i, _i, _i]),
+    "ltx25_linear_mx4": (_i, [_vp, _vp, ctypes.c_int64, _i, ctypes.POINTER(Mx4C), _vp, _i, _vp, _i,
+                              _vp, _sz]),
+    "ltx25_linear_mx4_workspace": (_sz, [_i, _i, _i]),
+    "ltx25_block_norm": (_i, [_vp, ctypes.POINTER(NormC), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                              _vp, _vp, _i]),
+    "ltx25_block_norm_mx4": (_i, [_vp, ctypes.POINTER(NormC), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                  _vp, _vp, ctypes.POINTER(Mx4C), _i]),
+    "ltx25_rope": (_i, [_vp, ctypes.POINTER(RotationC), _vp, _vp, _i, ctypes.c_int64,
+                        ctypes.c_int64, _vp, _vp, _i, ctypes.c_int64, ctypes.c_int64, _i]),
+    "ltx25_kv_append_rope": (_i, [_vp, ctypes.POINTER(KVCacheC), _vp, _i, _vp, _vp, ctypes.c_int64,
+                                  ctypes.c_int64, _vp, _vp, ctypes.POINTER(RotationC), _i, _i]),
 }
 
 _lib = None
@@ -565,6 +632,349 @@ def attention_cached(cache: KVCache, table, lens, q, out, q_len: int, max_len: i
                                         table.data_ptr(), pages, lens.data_ptr(), q.data_ptr(),
                                         out.data_ptr(), _ptr(lse), batch, q_len, max_len, at,
                                         held))
+
+
+# ---- microscaled 4 bits (include/ltx25_mx4.h) ------------------------------------------
+
+
+def _on_device(stream, *tensors) -> int:
+    """The stream to launch on. Without one given it is the current device's, where the tensors
+    must lie (pinned host memory is reached from any)."""
+    if stream is not None:
+        return stream
+    device = (_torch or _import_torch()).cuda.current_device()
+    for t in tensors:
+        if t is not None and t.is_cuda and t.get_device() != device:
+            raise ValueError(f"a tensor lies on {t.device}, the current device is cuda:{device}")
+    return _raw_stream(device)
+
+
+def _float_type(name: str, t) -> int:
+    if t.dtype is _torch.bfloat16:
+        return DT_BF16
+    if t.dtype is _torch.float32:
+        return DT_F32
+    raise TypeError(f"{name} must be bf16 or f32, got {t.dtype}")
+
+
+def _rows(name: str, t, width: int | None = None) -> int:
+    """The elements from a row to the next of a tensor [rows][width] whose rows lie in one piece
+    each."""
+    shape = t.shape
+    if len(shape) != 2 or (width is not None and shape[1] != width):
+        raise ValueError(f"{name} must be [rows][{'width' if width is None else width}], got "
+                         f"{tuple(shape)}")
+    stride = t.stride()
+    if shape[1] > 1 and stride[1] != 1:
+        raise ValueError(f"{name}: a row's values must lie side by side, got strides {stride}")
+    return stride[0] if shape[0] > 1 else (shape[1] + 7) // 8 * 8   # one row: there is no next
+
+
+class MX4:
+    """Rows in microscaled 4 bits, held in torch device tensors (ltx25_mx4): `codes` uint8
+    [rows][K / 2], two values a byte with the earlier one in the low half, and `scales`, uint8 with
+    the blocks' exponents in the order of the matrix cores' reads.
+
+    Calls work on the tensors given here, whose contents may change at will.
+    """
+
+    codes = property(lambda self: self._tensors[0])
+    scales = property(lambda self: self._tensors[1])
+
+    def __init__(self, codes, scales):
+        torch = _torch or _import_torch()
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
+            raise TypeError(f"codes must be contiguous uint8 [rows][K / 2], got {codes.dtype} "
+                            f"{tuple(codes.shape)}")
+        rows, half = codes.shape
+        if half == 0 or half % 16:
+            raise ValueError(f"rows of {2 * half} values: K is a multiple of 32")
+        need = mx4_scale_bytes(rows, 2 * half)
+        if scales.dtype != torch.uint8 or scales.numel() != need or not scales.is_contiguous():
+            raise TypeError(f"scales must be contiguous uint8 with {need} elements, got "
+                            f"{scales.dtype} {tuple(scales.shape)}")
+        if codes.device != scales.device:
+            raise ValueError(f"codes lie on {codes.device}, scales on {scales.device}")
+        self._tensors = (codes, scales)
+        self.rows, self.K = rows, 2 * half
+        self._c = Mx4C(_ptr(codes), _ptr(scales), rows, 2 * half)
+
+    @classmethod
+    def empty(cls, rows: int, K: int, device="cuda"):
+        torch = _torch or _import_torch()
+        return cls(torch.empty((rows, K // 2), dtype=torch.uint8, device=device),
+                   torch.empty(mx4_scale_bytes(rows, K), dtype=torch.uint8, device=device))
+
+    @classmethod
+    def packed(cls, codes, scales, stream=None):
+        """From codes and scales as checkpoints hold them, uint8 [rows][K / 32]
+        (ltx25_mx4_pack_scales)."""
+        torch = _torch or _import_torch()
+        rows, half = codes.shape
+        q = cls(codes, torch.empty(mx4_scale_bytes(rows, 2 * half), dtype=torch.uint8,
+                                   device=codes.device))
+        _check_scales(scales, q)
+        _reachable("scales codes", scales, codes)
+        check(load().ltx25_mx4_pack_scales(_on_device(stream, codes, scales), _ptr(scales),
+                                           ctypes.byref(q.c())))
+        return q
+
+    def unpacked_scales(self, stream=None):
+        """The scales as uint8 [rows][K / 32] (ltx25_mx4_unpack_scales)."""
+        out = self.scales.new_empty((self.rows, self.K // 32))
+        _reachable("scales", self.scales)
+        check(load().ltx25_mx4_unpack_scales(_on_device(stream, out), ctypes.byref(self.c()),
+                                             _ptr(out)))
+        return out
+
+    def c(self) -> Mx4C:
+        return self._c
+
+
+def _check_scales(scales, q: MX4) -> None:
+    if (scales.dtype != _torch.uint8 or tuple(scales.shape) != (q.rows, q.K // 32)
+            or not scales.is_contiguous()):
+        raise TypeError(f"scales must be contiguous uint8 [{q.rows}][{q.K // 32}], got "
+                        f"{scales.dtype} {tuple(scales.shape)}")
+
+
+def mx4_scale_bytes(rows: int, K: int) -> int:
+    return int(load().ltx25_mx4_scale_bytes(rows, K))
+
+
+def mx4_quantize_rows(x, q: MX4, stream=None) -> None:
+    """Codes of the rows of x, bf16 or f32 [rows][K] (ltx25_mx4_quantize_rows)."""
+    if _torch is None:
+        _import_torch()
+    kind = _float_type("x", x)
+    stride = _rows("x", x, q.K)
+    if x.shape[0] != q.rows:
+        raise ValueError(f"x {tuple(x.shape)} does not have q's {q.rows} rows")
+    if not (x.is_cuda and q.codes.is_cuda):
+        _reachable("x q.codes", x, q.codes)
+    check(load().ltx25_mx4_quantize_rows(_on_device(stream, x, q.codes), x.data_ptr(), kind, stride,
+                                         ctypes.byref(q.c())))
+
+
+def mx4_dequant(q: MX4, out, stream=None) -> None:
+    """The values as bf16 [rows][K] (ltx25_mx4_dequant)."""
+    if _torch is None:
+        _import_torch()
+    stride = _rows("out", out, q.K)
+    if out.dtype is not _torch.bfloat16 or out.shape[0] != q.rows:
+        raise TypeError(f"out must be bf16 [{q.rows}][{q.K}], got {out.dtype} {tuple(out.shape)}")
+    if not (out.is_cuda and q.codes.is_cuda):
+        _reachable("out q.codes", out, q.codes)
+    check(load().ltx25_mx4_dequant(_on_device(stream, out, q.codes), ctypes.byref(q.c()),
+                                   out.data_ptr(), stride))
+
+
+def mx4_gemm_workspace(M: int, K: int, N: int) -> int:
+    return int(load().ltx25_mx4_gemm_workspace(M, K, N))
+
+
+def linear_mx4_workspace(M: int, K: int, N: int) -> int:
+    return int(load().ltx25_linear_mx4_workspace(M, K, N))
+
+
+def _product(y, bias, M: int, N: int, workspace, need: int, stream):
+    """What the two products check alike; the workspace, allocated on torch's current stream
+    where none is given."""
+    if y.dtype is not _torch.bfloat16 or tuple(y.shape) != (M, N) or not y.is_contiguous():
+        raise TypeError(f"y must be contiguous bf16 [{M}][{N}], got {y.dtype} {tuple(y.shape)}")
+    if bias is not None and (tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+        raise TypeError(f"bias must be contiguous [{N}], got {tuple(bias.shape)}")
+    if need and workspace is None:
+        if stream is not None:
+            raise ValueError(f"on a stream of the caller's, {need} bytes of workspace are the "
+                             f"caller's too")
+        workspace = _torch.empty(need, dtype=_torch.uint8, device=y.device)
+    return workspace
+
+
+def _held(workspace) -> tuple:
+    if workspace is None:
+        return None, 0
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def mx4_gemm(x: MX4, w: MX4, bias, y, epilogue: int = EPI_NONE, workspace=None,
+             stream=None) -> None:
+    """y [M][N] = epilogue(x . w^T + bias) of two coded operands (ltx25_mx4_gemm)."""
+    if _torch is None:
+        _import_torch()
+    kind = bias_dtype_of(bias)
+    workspace = _product(y, bias, x.rows, w.rows, workspace,
+                         mx4_gemm_workspace(x.rows, x.K, w.rows), stream)
+    if not (y.is_cuda and x.codes.is_cuda and w.codes.is_cuda):
+        _reachable("x.codes w.codes y bias workspace", x.codes, w.codes, y, bias, workspace)
+    elif not ((bias is None or bias.is_cuda) and (workspace is None or workspace.is_cuda)):
+        _reachable("bias workspace", bias, workspace)
+    check(load().ltx25_mx4_gemm(_on_device(stream, y, x.codes, w.codes), ctypes.byref(x.c()),
+                                ctypes.byref(w.c()), _ptr(bias), kind, y.data_ptr(), epilogue,
+                                *_held(workspace)))
+
+
+def linear_mx4(x, w: MX4, bias, y, epilogue: int = EPI_NONE, workspace=None, stream=None) -> None:
+    """y [M][N] = epilogue(coded x . w^T + bias), x bf16 [M][K] (ltx25_linear_mx4)."""
+    if _torch is None:
+        _import_torch()
+    kind = bias_dtype_of(bias)
+    if x.dtype is not _torch.bfloat16:
+        raise TypeError(f"x must be bf16, got {x.dtype}")
+    stride = _rows("x", x, w.K)
+    M, N = x.shape[0], w.rows
+    workspace = _product(y, bias, M, N, workspace, linear_mx4_workspace(M, w.K, N), stream)
+    if not (x.is_cuda and y.is_cuda and w.codes.is_cuda):
+        _reachable("x w.codes y bias workspace", x, w.codes, y, bias, workspace)
+    elif not ((bias is None or bias.is_cuda) and (workspace is None or workspace.is_cuda)):
+        _reachable("bias workspace", bias, workspace)
+    check(load().ltx25_linear_mx4(_on_device(stream, x, y, w.codes), x.data_ptr(), stride, M,
+                                  ctypes.byref(w.c()), _ptr(bias), kind, y.data_ptr(), epilogue,
+                                  *_held(workspace)))
+
+
+# ---- around a block's linears and attention (include/ltx25_block.h) -----------------------
+
+
+def block_norm(x, out, *, y=None, x_out=None, gate=None, post_weight=None, weight=None, scale=None,
+               shift=None, rows=None, layer: bool = False, eps: float = 1e-6,
+               residual_scale: float = 1.0, stream=None) -> None:
+    """The end of one block and the start of the next (ltx25_block_norm):
+
+        u = y, or norm(y) post_weight;  x_out = residual_scale x + gate u
+        out = norm(x_out) weight (1 + scale) + shift
+
+    x, x_out bf16 or f32 [tokens][width]; y bf16; weight, post_weight [width]; gate, scale, shift
+    [mod_rows][width] of one type and row stride; rows int32 [tokens]. Without y, out is of x. out
+    is bf16, an MX4 (ltx25_block_norm_mx4), or None where y is given."""
+    if _torch is None:
+        _import_torch()
+    kind = _float_type("x", x)
+    xs = _rows("x", x)
+    tokens, width = x.shape
+    n = NormC(width, 1 if layer else 0, eps, residual_scale, kind, DT_BF16, DT_BF16, 0, xs, 0, 0, 0,
+              0)
+    if y is not None:
+        n.y_stride = _rows("y", y, width)
+        if y.dtype is not _torch.bfloat16 or y.shape[0] != tokens:
+            raise TypeError(f"y must be bf16 [{tokens}][{width}], got {y.dtype} {tuple(y.shape)}")
+        if x_out is None:
+            raise ValueError("x_out must be given with y (it may be x)")
+    if x_out is not None:
+        n.x_out_stride = _rows("x_out", x_out, width)
+        if x_out.dtype != x.dtype or x_out.shape[0] != tokens:
+            raise TypeError(f"x_out must be {x.dtype} [{tokens}][{width}], got {x_out.dtype} "
+                            f"{tuple(x_out.shape)}")
+    first = None
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is None:
+            continue
+        at = (_float_type(name, t), _rows(name, t, width), t.shape[0])
+        if first is None:
+            first = at
+            n.mod_dtype, n.mod_stride, n.mod_rows = at
+        elif at != first:
+            raise ValueError(f"{name}: gate, scale and shift must be alike in type, rows and row "
+                             f"stride")
+    if rows is not None:
+        _int32("rows", rows, tokens)
+    first = None
+    for name, t in (("post_weight", post_weight), ("weight", weight)):
+        if t is None:
+            continue
+        n.weight_dtype = _float_type(name, t)
+        if tuple(t.shape) != (width,) or not t.is_contiguous() or first not in (None, t.dtype):
+            raise TypeError(f"{name} must be contiguous [{width}], and of one type with the other "
+                            f"weight, got {t.dtype} {tuple(t.shape)}")
+        first = t.dtype
+    coded = isinstance(out, MX4)
+    if coded:
+        if out.rows != tokens or out.K != width:
+            raise ValueError(f"out has {out.rows} rows of {out.K}, not {tokens} of {width}")
+    elif out is not None:
+        n.out_stride = _rows("out", out, width)
+        if out.dtype is not _torch.bfloat16 or out.shape[0] != tokens:
+            raise TypeError(f"out must be bf16 [{tokens}][{width}] or an MX4, got {out.dtype} "
+                            f"{tuple(out.shape)}")
+    held = out.codes if coded else out
+    tensors = (x, held, y, x_out, gate, post_weight, weight, scale, shift, rows)
+    _reachable("x out y x_out gate post_weight weight scale shift rows", *tensors)
+    if coded:
+        fn, to = load().ltx25_block_norm_mx4, ctypes.byref(out.c())
+    else:
+        fn, to = load().ltx25_block_norm, _ptr(out)
+    check(fn(_on_device(stream, *tensors), ctypes.byref(n), _ptr(x), _ptr(y), _ptr(x_out),
+             _ptr(post_weight), _ptr(gate), _ptr(weight), _ptr(scale), _ptr(shift), _ptr(rows), to,
+             tokens))
+
+
+def _rotation(head_dim: int, freqs, axes, positions, tokens: int, interleaved: bool) -> RotationC:
+    if (freqs.dtype is not _torch.float32 or freqs.dim() != 2 or not freqs.is_contiguous()):
+        raise TypeError(f"freqs must be contiguous float32 [1 or heads][pairs], got {freqs.dtype} "
+                        f"{tuple(freqs.shape)}")
+    if axes is not None and (axes.dtype is not _torch.int32 or axes.shape != freqs.shape
+                             or not axes.is_contiguous()):
+        raise TypeError(f"axes must be contiguous int32 {tuple(freqs.shape)}, got {axes.dtype} "
+                        f"{tuple(axes.shape)}")
+    r = RotationC(head_dim, 2 * freqs.shape[1], 1 if interleaved else 0, 1, freqs.shape[0], DT_F32,
+                  _ptr(freqs), _ptr(axes), None)
+    if freqs.shape[1] == 0:
+        raise ValueError("freqs has no pairs")
+    if positions is not None:
+        if positions.dim() != 2 or positions.shape[0] != tokens or not positions.is_contiguous():
+            raise TypeError(f"positions must be contiguous [{tokens}][axes], got "
+                            f"{tuple(positions.shape)}")
+        if positions.dtype is _torch.int32:
+            r.pos_dtype = DT_I32
+        elif positions.dtype is not _torch.float32:
+            raise TypeError(f"positions must be int32 or float32, got {positions.dtype}")
+        r.n_axes, r.positions = positions.shape[1], _ptr(positions)
+    return r
+
+
+def rope(q, k, positions, freqs, axes=None, *, q_out=None, k_out=None, interleaved: bool = False,
+         stream=None) -> None:
+    """Rotates queries and keys, bf16 [tokens][heads][head_dim], by their positions (ltx25_rope), in
+    place or into q_out and k_out. Either of q and k may be None.
+
+    positions int32 or float32 [tokens][axes]; freqs float32 [1 or heads][pairs], axes int32 of the
+    same shape: pair p turns by positions[token][axes[p]] * freqs[p]. interleaved: pair p is
+    channels 2 p and 2 p + 1, else p and p + pairs."""
+    if _torch is None:
+        _import_torch()
+    given = q if q is not None else k
+    if given is None or (q is None and q_out is not None) or (k is None and k_out is not None):
+        raise ValueError("rope rotates q, k or both, and an output goes with its input")
+    tokens, _, dim = given.shape
+    args = []
+    for name, t, to in (("q", q, q_out), ("k", k, k_out)):
+        if t is None:
+            args += [None, None, 0, 0, 0]
+            continue
+        to = t if to is None else to
+        ts, os_ = _tokens(name, t, t.shape), _tokens(name + "_out", to, to.shape)
+        if t.shape != to.shape or t.shape[0] != tokens or t.shape[2] != dim:
+            raise ValueError(f"{name} {tuple(t.shape)} and {name}_out {tuple(to.shape)} are not "
+                             f"both {tokens} tokens of heads of {dim}")
+        args += [t.data_ptr(), to.data_ptr(), t.shape[1], ts, os_]
+    r = _rotation(dim, freqs, axes, positions, tokens, interleaved)
+    tensors = (q, k, positions, freqs, axes, q_out, k_out)
+    _reachable("q k positions freqs axes q_out k_out", *tensors)
+    check(load().ltx25_rope(_on_device(stream, *tensors), ctypes.byref(r), *args, tokens))
+
+
+def kv_append_rope(cache: KVCache, table, k, v, cu, start, freqs, axes=None, positions=None, *,
+                   interleaved: bool = False, stream=None) -> None:
+    """kv_append with the keys rotated on the way (ltx25_kv_append_rope): the bits of rope on k and
+    kv_append. positions [total][axes] as for rope, or None: a token's place in its sequence on
+    every axis."""
+    args = _moved(cache, table, k, v, cu, start)
+    r = _rotation(cache.head_dim, freqs, axes, positions, k.shape[0], interleaved)
+    tensors = (freqs, axes, positions)
+    _reachable("freqs axes positions", *tensors)
+    check(load().ltx25_kv_append_rope(_on_device(stream, k, v, table, *tensors), *args[:9],
+                                      ctypes.byref(r), *args[9:]))
 
 
 def probe_read(src, nbytes: int, sink, blocks: int, stream=None) -> None:

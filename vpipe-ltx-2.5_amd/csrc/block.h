@@ -1,0 +1,169 @@
+// Rotations on the device, and the launchers of the norms and rotations
+// (norm.hip, rope.hip, kv_cache.hip) that their C ABI layer (capi_block.cpp) calls.
+#pragma once
+
+#include "attention.h"
+#include "mx4.h"
+
+namespace ltx25 {
+
+constexpr int kAxesMax = 4;
+
+// ltx25_rotation as the kernels take it
+struct Rotation {
+  const float* freqs = nullptr;
+  const int* axes = nullptr;         // null: axis 0
+  const void* positions = nullptr;   // null: a token's place in its sequence
+  int pairs = 0;                     // rot_dim / 2
+  int n_axes = 1;
+  bool whole = false;                // positions are int32
+  bool per_head = false;
+  bool interleaved = false;
+};
+
+// A token's positions in turns (divided by 2 pi), in 64 bits
+struct Turns {
+  double at[kAxesMax];
+};
+
+__device__ __forceinline__ Turns turns_of(const Rotation& r, long token)
+{
+  constexpr double kInv2Pi = 0.15915494309189533577;
+  Turns t;
+#pragma unroll
+  for (int a = 0; a < kAxesMax; ++a) {
+    const long at = token * r.n_axes + min(a, r.n_axes - 1);
+    t.at[a] = (r.whole ? (double)((const int*)r.positions)[at]
+                       : (double)((const float*)r.positions)[at]) * kInv2Pi;
+  }
+  return t;
+}
+
+__device__ __forceinline__ Turns turns_at(long place)
+{
+  constexpr double kInv2Pi = 0.15915494309189533577;
+  const double t = (double)place * kInv2Pi;
+  return {{t, t, t, t}};
+}
+
+// The sine and cosine of one pair's angle. The product and the removal of whole turns in 64
+// bits: an angle of 2^20 radians has 2^-4 left of its own last bits in 32. What is left, at
+// most half a turn, goes to the hardware's sine and cosine, whose argument is in turns.
+__device__ __forceinline__ void sin_cos(const Turns& t, float freq, int axis, float& sn, float& cs)
+{
+  double at = t.at[0];
+  at = axis == 1 ? t.at[1] : at;
+  at = axis == 2 ? t.at[2] : at;
+  at = axis >= 3 ? t.at[3] : at;
+  const double turns = at * (double)freq;
+  const float left = (float)(turns - rint(turns));
+  sn = __builtin_amdgcn_sinf(left);
+  cs = __builtin_amdgcn_cosf(left);
+}
+
+// N consecutive pairs' frequencies and axes (N 4 or 8, the first a multiple of 4)
+template <int N>
+struct Pairs {
+  float freq[N];
+  int axis[N];
+};
+template <int N>
+__device__ __forceinline__ Pairs<N> pairs_of(const Rotation& r, int head, int first)
+{
+  Pairs<N> p;
+  const long at = (long)(r.per_head ? head : 0) * r.pairs + first;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const f32x4 f = *(const f32x4*)(r.freqs + at + i);
+    const i32x4 a = r.axes != nullptr ? *(const i32x4*)(r.axes + at + i) : i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      p.freq[i + k] = f[k];
+      p.axis[i + k] = min(a[k], r.n_axes - 1);
+    }
+  }
+  return p;
+}
+
+// Two bf16 (low, high half) as floats
+__device__ __forceinline__ float low_f32(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_f32(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// (a, b) turned: a cos - b sin, a sin + b cos
+__device__ __forceinline__ float turned_a(float a, float b, float sn, float cs)
+{
+  return fmaf(a, cs, -(b * sn));
+}
+__device__ __forceinline__ float turned_b(float a, float b, float sn, float cs)
+{
+  return fmaf(a, sn, b * cs);
+}
+
+// Eight channels of pairs side by side, turned
+__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pairs<4>& p)
+{
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float sn, cs;
+    sin_cos(t, p.freq[i], p.axis[i], sn, cs);
+    const float a = low_f32(w[i]), b = high_f32(w[i]);
+    w[i] = pack_bf16x2(turned_a(a, b, sn, cs), turned_b(a, b, sn, cs));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Eight pairs, their first channels in xa and their second in xb
+__device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns& t,
+                                              const Pairs<8>& p)
+{
+  uint32_t a[4] = {xa.x, xa.y, xa.z, xa.w}, b[4] = {xb.x, xb.y, xb.z, xb.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float s0, c0, s1, c1;
+    sin_cos(t, p.freq[2 * i], p.axis[2 * i], s0, c0);
+    sin_cos(t, p.freq[2 * i + 1], p.axis[2 * i + 1], s1, c1);
+    const float a0 = low_f32(a[i]), a1 = high_f32(a[i]), b0 = low_f32(b[i]), b1 = high_f32(b[i]);
+    a[i] = pack_bf16x2(turned_a(a0, b0, s0, c0), turned_a(a1, b1, s1, c1));
+    b[i] = pack_bf16x2(turned_b(a0, b0, s0, c0), turned_b(a1, b1, s1, c1));
+  }
+  xa = make_uint4(a[0], a[1], a[2], a[3]);
+  xb = make_uint4(b[0], b[1], b[2], b[3]);
+}
+
+// ---- launchers --------------------------------------------------------------
+
+struct RopeArgs {
+  Rotation r;
+  const uint16_t* in[2] = {nullptr, nullptr};   // queries, keys
+  uint16_t* out[2] = {nullptr, nullptr};
+  int64_t in_stride[2] = {0, 0}, out_stride[2] = {0, 0};
+  int heads[2] = {0, 0};
+  int head_dim = 0, tokens = 0;
+};
+hipError_t launch_rope(const RopeArgs& a, hipStream_t stream);
+
+hipError_t launch_kv_append_rope(const CacheArgs& c, const uint16_t* k, const uint16_t* v,
+                                 int64_t ks, int64_t vs, const int* cu, const int* start,
+                                 const Rotation& r, int batch, int total, hipStream_t stream);
+
+struct NormArgs {
+  const void* x = nullptr;
+  const uint16_t* y = nullptr;
+  void* x_out = nullptr;
+  const void* after = nullptr;    // post_weight
+  const void* gate = nullptr;
+  const void* weight = nullptr;
+  const void* scale = nullptr;
+  const void* shift = nullptr;
+  const int* rows = nullptr;
+  uint16_t* out = nullptr;
+  Mx4Args q;                      // codes null: out is bf16 (or none)
+  int64_t xs = 0, xos = 0, ys = 0, ms = 0, os = 0;
+  int width = 0, tokens = 0, mod_rows = 0, run = 1;   // run: tokens of a modulation row
+  bool layer = false, wide = false, mod_wide = false, weight_wide = false;
+  float eps = 0.0f, alpha = 1.0f;
+};
+hipError_t launch_norm(const NormArgs& a, hipStream_t stream);
+
+}  // namespace ltx25

@@ -1,9 +1,10 @@
 // The C ABI of attention and its cache (include/ltx25_attention.h): argument
 // validation ahead of any HIP call, then the launch. No state: what a call
 // needs is its own tensors and the caller's workspace.
-#include "ltx25_attention.h"
+#include "ltx25_block.h"
 
-#include "attention.h"
+#include "block.h"
+#include "checks.h"
 
 #include <hip/hip_runtime.h>
 
@@ -11,32 +12,14 @@
 
 namespace {
 
+using namespace ltx25::checks;
 using ltx25::set_error;
-
-int hip_error(hipError_t e, const char* what)
-{
-  return set_error(LTX25_E_HIP, "%s: %s", what, hipGetErrorString(e));
-}
-
-bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
-
-int check_pointer(const char* name, const void* p, uintptr_t align)
-{
-  if (p == nullptr) { return set_error(LTX25_E_INVAL, "%s is null", name); }
-  if (!aligned(p, align)) {
-    return set_error(LTX25_E_INVAL, "%s (%p) is not %d-byte aligned", name, p, (int)align);
-  }
-  return LTX25_OK;
-}
 
 // The kernels form a 64-token tile's offsets in 32 bits.
 constexpr int64_t kStrideMax = (int64_t)1 << 23;
 // Tokens of a cached sequence; positions past them would not fit the kernels' 32-bit
 // token numbers.
 constexpr int kTokensMax = 1 << 30;
-// Packed tokens of a call: no sequence then has more than 2^24 units of work
-// (find_unit's bound), nor 64 sequences' units more than 32 bits hold.
-constexpr int kPackedMax = 1 << 27;
 
 int check_stride(const char* name, int64_t stride, int heads, int head_dim)
 {
@@ -110,24 +93,6 @@ int check_cache(const ltx25_kv_cache* c, const int* table, int table_stride, int
   out->table = table;
   out->table_stride = table_stride;
   return LTX25_OK;
-}
-
-int check_tokens(const char* name, long tokens, int most)
-{
-  if (tokens < 0 || tokens > most) {
-    return set_error(LTX25_E_INVAL, "%s=%ld is not in 0 .. %d", name, tokens, most);
-  }
-  return LTX25_OK;
-}
-
-int check_workspace(const void* workspace, size_t bytes, size_t need)
-{
-  const int rc = check_pointer("workspace", workspace, 16);
-  if (rc == LTX25_OK && bytes < need) {
-    return set_error(LTX25_E_INVAL, "the workspace has %zu bytes; this call needs %zu", bytes,
-                     need);
-  }
-  return rc;
 }
 
 // What append and read share.
@@ -260,6 +225,34 @@ int ltx25_kv_append(void* stream, const ltx25_kv_cache* cache, const int* table,
       ltx25::launch_kv_append(c, (const uint16_t*)k, (const uint16_t*)v, k_stride, v_stride, cu,
                               start, batch, total, (hipStream_t)stream);
   return e == hipSuccess ? LTX25_OK : hip_error(e, "kv_append launch");
+}
+
+int ltx25_kv_append_rope(void* stream, const ltx25_kv_cache* cache, const int* table,
+                         int table_stride, const void* k, const void* v, int64_t k_stride,
+                         int64_t v_stride, const int* cu, const int* start,
+                         const ltx25_rotation* r, int batch, int total)
+{
+  ltx25::CacheArgs c;
+  ltx25::Rotation rot;
+  int rc = check_move(cache, table, table_stride, k, v, k_stride, v_stride, cu, start, batch, total,
+                      &c);
+  if (rc != LTX25_OK) { return rc; }
+  const bool work = batch > 0 && total > 0;
+  if ((rc = ltx25::check_rotation(r, work, true, &rot)) != LTX25_OK) { return rc; }
+  if (r->head_dim != c.head_dim) {
+    return set_error(LTX25_E_INVAL, "the rotation is of heads of width %d, the cache's are of %d",
+                     r->head_dim, c.head_dim);
+  }
+  if (r->freq_heads != 1 && r->freq_heads != c.kv_heads) {
+    return set_error(LTX25_E_INVAL, "freq_heads=%d is neither 1 nor the cache's kv_heads=%d",
+                     r->freq_heads, c.kv_heads);
+  }
+  if (!work) { return LTX25_OK; }
+  if ((rc = ltx25::check_device()) != LTX25_OK) { return rc; }
+  const hipError_t e =
+      ltx25::launch_kv_append_rope(c, (const uint16_t*)k, (const uint16_t*)v, k_stride, v_stride,
+                                   cu, start, rot, batch, total, (hipStream_t)stream);
+  return e == hipSuccess ? LTX25_OK : hip_error(e, "kv_append_rope launch");
 }
 
 int ltx25_kv_read(void* stream, const ltx25_kv_cache* cache, const int* table, int table_stride,

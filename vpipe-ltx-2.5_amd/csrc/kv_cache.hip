@@ -1,7 +1,7 @@
 // The paged cache of 8-bit keys and values: appending to it, reading it back,
 // and attention over it (ltx25_kv_append, ltx25_kv_read,
 // ltx25_attention_cached).
-#include "attention.h"
+#include "block.h"
 
 #include <algorithm>
 #include <climits>
@@ -120,6 +120,7 @@ struct Span {
   const int* id;   // where the page's id is; null past the table
   int lo, hi;
   long first;
+  long place;      // of the page's token 0 in its sequence
 };
 
 // The unit blockIdx.x of all sequences' touched pages; false past the last.
@@ -143,6 +144,7 @@ __device__ __forceinline__ bool find_span(const MoveParams& p, Span& s)
   s.lo = (int)(max((long)at, t0) - t0);
   s.hi = (int)(min((long)at + n, t0 + (1 << p.c.pl)) - t0);
   s.first = c0 + (t0 - at);
+  s.place = t0;
   s.id = page < p.c.table_stride ? p.c.table + (long)seq * p.c.table_stride + page : nullptr;
   return true;
 }
@@ -197,8 +199,12 @@ __device__ __forceinline__ uint2 quantize8(uint4 x, float s, float rs)
 //
 // Bound by memory where there is much to do: 8192 tokens of 8 heads of 128, 50 MB read
 // and written, 14.9 us (3.4 TB/s; a page's first code waits for all its values).
-template <int D>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
+//
+// ROPE: the keys are turned in registers as they arrive and rounded to bf16, and from there on
+// are the keys of a plain append. Pairs half of the rotated channels apart meet by an exchange
+// of 16-byte pieces between lanes of one token.
+template <int D, bool ROPE = false>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotation rot)
 {
   constexpr int kMaxP = 128;
   constexpr int kPer = D / 8;   // 16-byte pieces of a token
@@ -221,6 +227,34 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
   const int pid = *sp.id;
   const int quad0 = sp.lo >> 2;
   const int pieces = few ? (sp.hi - sp.lo) * kPer : (((sp.hi + 3) >> 2) - quad0) * kPer;
+  // a key of the page's token `tok`, the lane's piece of it; every lane of a wave takes part
+  auto rotate = [&](uint4& w, int tok) {
+    if constexpr (ROPE) {
+      const int piece = tid % kPer;
+      const bool there = tok >= sp.lo && tok < sp.hi && piece * 8 < 2 * rot.pairs;
+      const int first = rot.interleaved ? piece * 4 : piece * 8 % rot.pairs;
+      const int apart = rot.interleaved ? 0 : rot.pairs / 8;
+      const bool second = !rot.interleaved && piece >= apart;
+      uint4 other = w;
+      if (!rot.interleaved) {
+        const int from = (tid & 63) + (second ? -apart : apart);
+        other.x = __shfl((int)w.x, from);
+        other.y = __shfl((int)w.y, from);
+        other.z = __shfl((int)w.z, from);
+        other.w = __shfl((int)w.w, from);
+      }
+      if (!there) { return; }
+      const Turns t = rot.positions != nullptr ? turns_of(rot, sp.first + tok)
+                                               : turns_at(sp.place + tok);
+      if (rot.interleaved) {
+        w = rotate_side(w, t, pairs_of<4>(rot, g, first));
+      } else {
+        uint4 a = second ? other : w, b = second ? w : other;
+        rotate_halves(a, b, t, pairs_of<8>(rot, g, first));
+        w = second ? b : a;
+      }
+    }
+  };
   uint4 held[kHeld][4];
   uint32_t top = 0;
   bool odd = false;   // an infinity or a NaN among the lane's values
@@ -229,6 +263,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
     if (tid < pieces) {
       held[0][0] = *(const uint4*)(x + (sp.first + sp.lo + tid / kPer) * stride + (tid % kPer) * 8);
     }
+    if (ROPE && !values) { rotate(held[0][0], sp.lo + tid / kPer); }
     const u16x2 tops = max_magnitudes(u16x2{0, 0}, held[0][0]);
     top = max((uint32_t)tops[0], (uint32_t)tops[1]);
     odd = top >= 0x7f80u;
@@ -244,6 +279,15 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p)
         held[i][j] = make_uint4(0, 0, 0, 0);
         if (at < pieces && tok >= sp.lo && tok < sp.hi) {
           held[i][j] = *(const uint4*)(x + (sp.first + tok) * stride + (at % kPer) * 8);
+        }
+      }
+    }
+    if (ROPE && !values) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          rotate(held[i][j], (quad0 + (tid + i * kThreads) / kPer) * 4 + j);
         }
       }
     }
@@ -877,9 +921,25 @@ hipError_t launch_kv_append(const CacheArgs& c, const uint16_t* k, const uint16_
   dim3 grid;
   if (!move_grid(p, grid)) { return hipErrorInvalidConfiguration; }
   if (c.head_dim == 128) {
-    kv_append_kernel<128><<<grid, kThreads, 0, stream>>>(p);
+    kv_append_kernel<128><<<grid, kThreads, 0, stream>>>(p, Rotation());
   } else {
-    kv_append_kernel<64><<<grid, kThreads, 0, stream>>>(p);
+    kv_append_kernel<64><<<grid, kThreads, 0, stream>>>(p, Rotation());
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_append_rope(const CacheArgs& c, const uint16_t* k, const uint16_t* v,
+                                 int64_t ks, int64_t vs, const int* cu, const int* start,
+                                 const Rotation& r, int batch, int total, hipStream_t stream)
+{
+  const MoveParams p = {view_of(c), k, v, nullptr, nullptr, (long)ks, (long)vs, cu, start, batch,
+                        total};
+  dim3 grid;
+  if (!move_grid(p, grid)) { return hipErrorInvalidConfiguration; }
+  if (c.head_dim == 128) {
+    kv_append_kernel<128, true><<<grid, kThreads, 0, stream>>>(p, r);
+  } else {
+    kv_append_kernel<64, true><<<grid, kThreads, 0, stream>>>(p, r);
   }
   return hipGetLastError();
 }

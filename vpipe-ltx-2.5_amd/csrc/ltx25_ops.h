@@ -16,6 +16,8 @@
 #pragma once
 
 #include "ltx25_attention.h"
+#include "ltx25_block.h"
+#include "ltx25_mx4.h"
 #include "ltx25_qlinear.h"
 
 #include <hip/hip_runtime.h>
@@ -179,6 +181,70 @@ public:
   static size_t attention_cached_workspace(const ltx25_attn& a, int batch, int q_len, int max_len)
   {
     return ltx25_attention_cached_workspace(batch, q_len, a.heads, a.kv_heads, a.head_dim, max_len);
+  }
+
+  // The microscaled 4-bit tier: rows to codes and back, the product of two coded
+  // operands, and a linear that codes its activations on the way.
+  void mx4_quantize_rows(hipStream_t enc, const void* x, int x_dtype, int64_t x_stride,
+                         const ltx25_mx4& q) const
+  {
+    note(ltx25_mx4_quantize_rows(enc, x, x_dtype, x_stride, &q));
+  }
+  void mx4_dequant(hipStream_t enc, const ltx25_mx4& q, void* out, int64_t out_stride) const
+  {
+    note(ltx25_mx4_dequant(enc, &q, out, out_stride));
+  }
+  void mx4_gemm(hipStream_t enc, const ltx25_mx4& x, const ltx25_mx4& w, const void* bias, void* y,
+                bool gelu, void* workspace, size_t workspace_bytes) const
+  {
+    note(ltx25_mx4_gemm(enc, &x, &w, bias, bias != nullptr ? LTX25_DT_BF16 : LTX25_DT_NONE, y,
+                        gelu ? LTX25_EPI_GELU_TANH : LTX25_EPI_NONE, workspace, workspace_bytes));
+  }
+  void linear_mx4(hipStream_t enc, const void* x, int64_t x_stride, int M, const ltx25_mx4& w,
+                  const void* bias, void* y, bool gelu, void* workspace,
+                  size_t workspace_bytes) const
+  {
+    note(ltx25_linear_mx4(enc, x, x_stride, M, &w, bias,
+                          bias != nullptr ? LTX25_DT_BF16 : LTX25_DT_NONE, y,
+                          gelu ? LTX25_EPI_GELU_TANH : LTX25_EPI_NONE, workspace, workspace_bytes));
+  }
+  static size_t mx4_gemm_workspace(int M, int K, int N) { return ltx25_mx4_gemm_workspace(M, K, N); }
+  static size_t linear_mx4_workspace(int M, int K, int N)
+  {
+    return ltx25_linear_mx4_workspace(M, K, N);
+  }
+
+  // Around the linears and the attention: a block's end and the next one's norm, with a
+  // bf16 or a 4-bit output, and rotated positions.
+  void block_norm(hipStream_t enc, const ltx25_norm& n, const void* x, const void* y, void* x_out,
+                  const void* post_weight, const void* gate, const void* weight, const void* scale,
+                  const void* shift, const int* rows, void* out, int tokens) const
+  {
+    note(ltx25_block_norm(enc, &n, x, y, x_out, post_weight, gate, weight, scale, shift, rows, out,
+                          tokens));
+  }
+  void block_norm_mx4(hipStream_t enc, const ltx25_norm& n, const void* x, const void* y,
+                      void* x_out, const void* post_weight, const void* gate, const void* weight,
+                      const void* scale, const void* shift, const int* rows, const ltx25_mx4& q,
+                      int tokens) const
+  {
+    note(ltx25_block_norm_mx4(enc, &n, x, y, x_out, post_weight, gate, weight, scale, shift, rows,
+                              &q, tokens));
+  }
+  // In place, q and k at a.q_stride and a.k_stride.
+  void rope(hipStream_t enc, const ltx25_rotation& r, const ltx25_attn& a, void* q, void* k,
+            int tokens) const
+  {
+    note(ltx25_rope(enc, &r, q, q, a.heads, a.q_stride, a.q_stride, k, k, a.kv_heads, a.k_stride,
+                    a.k_stride, tokens));
+  }
+  void kv_append_rope(hipStream_t enc, const ltx25_attn& a, const ltx25_kv_cache& cache,
+                      const int* table, int table_stride, const void* k, const void* v,
+                      const int* cu, const int* start, const ltx25_rotation& r, int batch,
+                      int total) const
+  {
+    note(ltx25_kv_append_rope(enc, &cache, table, table_stride, k, v, a.k_stride, a.v_stride, cu,
+                              start, &r, batch, total));
   }
 
   // The dequant-once arm (src/ltx25-metal-ops.cc:467-502): LTX25_DEQUANT_ONCE_*.

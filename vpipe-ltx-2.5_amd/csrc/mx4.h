@@ -1,0 +1,118 @@
+// Device helpers of the microscaled 4-bit formats (E2M1 codes, an E8M0 exponent for
+// each block of 32), and the launchers that their C ABI layer (capi_mx4.cpp) calls.
+#pragma once
+
+#include "common.h"
+
+namespace ltx25 {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// Where the scales of a block lie (include/ltx25_mx4.h): tiles of 16 rows x 16 blocks,
+// 256 bytes; lane l of a wave reads dword l of a tile, the four blocks b % 4 = l / 16 of
+// row l % 16, one for each of the four matrix instructions that span the tile's 512
+// values. The instruction takes a lane's block and scale from the same lane, so that no
+// byte changes lanes.
+constexpr int kMx4Tile = 256;
+__host__ __device__ inline int mx4_spans(int K) { return (K + 511) / 512; }
+__host__ __device__ inline size_t mx4_scale_bytes(long rows, int K)
+{
+  return (size_t)((rows + 15) / 16) * mx4_spans(K) * kMx4Tile;
+}
+__device__ __forceinline__ int mx4_scale_at(int row, int block)   // within its tile
+{
+  return ((block & 3) * 16 + (row & 15)) * 4 + ((block >> 2) & 3);
+}
+
+// The exponent byte of a block whose largest magnitude has these bits (as f32):
+// floor(log2) - 2 + 127, not below 0; 255 where it is no finite number.
+__device__ __forceinline__ uint32_t mx4_scale(uint32_t top)
+{
+  const uint32_t e = top >> 23;
+  return e == 255 ? 255u : (uint32_t)max((int)e - 2, 0);
+}
+// 2^-exponent of a finite block: within 2^-125 .. 2^127
+__device__ __forceinline__ float mx4_factor(uint32_t scale)
+{
+  return __uint_as_float((254u - min(scale, 253u)) << 23);
+}
+
+// Eight values times 2^-exponent to codes, the first in the low bits: to the nearest,
+// ties to the even code, beyond 6 to 6 (the conversion's own rule).
+__device__ __forceinline__ uint32_t mx4_codes(const float (&v)[8], float f)
+{
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0] * f, v[1] * f, 1.0f, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2] * f, v[3] * f, 1.0f, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4] * f, v[5] * f, 1.0f, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6] * f, v[7] * f, 1.0f, 3);
+  return r;
+}
+
+// The larger of v over the lane's four (lanes 4 n .. 4 n + 3)
+__device__ __forceinline__ uint32_t quad_max(uint32_t v)
+{
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));   // 1 0 3 2
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // 2 3 0 1
+  return v;
+}
+
+// A block of 32 held by four lanes, eight values each: its exponent byte and the
+// lane's eight codes
+__device__ __forceinline__ uint32_t mx4_code_quad(const float (&v)[8], uint32_t& scale)
+{
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { top = max(top, __float_as_uint(v[i]) & 0x7fffffffu); }
+  scale = mx4_scale(quad_max(top));
+  return scale == 255u ? 0u : mx4_codes(v, mx4_factor(scale));
+}
+
+// A matrix operand of a lane: 32 codes, in the low half of the instruction's register
+// list (4-bit operands do not use the rest)
+__device__ __forceinline__ i32x8 mx4_operand(i32x4 v)
+{
+  return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+}
+constexpr int kMfmaFp4 = 4;   // the instruction's format number of E2M1
+
+// ---- launchers --------------------------------------------------------------
+
+// An operand: `rows` rows of K values
+struct Mx4Args {
+  uint8_t* codes = nullptr;
+  uint8_t* scales = nullptr;
+  int rows = 0, K = 0;
+};
+hipError_t launch_mx4_quantize(const void* x, bool wide, int64_t stride, const Mx4Args& q,
+                               hipStream_t stream);
+hipError_t launch_mx4_dequant(const Mx4Args& q, uint16_t* out, int64_t stride, hipStream_t stream);
+hipError_t launch_mx4_scales(const uint8_t* in, uint8_t* out, int rows, int K, bool pack,
+                             hipStream_t stream);
+
+// y = epilogue(x . w^T + bias). `xb` set: bf16 activations at xb_stride, coded on the
+// way; x then says where their codes go where the plan codes them ahead.
+struct Mx4Gemm {
+  Mx4Args x, w;
+  const uint16_t* xb = nullptr;
+  int64_t xb_stride = 0;
+  const void* bias = nullptr;
+  int bias_type = kBiasNone;
+  int epilogue = kEpiNone;
+  uint16_t* y = nullptr;
+  float* partial = nullptr;   // plan.partial_bytes
+};
+// How a product is cut; a function of the sizes alone, so that the workspace can be
+// asked for ahead.
+struct Mx4Plan {
+  int tile = 0;         // rows x columns of a workgroup: 0 128 x 128, 1 64 x 64
+  int splits = 1;       // parts of K
+  int span_chunk = 0;   // 512-value spans of a part
+  bool codes_ahead = false;   // bf16 activations are coded by a launch ahead
+  size_t partial_bytes = 0;
+};
+// `bf16`: the activations come in bf16
+Mx4Plan plan_mx4(int M, int K, int N, bool bf16);
+hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t stream);
+
+}  // namespace ltx25

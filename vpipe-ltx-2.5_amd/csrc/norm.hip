@@ -1,0 +1,227 @@
+// Norms fused with the gate, the residual and the modulation (ltx25_block_norm,
+// ltx25_block_norm_mx4).
+#include "block.h"
+
+#include <algorithm>
+
+namespace ltx25 {
+namespace {
+
+// 8 values from element `at` of a bf16 or f32 tensor
+__device__ __forceinline__ void load8(const void* p, bool wide, long at, float (&v)[8])
+{
+  if (wide) {
+    const f32x4 a = ((const f32x4*)((const float*)p + at))[0];
+    const f32x4 b = ((const f32x4*)((const float*)p + at))[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = a[i];
+      v[4 + i] = b[i];
+    }
+  } else {
+    const uint4 w = *(const uint4*)((const uint16_t*)p + at);
+    v[0] = low_f32(w.x), v[1] = high_f32(w.x), v[2] = low_f32(w.y), v[3] = high_f32(w.y);
+    v[4] = low_f32(w.z), v[5] = high_f32(w.z), v[6] = low_f32(w.w), v[7] = high_f32(w.w);
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8])
+{
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                    pack_bf16x2(v[6], v[7]));
+}
+
+// WAVES waves hold a token, CH chunks of eight values a lane: lane l of wave w has the
+// chunks w * 64 + l + i * 64 * WAVES. A single wave's tokens share a workgroup of four.
+//
+// Sums in f32, the mean taken off before the squares are added; where a sum leaves f32's
+// range the values are taken 2^-80 times as large, which leaves every square that counts
+// inside it.
+template <int WAVES, int CH>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(NormArgs p, long first)
+{
+  __shared__ float part[4][WAVES];
+  const int lane = threadIdx.x & 63;
+  const int wave = WAVES == 1 ? 0 : (int)(threadIdx.x >> 6);
+  const long token =
+      first + (WAVES == 1 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x);
+  if (token >= p.tokens) { return; }
+  int turn = 0;
+  auto total = [&](float v) {
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) { v += __shfl_xor(v, i); }
+    if constexpr (WAVES > 1) {
+      // the next sum's slots are others: its writers do not meet this one's readers
+      float* const at = part[turn & 3];
+      ++turn;
+      if (lane == 0) { at[wave] = v; }
+      __syncthreads();
+      v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) { v += at[w]; }
+    }
+    return v;
+  };
+  int col[CH];
+  bool in[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    col[i] = (i * 64 * WAVES + wave * 64 + lane) * 8;
+    in[i] = col[i] < p.width;
+  }
+  const float over = 1.0f / (float)p.width;
+  // v -> (v - mean) / sqrt(mean square + eps), zeros past the width kept
+  auto normalise = [&](float (&v)[CH][8]) {
+#pragma unroll 1
+    for (int far = 0; far < 2; ++far) {
+      const float unit = far ? 0x1p-80f : 1.0f;
+      float mean = 0.0f;
+      if (p.layer) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) { s += in[i] ? v[i][k] * unit : 0.0f; }
+        }
+        mean = total(s) * over;
+      }
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float d = fmaf(v[i][k], unit, -mean);
+          s += in[i] ? d * d : 0.0f;
+        }
+      }
+      const float square = total(s) * over;
+      if (far == 0 && !(square < INFINITY)) { continue; }
+      const float eps = far ? 0x1p-126f : p.eps;
+      const float rs = 1.0f / sqrtf(square + eps);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { v[i][k] = fmaf(v[i][k], unit, -mean) * rs; }
+      }
+      break;
+    }
+  };
+
+  float x[CH][8];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { x[i][k] = 0.0f; }
+    if (in[i]) { load8(p.x, p.wide, token * p.xs + col[i], x[i]); }
+  }
+  long row = 0;
+  if (p.mod_rows > 0) {
+    row = p.rows != nullptr ? clampi(p.rows[token], 0, p.mod_rows - 1) : token / p.run;
+    row *= p.ms;
+  }
+  if (p.y != nullptr) {
+    float y[CH][8];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { y[i][k] = 0.0f; }
+      if (in[i]) { load8(p.y, false, token * p.ys + col[i], y[i]); }
+    }
+    if (p.after != nullptr) { normalise(y); }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      if (!in[i]) { continue; }
+      float m[8];
+      if (p.after != nullptr) {
+        load8(p.after, p.weight_wide, col[i], m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { y[i][k] *= m[k]; }
+      }
+      if (p.gate != nullptr) {
+        load8(p.gate, p.mod_wide, row + col[i], m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { y[i][k] *= m[k]; }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { x[i][k] = fmaf(p.alpha, x[i][k], y[i][k]); }
+      if (p.wide) {
+        f32x4* const o = (f32x4*)((float*)p.x_out + token * p.xos + col[i]);
+        o[0] = f32x4{x[i][0], x[i][1], x[i][2], x[i][3]};
+        o[1] = f32x4{x[i][4], x[i][5], x[i][6], x[i][7]};
+      } else {
+        *(uint4*)((uint16_t*)p.x_out + token * p.xos + col[i]) = pack8(x[i]);
+      }
+    }
+  }
+  if (p.out == nullptr && p.q.codes == nullptr) { return; }
+  normalise(x);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    if (in[i]) {
+      float m[8];
+      if (p.weight != nullptr) {
+        load8(p.weight, p.weight_wide, col[i], m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { x[i][k] *= m[k]; }
+      }
+      if (p.scale != nullptr) {
+        load8(p.scale, p.mod_wide, row + col[i], m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { x[i][k] *= 1.0f + m[k]; }
+      }
+      if (p.shift != nullptr) {
+        load8(p.shift, p.mod_wide, row + col[i], m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { x[i][k] += m[k]; }
+      }
+      if (p.out != nullptr) { *(uint4*)(p.out + token * p.os + col[i]) = pack8(x[i]); }
+    }
+    if (p.q.codes != nullptr) {
+      // a block's four lanes are in or out together: the width is a multiple of 32
+      const int block = col[i] >> 5, spans = mx4_spans(p.width);
+      if (in[i]) {
+        uint32_t scale;
+        const uint32_t codes = mx4_code_quad(x[i], scale);
+        *(uint32_t*)(p.q.codes + token * (p.width >> 1) + (col[i] >> 1)) = codes;
+        if ((lane & 3) == 0) {
+          p.q.scales[((token >> 4) * spans + (block >> 4)) * kMx4Tile +
+                     mx4_scale_at((int)(token & 15), block)] = (uint8_t)scale;
+        }
+      } else if ((lane & 3) == 0 && block < spans * 16) {
+        p.q.scales[((token >> 4) * spans + (block >> 4)) * kMx4Tile +
+                   mx4_scale_at((int)(token & 15), block)] = 0;
+      }
+    }
+  }
+}
+
+template <int WAVES, int CH>
+hipError_t run(const NormArgs& a, hipStream_t stream)
+{
+  // a launch has fewer than 2^32 threads
+  constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES, kTokens = WAVES == 1 ? 4 : 1;
+  constexpr long kMost = ((1L << 32) / kThreads - 1) * kTokens;
+  for (long first = 0; first < a.tokens; first += kMost) {
+    const long n = std::min(kMost, a.tokens - first);
+    norm_kernel<WAVES, CH><<<(unsigned)((n + kTokens - 1) / kTokens), kThreads, 0, stream>>>(a, first);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) { return e; }
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_norm(const NormArgs& a, hipStream_t stream)
+{
+  // the padded blocks of a 4-bit output's last span are the lanes' past the width, too
+  const int width = a.q.codes != nullptr ? (a.width + 511) / 512 * 512 : a.width;
+  if (width <= 512) { return run<1, 1>(a, stream); }
+  if (width <= 1024) { return run<1, 2>(a, stream); }
+  if (width <= 2048) { return run<4, 1>(a, stream); }
+  if (width <= 4096) { return run<4, 2>(a, stream); }
+  if (width <= 8192) { return run<8, 2>(a, stream); }
+  return run<8, 4>(a, stream);
+}
+
+}  // namespace ltx25

@@ -1,0 +1,290 @@
+"""Microscaled 4-bit rows on the GPU: codes and scales exactly, products against 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import mx4_ref as ref
+from gpu_util import say
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(1, 32), (1, 512), (3, 64), (15, 480), (16, 512), (17, 544), (33, 1056), (64, 2048),
+          (5, 16384), (200, 96)]
+
+
+def _bits(rng, shape, wide):
+    """Values of any bits: denormals, zeros, and here and there an infinity or a NaN."""
+    if wide:
+        b = rng.integers(0, 1 << 32, shape, dtype=np.uint64).astype(np.uint32)
+        x = torch.from_numpy(b.view(np.int32).copy()).view(torch.float32)
+    else:
+        b = rng.integers(0, 1 << 16, shape).astype(np.uint16)
+        x = torch.from_numpy(b.view(np.int16).copy()).view(torch.bfloat16)
+    # exponents side by side within a block, and blocks without a value that is not finite
+    base = 2.0 ** torch.from_numpy(rng.integers(-130, 120, (shape[0], shape[1] // 32, 1))).double()
+    near = torch.from_numpy(rng.standard_normal((shape[0], shape[1] // 32, 32))) * base
+    near = near.reshape(shape).to(x.dtype)
+    keep = torch.from_numpy(rng.random((shape[0], shape[1] // 32, 1)) < 0.2).expand(
+        -1, -1, 32).reshape(shape)
+    x = torch.where(keep, x, near)
+    x[-1, :32] = 0
+    return x
+
+
+def _strided(x, extra=16):
+    """The same rows with a gap between them."""
+    wide = torch.empty((len(x), x.shape[1] + extra), dtype=x.dtype, device="cuda")
+    wide.fill_(float("nan"))
+    wide[:, :x.shape[1]] = x.cuda()
+    return wide[:, :x.shape[1]]
+
+
+def _same_codes(q, want):
+    codes, scales = ref.download(q)
+    assert (scales == want[1]).all()
+    ok = np.repeat(want[1] != 255, 32, 1)
+    assert (codes[ok] == want[0][ok]).all()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_codes_and_scales(pkg, dev, shape, wide):
+    say(f"mx4 quantize {shape} wide={wide}")
+    x = _bits(np.random.default_rng(shape[0] * 7 + shape[1] + wide), shape, wide)
+    q = pkg.MX4.empty(*shape)
+    q.codes.fill_(0xAA)
+    q.scales.fill_(0xAA)
+    pkg.mx4_quantize_rows(_strided(x), q)
+    want = ref.code(x.double().numpy())
+    _same_codes(q, want)
+    # bytes of blocks past the row's end are zeros
+    got, tiled = q.scales.cpu().numpy(), ref.tiles(np.full_like(want[1], 1))
+    rows = np.zeros(len(got), bool)
+    full = ref.tiles(np.ones((shape[0], -(-shape[1] // 512) * 16), np.uint8))
+    rows[full == 1] = True
+    assert (got[rows & (tiled == 0)] == 0).all()
+
+
+def test_every_value_of_bf16(pkg, dev):
+    """Each of the 65536 patterns as a value beside each of a few largest ones, so that every rounding
+    and tie is met at every place of the exponent."""
+    say("mx4 every bf16 value")
+    allb = np.arange(65536, dtype=np.uint16)
+    x = torch.from_numpy(allb.view(np.int16).copy()).view(torch.bfloat16).double().numpy()
+    x = np.where(np.isfinite(x), x, 1.0).reshape(-1, 1)
+    # the block's largest is the value times 1, 1.3, 3 or 9 where that is finite
+    rows = []
+    for f in (1.0, 1.3, 3.0, 9.0):
+        top = torch.from_numpy(np.clip(np.abs(x) * f, 0, 3e38)).bfloat16().double().numpy()
+        rows.append(np.concatenate([x, -x, top, np.repeat(0 * x, 29, 1)], 1))
+    x = np.concatenate(rows).reshape(-1, 512)
+    q = pkg.MX4.empty(*x.shape)
+    pkg.mx4_quantize_rows(torch.from_numpy(x).bfloat16().cuda(), q)
+    _same_codes(q, ref.code(x))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_values_back(pkg, dev, shape):
+    say(f"mx4 dequant {shape}")
+    rng = np.random.default_rng(shape[1])
+    codes = rng.integers(0, 16, shape).astype(np.uint8)
+    scales = rng.integers(0, 256, (shape[0], shape[1] // 32)).astype(np.uint8)
+    scales[0, 0] = 255
+    q = ref.upload(pkg, codes, scales)
+    out = _strided(torch.zeros(shape, dtype=torch.bfloat16))
+    pkg.mx4_dequant(q, out)
+    want = torch.from_numpy(ref.values(codes, scales)).float().bfloat16()
+    got = out.cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got, nan=0.0, posinf=1, neginf=-1),
+                       torch.nan_to_num(want, nan=0.0, posinf=1, neginf=-1))
+    gap = torch.as_strided(out, (shape[0], 16), (out.stride(0), 1), out.storage_offset() + shape[1])
+    assert bool(torch.isnan(gap).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scales_between_the_two_orders(pkg, dev, shape):
+    rng = np.random.default_rng(1)
+    codes, _ = ref.random_operand(rng, *shape)
+    scales = rng.integers(0, 256, (shape[0], shape[1] // 32)).astype(np.uint8)
+    q = pkg.MX4.packed(torch.from_numpy(ref.packed(codes)).cuda(), torch.from_numpy(scales).cuda())
+    assert (q.scales.cpu().numpy() == ref.tiles(scales)).all()
+    assert (q.unpacked_scales().cpu().numpy() == scales).all()
+
+
+# sizes around each kernel's rows, columns and steps, and around the changes from one to another
+PRODUCTS = [(1, 32, 1), (1, 64, 16), (2, 512, 17), (5, 544, 40), (16, 1024, 64), (17, 1056, 63),
+            (31, 96, 100), (33, 2080, 129), (64, 4096, 96), (65, 512, 257), (100, 2048, 1000),
+            (127, 160, 130), (129, 4096, 72), (200, 8192, 24), (255, 256, 255), (257, 768, 520),
+            (300, 1568, 1001), (520, 2048, 776), (1, 16384, 48), (1000, 288, 1500), (3, 8224, 9)]
+
+
+def _bias(rng, n, kind):
+    if kind is None:
+        return None, None
+    b = torch.from_numpy(rng.standard_normal(n)).to(kind)
+    return b.cuda(), b.double().numpy()
+
+
+def _guarded(m, n):
+    """An output between two stretches that no call may write."""
+    flat = torch.full((m * n + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
+    return flat[2048:2048 + m * n].view(m, n), flat
+
+
+def _untouched(flat, n):
+    assert bool((flat[:2048] == 7).all()) and bool((flat[2048 + n:] == 7).all())
+
+
+@pytest.mark.parametrize("kind,gelu", [(None, False), (torch.float32, True), (torch.bfloat16, False)])
+@pytest.mark.parametrize("m,k,n", PRODUCTS)
+def test_product(pkg, dev, m, k, n, kind, gelu):
+    say(f"mx4 gemm {m}x{k}->{n} bias={kind} gelu={gelu}")
+    rng = np.random.default_rng(m * 31 + k + n)
+    x, w = ref.random_operand(rng, m, k), ref.random_operand(rng, n, k, low=118)
+    bias, b = _bias(rng, n, kind)
+    y, flat = _guarded(m, n)
+    pkg.mx4_gemm(ref.upload(pkg, *x), ref.upload(pkg, *w), bias, y,
+                 pkg.EPI_GELU_TANH if gelu else pkg.EPI_NONE)
+    ref.check_product(y, ref.values(*x), ref.values(*w), b, gelu, f"{m}x{k}->{n}")
+    _untouched(flat, m * n)
+
+
+@pytest.mark.parametrize("m,k,n", PRODUCTS)
+def test_linear_is_coding_and_product(pkg, dev, m, k, n):
+    say(f"linear_mx4 {m}x{k}->{n}")
+    rng = np.random.default_rng(m + k * 3 + n)
+    x = torch.from_numpy(rng.standard_normal((m, k)) * np.exp(rng.standard_normal(k))).bfloat16()
+    w = ref.random_operand(rng, n, k, low=118)
+    weight = ref.upload(pkg, *w)
+    bias, b = _bias(rng, n, torch.float32)
+    y, flat = _guarded(m, n)
+    need = pkg.linear_mx4_workspace(m, k, n)
+    ws = torch.full((need + 4096,), 0xAB, dtype=torch.uint8, device="cuda")
+    pkg.linear_mx4(_strided(x), weight, bias, y, workspace=ws[:need])
+    ref.check_product(y, ref.values(*ref.code(x.double().numpy())), ref.values(*w), b, False)
+    _untouched(flat, m * n)
+    assert bool((ws[need:] == 0xAB).all())
+    q = pkg.MX4.empty(m, k)
+    pkg.mx4_quantize_rows(x.cuda(), q)
+    two = torch.empty_like(y)
+    pkg.mx4_gemm(q, weight, bias, two)
+    assert torch.equal(y, two)
+    pkg.linear_mx4(x.cuda(), weight, bias, two)
+    assert torch.equal(y, two)
+
+
+def test_large_products(pkg, dev):
+    """Tiles of the largest kind, with rows, columns and K that end inside one, against torch in
+    64 bits on the GPU."""
+    for m, k, n, gelu in [(2100, 4096, 3000, True), (4097, 1056, 4104, False), (1500, 8192, 2049, False),
+                          (8160, 512, 4096, False)]:
+        say(f"mx4 large {m}x{k}->{n}")
+        gen = torch.Generator(device="cuda")
+        gen.manual_seed(m)
+        ops, vals = [], []
+        for rows in (m, n):
+            codes = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
+            scales = torch.randint(118, 122, (rows, k // 32), dtype=torch.uint8, device="cuda",
+                                   generator=gen)
+            ops.append(pkg.MX4.packed(codes, scales))
+            lut = torch.tensor(ref.VALUES, device="cuda")
+            v = lut[torch.stack([codes & 15, codes >> 4], 2).flatten(1).int()]
+            vals.append(v * (2.0 ** (scales.double() - 127)).repeat_interleave(32, 1))
+        y, flat = _guarded(m, n)
+        pkg.mx4_gemm(*ops, None, y, pkg.EPI_GELU_TANH if gelu else pkg.EPI_NONE)
+        want, mag = vals[0] @ vals[1].T, vals[0].abs() @ vals[1].abs().T
+        slack = 1.13 * (k + 1) * 2.0 ** -24 * mag
+        if gelu:
+            want = torch.nn.functional.gelu(want, approximate="tanh")
+        err = (y.double() - want).abs() - (1.01 * 2.0 ** -8 * want.abs() + slack)
+        assert float(err.max()) <= 0, float(err.max())
+        _untouched(flat, m * n)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1024, 64), (20, 1024, 64), (300, 1024, 520), (2000, 1024, 4000)])
+def test_blocks_of_nan_stay_in_their_rows(pkg, dev, m, k, n):
+    say(f"mx4 NaN blocks {m}x{k}->{n}")
+    rng = np.random.default_rng(5)
+    x, w = ref.random_operand(rng, m, k), ref.random_operand(rng, n, k)
+    x[1][m // 2, 7] = 255
+    w[1][n // 3, 30] = 255
+    # a block of zero codes with a scale of NaN is one of NaN, too
+    w[0][n // 3, 960:992] = 0
+    y = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    pkg.mx4_gemm(ref.upload(pkg, *x), ref.upload(pkg, *w), None, y)
+    bad = torch.isnan(y).cpu().numpy()
+    want = np.zeros((m, n), bool)
+    want[m // 2], want[:, n // 3] = True, True
+    assert (bad == want).all()
+
+
+def test_scales_at_both_ends(pkg, dev):
+    """Exponents far apart in the two operands whose products are ordinary numbers; products beyond
+    f32's range are infinite, those below it zero."""
+    say("mx4 scales at both ends")
+    rng = np.random.default_rng(6)
+    m, k, n = 33, 512, 48
+    for a, b in [(0, 254), (254, 0), (10, 230), (127, 127), (60, 200)]:
+        x, w = ref.random_operand(rng, m, k, 1, a), ref.random_operand(rng, n, k, 1, b)
+        y = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+        pkg.mx4_gemm(ref.upload(pkg, *x), ref.upload(pkg, *w), None, y)
+        ref.check_product(y, ref.values(*x), ref.values(*w), None, False, f"{a} {b}")
+    x, w = ref.random_operand(rng, m, k, 1, 254), ref.random_operand(rng, n, k, 1, 254)
+    y = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    x = (np.full_like(x[0], 7), x[1])
+    w = (np.full_like(w[0], 2), w[1])
+    pkg.mx4_gemm(ref.upload(pkg, *x), ref.upload(pkg, *w), None, y)
+    assert bool((y == float("inf")).all())
+    low = np.zeros_like(x[1])
+    pkg.mx4_gemm(ref.upload(pkg, x[0], low), ref.upload(pkg, w[0], np.zeros_like(w[1])), None, y)
+    assert bool((y == 0).all())
+
+
+def test_no_rows_and_no_columns(pkg, dev):
+    w = ref.upload(pkg, *ref.random_operand(np.random.default_rng(0), 16, 64))
+    none = pkg.MX4(w.codes[:0], w.scales[:0])
+    y = torch.empty((0, 16), dtype=torch.bfloat16, device="cuda")
+    pkg.mx4_gemm(none, w, None, y)
+    pkg.linear_mx4(torch.empty((0, 64), dtype=torch.bfloat16, device="cuda"), w, None, y)
+    pkg.mx4_gemm(w, none, None, torch.empty((16, 0), dtype=torch.bfloat16, device="cuda"))
+    pkg.mx4_quantize_rows(torch.empty((0, 64), device="cuda"), none)
+    pkg.mx4_dequant(none, torch.empty((0, 64), dtype=torch.bfloat16, device="cuda"))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 512), (24, 2048, 264), (150, 4096, 1000), (1100, 1024, 2048)])
+def test_captured_on_a_stream_and_repeated(pkg, dev, m, k, n):
+    """Captured with its workspace, replayed with other inputs and other work between, on a side
+    stream and twice: the same bits."""
+    say(f"mx4 graph {m}x{k}->{n}")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(3)
+    w = ref.upload(pkg, *ref.random_operand(np.random.default_rng(2), n, k))
+    bias = torch.randn(n, device="cuda", generator=gen)
+    xs = [torch.randn((m, k), device="cuda", generator=gen).bfloat16() for _ in range(4)]
+    want = []
+    for x in xs:
+        y = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+        pkg.linear_mx4(x, w, bias, y)
+        want.append(y)
+    ws = torch.empty(pkg.linear_mx4_workspace(m, k, n), dtype=torch.uint8, device="cuda")
+    x, y = xs[0].clone(), torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.linear_mx4(x, w, bias, y, workspace=ws)
+    for i in (1, 0, 3, 2, 1):
+        x.copy_(xs[i])
+        ws.fill_(0x5A)
+        graph.replay()
+        assert torch.equal(y, want[i])
+        (xs[i].float() @ xs[i].float().T).sum()
+        torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        outs = [torch.empty_like(y) for _ in xs]
+        for a, o in zip(xs, outs):
+            pkg.linear_mx4(a, w, bias, o)
+    side.synchronize()
+    assert all(torch.equal(o, t) for o, t in zip(outs, want))

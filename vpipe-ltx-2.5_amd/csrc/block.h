@@ -89,18 +89,19 @@ __device__ __forceinline__ Pairs<N> pairs_of(const Rotation& r, int head, int fi
 __device__ __forceinline__ float low_f32(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_f32(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// (a, b) turned: a cos - b sin, a sin + b cos
+// A pair (a, b) turned: a cos - b sin, b cos + a sin
 __device__ __forceinline__ float turned_a(float a, float b, float sn, float cs)
 {
   return fmaf(a, cs, -(b * sn));
 }
 __device__ __forceinline__ float turned_b(float a, float b, float sn, float cs)
 {
-  return fmaf(a, sn, b * cs);
+  return fmaf(b, cs, a * sn);
 }
 
-// Eight channels of pairs side by side, turned
-__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pairs<4>& p)
+// Eight channels of pairs side by side, turned by four frequencies
+template <int N>
+__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pairs<N>& p)
 {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -129,6 +130,29 @@ __device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns&
   }
   xa = make_uint4(a[0], a[1], a[2], a[3]);
   xb = make_uint4(b[0], b[1], b[2], b[3]);
+}
+
+// The same where one lane has the pairs' first channels and another their second: the
+// lane's own half of it, of its channels x and the other lane's.
+__device__ __forceinline__ uint4 rotate_half(uint4 x, uint4 other, bool second, const Turns& t,
+                                             const Pairs<8>& p)
+{
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  const uint32_t o[4] = {other.x, other.y, other.z, other.w};
+  const uint32_t sign = second ? 0u : 0x80000000u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float sn[2], cs[2], v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sin_cos(t, p.freq[2 * i + h], p.axis[2 * i + h], sn[h], cs[h]);
+      const float mine = h ? high_f32(w[i]) : low_f32(w[i]);
+      const float his = h ? high_f32(o[i]) : low_f32(o[i]);
+      v[h] = fmaf(mine, cs[h], __uint_as_float(__float_as_uint(his * sn[h]) ^ sign));
+    }
+    w[i] = pack_bf16x2(v[0], v[1]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---- launchers --------------------------------------------------------------

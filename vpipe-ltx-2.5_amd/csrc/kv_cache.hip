@@ -227,32 +227,39 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
   const int pid = *sp.id;
   const int quad0 = sp.lo >> 2;
   const int pieces = few ? (sp.hi - sp.lo) * kPer : (((sp.hi + 3) >> 2) - quad0) * kPer;
-  // a key of the page's token `tok`, the lane's piece of it; every lane of a wave takes part
-  auto rotate = [&](uint4& w, int tok) {
-    if constexpr (ROPE) {
-      const int piece = tid % kPer;
-      const bool there = tok >= sp.lo && tok < sp.hi && piece * 8 < 2 * rot.pairs;
-      const int first = rot.interleaved ? piece * 4 : piece * 8 % rot.pairs;
-      const int apart = rot.interleaved ? 0 : rot.pairs / 8;
-      const bool second = !rot.interleaved && piece >= apart;
-      uint4 other = w;
-      if (!rot.interleaved) {
-        const int from = (tid & 63) + (second ? -apart : apart);
-        other.x = __shfl((int)w.x, from);
-        other.y = __shfl((int)w.y, from);
-        other.z = __shfl((int)w.z, from);
-        other.w = __shfl((int)w.w, from);
+  // The lane's piece of a key is the same in all its tokens, so are its pairs. A key of the
+  // page's token `tok`: every lane of a wave takes part.
+  const int piece = tid % kPer;
+  const int apart = ROPE && !rot.interleaved ? rot.pairs / 8 : 0;   // pieces between a pair's two
+  const bool second = apart > 0 && piece >= apart;
+  const bool turning = ROPE && piece * 8 < 2 * rot.pairs;
+  Pairs<8> pairs;
+  if (ROPE && !values && turning) {
+    if (rot.interleaved) {
+      const Pairs<4> four = pairs_of<4>(rot, g, piece * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pairs.freq[i] = four.freq[i];
+        pairs.axis[i] = four.axis[i];
       }
-      if (!there) { return; }
+    } else {
+      pairs = pairs_of<8>(rot, g, (piece - (second ? apart : 0)) * 8);
+    }
+  }
+  auto rotate = [&](uint4& w, int tok) {
+    const bool there = turning && tok >= sp.lo && tok < sp.hi;
+    const int from = (tid & 63) + (second ? -apart : apart);
+    uint4 other = w;
+    if (!rot.interleaved) {
+      other.x = __shfl((int)w.x, from);
+      other.y = __shfl((int)w.y, from);
+      other.z = __shfl((int)w.z, from);
+      other.w = __shfl((int)w.w, from);
+    }
+    if (there) {
       const Turns t = rot.positions != nullptr ? turns_of(rot, sp.first + tok)
                                                : turns_at(sp.place + tok);
-      if (rot.interleaved) {
-        w = rotate_side(w, t, pairs_of<4>(rot, g, first));
-      } else {
-        uint4 a = second ? other : w, b = second ? w : other;
-        rotate_halves(a, b, t, pairs_of<8>(rot, g, first));
-        w = second ? b : a;
-      }
+      w = rot.interleaved ? rotate_side(w, t, pairs) : rotate_half(w, other, second, t, pairs);
     }
   };
   uint4 held[kHeld][4];
@@ -263,7 +270,9 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
     if (tid < pieces) {
       held[0][0] = *(const uint4*)(x + (sp.first + sp.lo + tid / kPer) * stride + (tid % kPer) * 8);
     }
-    if (ROPE && !values) { rotate(held[0][0], sp.lo + tid / kPer); }
+    if constexpr (ROPE) {
+      if (!values) { rotate(held[0][0], sp.lo + tid / kPer); }
+    }
     const u16x2 tops = max_magnitudes(u16x2{0, 0}, held[0][0]);
     top = max((uint32_t)tops[0], (uint32_t)tops[1]);
     odd = top >= 0x7f80u;
@@ -282,12 +291,14 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
         }
       }
     }
-    if (ROPE && !values) {
+    if constexpr (ROPE) {
+      if (!values) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
+        for (int i = 0; i < kHeld; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          rotate(held[i][j], (quad0 + (tid + i * kThreads) / kPer) * 4 + j);
+          for (int j = 0; j < 4; ++j) {
+            rotate(held[i][j], (quad0 + (tid + i * kThreads) / kPer) * 4 + j);
+          }
         }
       }
     }

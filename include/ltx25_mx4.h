@@ -21,20 +21,21 @@
 extern "C" {
 #endif
 
-/* `rows` rows of K values in blocks of 32 along K; K a multiple of 32.
- *   codes   u8 [rows][K / 2], 16-byte aligned: two values a byte, the earlier one
- *           in the low half. A code is a sign and one of the magnitudes 0, 0.5, 1,
- *           1.5, 2, 3, 4, 6 (E2M1).
- *   scales  ltx25_mx4_scale_bytes(rows, K) bytes, 4-byte aligned: a block's
- *           exponent plus 127 (E8M0), its values are code * 2^exponent; 255 stands
- *           for a block of NaN. In tiles of 16 rows by 16 blocks, a tile's bytes in
- *           the order in which a wave of the matrix cores reads them: block b of
- *           row r at
+/* `rows` rows of K values in blocks of 32 along K; K a multiple of 32. A value is a
+ * code, a sign and one of the magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6 (E2M1), times its
+ * block's 2^exponent (E8M0: a byte, the exponent plus 127; 255 stands for a block of
+ * NaN). Both lie in the order in which a wave of the matrix cores takes them, so that
+ * its loads are whole lines (ltx25_mx4_pack lays out what a checkpoint holds):
+ *   codes   ltx25_mx4_code_bytes(rows, K) bytes, 16-byte aligned, two values a byte with
+ *           the earlier one in the low half; tiles of 16 rows by 128 values, the 16
+ *           bytes of block b of row r at
+ *             ((r / 16) * ceil(K / 128) + b / 4) * 1024 + ((b % 4) * 16 + r % 16) * 16
+ *   scales  ltx25_mx4_scale_bytes(rows, K) bytes, 4-byte aligned; tiles of 16 rows by 16
+ *           blocks, the byte of block b of row r at
  *             ((r / 16) * ceil(K / 512) + b / 16) * 256
- *               + ((b % 4) * 16 + r % 16) * 4 + (b / 4) % 4.
- *           The bytes of blocks past K in a row's last tile are 0; every call here
- *           that writes scales writes them so. Those of rows past the last are not
- *           read. */
+ *               + ((b % 4) * 16 + r % 16) * 4 + (b / 4) % 4
+ * The bytes of blocks past K in a row's last tile are 0; every call here that writes a
+ * row writes them so. Those of rows past the last may hold anything. */
 typedef struct ltx25_mx4 {
   void* codes;
   void* scales;
@@ -42,8 +43,9 @@ typedef struct ltx25_mx4 {
   int K;
 } ltx25_mx4;
 
-/* Bytes of the scales of `rows` rows of K values; 0 for sizes below 1 and a K that
- * is no multiple of 32. */
+/* Bytes of `rows` rows of K values; 0 for sizes below 1 and a K that is no multiple
+ * of 32. */
+size_t ltx25_mx4_code_bytes(int rows, int K);
 size_t ltx25_mx4_scale_bytes(int rows, int K);
 
 /* Codes of q->rows rows of x, bf16 or f32 (x_dtype), x_stride elements from a row
@@ -60,10 +62,10 @@ int ltx25_mx4_quantize_rows(void* stream, const void* x, int x_dtype, int64_t x_
  * (infinite) and below its smallest (rounded). */
 int ltx25_mx4_dequant(void* stream, const ltx25_mx4* q, void* out, int64_t out_stride);
 
-/* Scales from rows of K / 32 bytes, as checkpoints hold them, to q's tiles, and
- * back. */
-int ltx25_mx4_pack_scales(void* stream, const uint8_t* scales, const ltx25_mx4* q);
-int ltx25_mx4_unpack_scales(void* stream, const ltx25_mx4* q, uint8_t* scales);
+/* From u8 codes [rows][K / 2] and scales [rows][K / 32], as checkpoints hold them, to
+ * q's order, and back. Both 16-byte aligned. */
+int ltx25_mx4_pack(void* stream, const void* codes, const void* scales, const ltx25_mx4* q);
+int ltx25_mx4_unpack(void* stream, const ltx25_mx4* q, void* codes, void* scales);
 
 /* y[M][N] = epilogue(x . w^T + bias): M = x->rows, N = w->rows, both of one K. Both
  * operands are exact in the products, which are added in f32; bias (LTX25_DT_*) and

@@ -51,6 +51,16 @@ def tiles(scales):
     return out
 
 
+def code_tiles(b):
+    """Packed codes [R][K / 2] in the matrix cores' order; bytes that stand for no block are 0."""
+    rows, blocks = len(b), b.shape[1] // 16
+    slices = -(-blocks // 4)
+    out = np.zeros(((-(-rows // 16)) * slices * 64, 16), np.uint8)
+    r, k = np.meshgrid(np.arange(rows), np.arange(blocks), indexing="ij")
+    out[((r // 16) * slices + k // 4) * 64 + (k % 4) * 16 + r % 16] = b.reshape(rows, blocks, 16)
+    return out.reshape(-1)
+
+
 def random_operand(rng, rows, k, spread=3, low=120):
     codes = rng.integers(0, 16, (rows, k)).astype(np.uint8)
     scales = rng.integers(low, low + spread, (rows, k // 32)).astype(np.uint8)
@@ -58,12 +68,14 @@ def random_operand(rng, rows, k, spread=3, low=120):
 
 
 def upload(pkg, codes, scales):
-    return pkg.MX4(torch.from_numpy(packed(codes)).cuda(), torch.from_numpy(tiles(scales)).cuda())
+    return pkg.MX4(torch.from_numpy(code_tiles(packed(codes))).cuda(),
+                   torch.from_numpy(tiles(scales)).cuda(), *codes.shape)
 
 
 def download(q):
     """An MX4's codes [R][K] and scales [R][K / 32]."""
-    return unpacked(q.codes.cpu().numpy()), q.unpacked_scales().cpu().numpy()
+    codes, scales = q.unpacked()
+    return unpacked(codes.cpu().numpy()), scales.cpu().numpy()
 
 
 def gelu(y):

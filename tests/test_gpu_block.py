@@ -185,6 +185,7 @@ def test_norm_coded(pkg, dev, tokens, width):
     c["x_out"] = torch.empty_like(c["x"])
     q = pkg.MX4.empty(tokens, width)
     q.scales.fill_(0xAA)
+    q.codes.fill_(0xAA)
     pkg.block_norm(out=q, **c)
     h, _, mag, _ = _want(c, np.zeros(tokens, int))
     codes, scales = ref.download(q)
@@ -196,6 +197,9 @@ def test_norm_coded(pkg, dev, tokens, width):
     full = ref.tiles(np.ones((tokens, -(-width // 512) * 16), np.uint8)) == 1
     there = ref.tiles(np.ones((tokens, width // 32), np.uint8)) == 1
     assert (q.scales.cpu().numpy()[full & ~there] == 0).all()
+    full = ref.code_tiles(np.ones((tokens, -(-width // 128) * 64), np.uint8)) == 1
+    there = ref.code_tiles(np.ones((tokens, width // 2), np.uint8)) == 1
+    assert (q.codes.cpu().numpy()[full & ~there] == 0).all()
     out = torch.empty((tokens, width), dtype=BF16, device="cuda")
     xo = c["x_out"].clone()
     pkg.block_norm(out=out, **c)

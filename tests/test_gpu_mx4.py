@@ -58,11 +58,11 @@ def test_codes_and_scales(pkg, dev, shape, wide):
     want = ref.code(x.double().numpy())
     _same_codes(q, want)
     # bytes of blocks past the row's end are zeros
-    got, tiled = q.scales.cpu().numpy(), ref.tiles(np.full_like(want[1], 1))
-    rows = np.zeros(len(got), bool)
-    full = ref.tiles(np.ones((shape[0], -(-shape[1] // 512) * 16), np.uint8))
-    rows[full == 1] = True
-    assert (got[rows & (tiled == 0)] == 0).all()
+    for got, tiled, wide_ones in ((q.scales, ref.tiles, 1), (q.codes, ref.code_tiles, 16)):
+        whole = -(-want[1].shape[1] // (16 if wide_ones == 1 else 4)) * (16 if wide_ones == 1 else 4)
+        there = tiled(np.ones((shape[0], want[1].shape[1] * wide_ones), np.uint8)) == 1
+        rows = tiled(np.ones((shape[0], whole * wide_ones), np.uint8)) == 1
+        assert (got.cpu().numpy()[rows & ~there] == 0).all()
 
 
 def test_every_value_of_bf16(pkg, dev):
@@ -103,13 +103,18 @@ def test_values_back(pkg, dev, shape):
 
 
 @pytest.mark.parametrize("shape", SHAPES)
-def test_scales_between_the_two_orders(pkg, dev, shape):
+def test_the_two_orders(pkg, dev, shape):
+    say(f"mx4 orders {shape}")
     rng = np.random.default_rng(1)
-    codes, _ = ref.random_operand(rng, *shape)
+    codes = rng.integers(0, 16, shape).astype(np.uint8)
     scales = rng.integers(0, 256, (shape[0], shape[1] // 32)).astype(np.uint8)
-    q = pkg.MX4.packed(torch.from_numpy(ref.packed(codes)).cuda(), torch.from_numpy(scales).cuda())
-    assert (q.scales.cpu().numpy() == ref.tiles(scales)).all()
-    assert (q.unpacked_scales().cpu().numpy() == scales).all()
+    rows = [torch.from_numpy(t).cuda() for t in (ref.packed(codes), scales)]
+    q = pkg.MX4.packed(*rows)
+    pad = 16 * (-(-shape[0] // 16)) - shape[0]
+    assert (q.codes.cpu().numpy() == ref.code_tiles(np.pad(ref.packed(codes), ((0, pad), (0, 0))))).all()
+    assert (q.scales.cpu().numpy() == ref.tiles(np.pad(scales, ((0, pad), (0, 0))))).all()
+    back = q.unpacked()
+    assert torch.equal(back[0], rows[0]) and torch.equal(back[1], rows[1])
 
 
 # sizes around each kernel's rows, columns and steps, and around the changes from one to another
@@ -243,7 +248,7 @@ def test_scales_at_both_ends(pkg, dev):
 
 def test_no_rows_and_no_columns(pkg, dev):
     w = ref.upload(pkg, *ref.random_operand(np.random.default_rng(0), 16, 64))
-    none = pkg.MX4(w.codes[:0], w.scales[:0])
+    none = pkg.MX4(w.codes[:0], w.scales[:0], 0, 64)
     y = torch.empty((0, 16), dtype=torch.bfloat16, device="cuda")
     pkg.mx4_gemm(none, w, None, y)
     pkg.linear_mx4(torch.empty((0, 64), dtype=torch.bfloat16, device="cuda"), w, None, y)

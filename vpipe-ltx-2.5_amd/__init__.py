@@ -233,11 +233,12 @@ SIGNATURES = {
     "ltx25_attention_cached": (_i, [_vp, ctypes.POINTER(AttnC), ctypes.POINTER(KVCacheC), _vp, _i,
                                     _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _sz]),
     "ltx25_attention_cached_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "ltx25_mx4_code_bytes": (_sz, [_i, _i]),
     "ltx25_mx4_scale_bytes": (_sz, [_i, _i]),
     "ltx25_mx4_quantize_rows": (_i, [_vp, _vp, _i, ctypes.c_int64, ctypes.POINTER(Mx4C)]),
     "ltx25_mx4_dequant": (_i, [_vp, ctypes.POINTER(Mx4C), _vp, ctypes.c_int64]),
-    "ltx25_mx4_pack_scales": (_i, [_vp, _vp, ctypes.POINTER(Mx4C)]),
-    "ltx25_mx4_unpack_scales": (_i, [_vp, ctypes.POINTER(Mx4C), _vp]),
+    "ltx25_mx4_pack": (_i, [_vp, _vp, _vp, ctypes.POINTER(Mx4C)]),
+    "ltx25_mx4_unpack": (_i, [_vp, ctypes.POINTER(Mx4C), _vp, _vp]),
     "ltx25_mx4_gemm": (_i, [_vp, ctypes.POINTER(Mx4C), ctypes.POINTER(Mx4C), _vp, _i, _vp, _i, _vp,
                             _sz]),
     "ltx25_mx4_gemm_workspace": (_sz, [_i, _i, _i]),
@@ -671,9 +672,9 @@ def _rows(name: str, t, width: int | None = None) -> int:
 
 
 class MX4:
-    """Rows in microscaled 4 bits, held in torch device tensors (ltx25_mx4): `codes` uint8
-    [rows][K / 2], two values a byte with the earlier one in the low half, and `scales`, uint8 with
-    the blocks' exponents in the order of the matrix cores' reads.
+    """`rows` rows of K values in microscaled 4 bits, held in torch device tensors (ltx25_mx4): uint8
+    `codes` and `scales` in the order of the matrix cores' reads, mx4_code_bytes() and
+    mx4_scale_bytes() long.
 
     Calls work on the tensors given here, whose contents may change at will.
     """
@@ -681,61 +682,61 @@ class MX4:
     codes = property(lambda self: self._tensors[0])
     scales = property(lambda self: self._tensors[1])
 
-    def __init__(self, codes, scales):
+    def __init__(self, codes, scales, rows: int, K: int):
         torch = _torch or _import_torch()
-        if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
-            raise TypeError(f"codes must be contiguous uint8 [rows][K / 2], got {codes.dtype} "
-                            f"{tuple(codes.shape)}")
-        rows, half = codes.shape
-        if half == 0 or half % 16:
-            raise ValueError(f"rows of {2 * half} values: K is a multiple of 32")
-        need = mx4_scale_bytes(rows, 2 * half)
-        if scales.dtype != torch.uint8 or scales.numel() != need or not scales.is_contiguous():
-            raise TypeError(f"scales must be contiguous uint8 with {need} elements, got "
-                            f"{scales.dtype} {tuple(scales.shape)}")
-        if codes.device != scales.device:
+        if rows < 0 or K <= 0 or K % 32:
+            raise ValueError(f"{rows} rows of {K} values: K is a multiple of 32")
+        for name, t, need in (("codes", codes, mx4_code_bytes(rows, K)),
+                              ("scales", scales, mx4_scale_bytes(rows, K))):
+            if t.dtype != torch.uint8 or t.numel() != need or not t.is_contiguous():
+                raise TypeError(f"{name} must be contiguous uint8 with {need} elements, got "
+                                f"{t.dtype} {tuple(t.shape)}")
+        if codes.device != scales.device or codes.is_cuda != scales.is_cuda:
             raise ValueError(f"codes lie on {codes.device}, scales on {scales.device}")
         self._tensors = (codes, scales)
-        self.rows, self.K = rows, 2 * half
-        self._c = Mx4C(_ptr(codes), _ptr(scales), rows, 2 * half)
+        self.rows, self.K = rows, K
+        self._c = Mx4C(_ptr(codes), _ptr(scales), rows, K)
 
     @classmethod
     def empty(cls, rows: int, K: int, device="cuda"):
         torch = _torch or _import_torch()
-        return cls(torch.empty((rows, K // 2), dtype=torch.uint8, device=device),
-                   torch.empty(mx4_scale_bytes(rows, K), dtype=torch.uint8, device=device))
+        return cls(torch.empty(mx4_code_bytes(rows, K), dtype=torch.uint8, device=device),
+                   torch.empty(mx4_scale_bytes(rows, K), dtype=torch.uint8, device=device), rows, K)
 
     @classmethod
     def packed(cls, codes, scales, stream=None):
-        """From codes and scales as checkpoints hold them, uint8 [rows][K / 32]
-        (ltx25_mx4_pack_scales)."""
+        """From uint8 codes [rows][K / 2], the earlier of a byte's two values in its low half, and
+        scales [rows][K / 32], as checkpoints hold them (ltx25_mx4_pack)."""
         torch = _torch or _import_torch()
         rows, half = codes.shape
-        q = cls(codes, torch.empty(mx4_scale_bytes(rows, 2 * half), dtype=torch.uint8,
-                                   device=codes.device))
-        _check_scales(scales, q)
-        _reachable("scales codes", scales, codes)
-        check(load().ltx25_mx4_pack_scales(_on_device(stream, codes, scales), _ptr(scales),
-                                           ctypes.byref(q.c())))
+        if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or half % 16
+                or tuple(scales.shape) != (rows, half // 16)
+                or not (codes.is_contiguous() and scales.is_contiguous())):
+            raise TypeError(f"codes and scales must be contiguous uint8 [rows][K / 2] and "
+                            f"[rows][K / 32], got {codes.dtype} {tuple(codes.shape)}, "
+                            f"{scales.dtype} {tuple(scales.shape)}")
+        _reachable("codes scales", codes, scales)
+        q = cls.empty(rows, 2 * half, codes.device)
+        check(load().ltx25_mx4_pack(_on_device(stream, codes, scales), _ptr(codes), _ptr(scales),
+                                    ctypes.byref(q.c())))
         return q
 
-    def unpacked_scales(self, stream=None):
-        """The scales as uint8 [rows][K / 32] (ltx25_mx4_unpack_scales)."""
-        out = self.scales.new_empty((self.rows, self.K // 32))
-        _reachable("scales", self.scales)
-        check(load().ltx25_mx4_unpack_scales(_on_device(stream, out), ctypes.byref(self.c()),
-                                             _ptr(out)))
-        return out
+    def unpacked(self, stream=None):
+        """codes [rows][K / 2] and scales [rows][K / 32] as packed() takes them
+        (ltx25_mx4_unpack)."""
+        codes = self.codes.new_empty((self.rows, self.K // 2))
+        scales = self.codes.new_empty((self.rows, self.K // 32))
+        _reachable("codes", self.codes)
+        check(load().ltx25_mx4_unpack(_on_device(stream, codes), ctypes.byref(self.c()),
+                                      _ptr(codes), _ptr(scales)))
+        return codes, scales
 
     def c(self) -> Mx4C:
         return self._c
 
 
-def _check_scales(scales, q: MX4) -> None:
-    if (scales.dtype != _torch.uint8 or tuple(scales.shape) != (q.rows, q.K // 32)
-            or not scales.is_contiguous()):
-        raise TypeError(f"scales must be contiguous uint8 [{q.rows}][{q.K // 32}], got "
-                        f"{scales.dtype} {tuple(scales.shape)}")
+def mx4_code_bytes(rows: int, K: int) -> int:
+    return int(load().ltx25_mx4_code_bytes(rows, K))
 
 
 def mx4_scale_bytes(rows: int, K: int) -> int:

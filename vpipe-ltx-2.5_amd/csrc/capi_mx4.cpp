@@ -21,7 +21,7 @@ bool sizes_fit(long rows, long K)
   return rows > 0 && rows <= kRowsMax && K > 0 && K <= kWidthMax && K % 32 == 0;
 }
 
-// `empty`: no rows are an empty call rather than a mistake
+// No rows are an empty call rather than a mistake
 int check_operand(const char* name, const ltx25_mx4* q, ltx25::Mx4Args* out)
 {
   if (q == nullptr) { return set_error(LTX25_E_INVAL, "%s is null", name); }
@@ -72,9 +72,9 @@ int check_product(const ltx25::Mx4Args& w, int M, const void* bias, int bias_dty
   if (epilogue != LTX25_EPI_NONE && epilogue != LTX25_EPI_GELU_TANH) {
     return set_error(LTX25_E_INVAL, "epilogue=%d is none of LTX25_EPI_*", epilogue);
   }
-  if ((size_t)w.rows * (size_t)(w.K / 2) >= (size_t)1 << 31) {
+  if (ltx25::mx4_code_bytes(w.rows, w.K) >= (size_t)1 << 31) {
     return set_error(LTX25_E_UNSUPPORTED, "the weight's %zu bytes of codes are 2 GiB or more",
-                     (size_t)w.rows * (size_t)(w.K / 2));
+                     ltx25::mx4_code_bytes(w.rows, w.K));
   }
   if (M == 0 || w.rows == 0) { return LTX25_OK; }
   int rc = check_pointer("y", y, 16);
@@ -102,7 +102,7 @@ Inside inside(int M, int K, const ltx25::Mx4Plan& plan)
 {
   Inside r;
   if (plan.codes_ahead) {
-    r.scales = up((size_t)M * (K / 2));
+    r.scales = up(ltx25::mx4_code_bytes(M, K));
     r.partial = r.scales + up(ltx25::mx4_scale_bytes(M, K));
   }
   r.bytes = r.partial + plan.partial_bytes;
@@ -127,6 +127,11 @@ int run(void* stream, ltx25::Mx4Gemm& g, const ltx25::Mx4Plan& plan, const void*
 }  // namespace
 
 extern "C" {
+
+size_t ltx25_mx4_code_bytes(int rows, int K)
+{
+  return sizes_fit(rows, K) ? ltx25::mx4_code_bytes(rows, K) : 0;
+}
 
 size_t ltx25_mx4_scale_bytes(int rows, int K)
 {
@@ -165,32 +170,34 @@ int ltx25_mx4_dequant(void* stream, const ltx25_mx4* q, void* out, int64_t out_s
   return e == hipSuccess ? LTX25_OK : hip_error(e, "4-bit expansion launch");
 }
 
-int ltx25_mx4_pack_scales(void* stream, const uint8_t* scales, const ltx25_mx4* q)
+int ltx25_mx4_pack(void* stream, const void* codes, const void* scales, const ltx25_mx4* q)
 {
   ltx25::Mx4Args a;
   int rc = check_operand("q", q, &a);
   if (rc != LTX25_OK || a.rows == 0) { return rc; }
-  if ((rc = check_pointer("scales", scales, 1)) != LTX25_OK ||
+  if ((rc = check_pointer("codes", codes, 16)) != LTX25_OK ||
+      (rc = check_pointer("scales", scales, 16)) != LTX25_OK ||
       (rc = ltx25::check_device()) != LTX25_OK) {
     return rc;
   }
-  const hipError_t e =
-      ltx25::launch_mx4_scales(scales, a.scales, a.rows, a.K, true, (hipStream_t)stream);
-  return e == hipSuccess ? LTX25_OK : hip_error(e, "4-bit scales launch");
+  const hipError_t e = ltx25::launch_mx4_pack((const uint8_t*)codes, (const uint8_t*)scales, a,
+                                              (hipStream_t)stream);
+  return e == hipSuccess ? LTX25_OK : hip_error(e, "4-bit packing launch");
 }
 
-int ltx25_mx4_unpack_scales(void* stream, const ltx25_mx4* q, uint8_t* scales)
+int ltx25_mx4_unpack(void* stream, const ltx25_mx4* q, void* codes, void* scales)
 {
   ltx25::Mx4Args a;
   int rc = check_operand("q", q, &a);
   if (rc != LTX25_OK || a.rows == 0) { return rc; }
-  if ((rc = check_pointer("scales", scales, 1)) != LTX25_OK ||
+  if ((rc = check_pointer("codes", codes, 16)) != LTX25_OK ||
+      (rc = check_pointer("scales", scales, 16)) != LTX25_OK ||
       (rc = ltx25::check_device()) != LTX25_OK) {
     return rc;
   }
   const hipError_t e =
-      ltx25::launch_mx4_scales(a.scales, scales, a.rows, a.K, false, (hipStream_t)stream);
-  return e == hipSuccess ? LTX25_OK : hip_error(e, "4-bit scales launch");
+      ltx25::launch_mx4_unpack(a, (uint8_t*)codes, (uint8_t*)scales, (hipStream_t)stream);
+  return e == hipSuccess ? LTX25_OK : hip_error(e, "4-bit unpacking launch");
 }
 
 size_t ltx25_mx4_gemm_workspace(int M, int K, int N)

@@ -8,18 +8,31 @@ namespace ltx25 {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// Where the scales of a block lie (include/ltx25_mx4.h): tiles of 16 rows x 16 blocks,
-// 256 bytes; lane l of a wave reads dword l of a tile, the four blocks b % 4 = l / 16 of
-// row l % 16, one for each of the four matrix instructions that span the tile's 512
-// values. The instruction takes a lane's block and scale from the same lane, so that no
-// byte changes lanes.
+// Where codes and scales lie (include/ltx25_mx4.h). Codes: tiles of 16 rows x 128 values,
+// 1 KB; lane l of a wave reads the tile's 16 bytes l, block l / 16 of row l % 16. Scales:
+// tiles of 16 rows x 16 blocks, 256 bytes; lane l reads dword l, its four blocks' for the
+// four matrix instructions that span the tile's 512 values. An instruction takes a lane's
+// block and scale from the same lane, so that no byte changes lanes; and four lanes side by
+// side read 64 bytes: from rows of K / 2 bytes the same fragment takes the address unit four
+// times as long (a wave's rows straight to registers: 91% of the time, matrix cores 36%).
+constexpr int kMx4CodeTile = 1024;
 constexpr int kMx4Tile = 256;
+__host__ __device__ inline int mx4_slices(int K) { return (K + 127) / 128; }
 __host__ __device__ inline int mx4_spans(int K) { return (K + 511) / 512; }
+__host__ __device__ inline size_t mx4_code_bytes(long rows, int K)
+{
+  return (size_t)((rows + 15) / 16) * mx4_slices(K) * kMx4CodeTile;
+}
 __host__ __device__ inline size_t mx4_scale_bytes(long rows, int K)
 {
   return (size_t)((rows + 15) / 16) * mx4_spans(K) * kMx4Tile;
 }
-__device__ __forceinline__ int mx4_scale_at(int row, int block)   // within its tile
+// Within their tiles
+__device__ __forceinline__ int mx4_code_at(int row, int block)
+{
+  return ((block & 3) * 16 + (row & 15)) * 16;
+}
+__device__ __forceinline__ int mx4_scale_at(int row, int block)
 {
   return ((block & 3) * 16 + (row & 15)) * 4 + ((block >> 2) & 3);
 }
@@ -87,8 +100,9 @@ struct Mx4Args {
 hipError_t launch_mx4_quantize(const void* x, bool wide, int64_t stride, const Mx4Args& q,
                                hipStream_t stream);
 hipError_t launch_mx4_dequant(const Mx4Args& q, uint16_t* out, int64_t stride, hipStream_t stream);
-hipError_t launch_mx4_scales(const uint8_t* in, uint8_t* out, int rows, int K, bool pack,
-                             hipStream_t stream);
+hipError_t launch_mx4_pack(const uint8_t* codes, const uint8_t* scales, const Mx4Args& q,
+                           hipStream_t stream);
+hipError_t launch_mx4_unpack(const Mx4Args& q, uint8_t* codes, uint8_t* scales, hipStream_t stream);
 
 // y = epilogue(x . w^T + bias). `xb` set: bf16 activations at xb_stride, coded on the
 // way; x then says where their codes go where the plan codes them ahead.

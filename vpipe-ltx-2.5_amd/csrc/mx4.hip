@@ -1,5 +1,5 @@
 // Coding rows in microscaled 4 bits and back (ltx25_mx4_quantize_rows,
-// ltx25_mx4_dequant, ltx25_mx4_pack_scales, ltx25_mx4_unpack_scales).
+// ltx25_mx4_dequant, ltx25_mx4_pack, ltx25_mx4_unpack).
 #include "mx4.h"
 
 namespace ltx25 {
@@ -7,18 +7,57 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A workgroup codes one tile of scales, 16 rows x 512 values. A wave takes a row at a
-// time, eight values a lane, so that a block's largest value is found among four lanes
-// and every load and store is a whole line; the tile's 256 scales go out together.
+// The workgroup blockIdx.x's span of 512 values of 16 rows: four tiles of codes and one of
+// scales, in LDS on their way to or from memory.
+struct Span {
+  int row0, span, slices;   // slices: tiles of codes that the span has, 1 to 4
+  uint8_t* codes;
+  uint32_t* scales;
+};
+__device__ __forceinline__ Span span_of(const Mx4Args& q)
+{
+  const int spans = mx4_spans(q.K), slices = mx4_slices(q.K);
+  Span s;
+  s.span = (int)(blockIdx.x % (unsigned)spans);
+  const int block = (int)(blockIdx.x / (unsigned)spans);
+  s.row0 = block * 16;
+  s.slices = min(4, slices - 4 * s.span);
+  s.codes = q.codes + ((long)block * slices + 4 * s.span) * kMx4CodeTile;
+  s.scales = (uint32_t*)(q.scales + (long)blockIdx.x * kMx4Tile);
+  return s;
+}
+// Thread t's 16 bytes of the codes and word of the scales
+__device__ __forceinline__ void store_span(const Span& s, const uint4* codes, const uint32_t* scales)
+{
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t < s.slices * 64) { ((uint4*)s.codes)[t] = codes[t]; }
+  if (t < kMx4Tile / 4) { s.scales[t] = scales[t]; }
+}
+__device__ __forceinline__ void load_span(const Span& s, uint4* codes, uint32_t* scales)
+{
+  const int t = threadIdx.x;
+  if (t < s.slices * 64) { codes[t] = ((const uint4*)s.codes)[t]; }
+  if (t < kMx4Tile / 4) { scales[t] = s.scales[t]; }
+  __syncthreads();
+}
+// Where eight codes from value 8 `lane` of the span lie in LDS
+__device__ __forceinline__ int codes_at(int row, int lane)
+{
+  return (lane >> 4) * kMx4CodeTile + mx4_code_at(row, lane >> 2) + (lane & 3) * 4;
+}
+
+// A wave takes a row at a time, eight values a lane, so that a block's largest value is found
+// among four lanes and every load is whole lines.
 template <bool WIDE>
 __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const void* x, long stride,
-                                                                Mx4Args q, int spans)
+                                                                Mx4Args q)
 {
+  __shared__ uint4 held[4 * kMx4CodeTile / 16];
   __shared__ uint32_t tile[kMx4Tile / 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int span = (int)(blockIdx.x % (unsigned)spans);
-  const int row0 = (int)(blockIdx.x / (unsigned)spans) * 16;
-  const int col = span * 512 + lane * 8;
+  const Span s = span_of(q);
+  const int row0 = s.row0, col = s.span * 512 + lane * 8;
   const bool in = col < q.K;   // K is a multiple of 32: a block's four lanes agree
   uint4 raw[4][WIDE ? 2 : 1];
 #pragma unroll
@@ -50,50 +89,33 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const void* x, l
     }
     uint32_t scale;
     const uint32_t codes = mx4_code_quad(v, scale);
-    if (in && row0 + r < q.rows) {
-      *(uint32_t*)(q.codes + (long)(row0 + r) * (q.K >> 1) + (col >> 1)) = codes;
-    }
     // zeros in blocks past K (and in rows past the last, which nothing reads)
+    *(uint32_t*)((uint8_t*)held + codes_at(r, lane)) = codes;
     if ((lane & 3) == 0) { ((uint8_t*)tile)[mx4_scale_at(r, lane >> 2)] = in ? (uint8_t)scale : 0; }
   }
-  __syncthreads();
-  if (threadIdx.x < kMx4Tile / 4) {
-    ((uint32_t*)(q.scales + (long)blockIdx.x * kMx4Tile))[threadIdx.x] = tile[threadIdx.x];
-  }
+  store_span(s, held, tile);
 }
 
-// A workgroup expands the codes of one tile of scales.
-__global__ void __launch_bounds__(kThreads) mx4_dequant_kernel(Mx4Args q, uint16_t* out, long stride,
-                                                               int spans)
+// A workgroup expands a span.
+__global__ void __launch_bounds__(kThreads) mx4_dequant_kernel(Mx4Args q, uint16_t* out, long stride)
 {
+  __shared__ uint4 held[4 * kMx4CodeTile / 16];
   __shared__ uint32_t tile[kMx4Tile / 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int span = (int)(blockIdx.x % (unsigned)spans);
-  const int row0 = (int)(blockIdx.x / (unsigned)spans) * 16;
-  const int col = span * 512 + lane * 8;
+  const Span sp = span_of(q);
+  const int row0 = sp.row0, col = sp.span * 512 + lane * 8;
   const bool in = col < q.K;
-  uint32_t codes[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = row0 + wave + 4 * i;
-    codes[i] = 0;
-    if (in && row < q.rows) {
-      codes[i] = *(const uint32_t*)(q.codes + (long)row * (q.K >> 1) + (col >> 1));
-    }
-  }
-  if (threadIdx.x < kMx4Tile / 4) {
-    tile[threadIdx.x] = ((const uint32_t*)(q.scales + (long)blockIdx.x * kMx4Tile))[threadIdx.x];
-  }
-  __syncthreads();
+  load_span(sp, held, tile);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = wave + 4 * i;
     if (!in || row0 + r >= q.rows) { continue; }
     const int s = ((const uint8_t*)tile)[mx4_scale_at(r, lane >> 2)];
+    const uint32_t codes = *(const uint32_t*)((const uint8_t*)held + codes_at(r, lane));
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t c = codes[i] >> (4 * k);
+      const uint32_t c = codes >> (4 * k);
       // magnitudes m / 2: 0 1 2 3 4 6 8 12, a nibble each
       const float m = (float)((0xc8643210u >> (4 * (c & 7u))) & 15u);
       v[k] = s == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(c & 8u ? -m : m, s - 128);
@@ -104,24 +126,35 @@ __global__ void __launch_bounds__(kThreads) mx4_dequant_kernel(Mx4Args q, uint16
   }
 }
 
-// Scales between rows of K / 32 bytes and tiles; a thread moves one byte of a tile.
-__global__ void __launch_bounds__(kThreads) mx4_scales_kernel(const uint8_t* in, uint8_t* out,
-                                                              int rows, int blocks, int spans,
-                                                              bool pack)
+// Between rows and a span's tiles: thread t has block t % 16 of row t / 16.
+template <bool PACK>
+__global__ void __launch_bounds__(kThreads) mx4_order_kernel(Mx4Args q, uint8_t* codes,
+                                                             uint8_t* scales)
 {
-  const int row = (int)(blockIdx.x / (unsigned)spans) * 16 + (int)(threadIdx.x >> 4);
-  const int block = (int)(blockIdx.x % (unsigned)spans) * 16 + (int)(threadIdx.x & 15);
-  const long at = (long)blockIdx.x * kMx4Tile + mx4_scale_at(row, block);
-  const bool there = row < rows && block < blocks;
-  const long flat = (long)row * blocks + block;
-  if (pack) {
-    out[at] = there ? in[flat] : 0;
-  } else if (there) {
-    out[flat] = in[at];
+  __shared__ uint4 held[4 * kMx4CodeTile / 16];
+  __shared__ uint32_t tile[kMx4Tile / 4];
+  const Span s = span_of(q);
+  const int r = (int)threadIdx.x >> 4, b = (int)threadIdx.x & 15, blocks = q.K >> 5;
+  const int row = s.row0 + r, block = s.span * 16 + b;
+  const bool in = row < q.rows && block < blocks;
+  uint4* const code = (uint4*)codes + (long)row * blocks + block;
+  uint8_t* const scale = scales + (long)row * blocks + block;
+  uint4* const here = (uint4*)((uint8_t*)held + (b >> 2) * kMx4CodeTile + mx4_code_at(r, b));
+  uint8_t* const exponent = (uint8_t*)tile + mx4_scale_at(r, b);
+  if (PACK) {
+    *here = in ? *code : make_uint4(0, 0, 0, 0);
+    *exponent = in ? *scale : 0;
+    store_span(s, held, tile);
+  } else {
+    load_span(s, held, tile);
+    if (in) {
+      *code = *here;
+      *scale = *exponent;
+    }
   }
 }
 
-// One workgroup for each tile of scales
+// One workgroup for each span of 16 rows
 bool tiles_of(int rows, int K, int& grid)
 {
   const long n = (long)((rows + 15) / 16) * mx4_spans(K);
@@ -137,9 +170,9 @@ hipError_t launch_mx4_quantize(const void* x, bool wide, int64_t stride, const M
   int grid;
   if (!tiles_of(q.rows, q.K, grid)) { return hipErrorInvalidConfiguration; }
   if (wide) {
-    mx4_quantize_kernel<true><<<grid, kThreads, 0, stream>>>(x, (long)stride, q, mx4_spans(q.K));
+    mx4_quantize_kernel<true><<<grid, kThreads, 0, stream>>>(x, (long)stride, q);
   } else {
-    mx4_quantize_kernel<false><<<grid, kThreads, 0, stream>>>(x, (long)stride, q, mx4_spans(q.K));
+    mx4_quantize_kernel<false><<<grid, kThreads, 0, stream>>>(x, (long)stride, q);
   }
   return hipGetLastError();
 }
@@ -148,16 +181,25 @@ hipError_t launch_mx4_dequant(const Mx4Args& q, uint16_t* out, int64_t stride, h
 {
   int grid;
   if (!tiles_of(q.rows, q.K, grid)) { return hipErrorInvalidConfiguration; }
-  mx4_dequant_kernel<<<grid, kThreads, 0, stream>>>(q, out, (long)stride, mx4_spans(q.K));
+  mx4_dequant_kernel<<<grid, kThreads, 0, stream>>>(q, out, (long)stride);
   return hipGetLastError();
 }
 
-hipError_t launch_mx4_scales(const uint8_t* in, uint8_t* out, int rows, int K, bool pack,
-                             hipStream_t stream)
+hipError_t launch_mx4_pack(const uint8_t* codes, const uint8_t* scales, const Mx4Args& q,
+                           hipStream_t stream)
 {
   int grid;
-  if (!tiles_of(rows, K, grid)) { return hipErrorInvalidConfiguration; }
-  mx4_scales_kernel<<<grid, kThreads, 0, stream>>>(in, out, rows, K / 32, mx4_spans(K), pack);
+  if (!tiles_of(q.rows, q.K, grid)) { return hipErrorInvalidConfiguration; }
+  mx4_order_kernel<true><<<grid, kThreads, 0, stream>>>(q, const_cast<uint8_t*>(codes),
+                                                        const_cast<uint8_t*>(scales));
+  return hipGetLastError();
+}
+
+hipError_t launch_mx4_unpack(const Mx4Args& q, uint8_t* codes, uint8_t* scales, hipStream_t stream)
+{
+  int grid;
+  if (!tiles_of(q.rows, q.K, grid)) { return hipErrorInvalidConfiguration; }
+  mx4_order_kernel<false><<<grid, kThreads, 0, stream>>>(q, codes, scales);
   return hipGetLastError();
 }
 

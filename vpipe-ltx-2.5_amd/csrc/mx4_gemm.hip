@@ -32,6 +32,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, size_
                                            0x00020000);
 }
 
+// An offset past every operand, whose soffset still adds up within 32 bits
+constexpr uint32_t kPast = 0xc0000000u;
+
 // acc += w . x over 128 values, scales in byte J of the lanes' registers
 template <int J>
 __device__ __forceinline__ f32x4 mfma_mx4(i32x4 w, i32x4 x, f32x4 acc, int ws, int xs)
@@ -40,193 +43,208 @@ __device__ __forceinline__ f32x4 mfma_mx4(i32x4 w, i32x4 x, f32x4 acc, int ws, i
                                                           kMfmaFp4, kMfmaFp4, J, ws, J, xs);
 }
 
-// 32 RB x 32 CB outputs of a workgroup of four waves, 2 x 2; a wave has RB x CB blocks of
-// 16 x 16. A step is 256 values of K: 128 bytes of a row, which go from memory straight into
-// one of two LDS stages, 8 rows an instruction, the row's 16-byte pieces at slot piece ^ (row
-// % 8), so that a fragment's reads (16 rows x 4 pieces) are free of bank conflicts. Scales go
-// to registers, a dword of a lane for each block of rows and two steps.
+// 64 RB x 16 CB outputs of a workgroup of four waves, one below the other: a wave has RB x CB
+// blocks of 16 x 16. The weight's rows, which all four read, go through LDS; a wave's rows of x
+// are its own and go from memory straight to its registers, two slices of 128 values ahead: LDS
+// then carries (16 CB rows x 5) bytes of K where both operands through LDS and 2 x 2 waves of
+// the same size carry (32 RB + 16 CB) x 3.
+//
+// A span is 512 values: two LDS stages of CB tiles x 4 slices take turns, filled a span ahead
+// by loads that go straight into LDS, one barrier a span. Tiles lie in LDS as in memory, and a
+// fragment's read is the tile's 1 KB in the order of the lanes.
 template <int RB, int CB>
-__global__ void __launch_bounds__(256, 2) mx4_tile_kernel(GemmParams p)
+__global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 {
-  constexpr int BM = 32 * RB, BN = 32 * CB;
-  constexpr int kStage = (BM + BN) * 128;
-  constexpr int kEP = BN + 8;   // staged output row
-  static_assert(BM * kEP * 2 <= 2 * kStage, "the staged tile fits the stages");
+  constexpr int BM = 64 * RB, BN = 16 * CB;
+  constexpr int kStage = 4 * CB * kMx4CodeTile;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
   map_tile(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
+  const int n0 = tn * BN, row0 = tm * BM + wave * 16 * RB;   // the wave's rows
 
   const int spans = mx4_spans(p.K);
   const int span0 = (int)blockIdx.y * p.span_chunk;
   const int span1 = min(span0 + p.span_chunk, spans);
-  const int blocks = p.K >> 5;
-  const int step1 = min(2 * span1, (blocks + 7) >> 3);
-  const uint32_t pitch = (uint32_t)p.K >> 1;
-
-  const size_t xbytes = (size_t)p.M * pitch, wbytes = (size_t)p.N * pitch;
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, xbytes), wr = make_rsrc(p.w, wbytes);
+  const int slices = mx4_slices(p.K);
+  const uint32_t pitch = (uint32_t)slices * kMx4CodeTile;   // of 16 rows
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, mx4_code_bytes(p.M, p.K));
+  const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.w, mx4_code_bytes(p.N, p.K));
   const __amdgpu_buffer_rsrc_t xsr = make_rsrc(p.xs, mx4_scale_bytes(p.M, p.K));
   const __amdgpu_buffer_rsrc_t wsr = make_rsrc(p.ws, mx4_scale_bytes(p.N, p.K));
 
-  // wave w issues instructions RB w + i of X and CB w + i of W
-  const int piece = (lane & 7) ^ (lane >> 3);
-  const uint32_t xoff = (uint32_t)(m0 + 8 * RB * wave + (lane >> 3)) * pitch + piece * 16;
-  const uint32_t woff = (uint32_t)(n0 + 8 * CB * wave + (lane >> 3)) * pitch + piece * 16;
-  auto load = [&](int s) {
-    uint8_t* const xd = lds + (s & 1) * kStage + RB * wave * 1024;
-    uint8_t* const wd = lds + (s & 1) * kStage + BM * 128 + CB * wave * 1024;
-    // pieces past the row's end would be the next row's: an offset past the operand gives zeros
-    const bool in = 8 * s + piece < blocks;
+  // Stage: [tile row][slice]. Wave w loads slice w of every tile row. Slices past the rows' end
+  // would be the next rows': an offset past the operand gives zeros.
+  const uint32_t woff = (uint32_t)(n0 / 16) * pitch + lane * 16;
+  auto load_w = [&](int span) {
+    const int t = 4 * span + wave;
+    uint8_t* const at = lds + (span & 1) * kStage + wave * kMx4CodeTile;
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          xr, (lds_u32*)(xd + i * 1024), 16, (int)(in ? xoff + 8u * i * pitch : (uint32_t)xbytes),
-          s * 128, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < CB; ++i) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          wr, (lds_u32*)(wd + i * 1024), 16, (int)(in ? woff + 8u * i * pitch : (uint32_t)wbytes),
-          s * 128, 0, 0);
+    for (int j = 0; j < CB; ++j) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_u32*)(at + j * 4 * kMx4CodeTile), 16,
+                                               (int)(t < slices ? woff + j * pitch : kPast),
+                                               t * kMx4CodeTile, 0, 0);
     }
   };
-  int xs[RB], ws[CB];
+  const uint32_t xoff = (uint32_t)(row0 / 16) * pitch + lane * 16;
+  i32x4 x[4][RB];
+  auto load_x = [&](int t, int buf) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      x[buf][i] = __builtin_bit_cast(
+          i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                     xr, (int)(t < slices ? xoff + i * pitch : kPast), t * kMx4CodeTile, 0));
+    }
+  };
+  int xs[RB], ws[CB], nxs[RB], nws[CB];
   auto load_scales = [&](int span) {
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
-      const uint32_t at = (uint32_t)((m0 + wm * 16 * RB) / 16 + i) * spans * kMx4Tile + lane * 4;
-      xs[i] = __builtin_amdgcn_raw_buffer_load_b32(xsr, (int)at, span * kMx4Tile, 0);
+      nxs[i] = __builtin_amdgcn_raw_buffer_load_b32(
+          xsr, (int)((uint32_t)(row0 / 16 + i) * spans * kMx4Tile + lane * 4), span * kMx4Tile, 0);
     }
 #pragma unroll
     for (int j = 0; j < CB; ++j) {
-      const uint32_t at = (uint32_t)((n0 + wn * 16 * CB) / 16 + j) * spans * kMx4Tile + lane * 4;
-      ws[j] = __builtin_amdgcn_raw_buffer_load_b32(wsr, (int)at, span * kMx4Tile, 0);
+      nws[j] = __builtin_amdgcn_raw_buffer_load_b32(
+          wsr, (int)((uint32_t)(n0 / 16 + j) * spans * kMx4Tile + lane * 4), span * kMx4Tile, 0);
     }
   };
-  const int fo0 = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
-  const int fo1 = (lane & 15) * 128 + (((4 + (lane >> 4)) ^ (lane & 7)) * 16);
   f32x4 acc[RB][CB] = {};
-  int cxs[RB], cws[CB];
-  auto step = [&](int s, auto half) {
-    constexpr int H = decltype(half)::value;
-    const uint8_t* const xb = lds + (s & 1) * kStage + wm * 16 * RB * 128;
-    const uint8_t* const wb = lds + (s & 1) * kStage + BM * 128 + wn * 16 * CB * 128;
-    auto slice = [&](auto sl) {
-      constexpr int J = 2 * H + decltype(sl)::value;
-      const int fo = decltype(sl)::value ? fo1 : fo0;
-      i32x4 a[RB], b[CB];
+  auto slice = [&](int span, auto sl) {
+    constexpr int J = decltype(sl)::value;
+    const uint8_t* const wb = lds + (span & 1) * kStage + J * kMx4CodeTile + lane * 16;
+    i32x4 w[CB];
 #pragma unroll
-      for (int i = 0; i < RB; ++i) { a[i] = *(const i32x4*)(xb + fo + i * 16 * 128); }
+    for (int j = 0; j < CB; ++j) { w[j] = *(const i32x4*)(wb + j * 4 * kMx4CodeTile); }
 #pragma unroll
-      for (int j = 0; j < CB; ++j) { b[j] = *(const i32x4*)(wb + fo + j * 16 * 128); }
+    for (int j = 0; j < CB; ++j) {
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
-#pragma unroll
-        for (int j = 0; j < CB; ++j) {
-          acc[i][j] = mfma_mx4<J>(b[j], a[i], acc[i][j], cws[j], cxs[i]);
-        }
+        acc[i][j] = mfma_mx4<J>(w[j], x[J][i], acc[i][j], ws[j], xs[i]);
       }
-    };
-    slice(std::integral_constant<int, 0>{});
-    slice(std::integral_constant<int, 1>{});
-  };
-  // every load in flight has landed, in all waves
-  auto landed = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-    __syncthreads();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (J & 1) {
+      load_x(4 * span + J + 3, J - 1);
+      load_x(4 * span + J + 4, J);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  load(2 * span0);
+  load_w(span0);
   load_scales(span0);
-  for (int s = 2 * span0; s < step1; s += 2) {
-    landed();
+  load_x(4 * span0, 0);
+  load_x(4 * span0 + 1, 1);
+  load_x(4 * span0 + 2, 2);
+  load_x(4 * span0 + 3, 3);
+  for (int span = span0; span < span1; ++span) {
+    // this span's weight loads have landed: two slices of x and no more came after them
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * RB));
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < RB; ++i) { cxs[i] = xs[i]; }
+    for (int i = 0; i < RB; ++i) { xs[i] = nxs[i]; }
 #pragma unroll
-    for (int j = 0; j < CB; ++j) { cws[j] = ws[j]; }
-    if (s + 1 < step1) { load(s + 1); }
-    if (s + 2 < step1) { load_scales((s + 2) / 2); }
-    step(s, std::integral_constant<int, 0>{});
-    landed();
-    if (s + 1 >= step1) { break; }
-    if (s + 2 < step1) { load(s + 2); }
-    step(s + 1, std::integral_constant<int, 1>{});
+    for (int j = 0; j < CB; ++j) { ws[j] = nws[j]; }
+    // Unconditionally, so that the compiler knows how many loads there are behind a slice of x;
+    // past the row's end they give zeros.
+    load_w(span + 1);
+    load_scales(span + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    slice(span, std::integral_constant<int, 0>{});
+    slice(span, std::integral_constant<int, 1>{});
+    slice(span, std::integral_constant<int, 2>{});
+    slice(span, std::integral_constant<int, 3>{});
   }
-  __syncthreads();
+
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // no load into LDS outlives the wave
 
   // block (i, j), lane l, register r: row 16 i + l % 16, column 16 j + 4 (l / 16) + r
-  const int lrow = lane & 15, lcol = (lane >> 4) * 4;
-  if (p.partial != nullptr) {
-    float* const out = p.partial + (size_t)blockIdx.y * p.M * p.N;
+  const int g = lane >> 4;
+  if (p.partial != nullptr || p.N % 8 != 0) {
+    float* const part = p.partial == nullptr ? nullptr : p.partial + (size_t)blockIdx.y * p.M * p.N;
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      const int m = m0 + (wm * RB + i) * 16 + lrow;
-      if (m >= p.M) { continue; }
+    for (int j = 0; j < CB; ++j) {
 #pragma unroll
-      for (int j = 0; j < CB; ++j) {
-        const int n = n0 + (wn * CB + j) * 16 + lcol;
+      for (int r = 0; r < 4; ++r) {
+        const int n = n0 + 16 * j + 4 * g + r;
+        const float bias = load_bias(p.bias, p.bias_type, min(n, p.N - 1));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (n + r < p.N) { out[(size_t)m * p.N + n + r] = acc[i][j][r]; }
+        for (int i = 0; i < RB; ++i) {
+          const int m = row0 + 16 * i + (lane & 15);
+          if (m >= p.M || n >= p.N) { continue; }
+          if (part != nullptr) {
+            part[(size_t)m * p.N + n] = acc[i][j][r];
+          } else {
+            const float v = acc[i][j][r] + bias;
+            p.y[(size_t)m * p.N + n] = f32_to_bf16(p.epilogue == kEpiGelu ? gelu_tanh(v) : v);
+          }
         }
       }
     }
     return;
   }
-  uint16_t* const stage = (uint16_t*)lds;
+  // Two blocks side by side: the lanes' rows of 16 are exchanged so that each lane has eight
+  // columns of one of them, 16 bytes.
+  auto store = [&](auto gelu) {
 #pragma unroll
-  for (int j = 0; j < CB; ++j) {
-    const int c = (wn * CB + j) * 16 + lcol;
-    float bias[4];
+    for (int j = 0; j < CB; j += 2) {
+      float bias[2][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) { bias[r] = load_bias(p.bias, p.bias_type, min(n0 + c + r, p.N - 1)); }
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      float v[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[r] = acc[i][j][r] + bias[r];
-        if (p.epilogue == kEpiGelu) { v[r] = gelu_tanh(v[r]); }
+        for (int r = 0; r < 4; ++r) {
+          bias[h][r] =
+              load_bias(p.bias, p.bias_type, min(n0 + 16 * (j + h) + 4 * g + r, p.N - 1));
+        }
       }
-      *(uint2*)(stage + ((wm * RB + i) * 16 + lrow) * kEP + c) =
-          make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    }
-  }
-  __syncthreads();
-  if (p.N % 8 == 0) {
-    for (int q = tid; q < BM * BN / 8; q += 256) {
-      const int r = q / (BN / 8), c = (q % (BN / 8)) * 8;
-      if (m0 + r < p.M && n0 + c < p.N) {
-        *(uint4*)(p.y + (size_t)(m0 + r) * p.N + n0 + c) = *(const uint4*)(stage + r * kEP + c);
+      const int n = n0 + 16 * (j + (g & 1)) + 8 * (g >> 1);
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        uint32_t w[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            v[r] = acc[i][j + h][r] + bias[h][r];
+            if constexpr (decltype(gelu)::value) { v[r] = gelu_tanh(v[r]); }
+          }
+          w[h][0] = pack_bf16x2(v[0], v[1]);
+          w[h][1] = pack_bf16x2(v[2], v[3]);
+        }
+        const auto a = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+        const int m = row0 + 16 * i + (lane & 15);
+        if (m < p.M && n < p.N) {
+          const i32x4 v = {(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
+          __builtin_nontemporal_store(v, (i32x4*)(p.y + (size_t)m * p.N + n));
+        }
       }
     }
+  };
+  if (p.epilogue == kEpiGelu) {
+    store(std::true_type{});
   } else {
-    for (int q = tid; q < BM * BN; q += 256) {
-      const int r = q / BN, c = q % BN;
-      if (m0 + r < p.M && n0 + c < p.N) {
-        p.y[(size_t)(m0 + r) * p.N + n0 + c] = stage[r * kEP + c];
-      }
-    }
+    store(std::false_type{});
   }
 }
 
 template <int RB, int CB>
-hipError_t run_tile(GemmParams& p, const Mx4Plan& plan, hipStream_t stream)
+hipError_t run_wide(GemmParams& p, const Mx4Plan& plan, hipStream_t stream)
 {
-  p.tiles_m = (p.M + 32 * RB - 1) / (32 * RB);
-  p.tiles_n = (p.N + 32 * CB - 1) / (32 * CB);
+  p.tiles_m = (p.M + 64 * RB - 1) / (64 * RB);
+  p.tiles_n = (p.N + 16 * CB - 1) / (16 * CB);
   const long tiles = (long)p.tiles_m * p.tiles_n;
   if (tiles * 256 >= 1L << 32) { return hipErrorInvalidConfiguration; }
-  mx4_tile_kernel<RB, CB><<<dim3((unsigned)tiles, (unsigned)plan.splits), 256, 0, stream>>>(p);
+  mx4_wide_kernel<RB, CB><<<dim3((unsigned)tiles, (unsigned)plan.splits), 256, 0, stream>>>(p);
   return hipGetLastError();
 }
 
-// Rows of x below 2 GiB of codes and scales
-constexpr size_t kSlabBytes = (size_t)1 << 31;
+// Bytes of a launch's rows of x
+constexpr size_t kSlabBytes = (size_t)1 << 30;
 
 }  // namespace
 
@@ -254,10 +272,10 @@ hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t st
   }
   const int K = g.w.K, M = g.x.rows, N = g.w.rows;
   // rows of a launch: whole tiles, operands that 32-bit offsets reach
-  const long most = (long)((kSlabBytes - 1) / (size_t)(K / 2)) & ~255L;
+  const long most = (long)(kSlabBytes / ((size_t)mx4_slices(K) * (kMx4CodeTile / 16))) & ~255L;
   for (long m = 0; m < M; m += most) {
     GemmParams p;
-    p.x = g.x.codes + (size_t)m * (K / 2);
+    p.x = g.x.codes + (size_t)(m / 16) * mx4_slices(K) * kMx4CodeTile;
     p.xs = g.x.scales + (size_t)(m / 16) * mx4_spans(K) * kMx4Tile;
     p.w = g.w.codes;
     p.ws = g.w.scales;
@@ -270,7 +288,7 @@ hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t st
     p.bias_type = g.bias_type;
     p.epilogue = g.epilogue;
     p.span_chunk = plan.span_chunk;
-    hipError_t e = plan.tile == 0 ? run_tile<4, 4>(p, plan, stream) : run_tile<2, 2>(p, plan, stream);
+    hipError_t e = plan.tile == 0 ? run_wide<4, 8>(p, plan, stream) : run_wide<1, 4>(p, plan, stream);
     if (e == hipSuccess && p.partial != nullptr) {
       e = launch_splitk_reduce(p.partial, plan.splits, g.bias, g.bias_type, g.epilogue, nullptr,
                                p.y, p.M, N, stream);

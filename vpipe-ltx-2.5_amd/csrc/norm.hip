@@ -177,19 +177,18 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
       if (p.out != nullptr) { *(uint4*)(p.out + token * p.os + col[i]) = pack8(x[i]); }
     }
     if (p.q.codes != nullptr) {
-      // a block's four lanes are in or out together: the width is a multiple of 32
-      const int block = col[i] >> 5, spans = mx4_spans(p.width);
-      if (in[i]) {
-        uint32_t scale;
-        const uint32_t codes = mx4_code_quad(x[i], scale);
-        *(uint32_t*)(p.q.codes + token * (p.width >> 1) + (col[i] >> 1)) = codes;
-        if ((lane & 3) == 0) {
-          p.q.scales[((token >> 4) * spans + (block >> 4)) * kMx4Tile +
-                     mx4_scale_at((int)(token & 15), block)] = (uint8_t)scale;
-        }
-      } else if ((lane & 3) == 0 && block < spans * 16) {
+      // a block's four lanes are in or out together: the width is a multiple of 32; blocks past
+      // it in the row's last tiles are zeros
+      const int block = col[i] >> 5, slices = mx4_slices(p.width), spans = mx4_spans(p.width);
+      uint32_t scale = 0, codes = 0;
+      if (in[i]) { codes = mx4_code_quad(x[i], scale); }
+      if (block < slices * 4) {
+        *(uint32_t*)(p.q.codes + ((token >> 4) * slices + (block >> 2)) * kMx4CodeTile +
+                     mx4_code_at((int)(token & 15), block) + (lane & 3) * 4) = codes;
+      }
+      if ((lane & 3) == 0 && block < spans * 16) {
         p.q.scales[((token >> 4) * spans + (block >> 4)) * kMx4Tile +
-                   mx4_scale_at((int)(token & 15), block)] = 0;
+                   mx4_scale_at((int)(token & 15), block)] = (uint8_t)scale;
       }
     }
   }

@@ -91,23 +91,8 @@ int check_source(const char* name, const void* x, int64_t stride, int K, bool wi
   return rc != LTX25_OK ? rc : check_pointer("x", x, 16);
 }
 
-size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
-
-// The activations' codes and scales in linear_mx4's workspace, the products' parts
-// behind them
-struct Inside {
-  size_t scales = 0, partial = 0, bytes = 0;
-};
-Inside inside(int M, int K, const ltx25::Mx4Plan& plan)
-{
-  Inside r;
-  if (plan.codes_ahead) {
-    r.scales = up(ltx25::mx4_code_bytes(M, K));
-    r.partial = r.scales + up(ltx25::mx4_scale_bytes(M, K));
-  }
-  r.bytes = r.partial + plan.partial_bytes;
-  return r;
-}
+// Where the activations' scales lie in linear_mx4's workspace, behind their codes
+size_t scales_at(int M, int K) { return (ltx25::mx4_code_bytes(M, K) + 255) & ~(size_t)255; }
 
 int run(void* stream, ltx25::Mx4Gemm& g, const ltx25::Mx4Plan& plan, const void* bias,
         int bias_dtype, void* y, int epilogue)
@@ -203,7 +188,7 @@ int ltx25_mx4_unpack(void* stream, const ltx25_mx4* q, void* codes, void* scales
 size_t ltx25_mx4_gemm_workspace(int M, int K, int N)
 {
   if (!sizes_fit(M, K) || !sizes_fit(N, K)) { return 0; }
-  return ltx25::plan_mx4(M, K, N, false).partial_bytes;
+  return 0;   // the waves' sums meet in LDS
 }
 
 int ltx25_mx4_gemm(void* stream, const ltx25_mx4* x, const ltx25_mx4* w, const void* bias,
@@ -218,7 +203,6 @@ int ltx25_mx4_gemm(void* stream, const ltx25_mx4* x, const ltx25_mx4* w, const v
   const size_t need = ltx25_mx4_gemm_workspace(g.x.rows, g.x.K, g.w.rows);
   rc = check_product(g.w, g.x.rows, bias, bias_dtype, y, epilogue, workspace, workspace_bytes, need);
   if (rc != LTX25_OK || g.x.rows == 0 || g.w.rows == 0) { return rc; }
-  g.partial = (float*)workspace;
   return run(stream, g, ltx25::plan_mx4(g.x.rows, g.x.K, g.w.rows, false), bias, bias_dtype, y,
              epilogue);
 }
@@ -226,7 +210,8 @@ int ltx25_mx4_gemm(void* stream, const ltx25_mx4* x, const ltx25_mx4* w, const v
 size_t ltx25_linear_mx4_workspace(int M, int K, int N)
 {
   if (!sizes_fit(M, K) || !sizes_fit(N, K)) { return 0; }
-  return inside(M, K, ltx25::plan_mx4(M, K, N, true)).bytes;
+  if (!ltx25::plan_mx4(M, K, N, true).codes_ahead) { return 0; }
+  return scales_at(M, K) + ltx25::mx4_scale_bytes(M, K);
 }
 
 int ltx25_linear_mx4(void* stream, const void* x, int64_t x_stride, int M, const ltx25_mx4* w,
@@ -241,14 +226,12 @@ int ltx25_linear_mx4(void* stream, const void* x, int64_t x_stride, int M, const
   if (rc != LTX25_OK || M == 0 || g.w.rows == 0) { return rc; }
   if ((rc = check_source("x_stride", x, x_stride, g.w.K, false)) != LTX25_OK) { return rc; }
   const ltx25::Mx4Plan plan = ltx25::plan_mx4(M, g.w.K, g.w.rows, true);
-  const Inside at = inside(M, g.w.K, plan);
   g.x.codes = (uint8_t*)workspace;
-  g.x.scales = (uint8_t*)workspace + at.scales;
+  g.x.scales = (uint8_t*)workspace + scales_at(M, g.w.K);
   g.x.rows = M;
   g.x.K = g.w.K;
   g.xb = (const uint16_t*)x;
   g.xb_stride = x_stride;
-  g.partial = (float*)((uint8_t*)workspace + at.partial);
   return run(stream, g, plan, bias, bias_dtype, y, epilogue);
 }
 

@@ -81,6 +81,27 @@ __device__ __forceinline__ uint32_t mx4_code_quad(const float (&v)[8], uint32_t&
   return scale == 255u ? 0u : mx4_codes(v, mx4_factor(scale));
 }
 
+// The same of bf16 values as they lie in memory. The conversion divides by 2^exponent, of
+// which its scale operand holds the bits: the exponent byte is f32's own, 0 for 2^-127 too.
+__device__ __forceinline__ uint32_t mx4_code_bf16_quad(uint4 raw, uint32_t& scale)
+{
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  u16x2 top = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  }
+  scale = mx4_scale(quad_max((uint32_t)max((int)top[0], (int)top[1]) << 16));
+  const float unit = __uint_as_float(scale << 23);
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[0]), unit, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[1]), unit, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[2]), unit, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[3]), unit, 3);
+  return scale == 255u ? 0u : r;
+}
+
 // A matrix operand of a lane: 32 codes, in the low half of the instruction's register
 // list (4-bit operands do not use the rest)
 __device__ __forceinline__ i32x8 mx4_operand(i32x4 v)
@@ -114,16 +135,11 @@ struct Mx4Gemm {
   int bias_type = kBiasNone;
   int epilogue = kEpiNone;
   uint16_t* y = nullptr;
-  float* partial = nullptr;   // plan.partial_bytes
 };
-// How a product is cut; a function of the sizes alone, so that the workspace can be
-// asked for ahead.
+// The kernel and tile of a product; a function of the sizes alone.
 struct Mx4Plan {
-  int tile = 0;         // rows x columns of a workgroup: 0 128 x 128, 1 64 x 64
-  int splits = 1;       // parts of K
-  int span_chunk = 0;   // 512-value spans of a part
+  int tile = 0;
   bool codes_ahead = false;   // bf16 activations are coded by a launch ahead
-  size_t partial_bytes = 0;
 };
 // `bf16`: the activations come in bf16
 Mx4Plan plan_mx4(int M, int K, int N, bool bf16);

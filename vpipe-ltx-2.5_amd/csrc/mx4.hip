@@ -74,21 +74,17 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const void* x, l
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = wave + 4 * i;
-    float v[8];
+    uint32_t scale, codes;
     if constexpr (WIDE) {
       const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w,
                              raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+      float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) { v[k] = __uint_as_float(w[k]); }
+      codes = mx4_code_quad(v, scale);
     } else {
-      const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
-      }
+      codes = mx4_code_bf16_quad(raw[i][0], scale);
     }
-    uint32_t scale;
-    const uint32_t codes = mx4_code_quad(v, scale);
     // zeros in blocks past K (and in rows past the last, which nothing reads)
     *(uint32_t*)((uint8_t*)held + codes_at(r, lane)) = codes;
     if ((lane & 3) == 0) { ((uint8_t*)tile)[mx4_scale_at(r, lane >> 2)] = in ? (uint8_t)scale : 0; }

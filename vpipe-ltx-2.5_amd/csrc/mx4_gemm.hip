@@ -4,7 +4,10 @@
 #include "mx4.h"
 
 #include <algorithm>
+#include <cstdio>
+#include <cstdlib>
 #include <type_traits>
+#include <utility>
 
 namespace ltx25 {
 namespace {
@@ -18,11 +21,9 @@ struct GemmParams {
   const uint8_t* ws;
   const void* bias;
   uint16_t* y;
-  float* partial;   // null: y is written
   int M, N, K;
   int bias_type, epilogue;
   int tiles_m, tiles_n;
-  int span_chunk;
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, size_t bytes)
@@ -30,6 +31,18 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, size_
   // loads past `bytes` return zeros
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)(uint32_t)bytes,
                                            0x00020000);
+}
+
+// f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>)
+template <typename F, int... I>
+__device__ __forceinline__ void unroll_seq(F&& f, std::integer_sequence<int, I...>)
+{
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unroll(F&& f)
+{
+  unroll_seq(f, std::make_integer_sequence<int, N>{});
 }
 
 // An offset past every operand, whose soffset still adds up within 32 bits
@@ -45,126 +58,148 @@ __device__ __forceinline__ f32x4 mfma_mx4(i32x4 w, i32x4 x, f32x4 acc, int ws, i
 
 // 64 RB x 16 CB outputs of a workgroup of four waves, one below the other: a wave has RB x CB
 // blocks of 16 x 16. The weight's rows, which all four read, go through LDS; a wave's rows of x
-// are its own and go from memory straight to its registers, two slices of 128 values ahead: LDS
-// then carries (16 CB rows x 5) bytes of K where both operands through LDS and 2 x 2 waves of
-// the same size carry (32 RB + 16 CB) x 3.
+// are its own and go from memory straight to its registers, DEPTH slices of 128 values ahead: LDS
+// then carries 5 x 16 CB rows of K where both operands through LDS and 2 x 2 waves of the same
+// size carry 3 x (64 RB + 16 CB).
 //
-// A span is 512 values: two LDS stages of CB tiles x 4 slices take turns, filled a span ahead
-// by loads that go straight into LDS, one barrier a span. Tiles lie in LDS as in memory, and a
-// fragment's read is the tile's 1 KB in the order of the lanes.
-template <int RB, int CB>
+// A span is 512 values: STAGES LDS stages of CB x 4 tiles of codes and all the workgroup's scales
+// take turns, filled STAGES - 1 spans ahead by loads that go straight into LDS, one barrier a
+// span. Tiles lie in LDS as in memory, and a fragment's read is the tile's 1 KB in the order of
+// the lanes.
+template <int RB, int CB, int STAGES, int DEPTH>
 __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 {
-  constexpr int BM = 64 * RB, BN = 16 * CB;
-  constexpr int kStage = 4 * CB * kMx4CodeTile;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  static_assert(DEPTH == 4 || DEPTH == 8, "slices in flight, a span's or two");
+  constexpr int kCodes = 4 * CB * kMx4CodeTile;
+  constexpr int kScaleTiles = 4 * RB + CB, kScaleLoads = (kScaleTiles + 15) / 16;
+  constexpr int kStage = kCodes + 16 * kScaleLoads * kMx4Tile;
+  static_assert(STAGES * kStage <= 80 * 1024, "two workgroups a CU");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
   map_tile(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
-  const int n0 = tn * BN, row0 = tm * BM + wave * 16 * RB;   // the wave's rows
+  const int n0 = tn * 16 * CB, row0 = (tm * 4 + wave) * 16 * RB;   // the wave's rows
 
-  const int spans = mx4_spans(p.K);
-  const int span0 = (int)blockIdx.y * p.span_chunk;
-  const int span1 = min(span0 + p.span_chunk, spans);
-  const int slices = mx4_slices(p.K);
+  const int slices = mx4_slices(p.K), spans = mx4_spans(p.K);
   const uint32_t pitch = (uint32_t)slices * kMx4CodeTile;   // of 16 rows
+  const uint32_t spitch = (uint32_t)spans * kMx4Tile;
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, mx4_code_bytes(p.M, p.K));
   const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.w, mx4_code_bytes(p.N, p.K));
   const __amdgpu_buffer_rsrc_t xsr = make_rsrc(p.xs, mx4_scale_bytes(p.M, p.K));
   const __amdgpu_buffer_rsrc_t wsr = make_rsrc(p.ws, mx4_scale_bytes(p.N, p.K));
 
-  // Stage: [tile row][slice]. Wave w loads slice w of every tile row. Slices past the rows' end
-  // would be the next rows': an offset past the operand gives zeros.
+  // Codes of a stage: [tile row][slice], wave w loads slice w of every tile row. Slices past the
+  // rows' end would be the next rows': an offset past the operand gives zeros. Scales: tiles of
+  // x, then of w, four a load; wave w has loads w, w + 4 (those past the last tile zeros).
   const uint32_t woff = (uint32_t)(n0 / 16) * pitch + lane * 16;
-  auto load_w = [&](int span) {
-    const int t = 4 * span + wave;
-    uint8_t* const at = lds + (span & 1) * kStage + wave * kMx4CodeTile;
+  uint32_t soff[kScaleLoads];
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_u32*)(at + j * 4 * kMx4CodeTile), 16,
-                                               (int)(t < slices ? woff + j * pitch : kPast),
-                                               t * kMx4CodeTile, 0, 0);
+  for (int i = 0; i < kScaleLoads; ++i) {
+    const int q = wave + 4 * i, tile = 4 * q + (lane >> 4);
+    const uint32_t at = q < RB ? (uint32_t)(tm * 4 * RB + tile) : (uint32_t)(tn * CB + tile - 4 * RB);
+    soff[i] = tile < kScaleTiles ? at * spitch + (lane & 15) * 16 : kPast;
+  }
+  constexpr int kW = CB + kScaleLoads;   // loads of a wave into a stage
+  auto load_w = [&](int span, int stage, int k) {   // the k-th of them
+    uint8_t* const at = lds + stage * kStage;
+    if (k < CB) {
+      const int t = 4 * span + wave;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          wr, (lds_u32*)(at + (4 * k + wave) * kMx4CodeTile), 16,
+          (int)(t < slices ? woff + k * pitch : kPast), t * kMx4CodeTile, 0, 0);
+    } else {
+      const int q = wave + 4 * (k - CB);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(q < RB ? xsr : wsr,
+                                               (lds_u32*)(at + kCodes + q * 4 * kMx4Tile), 16,
+                                               (int)(span < spans ? soff[k - CB] : kPast),
+                                               span * kMx4Tile, 0, 0);
     }
   };
   const uint32_t xoff = (uint32_t)(row0 / 16) * pitch + lane * 16;
-  i32x4 x[4][RB];
-  auto load_x = [&](int t, int buf) {
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      x[buf][i] = __builtin_bit_cast(
-          i32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                     xr, (int)(t < slices ? xoff + i * pitch : kPast), t * kMx4CodeTile, 0));
-    }
+  i32x4 x[DEPTH][RB];
+  auto load_x = [&](int t, int buf, int i) {
+    x[buf][i] = __builtin_bit_cast(
+        i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                   xr, (int)(t < slices ? xoff + i * pitch : kPast), t * kMx4CodeTile, 0));
   };
-  int xs[RB], ws[CB], nxs[RB], nws[CB];
-  auto load_scales = [&](int span) {
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      nxs[i] = __builtin_amdgcn_raw_buffer_load_b32(
-          xsr, (int)((uint32_t)(row0 / 16 + i) * spans * kMx4Tile + lane * 4), span * kMx4Tile, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < CB; ++j) {
-      nws[j] = __builtin_amdgcn_raw_buffer_load_b32(
-          wsr, (int)((uint32_t)(n0 / 16 + j) * spans * kMx4Tile + lane * 4), span * kMx4Tile, 0);
-    }
-  };
+  // A span is 4 CB fragments of w, RB matrix instructions each. Its loads go out one by one among
+  // them, since a wave waits until the address unit has taken its load (all of a span's loads to
+  // LDS at its start and a slice's of x behind the slice: 2.5 us a span of one workgroup a CU;
+  // without those of x 1.9, without those to LDS 2.1): the k-th load to LDS at fragment 2 k,
+  // and slice J - 1's registers are filled anew during slice J.
+  static_assert(2 * (kW - 1) < 4 * CB && CB % RB == 0, "a span has room for its loads");
+  constexpr int kXEvery = CB / RB;
+  // loads of x behind the last one to LDS
+  constexpr int kXBehind = (4 * CB - 1 - 2 * (kW - 1)) / kXEvery;
   f32x4 acc[RB][CB] = {};
-  auto slice = [&](int span, auto sl) {
-    constexpr int J = decltype(sl)::value;
-    const uint8_t* const wb = lds + (span & 1) * kStage + J * kMx4CodeTile + lane * 16;
-    i32x4 w[CB];
-#pragma unroll
-    for (int j = 0; j < CB; ++j) { w[j] = *(const i32x4*)(wb + j * 4 * kMx4CodeTile); }
-#pragma unroll
-    for (int j = 0; j < CB; ++j) {
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        acc[i][j] = mfma_mx4<J>(w[j], x[J][i], acc[i][j], ws[j], xs[i]);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (J & 1) {
-      load_x(4 * span + J + 3, J - 1);
-      load_x(4 * span + J + 4, J);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-
-  load_w(span0);
-  load_scales(span0);
-  load_x(4 * span0, 0);
-  load_x(4 * span0 + 1, 1);
-  load_x(4 * span0 + 2, 2);
-  load_x(4 * span0 + 3, 3);
-  for (int span = span0; span < span1; ++span) {
-    // this span's weight loads have landed: two slices of x and no more came after them
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * RB));
+  int stage = 0;   // of the span
+  auto step = [&](int span, auto parity) {
+    constexpr int B = DEPTH == 8 ? 4 * decltype(parity)::value : 0;
+    // The span's loads into LDS have landed: behind them came those of x of the span that issued
+    // them, and STAGES - 2 spans' since. Then the stage that the last span used is free.
+    constexpr int kBehind = kXBehind + (STAGES - 2) * (kW + 4 * RB);
+    constexpr int kWait = kBehind < 63 ? kBehind : 63;
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (kWait & 15) | ((kWait >> 4) << 14));
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
+    const int next = stage == 0 ? STAGES - 1 : stage - 1;
+    const uint8_t* const at = lds + stage * kStage + lane * 16;
+    const uint8_t* const sat = lds + stage * kStage + kCodes + lane * 4;
+    int xs[RB], ws[CB];
 #pragma unroll
-    for (int i = 0; i < RB; ++i) { xs[i] = nxs[i]; }
+    for (int i = 0; i < RB; ++i) { xs[i] = *(const int*)(sat + (wave * RB + i) * kMx4Tile); }
 #pragma unroll
-    for (int j = 0; j < CB; ++j) { ws[j] = nws[j]; }
-    // Unconditionally, so that the compiler knows how many loads there are behind a slice of x;
-    // past the row's end they give zeros.
-    load_w(span + 1);
-    load_scales(span + 1);
+    for (int j = 0; j < CB; ++j) { ws[j] = *(const int*)(sat + (4 * RB + j) * kMx4Tile); }
+    // Fragment f is slice f / CB of tile row f % CB; three are on their way from LDS while one
+    // is multiplied (left to itself the compiler asks for two and waits for them).
+    auto fragment = [&](int f) { return *(const i32x4*)(at + (4 * (f % CB) + f / CB) * kMx4CodeTile); };
+    i32x4 w[4] = {fragment(0), fragment(1), fragment(2)};
     __builtin_amdgcn_sched_barrier(0);
-    slice(span, std::integral_constant<int, 0>{});
-    slice(span, std::integral_constant<int, 1>{});
-    slice(span, std::integral_constant<int, 2>{});
-    slice(span, std::integral_constant<int, 3>{});
-  }
+    unroll<4 * CB>([&](auto ff) {
+      constexpr int f = decltype(ff)::value, J = f / CB, j = f % CB;
+      if constexpr (f + 3 < 4 * CB) { w[(f + 3) % 4] = fragment(f + 3); }
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        acc[i][j] = mfma_mx4<J>(w[f % 4], x[B + J][i], acc[i][j], ws[j], xs[i]);
+      }
+      // Unconditionally, so that the number of loads behind others is known; past the end they
+      // give zeros.
+      if constexpr (f % 2 == 0 && f / 2 < kW) { load_w(span + STAGES - 1, next, f / 2); }
+      if constexpr (j % kXEvery == kXEvery - 1) {
+        constexpr int kBuf = J > 0 ? B + J - 1 : DEPTH == 8 ? 7 - B : 3;
+        load_x(4 * span + J - 1 + DEPTH, kBuf, j / kXEvery);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+  };
 
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+#pragma unroll
+    for (int k = 0; k < kW; ++k) { load_w(i, i, k); }
+  }
+#pragma unroll
+  for (int t = 0; t < DEPTH - 1; ++t) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i) { load_x(t, t, i); }
+  }
+  // the first stages have landed, for what the count above does not see
+  constexpr int kFirst = (DEPTH - 1) * RB;
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (kFirst < 15 ? kFirst : 15));
+  int span = 0;
+  for (; span + 1 < spans; span += 2) {
+    step(span, std::integral_constant<int, 0>{});
+    step(span + 1, std::integral_constant<int, 1>{});
+  }
+  if (span < spans) { step(span, std::integral_constant<int, 0>{}); }
   __builtin_amdgcn_s_waitcnt(0x0f70);   // no load into LDS outlives the wave
 
   // block (i, j), lane l, register r: row 16 i + l % 16, column 16 j + 4 (l / 16) + r
   const int g = lane >> 4;
-  if (p.partial != nullptr || p.N % 8 != 0) {
-    float* const part = p.partial == nullptr ? nullptr : p.partial + (size_t)blockIdx.y * p.M * p.N;
+  if (p.N % 8 != 0) {
 #pragma unroll
     for (int j = 0; j < CB; ++j) {
 #pragma unroll
@@ -175,12 +210,8 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
         for (int i = 0; i < RB; ++i) {
           const int m = row0 + 16 * i + (lane & 15);
           if (m >= p.M || n >= p.N) { continue; }
-          if (part != nullptr) {
-            part[(size_t)m * p.N + n] = acc[i][j][r];
-          } else {
-            const float v = acc[i][j][r] + bias;
-            p.y[(size_t)m * p.N + n] = f32_to_bf16(p.epilogue == kEpiGelu ? gelu_tanh(v) : v);
-          }
+          const float v = acc[i][j][r] + bias;
+          p.y[(size_t)m * p.N + n] = f32_to_bf16(p.epilogue == kEpiGelu ? gelu_tanh(v) : v);
         }
       }
     }
@@ -232,14 +263,201 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   }
 }
 
-template <int RB, int CB>
-hipError_t run_wide(GemmParams& p, const Mx4Plan& plan, hipStream_t stream)
+template <int RB, int CB, int STAGES, int DEPTH>
+hipError_t run_wide(GemmParams& p, hipStream_t stream)
 {
   p.tiles_m = (p.M + 64 * RB - 1) / (64 * RB);
   p.tiles_n = (p.N + 16 * CB - 1) / (16 * CB);
   const long tiles = (long)p.tiles_m * p.tiles_n;
   if (tiles * 256 >= 1L << 32) { return hipErrorInvalidConfiguration; }
-  mx4_wide_kernel<RB, CB><<<dim3((unsigned)tiles, (unsigned)plan.splits), 256, 0, stream>>>(p);
+  mx4_wide_kernel<RB, CB, STAGES, DEPTH><<<(unsigned)tiles, 256, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+// ---- panels: few outputs -------------------------------------------------------
+
+// 16 RB x 16 CB outputs of a workgroup whose waves deal the spans of K among themselves: both
+// operands go from memory straight to registers, a tile's 1 KB an instruction, with four slices
+// in flight (the next span's slice is asked for when this span's has been multiplied), no
+// barrier before the waves' sums meet in LDS. For outputs of few tiles, where a workgroup that
+// walks all of K is a chain of its loads' latencies.
+//
+// CODED false: bf16 activations, up to 16 rows. A wave codes what it multiplies: four lanes
+// have a block and find its largest value, and the codes change to the matrix instruction's
+// lanes through LDS of the wave's own.
+template <int RB, int CB, int WAVES, bool CODED>
+__global__ void __launch_bounds__(64 * WAVES, WAVES >= 8 ? 2 : 1)
+mx4_panel_kernel(GemmParams p, const uint16_t* xb, long stride)
+{
+  static_assert(CODED || (RB == 1 && CB == 1), "more rows are coded ahead");
+  constexpr int kOut = 256 * RB * CB;
+  constexpr int kBuf = 5 * kMx4CodeTile;   // four slices' codes, and scales
+  __shared__ __attribute__((aligned(16))) uint8_t
+      lds[WAVES * (CODED ? kOut * 4 : (kOut * 4 > kBuf ? kOut * 4 : kBuf))];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane & 15, g = lane >> 4;
+  const int tn = (int)(blockIdx.x % (unsigned)p.tiles_n), tm = (int)(blockIdx.x / (unsigned)p.tiles_n);
+  const int slices = mx4_slices(p.K), spans = mx4_spans(p.K);
+  const uint32_t pitch = (uint32_t)slices * kMx4CodeTile, spitch = (uint32_t)spans * kMx4Tile;
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, CODED ? mx4_code_bytes(p.M, p.K) : 0);
+  const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.w, mx4_code_bytes(p.N, p.K));
+  const __amdgpu_buffer_rsrc_t xsr = make_rsrc(p.xs, CODED ? mx4_scale_bytes(p.M, p.K) : 0);
+  const __amdgpu_buffer_rsrc_t wsr = make_rsrc(p.ws, mx4_scale_bytes(p.N, p.K));
+  const uint32_t xoff = (uint32_t)(tm * RB) * pitch + lane * 16;
+  const uint32_t woff = (uint32_t)(tn * CB) * pitch + lane * 16;
+  const uint32_t xsoff = (uint32_t)(tm * RB) * spitch + lane * 4;
+  const uint32_t wsoff = (uint32_t)(tn * CB) * spitch + lane * 4;
+
+  i32x4 w[4][CB], x[4][RB];
+  uint4 raw[4][CODED ? 1 : 4];
+  int ws[CB], xs[RB], nws[CB], nxs[RB];
+  auto load = [&](int t, int j) {   // slice t; past the rows' end zeros
+    const bool in = t < slices;
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      w[j][c] = __builtin_bit_cast(
+          i32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, (int)(in ? woff + c * pitch : kPast),
+                                                       t * kMx4CodeTile, 0));
+    }
+    if constexpr (CODED) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        x[j][i] = __builtin_bit_cast(
+            i32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, (int)(in ? xoff + i * pitch : kPast),
+                                                         t * kMx4CodeTile, 0));
+      }
+    } else {
+      // lane l: values 8 (l % 16) .. of row 4 i + l / 16; past K the row's first ones, unused
+      const int at = t * 128 + row * 8;
+      const uint16_t* const from = xb + (at < p.K ? at : 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (4 * i < p.M) { raw[j][i] = *(const uint4*)(from + min(4 * i + g, p.M - 1) * stride); }
+      }
+    }
+  };
+  auto load_scales = [&](int span) {
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      nws[c] = __builtin_amdgcn_raw_buffer_load_b32(wsr, (int)(wsoff + c * spitch), span * kMx4Tile, 0);
+    }
+    if constexpr (CODED) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        nxs[i] = __builtin_amdgcn_raw_buffer_load_b32(xsr, (int)(xsoff + i * spitch), span * kMx4Tile, 0);
+      }
+    }
+  };
+  f32x4 acc[RB][CB] = {};
+  auto multiply = [&](auto sl) {
+    constexpr int J = decltype(sl)::value;
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        acc[i][c] = mfma_mx4<J>(w[J][c], x[J][i], acc[i][c], ws[c], xs[i]);
+      }
+    }
+  };
+  // the wave's rows of x coded, from raw to x and xs
+  uint8_t* const own = lds + wave * kBuf;
+  auto code = [&](int span) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = (4 * span + j) * 128 + row * 8 < p.K;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (4 * i >= p.M) { break; }
+        uint32_t scale;
+        const uint32_t codes = mx4_code_bf16_quad(raw[j][i], scale);
+        // row / 4 is the block of the slice, row % 4 the lane's place in it
+        const int at = (row >> 2) * 16 + 4 * i + g;
+        *(uint32_t*)(own + j * kMx4CodeTile + at * 16 + (row & 3) * 4) = in ? codes : 0u;
+        if ((row & 3) == 0) { own[4 * kMx4CodeTile + at * 4 + j] = in ? (uint8_t)scale : 0; }
+      }
+    }
+    xs[0] = *(const int*)(own + 4 * kMx4CodeTile + lane * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[j][0] = *(const i32x4*)(own + j * kMx4CodeTile + lane * 16); }
+  };
+
+  if (wave < spans) {
+    load_scales(wave);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { load(4 * wave + j, j); }
+  }
+  for (int span = wave; span < spans; span += WAVES) {
+    __builtin_amdgcn_sched_barrier(0);   // every load is asked for before the first is used
+#pragma unroll
+    for (int c = 0; c < CB; ++c) { ws[c] = nws[c]; }
+    if constexpr (CODED) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i) { xs[i] = nxs[i]; }
+    } else {
+      code(span);
+    }
+    const bool more = span + WAVES < spans;
+    if (more) { load_scales(span + WAVES); }
+    auto slice = [&](auto sl) {
+      multiply(sl);
+      if (more) {
+        __builtin_amdgcn_sched_barrier(0);
+        load(4 * (span + WAVES) + decltype(sl)::value, decltype(sl)::value);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    slice(std::integral_constant<int, 0>{});
+    slice(std::integral_constant<int, 1>{});
+    slice(std::integral_constant<int, 2>{});
+    slice(std::integral_constant<int, 3>{});
+  }
+
+  // the waves' sums, in one order; block (i, c), lane l: row 16 i + l % 16, columns 16 c +
+  // 4 (l / 16) .. of it
+  float* const red = (float*)lds;
+  if constexpr (!CODED) { __syncthreads(); }   // the codes' LDS is free
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      *(f32x4*)(red + wave * kOut + (i * 16 + row) * 16 * CB + c * 16 + g * 4) = acc[i][c];
+    }
+  }
+  __syncthreads();
+  const int used = min(WAVES, spans);
+  for (int t = threadIdx.x * 4; t < kOut; t += 256 * WAVES) {
+    const int m = tm * 16 * RB + t / (16 * CB), n = (tn * 16 * CB) + t % (16 * CB);
+    if (m >= p.M || n >= p.N) { continue; }
+    f32x4 v = *(const f32x4*)(red + t);
+    for (int k = 1; k < used; ++k) { v += *(const f32x4*)(red + k * kOut + t); }
+    uint16_t* const y = p.y + (size_t)m * p.N + n;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v[r] += load_bias(p.bias, p.bias_type, min(n + r, p.N - 1));
+      if (p.epilogue == kEpiGelu) { v[r] = gelu_tanh(v[r]); }
+    }
+    if (p.N % 4 == 0) {
+      *(uint2*)y = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (n + r < p.N) { y[r] = f32_to_bf16(v[r]); }
+      }
+    }
+  }
+}
+
+template <int RB, int CB, int WAVES, bool CODED = true>
+hipError_t run_panel(GemmParams& p, hipStream_t stream, const uint16_t* xb = nullptr,
+                     int64_t stride = 0)
+{
+  p.tiles_m = (p.M + 16 * RB - 1) / (16 * RB);
+  p.tiles_n = (p.N + 16 * CB - 1) / (16 * CB);
+  const long tiles = (long)p.tiles_m * p.tiles_n;
+  if (tiles * 64 * WAVES >= 1L << 32) { return hipErrorInvalidConfiguration; }
+  mx4_panel_kernel<RB, CB, WAVES, CODED>
+      <<<(unsigned)tiles, 64 * WAVES, 0, stream>>>(p, xb, (long)stride);
   return hipGetLastError();
 }
 
@@ -252,15 +470,15 @@ Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
 {
   Mx4Plan r;
   r.codes_ahead = bf16;
-  const int spans = mx4_spans(K);
-  const long big = (long)((M + 127) / 128) * ((N + 127) / 128);
-  const long small = (long)((M + 63) / 64) * ((N + 63) / 64);
-  r.tile = big >= 256 ? 0 : 1;
-  const long tiles = r.tile == 0 ? big : small;
-  r.splits = (int)std::max(1L, std::min((long)spans, 512 / std::max(1L, tiles)));
-  r.span_chunk = (spans + r.splits - 1) / r.splits;
-  r.splits = (spans + r.span_chunk - 1) / r.span_chunk;
-  r.partial_bytes = r.splits > 1 ? (size_t)r.splits * M * N * sizeof(float) : 0;
+  if (const char* force = getenv("MX4_TILE")) {
+    int a = 0, b = 0;
+    sscanf(force, "%d,%d", &a, &b);
+    r.tile = a >= 100 ? a : a * 16 + b;
+    r.codes_ahead = bf16 && !(a == 118 && M <= 16);
+    return r;
+  }
+  r.tile = M <= 16 ? 118 : M <= 32 ? 218 : 4 * 16 + 8;
+  r.codes_ahead = bf16 && M > 16;
   return r;
 }
 
@@ -281,17 +499,33 @@ hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t st
     p.ws = g.w.scales;
     p.bias = g.bias;
     p.y = g.y + (size_t)m * N;
-    p.partial = plan.splits > 1 ? g.partial : nullptr;
     p.M = (int)std::min(most, M - m);
     p.N = N;
     p.K = K;
     p.bias_type = g.bias_type;
     p.epilogue = g.epilogue;
-    p.span_chunk = plan.span_chunk;
-    hipError_t e = plan.tile == 0 ? run_wide<4, 8>(p, plan, stream) : run_wide<1, 4>(p, plan, stream);
-    if (e == hipSuccess && p.partial != nullptr) {
-      e = launch_splitk_reduce(p.partial, plan.splits, g.bias, g.bias_type, g.epilogue, nullptr,
-                               p.y, p.M, N, stream);
+    hipError_t e = hipSuccess;
+    switch (plan.tile) {
+      case 16:
+      case 118:
+        e = g.xb != nullptr ? run_panel<1, 1, 8, false>(p, stream, g.xb, g.xb_stride)
+                            : run_panel<1, 1, 8>(p, stream);
+        break;
+      case 32:
+      case 218: e = run_panel<2, 1, 8>(p, stream); break;
+      case 64:
+      case 418: e = run_panel<4, 1, 8>(p, stream); break;
+      case 228: e = run_panel<2, 2, 8>(p, stream); break;
+      case 224: e = run_panel<2, 2, 4>(p, stream); break;
+      case 428: e = run_panel<4, 2, 8>(p, stream); break;
+      case 424: e = run_panel<4, 2, 4>(p, stream); break;
+      case 248: e = run_panel<2, 4, 8>(p, stream); break;
+      case 448: e = run_panel<4, 4, 8>(p, stream); break;
+      case 444: e = run_panel<4, 4, 4>(p, stream); break;
+      case 1 * 16 + 4: e = run_wide<1, 4, 4, 8>(p, stream); break;
+      case 2 * 16 + 4: e = run_wide<2, 4, 4, 8>(p, stream); break;
+      case 4 * 16 + 4: e = run_wide<4, 4, 3, 4>(p, stream); break;
+      default: e = run_wide<4, 8, 2, 4>(p, stream); break;
     }
     if (e != hipSuccess) { return e; }
   }

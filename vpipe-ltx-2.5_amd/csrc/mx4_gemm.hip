@@ -66,21 +66,17 @@ __device__ __forceinline__ f32x4 mfma_mx4(i32x4 w, i32x4 x, f32x4 acc, int ws, i
 // take turns, filled STAGES - 1 spans ahead by loads that go straight into LDS, one barrier a
 // span. Tiles lie in LDS as in memory, and a fragment's read is the tile's 1 KB in the order of
 // the lanes.
-template <int RB, int CB, int STAGES, int DEPTH>
+template <int RB, int CB, int STAGES>
 __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 {
-  static_assert(DEPTH == 4 || DEPTH == 8, "slices in flight, a span's or two");
   constexpr int kCodes = 4 * CB * kMx4CodeTile;
   constexpr int kScaleTiles = 4 * RB + CB, kScaleLoads = (kScaleTiles + 15) / 16;
   constexpr int kStage = kCodes + 16 * kScaleLoads * kMx4Tile;
   static_assert(STAGES * kStage <= 80 * 1024, "two workgroups a CU");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int tm, tn;
-  map_tile(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
-  const int n0 = tn * 16 * CB, row0 = (tm * 4 + wave) * 16 * RB;   // the wave's rows
-
+  const int tiles = p.tiles_m * p.tiles_n;
   const int slices = mx4_slices(p.K), spans = mx4_spans(p.K);
   const uint32_t pitch = (uint32_t)slices * kMx4CodeTile;   // of 16 rows
   const uint32_t spitch = (uint32_t)spans * kMx4Tile;
@@ -89,39 +85,57 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   const __amdgpu_buffer_rsrc_t xsr = make_rsrc(p.xs, mx4_scale_bytes(p.M, p.K));
   const __amdgpu_buffer_rsrc_t wsr = make_rsrc(p.ws, mx4_scale_bytes(p.N, p.K));
 
-  // Codes of a stage: [tile row][slice], wave w loads slice w of every tile row. Slices past the
-  // rows' end would be the next rows': an offset past the operand gives zeros. Scales: tiles of
+  // The loads run ahead of the products, those into LDS STAGES - 1 spans, those of x one; with
+  // two stages over the end of a tile to the workgroup's next. Past the last tile, and in slices
+  // past the rows' end (which would be the next rows'), offsets lie past the operands and give
+  // zeros.
+  //
+  // Codes of a stage: [tile row][slice], wave w loads slice w of every tile row. Scales: tiles of
   // x, then of w, four a load; wave w has loads w, w + 4 (those past the last tile zeros).
-  const uint32_t woff = (uint32_t)(n0 / 16) * pitch + lane * 16;
-  uint32_t soff[kScaleLoads];
+  struct Place {
+    uint32_t w, x, s[kScaleLoads];
+  };
+  auto place_of = [&](int tile) {
+    int tm, tn;
+    map_tile(tile, p.tiles_m, p.tiles_n, tm, tn);
+    const bool in = tile < tiles;
+    Place at;
+    at.w = in ? (uint32_t)(tn * CB) * pitch + lane * 16 : kPast;
+    at.x = in ? (uint32_t)((tm * 4 + wave) * RB) * pitch + lane * 16 : kPast;
 #pragma unroll
-  for (int i = 0; i < kScaleLoads; ++i) {
-    const int q = wave + 4 * i, tile = 4 * q + (lane >> 4);
-    const uint32_t at = q < RB ? (uint32_t)(tm * 4 * RB + tile) : (uint32_t)(tn * CB + tile - 4 * RB);
-    soff[i] = tile < kScaleTiles ? at * spitch + (lane & 15) * 16 : kPast;
-  }
+    for (int i = 0; i < kScaleLoads; ++i) {
+      const int q = wave + 4 * i, t = 4 * q + g;
+      const uint32_t r = q < RB ? (uint32_t)(tm * 4 * RB + t) : (uint32_t)(tn * CB + t - 4 * RB);
+      at.s[i] = in && t < kScaleTiles ? r * spitch + (lane & 15) * 16 : kPast;
+    }
+    return at;
+  };
+  Place here = place_of(blockIdx.x), then = place_of(STAGES == 2 ? blockIdx.x + gridDim.x : tiles);
   constexpr int kW = CB + kScaleLoads;   // loads of a wave into a stage
   auto load_w = [&](int span, int stage, int k) {   // the k-th of them
+    const bool on = span >= spans;
+    const int from = on ? span - spans : span;
     uint8_t* const at = lds + stage * kStage;
     if (k < CB) {
-      const int t = 4 * span + wave;
+      const int t = 4 * from + wave;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           wr, (lds_u32*)(at + (4 * k + wave) * kMx4CodeTile), 16,
-          (int)(t < slices ? woff + k * pitch : kPast), t * kMx4CodeTile, 0, 0);
+          (int)(t < slices ? (on ? then.w : here.w) + k * pitch : kPast), t * kMx4CodeTile, 0, 0);
     } else {
       const int q = wave + 4 * (k - CB);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(q < RB ? xsr : wsr,
-                                               (lds_u32*)(at + kCodes + q * 4 * kMx4Tile), 16,
-                                               (int)(span < spans ? soff[k - CB] : kPast),
-                                               span * kMx4Tile, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          q < RB ? xsr : wsr, (lds_u32*)(at + kCodes + q * 4 * kMx4Tile), 16,
+          (int)(on ? then.s[k - CB] : here.s[k - CB]), from * kMx4Tile, 0, 0);
     }
   };
-  const uint32_t xoff = (uint32_t)(row0 / 16) * pitch + lane * 16;
-  i32x4 x[DEPTH][RB];
-  auto load_x = [&](int t, int buf, int i) {
-    x[buf][i] = __builtin_bit_cast(
+  i32x4 x[4][RB];
+  auto load_x = [&](int span, int slice, int i) {
+    const bool on = span >= spans;
+    const int t = 4 * (on ? span - spans : span) + slice;
+    x[slice][i] = __builtin_bit_cast(
         i32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                   xr, (int)(t < slices ? xoff + i * pitch : kPast), t * kMx4CodeTile, 0));
+                   xr, (int)(t < slices ? (on ? then.x : here.x) + i * pitch : kPast),
+                   t * kMx4CodeTile, 0));
   };
   // A span is 4 CB fragments of w, RB matrix instructions each. Its loads go out one by one among
   // them, since a wave waits until the address unit has taken its load (all of a span's loads to
@@ -132,12 +146,12 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   constexpr int kXEvery = CB / RB;
   // loads of x behind the last one to LDS
   constexpr int kXBehind = (4 * CB - 1 - 2 * (kW - 1)) / kXEvery;
-  f32x4 acc[RB][CB] = {};
+  f32x4 acc[RB][CB];
   int stage = 0;   // of the span
-  auto step = [&](int span, auto parity) {
-    constexpr int B = DEPTH == 8 ? 4 * decltype(parity)::value : 0;
+  auto step = [&](int span) {
     // The span's loads into LDS have landed: behind them came those of x of the span that issued
-    // them, and STAGES - 2 spans' since. Then the stage that the last span used is free.
+    // them, and STAGES - 2 spans' since (an epilogue's accesses only add to the count). Then the
+    // stage that the last span used is free.
     constexpr int kBehind = kXBehind + (STAGES - 2) * (kW + 4 * RB);
     constexpr int kWait = kBehind < 63 ? kBehind : 63;
     __builtin_amdgcn_s_waitcnt(0x0f70 | (kWait & 15) | ((kWait >> 4) << 14));
@@ -162,14 +176,12 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
       if constexpr (f + 3 < 4 * CB) { w[(f + 3) % 4] = fragment(f + 3); }
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
-        acc[i][j] = mfma_mx4<J>(w[f % 4], x[B + J][i], acc[i][j], ws[j], xs[i]);
+        acc[i][j] = mfma_mx4<J>(w[f % 4], x[J][i], acc[i][j], ws[j], xs[i]);
       }
-      // Unconditionally, so that the number of loads behind others is known; past the end they
-      // give zeros.
+      // Unconditionally, so that the number of loads behind others is known.
       if constexpr (f % 2 == 0 && f / 2 < kW) { load_w(span + STAGES - 1, next, f / 2); }
       if constexpr (j % kXEvery == kXEvery - 1) {
-        constexpr int kBuf = J > 0 ? B + J - 1 : DEPTH == 8 ? 7 - B : 3;
-        load_x(4 * span + J - 1 + DEPTH, kBuf, j / kXEvery);
+        load_x(J == 0 ? span : span + 1, (J + 3) % 4, j / kXEvery);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -182,95 +194,112 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
     for (int k = 0; k < kW; ++k) { load_w(i, i, k); }
   }
 #pragma unroll
-  for (int t = 0; t < DEPTH - 1; ++t) {
+  for (int t = 0; t < 3; ++t) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i) { load_x(t, t, i); }
+    for (int i = 0; i < RB; ++i) { load_x(0, t, i); }
   }
   // the first stages have landed, for what the count above does not see
-  constexpr int kFirst = (DEPTH - 1) * RB;
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (kFirst < 15 ? kFirst : 15));
-  int span = 0;
-  for (; span + 1 < spans; span += 2) {
-    step(span, std::integral_constant<int, 0>{});
-    step(span + 1, std::integral_constant<int, 1>{});
-  }
-  if (span < spans) { step(span, std::integral_constant<int, 0>{}); }
-  __builtin_amdgcn_s_waitcnt(0x0f70);   // no load into LDS outlives the wave
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (3 * RB));
 
-  // block (i, j), lane l, register r: row 16 i + l % 16, column 16 j + 4 (l / 16) + r
-  const int g = lane >> 4;
-  if (p.N % 8 != 0) {
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
+    for (int i = 0; i < RB; ++i) {
+#pragma unroll
+      for (int j = 0; j < CB; ++j) { acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+    }
+    for (int span = 0; span < spans; ++span) { step(span); }
+    here = then;
+    then = place_of(tile + 2 * (int)gridDim.x);
+
+    // Block (i, j), lane l, register r: row 16 i + l % 16, column 16 j + 4 (l / 16) + r. The
+    // loads of x that are in flight, the next tile's, have landed before anything is stored.
+    int tm, tn;
+    map_tile(tile, p.tiles_m, p.tiles_n, tm, tn);
+    const int n0 = tn * 16 * CB, row0 = (tm * 4 + wave) * 16 * RB;   // the wave's rows
+    auto bias_of = [&](int j, float (&bias)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int n = n0 + 16 * j + 4 * g + r;
-        const float bias = load_bias(p.bias, p.bias_type, min(n, p.N - 1));
-#pragma unroll
-        for (int i = 0; i < RB; ++i) {
-          const int m = row0 + 16 * i + (lane & 15);
-          if (m >= p.M || n >= p.N) { continue; }
-          const float v = acc[i][j][r] + bias;
-          p.y[(size_t)m * p.N + n] = f32_to_bf16(p.epilogue == kEpiGelu ? gelu_tanh(v) : v);
-        }
+        bias[r] = load_bias(p.bias, p.bias_type, min(n0 + 16 * j + 4 * g + r, p.N - 1));
       }
-    }
-    return;
-  }
-  // Two blocks side by side: the lanes' rows of 16 are exchanged so that each lane has eight
-  // columns of one of them, 16 bytes.
-  auto store = [&](auto gelu) {
+    };
+    if (p.N % 8 != 0) {
 #pragma unroll
-    for (int j = 0; j < CB; j += 2) {
-      float bias[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int j = 0; j < CB; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        float bias[4];
+        bias_of(j, bias);
+        __builtin_amdgcn_s_waitcnt(0x0f70);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          bias[h][r] =
-              load_bias(p.bias, p.bias_type, min(n0 + 16 * (j + h) + 4 * g + r, p.N - 1));
-        }
-      }
-      const int n = n0 + 16 * (j + (g & 1)) + 8 * (g >> 1);
+          const int n = n0 + 16 * j + 4 * g + r;
 #pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        uint32_t w[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            v[r] = acc[i][j + h][r] + bias[h][r];
-            if constexpr (decltype(gelu)::value) { v[r] = gelu_tanh(v[r]); }
+          for (int i = 0; i < RB; ++i) {
+            const int m = row0 + 16 * i + (lane & 15);
+            if (m >= p.M || n >= p.N) { continue; }
+            const float v = acc[i][j][r] + bias[r];
+            p.y[(size_t)m * p.N + n] = f32_to_bf16(p.epilogue == kEpiGelu ? gelu_tanh(v) : v);
           }
-          w[h][0] = pack_bf16x2(v[0], v[1]);
-          w[h][1] = pack_bf16x2(v[2], v[3]);
-        }
-        const auto a = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
-        const auto b = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
-        const int m = row0 + 16 * i + (lane & 15);
-        if (m < p.M && n < p.N) {
-          const i32x4 v = {(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
-          __builtin_nontemporal_store(v, (i32x4*)(p.y + (size_t)m * p.N + n));
         }
       }
+      continue;
     }
-  };
-  if (p.epilogue == kEpiGelu) {
-    store(std::true_type{});
-  } else {
-    store(std::false_type{});
+    // Two blocks side by side: the lanes' rows of 16 are exchanged so that each lane has eight
+    // columns of one of them, 16 bytes.
+    auto store = [&](auto gelu) {
+      unroll<CB / 2>([&](auto jj) {
+        constexpr int j = 2 * decltype(jj)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        float bias[2][4];
+        bias_of(j, bias[0]);
+        bias_of(j + 1, bias[1]);
+        const int n = n0 + 16 * (j + (g & 1)) + 8 * (g >> 1);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          uint32_t w[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              v[r] = acc[i][j + h][r] + bias[h][r];
+              if constexpr (decltype(gelu)::value) { v[r] = gelu_tanh(v[r]); }
+            }
+            w[h][0] = pack_bf16x2(v[0], v[1]);
+            w[h][1] = pack_bf16x2(v[2], v[3]);
+          }
+          const auto a = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+          const auto b = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+          if constexpr (j == 0) {
+            if (i == 0) { __builtin_amdgcn_s_waitcnt(0x0f70); }
+          }
+          const int m = row0 + 16 * i + (lane & 15);
+          if (m < p.M && n < p.N) {
+            const i32x4 v = {(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
+            __builtin_nontemporal_store(v, (i32x4*)(p.y + (size_t)m * p.N + n));
+          }
+        }
+      });
+    };
+    if (p.epilogue == kEpiGelu) {
+      store(std::true_type{});
+    } else {
+      store(std::false_type{});
+    }
   }
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // no load into LDS outlives the wave
 }
 
-template <int RB, int CB, int STAGES, int DEPTH>
+template <int RB, int CB, int STAGES>
 hipError_t run_wide(GemmParams& p, hipStream_t stream)
 {
   p.tiles_m = (p.M + 64 * RB - 1) / (64 * RB);
   p.tiles_n = (p.N + 16 * CB - 1) / (16 * CB);
   const long tiles = (long)p.tiles_m * p.tiles_n;
   if (tiles * 256 >= 1L << 32) { return hipErrorInvalidConfiguration; }
-  mx4_wide_kernel<RB, CB, STAGES, DEPTH><<<(unsigned)tiles, 256, 0, stream>>>(p);
+  // two workgroups on each of the 256 CUs; a multiple of the XCDs, so that a workgroup's tiles
+  // are its XCD's (map_tile)
+  const long grid = STAGES == 2 ? std::min(tiles, 512L) : tiles;
+  mx4_wide_kernel<RB, CB, STAGES><<<(unsigned)grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
 
@@ -522,10 +551,10 @@ hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t st
       case 248: e = run_panel<2, 4, 8>(p, stream); break;
       case 448: e = run_panel<4, 4, 8>(p, stream); break;
       case 444: e = run_panel<4, 4, 4>(p, stream); break;
-      case 1 * 16 + 4: e = run_wide<1, 4, 4, 8>(p, stream); break;
-      case 2 * 16 + 4: e = run_wide<2, 4, 4, 8>(p, stream); break;
-      case 4 * 16 + 4: e = run_wide<4, 4, 3, 4>(p, stream); break;
-      default: e = run_wide<4, 8, 2, 4>(p, stream); break;
+      case 1 * 16 + 4: e = run_wide<1, 4, 4>(p, stream); break;
+      case 2 * 16 + 4: e = run_wide<2, 4, 4>(p, stream); break;
+      case 4 * 16 + 4: e = run_wide<4, 4, 3>(p, stream); break;
+      default: e = run_wide<4, 8, 2>(p, stream); break;
     }
     if (e != hipSuccess) { return e; }
   }

@@ -33,6 +33,33 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, size_
                                            0x00020000);
 }
 
+// 2 W bf16 to columns n .. of a row of N, of which those past N are left alone. Rows of an
+// odd N begin anywhere: the store is one all the same.
+template <int W>
+struct Words {
+  uint32_t w[W];
+};
+template <int W>
+__device__ __forceinline__ void store_bf16(uint16_t* row, int n, int N, const Words<W>& v)
+{
+  typedef uint32_t words __attribute__((ext_vector_type(W), aligned(2)));
+  if (n + 2 * W <= N) {
+    words x;
+#pragma unroll
+    for (int i = 0; i < W; ++i) { x[i] = v.w[i]; }
+    if (N % 8 == 0) {
+      __builtin_nontemporal_store(x, (words*)(row + n));
+    } else {
+      *(words*)(row + n) = x;   // lines that the cache puts together
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) {
+      if (n + i < N) { row[n + i] = (uint16_t)(v.w[i >> 1] >> (16 * (i & 1))); }
+    }
+  }
+}
+
 // f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>)
 template <typename F, int... I>
 __device__ __forceinline__ void unroll_seq(F&& f, std::integer_sequence<int, I...>)
@@ -66,9 +93,10 @@ __device__ __forceinline__ f32x4 mfma_mx4(i32x4 w, i32x4 x, f32x4 acc, int ws, i
 // take turns, filled STAGES - 1 spans ahead by loads that go straight into LDS, one barrier a
 // span. Tiles lie in LDS as in memory, and a fragment's read is the tile's 1 KB in the order of
 // the lanes.
-template <int RB, int CB, int STAGES>
+template <int RB, int CB, int STAGES, int DEPTH>
 __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 {
+  static_assert(DEPTH == 4 || (DEPTH == 8 && STAGES > 2), "slices of x in flight: a span's or two");
   constexpr int kCodes = 4 * CB * kMx4CodeTile;
   constexpr int kScaleTiles = 4 * RB + CB, kScaleLoads = (kScaleTiles + 15) / 16;
   constexpr int kStage = kCodes + 16 * kScaleLoads * kMx4Tile;
@@ -128,11 +156,11 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
           (int)(on ? then.s[k - CB] : here.s[k - CB]), from * kMx4Tile, 0, 0);
     }
   };
-  i32x4 x[4][RB];
-  auto load_x = [&](int span, int slice, int i) {
+  i32x4 x[DEPTH][RB];
+  auto load_x = [&](int span, int slice, int buf, int i) {
     const bool on = span >= spans;
     const int t = 4 * (on ? span - spans : span) + slice;
-    x[slice][i] = __builtin_bit_cast(
+    x[buf][i] = __builtin_bit_cast(
         i32x4, __builtin_amdgcn_raw_buffer_load_b128(
                    xr, (int)(t < slices ? (on ? then.x : here.x) + i * pitch : kPast),
                    t * kMx4CodeTile, 0));
@@ -148,7 +176,8 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   constexpr int kXBehind = (4 * CB - 1 - 2 * (kW - 1)) / kXEvery;
   f32x4 acc[RB][CB];
   int stage = 0;   // of the span
-  auto step = [&](int span) {
+  auto step = [&](int span, auto parity) {
+    constexpr int B = DEPTH == 8 ? 4 * decltype(parity)::value : 0;
     // The span's loads into LDS have landed: behind them came those of x of the span that issued
     // them, and STAGES - 2 spans' since (an epilogue's accesses only add to the count). Then the
     // stage that the last span used is free.
@@ -176,12 +205,13 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
       if constexpr (f + 3 < 4 * CB) { w[(f + 3) % 4] = fragment(f + 3); }
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
-        acc[i][j] = mfma_mx4<J>(w[f % 4], x[J][i], acc[i][j], ws[j], xs[i]);
+        acc[i][j] = mfma_mx4<J>(w[f % 4], x[B + J][i], acc[i][j], ws[j], xs[i]);
       }
       // Unconditionally, so that the number of loads behind others is known.
       if constexpr (f % 2 == 0 && f / 2 < kW) { load_w(span + STAGES - 1, next, f / 2); }
       if constexpr (j % kXEvery == kXEvery - 1) {
-        load_x(J == 0 ? span : span + 1, (J + 3) % 4, j / kXEvery);
+        constexpr int kBuf = J > 0 ? B + J - 1 : DEPTH == 8 ? 7 - B : 3;
+        load_x(span + DEPTH / 4 - (J == 0 ? 1 : 0), (J + 3) % 4, kBuf, j / kXEvery);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -194,12 +224,13 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
     for (int k = 0; k < kW; ++k) { load_w(i, i, k); }
   }
 #pragma unroll
-  for (int t = 0; t < 3; ++t) {
+  for (int t = 0; t < DEPTH - 1; ++t) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i) { load_x(0, t, i); }
+    for (int i = 0; i < RB; ++i) { load_x(t / 4, t % 4, t, i); }
   }
   // the first stages have landed, for what the count above does not see
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (3 * RB));
+  constexpr int kFirst = (DEPTH - 1) * RB;
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (kFirst < 15 ? kFirst : 15));
 
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
 #pragma unroll
@@ -207,7 +238,16 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 #pragma unroll
       for (int j = 0; j < CB; ++j) { acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
     }
-    for (int span = 0; span < spans; ++span) { step(span); }
+    if constexpr (DEPTH == 8) {
+      int span = 0;
+      for (; span + 1 < spans; span += 2) {
+        step(span, std::integral_constant<int, 0>{});
+        step(span + 1, std::integral_constant<int, 1>{});
+      }
+      if (span < spans) { step(span, std::integral_constant<int, 0>{}); }
+    } else {
+      for (int span = 0; span < spans; ++span) { step(span, std::integral_constant<int, 0>{}); }
+    }
     here = then;
     then = place_of(tile + 2 * (int)gridDim.x);
 
@@ -222,27 +262,6 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
         bias[r] = load_bias(p.bias, p.bias_type, min(n0 + 16 * j + 4 * g + r, p.N - 1));
       }
     };
-    if (p.N % 8 != 0) {
-#pragma unroll
-      for (int j = 0; j < CB; ++j) {
-        __builtin_amdgcn_sched_barrier(0);
-        float bias[4];
-        bias_of(j, bias);
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int n = n0 + 16 * j + 4 * g + r;
-#pragma unroll
-          for (int i = 0; i < RB; ++i) {
-            const int m = row0 + 16 * i + (lane & 15);
-            if (m >= p.M || n >= p.N) { continue; }
-            const float v = acc[i][j][r] + bias[r];
-            p.y[(size_t)m * p.N + n] = f32_to_bf16(p.epilogue == kEpiGelu ? gelu_tanh(v) : v);
-          }
-        }
-      }
-      continue;
-    }
     // Two blocks side by side: the lanes' rows of 16 are exchanged so that each lane has eight
     // columns of one of them, 16 bytes.
     auto store = [&](auto gelu) {
@@ -273,10 +292,7 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
             if (i == 0) { __builtin_amdgcn_s_waitcnt(0x0f70); }
           }
           const int m = row0 + 16 * i + (lane & 15);
-          if (m < p.M && n < p.N) {
-            const i32x4 v = {(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
-            __builtin_nontemporal_store(v, (i32x4*)(p.y + (size_t)m * p.N + n));
-          }
+          if (m < p.M) { store_bf16<4>(p.y + (size_t)m * p.N, n, p.N, {a[0], b[0], a[1], b[1]}); }
         }
       });
     };
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   __builtin_amdgcn_s_waitcnt(0x0f70);   // no load into LDS outlives the wave
 }
 
-template <int RB, int CB, int STAGES>
+template <int RB, int CB, int STAGES, int DEPTH>
 hipError_t run_wide(GemmParams& p, hipStream_t stream)
 {
   p.tiles_m = (p.M + 64 * RB - 1) / (64 * RB);
@@ -299,7 +315,7 @@ hipError_t run_wide(GemmParams& p, hipStream_t stream)
   // two workgroups on each of the 256 CUs; a multiple of the XCDs, so that a workgroup's tiles
   // are its XCD's (map_tile)
   const long grid = STAGES == 2 ? std::min(tiles, 512L) : tiles;
-  mx4_wide_kernel<RB, CB, STAGES><<<(unsigned)grid, 256, 0, stream>>>(p);
+  mx4_wide_kernel<RB, CB, STAGES, DEPTH><<<(unsigned)grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
 
@@ -460,20 +476,12 @@ mx4_panel_kernel(GemmParams p, const uint16_t* xb, long stride)
     if (m >= p.M || n >= p.N) { continue; }
     f32x4 v = *(const f32x4*)(red + t);
     for (int k = 1; k < used; ++k) { v += *(const f32x4*)(red + k * kOut + t); }
-    uint16_t* const y = p.y + (size_t)m * p.N + n;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       v[r] += load_bias(p.bias, p.bias_type, min(n + r, p.N - 1));
       if (p.epilogue == kEpiGelu) { v[r] = gelu_tanh(v[r]); }
     }
-    if (p.N % 4 == 0) {
-      *(uint2*)y = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (n + r < p.N) { y[r] = f32_to_bf16(v[r]); }
-      }
-    }
+    store_bf16<2>(p.y + (size_t)m * p.N, n, p.N, {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
   }
 }
 
@@ -495,19 +503,41 @@ constexpr size_t kSlabBytes = (size_t)1 << 30;
 
 }  // namespace
 
+// Tiles of a wide workgroup, 64 RB x 16 CB, and of a panel, 16 RB x 16 CB
+enum Tile : int { kWide48, kWide44, kWide24, kWide14, kPanel22, kPanel22x8, kPanel21, kPanel11 };
+
 Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
 {
+  auto groups = [&](int rows, int columns) {
+    return (long)((M + rows - 1) / rows) * ((N + columns - 1) / columns);
+  };
   Mx4Plan r;
-  r.codes_ahead = bf16;
-  if (const char* force = getenv("MX4_TILE")) {
-    int a = 0, b = 0;
-    sscanf(force, "%d,%d", &a, &b);
-    r.tile = a >= 100 ? a : a * 16 + b;
-    r.codes_ahead = bf16 && !(a == 118 && M <= 16);
-    return r;
-  }
-  r.tile = M <= 16 ? 118 : M <= 32 ? 218 : 4 * 16 + 8;
   r.codes_ahead = bf16 && M > 16;
+  // The largest tile that is half full and still gives three CUs of four a workgroup, wide ones
+  // first (us; M x K
+  // -> N, replayed in a graph):
+  //                         256 x 128  256 x 64  128 x 64  64 x 64  32 x 32  32 x 16 (8 waves)
+  //   8160 x 4096 -> 4096        64        81        92      128      173
+  //   1024 x 4096 -> 4096        17.4      12.8      13.7     18.9     26.3
+  //    512 x 4096 -> 4096        17.2      12.0       9.8     11.4     16.0
+  //    256 x 4096 -> 4096        16.8      11.0       8.1      6.2      9.7
+  //    333 x 2080 -> 1001        21.0      12.7       8.5      6.7      4.7      5.7
+  //     64 x 4096 -> 4096                                      7.1      4.5      4.9
+  //     32 x 4096 -> 4096                                      7.0      4.0      3.8
+  //    128 x 16384 -> 64                                      19.1      6.7      5.6
+  // A panel of one block has the most workgroups (128 x 16384 -> 64: 4.6), and codes bf16
+  // activations itself.
+  constexpr long kEnough = 192;
+  r.tile = M <= 16                                    ? kPanel11
+           : M > 128 && groups(256, 128) >= kEnough ? kWide48
+           : M > 128 && groups(256, 64) >= kEnough  ? kWide44
+           : M > 64 && groups(128, 64) >= kEnough   ? kWide24
+           : groups(64, 64) >= kEnough              ? kWide14
+           : groups(32, 32) > 256                   ? kPanel22
+           : groups(32, 32) >= kEnough              ? kPanel22x8
+           : groups(32, 16) >= kEnough              ? kPanel21
+                                                    : kPanel11;
+  if (const char* force = getenv("MX4_TILE")) { r.tile = atoi(force); }
   return r;
 }
 
@@ -535,26 +565,18 @@ hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t st
     p.epilogue = g.epilogue;
     hipError_t e = hipSuccess;
     switch (plan.tile) {
-      case 16:
-      case 118:
-        e = g.xb != nullptr ? run_panel<1, 1, 8, false>(p, stream, g.xb, g.xb_stride)
-                            : run_panel<1, 1, 8>(p, stream);
+      case kWide48: e = run_wide<4, 8, 2, 4>(p, stream); break;
+      case kWide44: e = run_wide<4, 4, 3, 4>(p, stream); break;
+      case kWide24: e = run_wide<2, 4, 4, 8>(p, stream); break;
+      case kWide14: e = run_wide<1, 4, 4, 8>(p, stream); break;
+      case kPanel22: e = run_panel<2, 2, 4>(p, stream); break;
+      case kPanel22x8: e = run_panel<2, 2, 8>(p, stream); break;
+      case kPanel21: e = run_panel<2, 1, 8>(p, stream); break;
+      default:
+        e = g.xb != nullptr && !plan.codes_ahead
+                ? run_panel<1, 1, 8, false>(p, stream, g.xb, g.xb_stride)
+                : run_panel<1, 1, 8>(p, stream);
         break;
-      case 32:
-      case 218: e = run_panel<2, 1, 8>(p, stream); break;
-      case 64:
-      case 418: e = run_panel<4, 1, 8>(p, stream); break;
-      case 228: e = run_panel<2, 2, 8>(p, stream); break;
-      case 224: e = run_panel<2, 2, 4>(p, stream); break;
-      case 428: e = run_panel<4, 2, 8>(p, stream); break;
-      case 424: e = run_panel<4, 2, 4>(p, stream); break;
-      case 248: e = run_panel<2, 4, 8>(p, stream); break;
-      case 448: e = run_panel<4, 4, 8>(p, stream); break;
-      case 444: e = run_panel<4, 4, 4>(p, stream); break;
-      case 1 * 16 + 4: e = run_wide<1, 4, 4>(p, stream); break;
-      case 2 * 16 + 4: e = run_wide<2, 4, 4>(p, stream); break;
-      case 4 * 16 + 4: e = run_wide<4, 4, 3>(p, stream); break;
-      default: e = run_wide<4, 8, 2>(p, stream); break;
     }
     if (e != hipSuccess) { return e; }
   }

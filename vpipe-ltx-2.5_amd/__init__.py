@@ -638,16 +638,33 @@ def attention_cached(cache: KVCache, table, lens, q, out, q_len: int, max_len: i
 # ---- microscaled 4 bits (include/ltx25_mx4.h) ------------------------------------------
 
 
-def _on_device(stream, *tensors) -> int:
-    """The stream to launch on. Without one given it is the current device's, where the tensors
-    must lie (pinned host memory is reached from any)."""
+def _on_device(stream, names: str, tensors) -> int:
+    """The stream to launch on: the caller's, or the current one of the current device, where the
+    tensors must lie (pinned host memory is reached from any). One look at each tensor; what it
+    finds is named afterwards."""
     if stream is not None:
+        for t in tensors:
+            if t is not None and not t.is_cuda:
+                _reachable(names, *tensors)
         return stream
-    device = (_torch or _import_torch()).cuda.current_device()
+    device = _device_of(names, tensors)
     for t in tensors:
-        if t is not None and t.is_cuda and t.get_device() != device:
-            raise ValueError(f"a tensor lies on {t.device}, the current device is cuda:{device}")
+        if t is not None and t.get_device() != device:
+            _reachable(names, *tensors)
+            for name, u in zip(names.split(), tensors):
+                if u is not None and u.is_cuda and u.get_device() != device:
+                    raise ValueError(f"{name} lies on {u.device}, the current device is "
+                                     f"cuda:{device}")
+            break
     return _raw_stream(device)
+
+
+def _device_of(names: str, tensors) -> int:
+    try:
+        return _torch.cuda.current_device()
+    except Exception:
+        _reachable(names, *tensors)   # without a GPU: a tensor in host memory is what is wrong
+        raise
 
 
 def _float_type(name: str, t) -> int:
@@ -669,6 +686,16 @@ def _rows(name: str, t, width: int | None = None) -> int:
     if shape[1] > 1 and stride[1] != 1:
         raise ValueError(f"{name}: a row's values must lie side by side, got strides {stride}")
     return stride[0] if shape[0] > 1 else (shape[1] + 7) // 8 * 8   # one row: there is no next
+
+
+def _alike(name: str, t, shape, dtype) -> int:
+    """_rows of a tensor that must have this shape and type."""
+    if t.dtype is not dtype or t.shape != shape:
+        raise TypeError(f"{name} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: a row's values must lie side by side, got strides {stride}")
+    return stride[0] if shape[0] > 1 else (shape[1] + 7) // 8 * 8
 
 
 class MX4:
@@ -696,6 +723,7 @@ class MX4:
         self._tensors = (codes, scales)
         self.rows, self.K = rows, K
         self._c = Mx4C(_ptr(codes), _ptr(scales), rows, K)
+        self.by_reference = ctypes.byref(self._c)
 
     @classmethod
     def empty(cls, rows: int, K: int, device="cuda"):
@@ -715,10 +743,9 @@ class MX4:
             raise TypeError(f"codes and scales must be contiguous uint8 [rows][K / 2] and "
                             f"[rows][K / 32], got {codes.dtype} {tuple(codes.shape)}, "
                             f"{scales.dtype} {tuple(scales.shape)}")
-        _reachable("codes scales", codes, scales)
+        at = _on_device(stream, "codes scales", (codes, scales))
         q = cls.empty(rows, 2 * half, codes.device)
-        check(load().ltx25_mx4_pack(_on_device(stream, codes, scales), _ptr(codes), _ptr(scales),
-                                    ctypes.byref(q.c())))
+        check(load().ltx25_mx4_pack(at, _ptr(codes), _ptr(scales), ctypes.byref(q.c())))
         return q
 
     def unpacked(self, stream=None):
@@ -726,9 +753,8 @@ class MX4:
         (ltx25_mx4_unpack)."""
         codes = self.codes.new_empty((self.rows, self.K // 2))
         scales = self.codes.new_empty((self.rows, self.K // 32))
-        _reachable("codes", self.codes)
-        check(load().ltx25_mx4_unpack(_on_device(stream, codes), ctypes.byref(self.c()),
-                                      _ptr(codes), _ptr(scales)))
+        check(load().ltx25_mx4_unpack(_on_device(stream, "codes", (self.codes,)),
+                                      ctypes.byref(self.c()), _ptr(codes), _ptr(scales)))
         return codes, scales
 
     def c(self) -> Mx4C:
@@ -751,10 +777,8 @@ def mx4_quantize_rows(x, q: MX4, stream=None) -> None:
     stride = _rows("x", x, q.K)
     if x.shape[0] != q.rows:
         raise ValueError(f"x {tuple(x.shape)} does not have q's {q.rows} rows")
-    if not (x.is_cuda and q.codes.is_cuda):
-        _reachable("x q.codes", x, q.codes)
-    check(load().ltx25_mx4_quantize_rows(_on_device(stream, x, q.codes), x.data_ptr(), kind, stride,
-                                         ctypes.byref(q.c())))
+    check(load().ltx25_mx4_quantize_rows(_on_device(stream, "x q.codes", (x, q.codes)),
+                                         x.data_ptr(), kind, stride, q.by_reference))
 
 
 def mx4_dequant(q: MX4, out, stream=None) -> None:
@@ -764,10 +788,8 @@ def mx4_dequant(q: MX4, out, stream=None) -> None:
     stride = _rows("out", out, q.K)
     if out.dtype is not _torch.bfloat16 or out.shape[0] != q.rows:
         raise TypeError(f"out must be bf16 [{q.rows}][{q.K}], got {out.dtype} {tuple(out.shape)}")
-    if not (out.is_cuda and q.codes.is_cuda):
-        _reachable("out q.codes", out, q.codes)
-    check(load().ltx25_mx4_dequant(_on_device(stream, out, q.codes), ctypes.byref(q.c()),
-                                   out.data_ptr(), stride))
+    check(load().ltx25_mx4_dequant(_on_device(stream, "out q.codes", (out, q.codes)),
+                                   q.by_reference, out.data_ptr(), stride))
 
 
 def mx4_gemm_workspace(M: int, K: int, N: int) -> int:
@@ -807,13 +829,10 @@ def mx4_gemm(x: MX4, w: MX4, bias, y, epilogue: int = EPI_NONE, workspace=None,
     kind = bias_dtype_of(bias)
     workspace = _product(y, bias, x.rows, w.rows, workspace,
                          mx4_gemm_workspace(x.rows, x.K, w.rows), stream)
-    if not (y.is_cuda and x.codes.is_cuda and w.codes.is_cuda):
-        _reachable("x.codes w.codes y bias workspace", x.codes, w.codes, y, bias, workspace)
-    elif not ((bias is None or bias.is_cuda) and (workspace is None or workspace.is_cuda)):
-        _reachable("bias workspace", bias, workspace)
-    check(load().ltx25_mx4_gemm(_on_device(stream, y, x.codes, w.codes), ctypes.byref(x.c()),
-                                ctypes.byref(w.c()), _ptr(bias), kind, y.data_ptr(), epilogue,
-                                *_held(workspace)))
+    at = _on_device(stream, "x.codes w.codes y bias workspace",
+                    (x.codes, w.codes, y, bias, workspace))
+    check(load().ltx25_mx4_gemm(at, x.by_reference, w.by_reference, _ptr(bias), kind, y.data_ptr(),
+                                epilogue, *_held(workspace)))
 
 
 def linear_mx4(x, w: MX4, bias, y, epilogue: int = EPI_NONE, workspace=None, stream=None) -> None:
@@ -826,13 +845,9 @@ def linear_mx4(x, w: MX4, bias, y, epilogue: int = EPI_NONE, workspace=None, str
     stride = _rows("x", x, w.K)
     M, N = x.shape[0], w.rows
     workspace = _product(y, bias, M, N, workspace, linear_mx4_workspace(M, w.K, N), stream)
-    if not (x.is_cuda and y.is_cuda and w.codes.is_cuda):
-        _reachable("x w.codes y bias workspace", x, w.codes, y, bias, workspace)
-    elif not ((bias is None or bias.is_cuda) and (workspace is None or workspace.is_cuda)):
-        _reachable("bias workspace", bias, workspace)
-    check(load().ltx25_linear_mx4(_on_device(stream, x, y, w.codes), x.data_ptr(), stride, M,
-                                  ctypes.byref(w.c()), _ptr(bias), kind, y.data_ptr(), epilogue,
-                                  *_held(workspace)))
+    at = _on_device(stream, "x w.codes y bias workspace", (x, w.codes, y, bias, workspace))
+    check(load().ltx25_linear_mx4(at, x.data_ptr(), stride, M, w.by_reference, _ptr(bias), kind,
+                                  y.data_ptr(), epilogue, *_held(workspace)))
 
 
 # ---- around a block's linears and attention (include/ltx25_block.h) -----------------------
@@ -851,87 +866,94 @@ def block_norm(x, out, *, y=None, x_out=None, gate=None, post_weight=None, weigh
     is bf16, an MX4 (ltx25_block_norm_mx4), or None where y is given."""
     if _torch is None:
         _import_torch()
-    kind = _float_type("x", x)
-    xs = _rows("x", x)
-    tokens, width = x.shape
-    n = NormC(width, 1 if layer else 0, eps, residual_scale, kind, DT_BF16, DT_BF16, 0, xs, 0, 0, 0,
-              0)
+    shape = x.shape
+    kind, xs = _float_type("x", x), _rows("x", x)
+    tokens, width = shape
+    xos = ys = ms = os_ = mod_rows = 0
+    mod = weights = DT_BF16
     if y is not None:
-        n.y_stride = _rows("y", y, width)
-        if y.dtype is not _torch.bfloat16 or y.shape[0] != tokens:
-            raise TypeError(f"y must be bf16 [{tokens}][{width}], got {y.dtype} {tuple(y.shape)}")
+        ys = _alike("y", y, shape, _torch.bfloat16)
         if x_out is None:
             raise ValueError("x_out must be given with y (it may be x)")
     if x_out is not None:
-        n.x_out_stride = _rows("x_out", x_out, width)
-        if x_out.dtype != x.dtype or x_out.shape[0] != tokens:
-            raise TypeError(f"x_out must be {x.dtype} [{tokens}][{width}], got {x_out.dtype} "
-                            f"{tuple(x_out.shape)}")
-    first = None
-    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
-        if t is None:
-            continue
-        at = (_float_type(name, t), _rows(name, t, width), t.shape[0])
-        if first is None:
-            first = at
-            n.mod_dtype, n.mod_stride, n.mod_rows = at
-        elif at != first:
-            raise ValueError(f"{name}: gate, scale and shift must be alike in type, rows and row "
-                             f"stride")
+        xos = _alike("x_out", x_out, shape, x.dtype)
+    if gate is not None or scale is not None or shift is not None:
+        first = None
+        for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+            if t is None:
+                continue
+            if first is None:
+                first = t
+                mod, ms, mod_rows = _float_type(name, t), _rows(name, t, width), t.shape[0]
+            elif (t.dtype != first.dtype or t.shape != first.shape
+                  or _rows(name, t, width) != ms):
+                raise ValueError(f"{name}: gate, scale and shift must be alike in type, rows and "
+                                 f"row stride")
     if rows is not None:
         _int32("rows", rows, tokens)
-    first = None
     for name, t in (("post_weight", post_weight), ("weight", weight)):
         if t is None:
             continue
-        n.weight_dtype = _float_type(name, t)
-        if tuple(t.shape) != (width,) or not t.is_contiguous() or first not in (None, t.dtype):
+        weights = _float_type(name, t)
+        if (t.shape != shape[1:] or not t.is_contiguous()
+                or (weight is not None and t.dtype != weight.dtype)):
             raise TypeError(f"{name} must be contiguous [{width}], and of one type with the other "
                             f"weight, got {t.dtype} {tuple(t.shape)}")
-        first = t.dtype
-    coded = isinstance(out, MX4)
-    if coded:
+    if isinstance(out, MX4):
         if out.rows != tokens or out.K != width:
             raise ValueError(f"out has {out.rows} rows of {out.K}, not {tokens} of {width}")
-    elif out is not None:
-        n.out_stride = _rows("out", out, width)
-        if out.dtype is not _torch.bfloat16 or out.shape[0] != tokens:
-            raise TypeError(f"out must be bf16 [{tokens}][{width}] or an MX4, got {out.dtype} "
-                            f"{tuple(out.shape)}")
-    held = out.codes if coded else out
-    tensors = (x, held, y, x_out, gate, post_weight, weight, scale, shift, rows)
-    _reachable("x out y x_out gate post_weight weight scale shift rows", *tensors)
-    if coded:
-        fn, to = load().ltx25_block_norm_mx4, ctypes.byref(out.c())
+        held, fn, to = out.codes, load().ltx25_block_norm_mx4, out.by_reference
     else:
-        fn, to = load().ltx25_block_norm, _ptr(out)
-    check(fn(_on_device(stream, *tensors), ctypes.byref(n), _ptr(x), _ptr(y), _ptr(x_out),
-             _ptr(post_weight), _ptr(gate), _ptr(weight), _ptr(scale), _ptr(shift), _ptr(rows), to,
-             tokens))
+        if out is not None:
+            os_ = _alike("out", out, shape, _torch.bfloat16)
+        held, fn, to = out, load().ltx25_block_norm, _ptr(out)
+    at = _on_device(stream, "x out y x_out gate post_weight weight scale shift rows",
+                    (x, held, y, x_out, gate, post_weight, weight, scale, shift, rows))
+    n = NormC(width, 1 if layer else 0, eps, residual_scale, kind, mod, weights, mod_rows, xs, xos,
+              ys, ms, os_)
+    check(fn(at, ctypes.byref(n), x.data_ptr(), _ptr(y), _ptr(x_out), _ptr(post_weight), _ptr(gate),
+             _ptr(weight), _ptr(scale), _ptr(shift), _ptr(rows), to, tokens))
 
 
 def _rotation(head_dim: int, freqs, axes, positions, tokens: int, interleaved: bool) -> RotationC:
-    if (freqs.dtype is not _torch.float32 or freqs.dim() != 2 or not freqs.is_contiguous()):
+    shape = freqs.shape
+    if (freqs.dtype is not _torch.float32 or len(shape) != 2 or shape[1] == 0
+            or not freqs.is_contiguous()):
         raise TypeError(f"freqs must be contiguous float32 [1 or heads][pairs], got {freqs.dtype} "
-                        f"{tuple(freqs.shape)}")
-    if axes is not None and (axes.dtype is not _torch.int32 or axes.shape != freqs.shape
-                             or not axes.is_contiguous()):
-        raise TypeError(f"axes must be contiguous int32 {tuple(freqs.shape)}, got {axes.dtype} "
-                        f"{tuple(axes.shape)}")
-    r = RotationC(head_dim, 2 * freqs.shape[1], 1 if interleaved else 0, 1, freqs.shape[0], DT_F32,
-                  _ptr(freqs), _ptr(axes), None)
-    if freqs.shape[1] == 0:
-        raise ValueError("freqs has no pairs")
+                        f"{tuple(shape)}")
+    pa = pp = None
+    if axes is not None:
+        if axes.dtype is not _torch.int32 or axes.shape != shape or not axes.is_contiguous():
+            raise TypeError(f"axes must be contiguous int32 {tuple(shape)}, got {axes.dtype} "
+                            f"{tuple(axes.shape)}")
+        pa = axes.data_ptr()
+    kind, n_axes = DT_F32, 1
     if positions is not None:
-        if positions.dim() != 2 or positions.shape[0] != tokens or not positions.is_contiguous():
-            raise TypeError(f"positions must be contiguous [{tokens}][axes], got "
-                            f"{tuple(positions.shape)}")
+        ps = positions.shape
+        if len(ps) != 2 or ps[0] != tokens or not positions.is_contiguous():
+            raise TypeError(f"positions must be contiguous [{tokens}][axes], got {tuple(ps)}")
         if positions.dtype is _torch.int32:
-            r.pos_dtype = DT_I32
+            kind = DT_I32
         elif positions.dtype is not _torch.float32:
             raise TypeError(f"positions must be int32 or float32, got {positions.dtype}")
-        r.n_axes, r.positions = positions.shape[1], _ptr(positions)
-    return r
+        n_axes, pp = ps[1], positions.data_ptr()
+    return RotationC(head_dim, 2 * shape[1], 1 if interleaved else 0, n_axes, shape[0], kind,
+                     freqs.data_ptr(), pa, pp)
+
+
+def _rotated(name: str, t, to, tokens: int, dim: int) -> tuple:
+    """What ltx25_rope takes of a tensor: pointers, heads and strides."""
+    if t is None:
+        return (None, None, 0, 0, 0)
+    shape = t.shape
+    stride = _tokens(name, t, shape)
+    if shape[0] != tokens or shape[2] != dim:
+        raise ValueError(f"{name} {tuple(shape)} is not {tokens} tokens of heads of {dim}")
+    if to is None:
+        return (t.data_ptr(), t.data_ptr(), shape[1], stride, stride)
+    if to.shape != shape:
+        raise ValueError(f"{name}_out {tuple(to.shape)} is not {name}'s {tuple(shape)}")
+    return (t.data_ptr(), to.data_ptr(), shape[1], stride, _tokens(name + "_out", to, shape))
 
 
 def rope(q, k, positions, freqs, axes=None, *, q_out=None, k_out=None, interleaved: bool = False,
@@ -948,21 +970,11 @@ def rope(q, k, positions, freqs, axes=None, *, q_out=None, k_out=None, interleav
     if given is None or (q is None and q_out is not None) or (k is None and k_out is not None):
         raise ValueError("rope rotates q, k or both, and an output goes with its input")
     tokens, _, dim = given.shape
-    args = []
-    for name, t, to in (("q", q, q_out), ("k", k, k_out)):
-        if t is None:
-            args += [None, None, 0, 0, 0]
-            continue
-        to = t if to is None else to
-        ts, os_ = _tokens(name, t, t.shape), _tokens(name + "_out", to, to.shape)
-        if t.shape != to.shape or t.shape[0] != tokens or t.shape[2] != dim:
-            raise ValueError(f"{name} {tuple(t.shape)} and {name}_out {tuple(to.shape)} are not "
-                             f"both {tokens} tokens of heads of {dim}")
-        args += [t.data_ptr(), to.data_ptr(), t.shape[1], ts, os_]
+    args = _rotated("q", q, q_out, tokens, dim) + _rotated("k", k, k_out, tokens, dim)
     r = _rotation(dim, freqs, axes, positions, tokens, interleaved)
-    tensors = (q, k, positions, freqs, axes, q_out, k_out)
-    _reachable("q k positions freqs axes q_out k_out", *tensors)
-    check(load().ltx25_rope(_on_device(stream, *tensors), ctypes.byref(r), *args, tokens))
+    at = _on_device(stream, "q k positions freqs axes q_out k_out",
+                    (q, k, positions, freqs, axes, q_out, k_out))
+    check(load().ltx25_rope(at, ctypes.byref(r), *args, tokens))
 
 
 def kv_append_rope(cache: KVCache, table, k, v, cu, start, freqs, axes=None, positions=None, *,
@@ -972,10 +984,8 @@ def kv_append_rope(cache: KVCache, table, k, v, cu, start, freqs, axes=None, pos
     every axis."""
     args = _moved(cache, table, k, v, cu, start)
     r = _rotation(cache.head_dim, freqs, axes, positions, k.shape[0], interleaved)
-    tensors = (freqs, axes, positions)
-    _reachable("freqs axes positions", *tensors)
-    check(load().ltx25_kv_append_rope(_on_device(stream, k, v, table, *tensors), *args[:9],
-                                      ctypes.byref(r), *args[9:]))
+    at = _on_device(stream, "freqs axes positions k", (freqs, axes, positions, k))
+    check(load().ltx25_kv_append_rope(at, *args[:9], ctypes.byref(r), *args[9:]))
 
 
 def probe_read(src, nbytes: int, sink, blocks: int, stream=None) -> None:

@@ -50,7 +50,10 @@ __device__ __forceinline__ void store_bf16(uint16_t* row, int n, int N, const Wo
     if (N % 8 == 0) {
       __builtin_nontemporal_store(x, (words*)(row + n));
     } else {
-      *(words*)(row + n) = x;   // lines that the cache puts together
+      // parts of lines, which the cache puts together. (The empty statement keeps the compiler
+      // from making one ordinary store of the two: 8160 x 4096 -> 16384 340 us for 267.)
+      asm volatile("" ::: "memory");
+      *(words*)(row + n) = x;
     }
   } else {
 #pragma unroll
@@ -99,9 +102,12 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   static_assert(DEPTH == 4 || (DEPTH == 8 && STAGES > 2), "slices of x in flight: a span's or two");
   constexpr int kCodes = 4 * CB * kMx4CodeTile;
   constexpr int kScaleTiles = 4 * RB + CB, kScaleLoads = (kScaleTiles + 15) / 16;
-  constexpr int kStage = kCodes + 16 * kScaleLoads * kMx4Tile;
-  static_assert(STAGES * kStage <= 80 * 1024, "two workgroups a CU");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
+  constexpr int kStage = kCodes + kScaleTiles * kMx4Tile;
+  // behind the stages: where loads of no tile go, and a tile's bias, a copy a wave
+  constexpr int kNowhere = STAGES * kStage, kBias = kNowhere + 4 * kMx4Tile;
+  constexpr int kLds = kBias + 4 * 64 * CB;
+  static_assert(kScaleTiles % 4 == 0 && kLds <= 80 * 1024, "two workgroups a CU");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = p.tiles_m * p.tiles_n;
@@ -152,7 +158,8 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
     } else {
       const int q = wave + 4 * (k - CB);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          q < RB ? xsr : wsr, (lds_u32*)(at + kCodes + q * 4 * kMx4Tile), 16,
+          q < RB ? xsr : wsr,
+          (lds_u32*)(4 * q < kScaleTiles ? at + kCodes + q * 4 * kMx4Tile : lds + kNowhere), 16,
           (int)(on ? then.s[k - CB] : here.s[k - CB]), from * kMx4Tile, 0, 0);
     }
   };
@@ -228,6 +235,19 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 #pragma unroll
     for (int i = 0; i < RB; ++i) { load_x(t / 4, t % 4, t, i); }
   }
+  // The whole weight is asked for at the start, a word of each 64 bytes over all workgroups,
+  // so that later spans find it beside the memory: with each span's loads the first to see their
+  // lines, a span waits for the memory behind the stores (8160 x 4096 -> 16384 on a weight not
+  // read for a while: 360 us, so 275; on one just read 246 and 257). Up to half of what is kept.
+  auto touch = [&](__amdgpu_buffer_rsrc_t r, size_t bytes) {
+    const uint32_t end = (uint32_t)min(bytes, (size_t)128 << 20);
+    for (uint32_t at = (blockIdx.x * 4 + wave) * 4096; at < end; at += gridDim.x * 4 * 4096) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_u32*)(lds + kNowhere), 4, (int)(at + lane * 64),
+                                               0, 0, 0);
+    }
+  };
+  touch(wr, mx4_code_bytes(p.N, p.K));
+  touch(wsr, mx4_scale_bytes(p.N, p.K));
   // the first stages have landed, for what the count above does not see
   constexpr int kFirst = (DEPTH - 1) * RB;
   __builtin_amdgcn_s_waitcnt(0x0f70 | (kFirst < 15 ? kFirst : 15));
@@ -237,6 +257,16 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
     for (int i = 0; i < RB; ++i) {
 #pragma unroll
       for (int j = 0; j < CB; ++j) { acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+    }
+    // The tile's bias, a column or two a lane, which has landed long before the tile is done
+    // (asked for behind the products: 8160 x 4096 -> 16384 with bias and GELU 367 us)
+    int tm, tn;
+    map_tile(tile, p.tiles_m, p.tiles_n, tm, tn);
+    const int n0 = tn * 16 * CB, row0 = (tm * 4 + wave) * 16 * RB;   // the wave's rows
+    float bias[CB / 4];
+#pragma unroll
+    for (int i = 0; i < CB / 4; ++i) {
+      bias[i] = load_bias(p.bias, p.bias_type, min(n0 + 64 * i + lane, p.N - 1));
     }
     if constexpr (DEPTH == 8) {
       int span = 0;
@@ -253,24 +283,17 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 
     // Block (i, j), lane l, register r: row 16 i + l % 16, column 16 j + 4 (l / 16) + r. The
     // loads of x that are in flight, the next tile's, have landed before anything is stored.
-    int tm, tn;
-    map_tile(tile, p.tiles_m, p.tiles_n, tm, tn);
-    const int n0 = tn * 16 * CB, row0 = (tm * 4 + wave) * 16 * RB;   // the wave's rows
-    auto bias_of = [&](int j, float (&bias)[4]) {
+    float* const biases = (float*)(lds + kBias) + wave * 16 * CB;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        bias[r] = load_bias(p.bias, p.bias_type, min(n0 + 16 * j + 4 * g + r, p.N - 1));
-      }
-    };
+    for (int i = 0; i < CB / 4; ++i) { biases[64 * i + lane] = bias[i]; }
     // Two blocks side by side: the lanes' rows of 16 are exchanged so that each lane has eight
     // columns of one of them, 16 bytes.
     auto store = [&](auto gelu) {
       unroll<CB / 2>([&](auto jj) {
         constexpr int j = 2 * decltype(jj)::value;
         __builtin_amdgcn_sched_barrier(0);
-        float bias[2][4];
-        bias_of(j, bias[0]);
-        bias_of(j + 1, bias[1]);
+        const f32x4 bias[2] = {*(const f32x4*)(biases + 16 * j + 4 * g),
+                               *(const f32x4*)(biases + 16 * j + 16 + 4 * g)};
         const int n = n0 + 16 * (j + (g & 1)) + 8 * (g >> 1);
 #pragma unroll
         for (int i = 0; i < RB; ++i) {

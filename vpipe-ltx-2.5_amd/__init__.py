@@ -800,18 +800,20 @@ def linear_mx4_workspace(M: int, K: int, N: int) -> int:
     return int(load().ltx25_linear_mx4_workspace(M, K, N))
 
 
-def _product(y, bias, M: int, N: int, workspace, need: int, stream):
+def _product(y, bias, M: int, K: int, N: int, workspace, need_of, stream):
     """What the two products check alike; the workspace, allocated on torch's current stream
-    where none is given."""
-    if y.dtype is not _torch.bfloat16 or tuple(y.shape) != (M, N) or not y.is_contiguous():
+    where none is given (one that is given the library checks)."""
+    if y.dtype is not _torch.bfloat16 or y.shape != (M, N) or not y.is_contiguous():
         raise TypeError(f"y must be contiguous bf16 [{M}][{N}], got {y.dtype} {tuple(y.shape)}")
-    if bias is not None and (tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+    if bias is not None and (bias.shape != (N,) or not bias.is_contiguous()):
         raise TypeError(f"bias must be contiguous [{N}], got {tuple(bias.shape)}")
-    if need and workspace is None:
-        if stream is not None:
+    if workspace is None:
+        need = need_of(M, K, N)
+        if need and stream is not None:
             raise ValueError(f"on a stream of the caller's, {need} bytes of workspace are the "
                              f"caller's too")
-        workspace = _torch.empty(need, dtype=_torch.uint8, device=y.device)
+        if need:
+            workspace = _torch.empty(need, dtype=_torch.uint8, device=y.device)
     return workspace
 
 
@@ -827,8 +829,7 @@ def mx4_gemm(x: MX4, w: MX4, bias, y, epilogue: int = EPI_NONE, workspace=None,
     if _torch is None:
         _import_torch()
     kind = bias_dtype_of(bias)
-    workspace = _product(y, bias, x.rows, w.rows, workspace,
-                         mx4_gemm_workspace(x.rows, x.K, w.rows), stream)
+    workspace = _product(y, bias, x.rows, x.K, w.rows, workspace, mx4_gemm_workspace, stream)
     at = _on_device(stream, "x.codes w.codes y bias workspace",
                     (x.codes, w.codes, y, bias, workspace))
     check(load().ltx25_mx4_gemm(at, x.by_reference, w.by_reference, _ptr(bias), kind, y.data_ptr(),
@@ -844,7 +845,7 @@ def linear_mx4(x, w: MX4, bias, y, epilogue: int = EPI_NONE, workspace=None, str
         raise TypeError(f"x must be bf16, got {x.dtype}")
     stride = _rows("x", x, w.K)
     M, N = x.shape[0], w.rows
-    workspace = _product(y, bias, M, N, workspace, linear_mx4_workspace(M, w.K, N), stream)
+    workspace = _product(y, bias, M, w.K, N, workspace, linear_mx4_workspace, stream)
     at = _on_device(stream, "x w.codes y bias workspace", (x, w.codes, y, bias, workspace))
     check(load().ltx25_linear_mx4(at, x.data_ptr(), stride, M, w.by_reference, _ptr(bias), kind,
                                   y.data_ptr(), epilogue, *_held(workspace)))

@@ -21,17 +21,20 @@ struct Rotation {
   bool interleaved = false;
 };
 
-// A token's positions in turns (divided by 2 pi), in 64 bits
+constexpr double kInv2Pi = 0.15915494309189533577;
+
+// A token's positions in turns (divided by 2 pi), in 64 bits. MANY: more than one axis.
+template <bool MANY>
 struct Turns {
-  double at[kAxesMax];
+  double at[MANY ? kAxesMax : 1];
 };
 
-__device__ __forceinline__ Turns turns_of(const Rotation& r, long token)
+template <bool MANY>
+__device__ __forceinline__ Turns<MANY> turns_of(const Rotation& r, long token)
 {
-  constexpr double kInv2Pi = 0.15915494309189533577;
-  Turns t;
+  Turns<MANY> t;
 #pragma unroll
-  for (int a = 0; a < kAxesMax; ++a) {
+  for (int a = 0; a < (MANY ? kAxesMax : 1); ++a) {
     const long at = token * r.n_axes + min(a, r.n_axes - 1);
     t.at[a] = (r.whole ? (double)((const int*)r.positions)[at]
                        : (double)((const float*)r.positions)[at]) * kInv2Pi;
@@ -39,23 +42,20 @@ __device__ __forceinline__ Turns turns_of(const Rotation& r, long token)
   return t;
 }
 
-__device__ __forceinline__ Turns turns_at(long place)
-{
-  constexpr double kInv2Pi = 0.15915494309189533577;
-  const double t = (double)place * kInv2Pi;
-  return {{t, t, t, t}};
-}
-
 // The sine and cosine of one pair's angle. The product and the removal of whole turns in 64
 // bits: an angle of 2^20 radians has 2^-4 left of its own last bits in 32. What is left, at
 // most half a turn, goes to the hardware's sine and cosine, whose argument is in turns.
-__device__ __forceinline__ void sin_cos(const Turns& t, float freq, int axis, float& sn, float& cs)
+template <bool MANY>
+__device__ __forceinline__ void sin_cos(const Turns<MANY>& t, double freq, int axis, float& sn,
+                                        float& cs)
 {
   double at = t.at[0];
-  at = axis == 1 ? t.at[1] : at;
-  at = axis == 2 ? t.at[2] : at;
-  at = axis >= 3 ? t.at[3] : at;
-  const double turns = at * (double)freq;
+  if constexpr (MANY) {
+    at = axis == 1 ? t.at[1] : at;
+    at = axis == 2 ? t.at[2] : at;
+    at = axis >= 3 ? t.at[3] : at;
+  }
+  const double turns = at * freq;
   const float left = (float)(turns - rint(turns));
   sn = __builtin_amdgcn_sinf(left);
   cs = __builtin_amdgcn_cosf(left);
@@ -64,10 +64,10 @@ __device__ __forceinline__ void sin_cos(const Turns& t, float freq, int axis, fl
 // N consecutive pairs' frequencies and axes (N 4 or 8, the first a multiple of 4)
 template <int N>
 struct Pairs {
-  float freq[N];
+  double freq[N];
   int axis[N];
 };
-template <int N>
+template <bool MANY, int N>
 __device__ __forceinline__ Pairs<N> pairs_of(const Rotation& r, int head, int first)
 {
   Pairs<N> p;
@@ -75,10 +75,10 @@ __device__ __forceinline__ Pairs<N> pairs_of(const Rotation& r, int head, int fi
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
     const f32x4 f = *(const f32x4*)(r.freqs + at + i);
-    const i32x4 a = r.axes != nullptr ? *(const i32x4*)(r.axes + at + i) : i32x4{0, 0, 0, 0};
+    const i32x4 a = MANY && r.axes != nullptr ? *(const i32x4*)(r.axes + at + i) : i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      p.freq[i + k] = f[k];
+      p.freq[i + k] = (double)f[k];
       p.axis[i + k] = min(a[k], r.n_axes - 1);
     }
   }
@@ -100,8 +100,8 @@ __device__ __forceinline__ float turned_b(float a, float b, float sn, float cs)
 }
 
 // Eight channels of pairs side by side, turned by four frequencies
-template <int N>
-__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pairs<N>& p)
+template <bool MANY, int N>
+__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns<MANY>& t, const Pairs<N>& p)
 {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -115,7 +115,8 @@ __device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pair
 }
 
 // Eight pairs, their first channels in xa and their second in xb
-__device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns& t,
+template <bool MANY>
+__device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns<MANY>& t,
                                               const Pairs<8>& p)
 {
   uint32_t a[4] = {xa.x, xa.y, xa.z, xa.w}, b[4] = {xb.x, xb.y, xb.z, xb.w};
@@ -134,8 +135,9 @@ __device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns&
 
 // The same where one lane has the pairs' first channels and another their second: the
 // lane's own half of it, of its channels x and the other lane's.
-__device__ __forceinline__ uint4 rotate_half(uint4 x, uint4 other, bool second, const Turns& t,
-                                             const Pairs<8>& p)
+template <bool MANY>
+__device__ __forceinline__ uint4 rotate_half(uint4 x, uint4 other, bool second,
+                                             const Turns<MANY>& t, const Pairs<8>& p)
 {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
   const uint32_t o[4] = {other.x, other.y, other.z, other.w};

@@ -203,7 +203,8 @@ __device__ __forceinline__ uint2 quantize8(uint4 x, float s, float rs)
 // ROPE: the keys are turned in registers as they arrive and rounded to bf16, and from there on
 // are the keys of a plain append. Pairs half of the rotated channels apart meet by an exchange
 // of 16-byte pieces between lanes of one token.
-template <int D, bool ROPE = false>
+// ROPE 2: positions of several axes.
+template <int D, int ROPE = 0>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotation rot)
 {
   constexpr int kMaxP = 128;
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
   const int pieces = few ? (sp.hi - sp.lo) * kPer : (((sp.hi + 3) >> 2) - quad0) * kPer;
   // The lane's piece of a key is the same in all its tokens, so are its pairs. A key of the
   // page's token `tok`: every lane of a wave takes part.
+  constexpr bool kMany = ROPE == 2;
   const int piece = tid % kPer;
   const int apart = ROPE && !rot.interleaved ? rot.pairs / 8 : 0;   // pieces between a pair's two
   const bool second = apart > 0 && piece >= apart;
@@ -236,14 +238,14 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
   Pairs<8> pairs;
   if (ROPE && !values && turning) {
     if (rot.interleaved) {
-      const Pairs<4> four = pairs_of<4>(rot, g, piece * 4);
+      const Pairs<4> four = pairs_of<kMany, 4>(rot, g, piece * 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         pairs.freq[i] = four.freq[i];
         pairs.axis[i] = four.axis[i];
       }
     } else {
-      pairs = pairs_of<8>(rot, g, (piece - (second ? apart : 0)) * 8);
+      pairs = pairs_of<kMany, 8>(rot, g, (piece - (second ? apart : 0)) * 8);
     }
   }
   auto rotate = [&](uint4& w, int tok) {
@@ -257,8 +259,12 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
       other.w = __shfl((int)w.w, from);
     }
     if (there) {
-      const Turns t = rot.positions != nullptr ? turns_of(rot, sp.first + tok)
-                                               : turns_at(sp.place + tok);
+      Turns<kMany> t;
+      if (kMany || rot.positions != nullptr) {
+        t = turns_of<kMany>(rot, sp.first + tok);
+      } else {
+        t.at[0] = (double)(sp.place + tok) * kInv2Pi;
+      }
       w = rot.interleaved ? rotate_side(w, t, pairs) : rotate_half(w, other, second, t, pairs);
     }
   };
@@ -947,10 +953,12 @@ hipError_t launch_kv_append_rope(const CacheArgs& c, const uint16_t* k, const ui
                         total};
   dim3 grid;
   if (!move_grid(p, grid)) { return hipErrorInvalidConfiguration; }
+  // (a token's place is the same on every axis)
+  const bool many = r.positions != nullptr && r.n_axes > 1;
   if (c.head_dim == 128) {
-    kv_append_kernel<128, true><<<grid, kThreads, 0, stream>>>(p, r);
+    (many ? kv_append_kernel<128, 2> : kv_append_kernel<128, 1>)<<<grid, kThreads, 0, stream>>>(p, r);
   } else {
-    kv_append_kernel<64, true><<<grid, kThreads, 0, stream>>>(p, r);
+    (many ? kv_append_kernel<64, 2> : kv_append_kernel<64, 1>)<<<grid, kThreads, 0, stream>>>(p, r);
   }
   return hipGetLastError();
 }

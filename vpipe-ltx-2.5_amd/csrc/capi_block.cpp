@@ -117,8 +117,8 @@ int check_norm(const ltx25_norm* n, const void* x, const void* y, const void* x_
   a->run = modulated && rows == nullptr ? tokens / n->mod_rows : 1;
   a->layer = n->layer != 0;
   a->wide = n->x_dtype == LTX25_DT_F32;
-  a->mod_wide = n->mod_dtype == LTX25_DT_F32;
-  a->weight_wide = n->weight_dtype == LTX25_DT_F32;
+  a->mod_wide = modulated && n->mod_dtype == LTX25_DT_F32;
+  a->weight_wide = (weight != nullptr || after != nullptr) && n->weight_dtype == LTX25_DT_F32;
   a->eps = n->eps;
   a->alpha = n->residual_scale;
   return LTX25_OK;

@@ -3,25 +3,48 @@
 #include "block.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ltx25 {
 namespace {
 
-// 8 values from element `at` of a bf16 or f32 tensor
+// 8 values of a tensor as they lie in memory: 16 bytes of bf16, 32 of f32
+template <bool WIDE>
+struct Raw {
+  uint4 w[WIDE ? 2 : 1];
+};
+template <bool WIDE>
+__device__ __forceinline__ Raw<WIDE> fetch8(const void* p, long at)
+{
+  const uint4* const q = (const uint4*)((const char*)p + at * (WIDE ? 4 : 2));
+  Raw<WIDE> r;
+  r.w[0] = q[0];
+  if constexpr (WIDE) { r.w[1] = q[1]; }
+  return r;
+}
+template <bool WIDE>
+__device__ __forceinline__ void values8(const Raw<WIDE>& r, float (&v)[8])
+{
+#pragma unroll
+  for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
+    const uint32_t a[4] = {r.w[h].x, r.w[h].y, r.w[h].z, r.w[h].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (WIDE) {
+        v[4 * h + i] = __uint_as_float(a[i]);
+      } else {
+        v[2 * i] = low_f32(a[i]);
+        v[2 * i + 1] = high_f32(a[i]);
+      }
+    }
+  }
+}
 __device__ __forceinline__ void load8(const void* p, bool wide, long at, float (&v)[8])
 {
   if (wide) {
-    const f32x4 a = ((const f32x4*)((const float*)p + at))[0];
-    const f32x4 b = ((const f32x4*)((const float*)p + at))[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = a[i];
-      v[4 + i] = b[i];
-    }
+    values8(fetch8<true>(p, at), v);
   } else {
-    const uint4 w = *(const uint4*)((const uint16_t*)p + at);
-    v[0] = low_f32(w.x), v[1] = high_f32(w.x), v[2] = low_f32(w.y), v[3] = high_f32(w.y);
-    v[4] = low_f32(w.z), v[5] = high_f32(w.z), v[6] = low_f32(w.w), v[7] = high_f32(w.w);
+    values8(fetch8<false>(p, at), v);
   }
 }
 
@@ -37,14 +60,21 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8])
 // Sums in f32, the mean taken off before the squares are added; where a sum leaves f32's
 // range the values are taken 2^-80 times as large, which leaves every square that counts
 // inside it.
-template <int WAVES, int CH>
+//
+// WIDE: x is f32. EARLY: what multiplies and shifts is bf16 and asked for before the sums.
+template <int WAVES, int CH, bool WIDE, bool EARLY>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(NormArgs p, long first)
 {
   __shared__ float part[4][WAVES];
   const int lane = threadIdx.x & 63;
   const int wave = WAVES == 1 ? 0 : (int)(threadIdx.x >> 6);
-  const long token =
-      first + (WAVES == 1 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x);
+  // Coded rows lie four to 64 bytes and 16 to a tile: 16 tokens go to workgroups of one XCD
+  // (every eighth), whose cache puts their lines together.
+  long place = blockIdx.x;
+  if (p.q.codes != nullptr && (place | 127) < (long)gridDim.x) {
+    place = (place & ~127L) + (place & 7) * 16 + ((place >> 3) & 15);
+  }
+  const long token = first + (WAVES == 1 ? place * 4 + (threadIdx.x >> 6) : place);
   if (token >= p.tokens) { return; }
   int turn = 0;
   auto total = [&](float v) {
@@ -107,17 +137,46 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
     }
   };
 
+  long row = 0;
+  if (p.mod_rows > 0) {
+    row = p.rows != nullptr ? clampi(p.rows[token], 0, p.mod_rows - 1) : token / p.run;
+    row *= p.ms;
+  }
+  // lanes past the width read its last values again
+  int from[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) { from[i] = min(col[i], p.width - 8); }
+  Raw<WIDE> rx[CH];
+  Raw<false> ry[CH], after[CH], gate[CH], weight[CH], scale[CH], shift[CH];
+  auto fetch = [&](auto& to, const void* t, long at) {
+    constexpr bool kWide = std::is_same_v<decltype(to), Raw<true>(&)[CH]>;
+    if (t == nullptr) { return; }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) { to[i] = fetch8<kWide>(t, at + from[i]); }
+  };
+  fetch(rx, p.x, token * p.xs);
+  fetch(ry, p.y, token * p.ys);
+  if constexpr (EARLY) {
+    fetch(after, p.after, 0);
+    fetch(gate, p.gate, row);
+    fetch(weight, p.weight, 0);
+    fetch(scale, p.scale, row);
+    fetch(shift, p.shift, row);
+  }
+  // chunk i of one of them
+  auto values = [&](const Raw<false>& early, const void* t, bool wide, long at, float (&m)[8]) {
+    if constexpr (EARLY) {
+      values8(early, m);
+    } else {
+      load8(t, wide, at, m);
+    }
+  };
   float x[CH][8];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) { x[i][k] = 0.0f; }
-    if (in[i]) { load8(p.x, p.wide, token * p.xs + col[i], x[i]); }
-  }
-  long row = 0;
-  if (p.mod_rows > 0) {
-    row = p.rows != nullptr ? clampi(p.rows[token], 0, p.mod_rows - 1) : token / p.run;
-    row *= p.ms;
+    if (in[i]) { values8(rx[i], x[i]); }
   }
   if (p.y != nullptr) {
     float y[CH][8];
@@ -125,7 +184,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
     for (int i = 0; i < CH; ++i) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) { y[i][k] = 0.0f; }
-      if (in[i]) { load8(p.y, false, token * p.ys + col[i], y[i]); }
+      if (in[i]) { values8(ry[i], y[i]); }
     }
     if (p.after != nullptr) { normalise(y); }
 #pragma unroll
@@ -133,18 +192,18 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
       if (!in[i]) { continue; }
       float m[8];
       if (p.after != nullptr) {
-        load8(p.after, p.weight_wide, col[i], m);
+        values(after[i], p.after, p.weight_wide, col[i], m);
 #pragma unroll
         for (int k = 0; k < 8; ++k) { y[i][k] *= m[k]; }
       }
       if (p.gate != nullptr) {
-        load8(p.gate, p.mod_wide, row + col[i], m);
+        values(gate[i], p.gate, p.mod_wide, row + col[i], m);
 #pragma unroll
         for (int k = 0; k < 8; ++k) { y[i][k] *= m[k]; }
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) { x[i][k] = fmaf(p.alpha, x[i][k], y[i][k]); }
-      if (p.wide) {
+      if constexpr (WIDE) {
         f32x4* const o = (f32x4*)((float*)p.x_out + token * p.xos + col[i]);
         o[0] = f32x4{x[i][0], x[i][1], x[i][2], x[i][3]};
         o[1] = f32x4{x[i][4], x[i][5], x[i][6], x[i][7]};
@@ -160,17 +219,17 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
     if (in[i]) {
       float m[8];
       if (p.weight != nullptr) {
-        load8(p.weight, p.weight_wide, col[i], m);
+        values(weight[i], p.weight, p.weight_wide, col[i], m);
 #pragma unroll
         for (int k = 0; k < 8; ++k) { x[i][k] *= m[k]; }
       }
       if (p.scale != nullptr) {
-        load8(p.scale, p.mod_wide, row + col[i], m);
+        values(scale[i], p.scale, p.mod_wide, row + col[i], m);
 #pragma unroll
         for (int k = 0; k < 8; ++k) { x[i][k] *= 1.0f + m[k]; }
       }
       if (p.shift != nullptr) {
-        load8(p.shift, p.mod_wide, row + col[i], m);
+        values(shift[i], p.shift, p.mod_wide, row + col[i], m);
 #pragma unroll
         for (int k = 0; k < 8; ++k) { x[i][k] += m[k]; }
       }
@@ -194,19 +253,30 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
   }
 }
 
-template <int WAVES, int CH>
+template <int WAVES, int CH, bool WIDE, bool EARLY>
 hipError_t run(const NormArgs& a, hipStream_t stream)
 {
-  // a launch has fewer than 2^32 threads
+  // a launch has fewer than 2^32 threads; whole runs of 128 workgroups
   constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES, kTokens = WAVES == 1 ? 4 : 1;
-  constexpr long kMost = ((1L << 32) / kThreads - 1) * kTokens;
+  constexpr long kMost = (((1L << 32) / kThreads - 1) & ~127L) * kTokens;
   for (long first = 0; first < a.tokens; first += kMost) {
     const long n = std::min(kMost, a.tokens - first);
-    norm_kernel<WAVES, CH><<<(unsigned)((n + kTokens - 1) / kTokens), kThreads, 0, stream>>>(a, first);
+    norm_kernel<WAVES, CH, WIDE, EARLY>
+        <<<(unsigned)((n + kTokens - 1) / kTokens), kThreads, 0, stream>>>(a, first);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) { return e; }
   }
   return hipSuccess;
+}
+
+template <int WAVES, int CH>
+hipError_t run(const NormArgs& a, hipStream_t stream)
+{
+  const bool narrow = !a.mod_wide && !a.weight_wide;
+  if (CH <= 2 && narrow) {
+    return a.wide ? run<WAVES, CH, true, CH <= 2>(a, stream) : run<WAVES, CH, false, CH <= 2>(a, stream);
+  }
+  return a.wide ? run<WAVES, CH, true, false>(a, stream) : run<WAVES, CH, false, false>(a, stream);
 }
 
 }  // namespace

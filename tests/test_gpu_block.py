@@ -206,6 +206,37 @@ def test_norm_coded(pkg, dev, tokens, width):
     assert torch.equal(xo, c["x_out"])
 
 
+def test_norm_and_rope_past_32_bits(pkg, dev):
+    """Tensors of more than 2^31 elements: their last rows against calls on those alone."""
+    say("norm and rope past 32 bits")
+    t, w = 140_000, 16384
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(2)
+    x = torch.randn((1, w), device="cuda", generator=gen).bfloat16().expand(t, w).contiguous()
+    x[-40:] = torch.randn((40, w), device="cuda", generator=gen).bfloat16()
+    out, q = torch.empty_like(x), pkg.MX4.empty(t, w)
+    pkg.block_norm(x, out)
+    pkg.block_norm(x, q)
+    want, coded, back = torch.empty_like(x[-40:]), pkg.MX4.empty(40, w), torch.empty_like(x)
+    pkg.block_norm(x[-40:], want)
+    pkg.block_norm(x[-40:], coded)
+    assert torch.equal(out[-40:], want) and torch.equal(out[t // 2], out[0])
+    values = torch.empty_like(want)
+    pkg.mx4_dequant(coded, values)
+    pkg.mx4_dequant(q, back)
+    assert torch.equal(back[-40:], values) and torch.equal(back[t // 2], back[0])
+    heads = x.view(t, 128, 128)
+    pos = torch.zeros((t, 2), device="cuda")
+    pos[-40:] = torch.randn((40, 2), device="cuda", generator=gen)
+    freqs = torch.rand((1, 64), device="cuda", generator=gen)
+    which = (torch.arange(64, device="cuda", dtype=torch.int32) % 2)[None].contiguous()
+    for side in (False, True):
+        pkg.rope(heads, None, pos, freqs, which, q_out=out.view(t, 128, 128), interleaved=side)
+        small = torch.empty((40, 128, 128), dtype=BF16, device="cuda")
+        pkg.rope(heads[-40:], None, pos[-40:].contiguous(), freqs, which, q_out=small, interleaved=side)
+        assert torch.equal(out[-40:].view(40, 128, 128), small) and torch.equal(out[5], x[5])
+
+
 # ---- rotations ------------------------------------------------------------------------------
 
 

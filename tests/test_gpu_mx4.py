@@ -179,32 +179,77 @@ def test_linear_is_coding_and_product(pkg, dev, m, k, n):
     assert torch.equal(y, two)
 
 
-def test_large_products(pkg, dev):
-    """Tiles of the largest kind, with rows, columns and K that end inside one, against torch in
-    64 bits on the GPU."""
-    for m, k, n, gelu in [(2100, 4096, 3000, True), (4097, 1056, 4104, False), (1500, 8192, 2049, False),
-                          (8160, 512, 4096, False)]:
-        say(f"mx4 large {m}x{k}->{n}")
-        gen = torch.Generator(device="cuda")
-        gen.manual_seed(m)
-        ops, vals = [], []
-        for rows in (m, n):
-            codes = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
-            scales = torch.randint(118, 122, (rows, k // 32), dtype=torch.uint8, device="cuda",
-                                   generator=gen)
-            ops.append(pkg.MX4.packed(codes, scales))
-            lut = torch.tensor(ref.VALUES, device="cuda")
-            v = lut[torch.stack([codes & 15, codes >> 4], 2).flatten(1).int()]
-            vals.append(v * (2.0 ** (scales.double() - 127)).repeat_interleave(32, 1))
-        y, flat = _guarded(m, n)
-        pkg.mx4_gemm(*ops, None, y, pkg.EPI_GELU_TANH if gelu else pkg.EPI_NONE)
-        want, mag = vals[0] @ vals[1].T, vals[0].abs() @ vals[1].abs().T
-        slack = 1.13 * (k + 1) * 2.0 ** -24 * mag
-        if gelu:
-            want = torch.nn.functional.gelu(want, approximate="tanh")
-        err = (y.double() - want).abs() - (1.01 * 2.0 ** -8 * want.abs() + slack)
-        assert float(err.max()) <= 0, float(err.max())
-        _untouched(flat, m * n)
+# Outputs of enough tiles for each kind of workgroup in turn, the largest last, with rows, columns
+# and K that end inside a tile, spans of K fewer than and around the stages', and more tiles than
+# workgroups that walk them.
+LARGE = [(20, 512, 3100, True), (100, 2080, 1800, False), (200, 544, 1300, True), (200, 32, 3100, False),
+         (200, 1056, 3100, True), (250, 4608, 3101, False), (130, 32, 6151, True), (140, 1568, 6150, False),
+         (130, 2592, 6152, False), (300, 64, 6200, False), (290, 1024, 6200, True), (300, 5120, 6199, False),
+         (2100, 4096, 3000, True), (4097, 1056, 4104, False), (1500, 8192, 2049, False),
+         (8160, 512, 4096, False), (8160, 96, 4095, True), (5000, 544, 4100, True)]
+
+
+def _on_gpu(pkg, rows, k, gen):
+    codes = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    scales = torch.randint(118, 122, (rows, k // 32), dtype=torch.uint8, device="cuda", generator=gen)
+    lut = torch.tensor(ref.VALUES, device="cuda")
+    v = lut[torch.stack([codes & 15, codes >> 4], 2).flatten(1).int()]
+    return pkg.MX4.packed(codes, scales), v * (2.0 ** (scales.double() - 127)).repeat_interleave(32, 1)
+
+
+@pytest.mark.parametrize("m,k,n,gelu", LARGE)
+def test_large_products(pkg, dev, m, k, n, gelu):
+    """Against torch in 64 bits on the GPU, with the bounds of ref.check_product."""
+    say(f"mx4 large {m}x{k}->{n}")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(m + k)
+    (x, xv), (w, wv) = _on_gpu(pkg, m, k, gen), _on_gpu(pkg, n, k, gen)
+    bias = torch.randn(n, device="cuda", generator=gen).to(torch.bfloat16 if gelu else torch.float32)
+    y, flat = _guarded(m, n)
+    pkg.mx4_gemm(x, w, bias, y, pkg.EPI_GELU_TANH if gelu else pkg.EPI_NONE)
+    want = xv @ wv.T + bias.double()
+    slack = 1.13 * (k + 1) * 2.0 ** -24 * (xv.abs() @ wv.abs().T + bias.double().abs())
+    if gelu:
+        want = torch.nn.functional.gelu(want, approximate="tanh")
+    err = (y.double() - want).abs() - (1.01 * 2.0 ** -8 * want.abs() + slack)
+    assert float(err.max()) <= 0, float(err.max())
+    _untouched(flat, m * n)
+    again = torch.empty_like(y)
+    pkg.mx4_gemm(x, w, bias, again, pkg.EPI_GELU_TANH if gelu else pkg.EPI_NONE)
+    assert torch.equal(again, y)
+
+
+def test_sizes_past_32_bits(pkg, dev):
+    """Codes beyond 1 GiB go out in two launches, and outputs and activations of more than 2^31
+    elements: rows of the whole call against calls on those rows alone."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    for m, k, n in [(17_000_003, 96, 8), (140_001, 64, 16384)]:
+        say(f"mx4 past 32 bits {m}x{k}->{n}")
+        w = pkg.MX4.packed(torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=gen),
+                           torch.randint(118, 122, (n, k // 32), dtype=torch.uint8, device="cuda", generator=gen))
+        x = torch.randn((m, k), device="cuda", generator=gen).bfloat16()
+        y = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+        pkg.linear_mx4(x, w, None, y)
+        edge = (1 << 30) // 64
+        for lo in (0, 130_900, min(edge - 200, m - 600), m - 600):
+            part = torch.empty((600, n), dtype=torch.bfloat16, device="cuda")
+            pkg.linear_mx4(x[lo:lo + 600], w, None, part)
+            # (another kernel may take the smaller call: sums in another order)
+            d = (part.float() - y[lo:lo + 600].float()).abs()
+            assert float((d - 2.0 ** -7 * part.float().abs()).max()) <= 1e-3
+        del x, y
+    m, k = 270_001, 8192
+    say("mx4 quantize past 32 bits")
+    x = torch.randn((1, k), device="cuda", generator=gen).bfloat16().expand(m, k).contiguous()
+    x[-5:] = torch.randn((5, k), device="cuda", generator=gen).bfloat16()
+    q, part, back = pkg.MX4.empty(m, k), pkg.MX4.empty(5, k), torch.empty_like(x)
+    pkg.mx4_quantize_rows(x, q)
+    pkg.mx4_dequant(q, back)
+    want = torch.empty((5, k), dtype=torch.bfloat16, device="cuda")
+    pkg.mx4_quantize_rows(x[-5:], part)
+    pkg.mx4_dequant(part, want)
+    assert torch.equal(back[-5:], want) and torch.equal(back[m // 2], back[0])
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 1024, 64), (20, 1024, 64), (300, 1024, 520), (2000, 1024, 4000)])

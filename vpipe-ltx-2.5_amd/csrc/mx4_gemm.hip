@@ -4,8 +4,6 @@
 #include "mx4.h"
 
 #include <algorithm>
-#include <cstdio>
-#include <cstdlib>
 #include <type_traits>
 #include <utility>
 
@@ -560,7 +558,6 @@ Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
            : groups(32, 32) >= kEnough              ? kPanel22x8
            : groups(32, 16) >= kEnough              ? kPanel21
                                                     : kPanel11;
-  if (const char* force = getenv("MX4_TILE")) { r.tile = atoi(force); }
   return r;
 }
 

@@ -179,6 +179,24 @@ def test_linear_is_coding_and_product(pkg, dev, m, k, n):
     assert torch.equal(y, two)
 
 
+@pytest.mark.parametrize("m", [1, 3, 4, 5, 15, 16])
+@pytest.mark.parametrize("k", [32, 96, 512, 1056, 4128])
+def test_few_rows_are_coded_alike(pkg, dev, m, k):
+    """Up to 16 rows are coded by the product's own waves: values of any bits, NaN and infinities
+    among them, give what the two calls give."""
+    say(f"linear_mx4 of any bits {m}x{k}")
+    rng = np.random.default_rng(m * k)
+    x = _strided(_bits(rng, (m, k), False))
+    w = ref.upload(pkg, *ref.random_operand(rng, 40, k, low=118))
+    q = pkg.MX4.empty(m, k)
+    pkg.mx4_quantize_rows(x, q)
+    one, two = (torch.empty((m, 40), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pkg.linear_mx4(x, w, None, one)
+    pkg.mx4_gemm(q, w, None, two)
+    assert torch.equal(torch.isnan(one), torch.isnan(two))
+    assert torch.equal(torch.nan_to_num(one, nan=7.0), torch.nan_to_num(two, nan=7.0))
+
+
 # Outputs of enough tiles for each kind of workgroup in turn, the largest last, with rows, columns
 # and K that end inside a tile, spans of K fewer than and around the stages', and more tiles than
 # workgroups that walk them.

@@ -84,16 +84,6 @@ __device__ __forceinline__ f32x4 mfma_mx4(i32x4 w, i32x4 x, f32x4 acc, int ws, i
                                                           kMfmaFp4, kMfmaFp4, J, ws, J, xs);
 }
 
-// 64 RB x 16 CB outputs of a workgroup of four waves, one below the other: a wave has RB x CB
-// blocks of 16 x 16. The weight's rows, which all four read, go through LDS; a wave's rows of x
-// are its own and go from memory straight to its registers, DEPTH slices of 128 values ahead: LDS
-// then carries 5 x 16 CB rows of K where both operands through LDS and 2 x 2 waves of the same
-// size carry 3 x (64 RB + 16 CB).
-//
-// A span is 512 values: STAGES LDS stages of CB x 4 tiles of codes and all the workgroup's scales
-// take turns, filled STAGES - 1 spans ahead by loads that go straight into LDS, one barrier a
-// span. Tiles lie in LDS as in memory, and a fragment's read is the tile's 1 KB in the order of
-// the lanes.
 // Tile id -> (tile_m, tile_n): ids are dealt to the eight XCDs in turn, so each XCD gets a run of
 // tiles, walked in groups of p.group rows of tiles. Few, so that a group's rows of x stay in the
 // XCD's cache from one round to the next and the stores run along the output's rows: 8160 x 4096
@@ -111,6 +101,16 @@ __device__ __forceinline__ void tile_at(int id, const GemmParams& p, int& tm, in
   tn = r / rows;
 }
 
+// 64 RB x 16 CB outputs of a workgroup of four waves, one below the other: a wave has RB x CB
+// blocks of 16 x 16. The weight's rows, which all four read, go through LDS; a wave's rows of x
+// are its own and go from memory straight to its registers, DEPTH slices of 128 values ahead: LDS
+// then carries 5 x 16 CB rows of K where both operands through LDS and 2 x 2 waves of the same
+// size carry 3 x (64 RB + 16 CB).
+//
+// A span is 512 values: STAGES LDS stages of CB x 4 tiles of codes and all the workgroup's scales
+// take turns, filled STAGES - 1 spans ahead by loads that go straight into LDS, one barrier a
+// span. Tiles lie in LDS as in memory, and a fragment's read is the tile's 1 KB in the order of
+// the lanes.
 template <int RB, int CB, int STAGES, int DEPTH>
 __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 {
@@ -250,10 +250,12 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 #pragma unroll
     for (int i = 0; i < RB; ++i) { load_x(t / 4, t % 4, t, i); }
   }
-  // The whole weight is asked for at the start, a word of each 64 bytes over all workgroups,
-  // so that later spans find it beside the memory: with each span's loads the first to see their
-  // lines, a span waits for the memory behind the stores (8160 x 4096 -> 16384 on a weight not
-  // read for a while: 360 us, so 275; on one just read 246 and 257). Up to half of what is kept.
+  // With more than a workgroup a CU the whole weight is asked for at the start, a word of each 64
+  // bytes over all workgroups, so that later spans find it beside the memory: with each span's
+  // loads the first to see their lines, a span waits for the memory behind the stores. On weights
+  // not read for a while, and just read: 8160 x 4096 -> 16384 275 us for 360, and 257 for 246;
+  // 4096 x 4096 -> 4096 39 for 43, 35 both; 2048 rows, one workgroup a CU, 25 for 24; tiles of
+  // 128 x 64, 300 x 16384 -> 4096, 34 for 31. Up to half of what is kept.
   auto touch = [&](__amdgpu_buffer_rsrc_t r, size_t bytes) {
     const uint32_t end = (uint32_t)min(bytes, (size_t)128 << 20);
     for (uint32_t at = (blockIdx.x * 4 + wave) * 4096; at < end; at += gridDim.x * 4 * 4096) {
@@ -261,8 +263,10 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
                                                0, 0, 0);
     }
   };
-  touch(wr, mx4_code_bytes(p.N, p.K));
-  touch(wsr, mx4_scale_bytes(p.N, p.K));
+  if (STAGES == 2 && tiles > 256) {
+    touch(wr, mx4_code_bytes(p.N, p.K));
+    touch(wsr, mx4_scale_bytes(p.N, p.K));
+  }
   // the first stages have landed, for what the count above does not see
   constexpr int kFirst = (DEPTH - 1) * RB;
   __builtin_amdgcn_s_waitcnt(0x0f70 | (kFirst < 15 ? kFirst : 15));
@@ -274,7 +278,6 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
       for (int j = 0; j < CB; ++j) { acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
     }
     // The tile's bias, a column or two a lane, which has landed long before the tile is done
-    // (asked for behind the products: 8160 x 4096 -> 16384 with bias and GELU 367 us)
     int tm, tn;
     tile_at(tile, p, tm, tn);
     const int n0 = tn * 16 * CB, row0 = (tm * 4 + wave) * 16 * RB;   // the wave's rows
@@ -553,8 +556,7 @@ Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
   Mx4Plan r;
   r.codes_ahead = bf16 && M > 16;
   // The largest tile that is half full and still gives three CUs of four a workgroup, wide ones
-  // first (us; M x K
-  // -> N, replayed in a graph):
+  // first (us; M x K -> N, replayed in a graph):
   //                         256 x 128  256 x 64  128 x 64  64 x 64  32 x 32  32 x 16 (8 waves)
   //   8160 x 4096 -> 4096        64        81        92      128      173
   //   1024 x 4096 -> 4096        17.4      12.8      13.7     18.9     26.3

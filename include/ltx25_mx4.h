@@ -58,8 +58,8 @@ int ltx25_mx4_quantize_rows(void* stream, const void* x, int x_dtype, int64_t x_
                             const ltx25_mx4* q);
 
 /* The values as bf16, out_stride elements from a row to the next (a multiple of 8,
- * at least K; out 16-byte aligned). Exact, but for values above bf16's largest
- * (infinite) and below its smallest (rounded). */
+ * at least K; out 16-byte aligned). Exact, but for values above bf16's largest, which
+ * are infinite. */
 int ltx25_mx4_dequant(void* stream, const ltx25_mx4* q, void* out, int64_t out_stride);
 
 /* From u8 codes [rows][K / 2] and scales [rows][K / 32], as checkpoints hold them, to
@@ -74,13 +74,15 @@ int ltx25_mx4_unpack(void* stream, const ltx25_mx4* q, void* codes, void* scales
  * workspace: at least ltx25_mx4_gemm_workspace(M, K, N) bytes. */
 int ltx25_mx4_gemm(void* stream, const ltx25_mx4* x, const ltx25_mx4* w, const void* bias,
                    int bias_dtype, void* y, int epilogue, void* workspace, size_t workspace_bytes);
-/* 0 where none is needed and for sizes that the call refuses. Not monotone in the sizes. */
+/* 0 where none is needed (every size, at present) and for sizes that the call refuses. */
 size_t ltx25_mx4_gemm_workspace(int M, int K, int N);
 
 /* The same with M rows of bf16 activations (x_stride elements from a row to the next,
  * a multiple of 8; x 16-byte aligned), which are coded as ltx25_mx4_quantize_rows
  * codes them on the way: the bits of the two calls.
- * workspace: at least ltx25_linear_mx4_workspace(M, K, N) bytes. */
+ * workspace: at least ltx25_linear_mx4_workspace(M, K, N) bytes, the coded rows' (0 for
+ * few rows, which are coded in the product's own kernel, and for sizes that the call
+ * refuses). */
 int ltx25_linear_mx4(void* stream, const void* x, int64_t x_stride, int M, const ltx25_mx4* w,
                      const void* bias, int bias_dtype, void* y, int epilogue, void* workspace,
                      size_t workspace_bytes);

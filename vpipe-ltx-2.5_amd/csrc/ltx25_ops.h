@@ -194,6 +194,16 @@ public:
   {
     note(ltx25_mx4_dequant(enc, &q, out, out_stride));
   }
+  // What a checkpoint holds, u8 codes [rows][K / 2] and scales [rows][K / 32], to q's order
+  // and back.
+  void mx4_pack(hipStream_t enc, const void* codes, const void* scales, const ltx25_mx4& q) const
+  {
+    note(ltx25_mx4_pack(enc, codes, scales, &q));
+  }
+  void mx4_unpack(hipStream_t enc, const ltx25_mx4& q, void* codes, void* scales) const
+  {
+    note(ltx25_mx4_unpack(enc, &q, codes, scales));
+  }
   void mx4_gemm(hipStream_t enc, const ltx25_mx4& x, const ltx25_mx4& w, const void* bias, void* y,
                 bool gelu, void* workspace, size_t workspace_bytes) const
   {

@@ -156,6 +156,19 @@ def test_norm_of_values_at_both_ends(pkg, dev, width, layer):
     assert bool(torch.isnan(out[5, -1])) or layer
 
 
+@pytest.mark.parametrize("layer", [False, True])
+@pytest.mark.parametrize("scale,eps", [(1e19, 3.2e38), (1e19, 1e38), (1e18, 3e37), (1e20, 1e38), (1.0, 1e38)])
+def test_norm_of_a_large_eps(pkg, dev, scale, eps, layer):
+    """It counts where the squares or their sum with it leave f32's range, too."""
+    say(f"block_norm eps {scale} {eps} {layer}")
+    x = _t(np.random.default_rng(3), (5, 1024), F32, scale)
+    out = torch.empty((5, 1024), dtype=BF16, device="cuda")
+    pkg.block_norm(x, out, layer=layer, eps=eps)
+    h, _, mag, _ = ref.block_norm(_f64(x), None, None, None, None, None, None, None, layer,
+                                  float(np.float32(eps)), 1.0)
+    _close(out, h, mag, BF16, "out")
+
+
 def test_norm_in_place(pkg, dev):
     """out in x (queries normed over all heads in the projection's output), and in y."""
     say("block_norm in place")

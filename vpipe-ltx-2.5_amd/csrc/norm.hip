@@ -124,10 +124,10 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
           s += in[i] ? d * d : 0.0f;
         }
       }
-      const float square = total(s) * over;
+      const float eps = far ? fmaxf(p.eps * 0x1p-80f * 0x1p-80f, 0x1p-126f) : p.eps;
+      const float square = total(s) * over + eps;
       if (far == 0 && !(square < INFINITY)) { continue; }
-      const float eps = far ? 0x1p-126f : p.eps;
-      const float rs = 1.0f / sqrtf(square + eps);
+      const float rs = 1.0f / sqrtf(square);
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
 #pragma unroll

@@ -29,8 +29,8 @@ def _rotation(pkg, **kw):
 
 
 def _run_norm(pkg, lib, n=None, coded=False, q=None, tokens=4, **kw):
-    a = dict(x=FAKE, y=FAKE, x_out=FAKE, post=FAKE, gate=FAKE, weight=FAKE, scale=FAKE, shift=FAKE,
-             rows=None, out=FAKE)
+    a = dict(x=FAKE, y=2 * FAKE, x_out=3 * FAKE, post=FAKE, gate=FAKE, weight=FAKE, scale=FAKE,
+             shift=FAKE, rows=None, out=4 * FAKE)
     a.update(kw)
     n = n if n is not None else _norm(pkg)
     args = [None, ctypes.byref(n), *(a[k] for k in ("x", "y", "x_out", "post", "gate", "weight",
@@ -175,6 +175,24 @@ def test_norm_pointers(pkg, lib):
     assert _run_norm(pkg, lib, tokens=-1) == pkg.E_INVAL
     assert _run_norm(pkg, lib, tokens=(1 << 27) + 1) == pkg.E_INVAL
     assert _run_norm(pkg, lib, tokens=0, x=None) == pkg.OK
+
+
+def test_norm_outputs_in_an_inputs_place(pkg, lib):
+    """Token for token, or not at all."""
+    x, y, xo = FAKE, 2 * FAKE, 3 * FAKE
+    alone = dict(y=None, x_out=None, post=None, gate=None)
+    for sizes, kw in [(dict(x_out_stride=128), dict(x_out=x)), (dict(out_stride=128), dict(out=y)),
+                      (dict(out_stride=128), dict(alone, out=x)),
+                      (dict(x_dtype=F32), dict(alone, out=x)), (dict(), dict(out=x)),
+                      (dict(), dict(out=xo)), (dict(), dict(x_out=y))]:
+        assert _run_norm(pkg, lib, _norm(pkg, **sizes), **kw) == pkg.E_INVAL, (sizes, kw)
+        assert " is " in pkg.last_error(), pkg.last_error()
+
+
+def test_rope_in_place_at_another_stride(pkg, lib):
+    for kw in (dict(qos=512), dict(kos=256, q=2 * FAKE), dict(qs=512, kos=128)):
+        assert _rope(pkg, lib, **kw) == pkg.E_INVAL
+        assert "stride" in pkg.last_error() and "_out is " in pkg.last_error()
 
 
 def test_norm_coded_output(pkg, lib):

@@ -33,6 +33,17 @@ int check_float_type(const char* name, int type)
   return LTX25_OK;
 }
 
+// An output in an input's place is there token for token, or one would be written over before
+// it is read. `alike`: of one type.
+int check_in_place(const char* name, const void* out, int64_t out_stride, const char* of,
+                   const void* in, int64_t in_stride, bool alike, int tokens)
+{
+  if (out == nullptr || out != in || (alike && (tokens <= 1 || out_stride == in_stride))) {
+    return LTX25_OK;
+  }
+  return set_error(LTX25_E_INVAL, "%s is %s but not of its type and stride", name, of);
+}
+
 // Everything but the output's own pointer and type. `out`: there is one.
 int check_norm(const ltx25_norm* n, const void* x, const void* y, const void* x_out,
                const void* after, const void* gate, const void* weight, const void* scale,
@@ -94,9 +105,12 @@ int check_norm(const ltx25_norm* n, const void* x, const void* y, const void* x_
       (rc = check_aligned("weight", weight, 16)) != LTX25_OK ||
       (rc = check_aligned("scale", scale, 16)) != LTX25_OK ||
       (rc = check_aligned("shift", shift, 16)) != LTX25_OK ||
-      (rc = check_aligned("rows", rows, 4)) != LTX25_OK) {
+      (rc = check_aligned("rows", rows, 4)) != LTX25_OK ||
+      (rc = check_in_place("x_out", x_out, n->x_out_stride, "x", x, n->x_stride, true, tokens)) !=
+          LTX25_OK) {
     return rc;
   }
+  if (x_out != nullptr && x_out == y) { return set_error(LTX25_E_INVAL, "x_out is y"); }
   a->x = x;
   a->y = (const uint16_t*)y;
   a->x_out = const_cast<void*>(x_out);
@@ -191,7 +205,16 @@ int ltx25_block_norm(void* stream, const ltx25_norm* n, const void* x, const voi
     return rc;
   }
   if (tokens == 0) { return LTX25_OK; }
-  if ((rc = check_aligned("out", out, 16)) != LTX25_OK) { return rc; }
+  if ((rc = check_aligned("out", out, 16)) != LTX25_OK ||
+      (rc = check_in_place("out", out, n->out_stride, "x", x, n->x_stride,
+                           n->x_dtype == LTX25_DT_BF16, tokens)) != LTX25_OK ||
+      (rc = check_in_place("out", out, n->out_stride, "y", y, n->y_stride, true, tokens)) !=
+          LTX25_OK) {
+    return rc;
+  }
+  if (out != nullptr && (out == x_out || (out == x && y != nullptr))) {
+    return set_error(LTX25_E_INVAL, "out is %s", out == x_out ? "x_out" : "x, and y is given");
+  }
   a.out = (uint16_t*)out;
   return run_norm(stream, a);
 }
@@ -261,7 +284,9 @@ int ltx25_rope(void* stream, const ltx25_rotation* r, const void* q, void* q_out
     }
     if (tokens == 0) { continue; }
     if ((rc = check_pointer(names[i][0], in[i], 16)) != LTX25_OK ||
-        (rc = check_pointer(names[i][1], out[i], 16)) != LTX25_OK) {
+        (rc = check_pointer(names[i][1], out[i], 16)) != LTX25_OK ||
+        (rc = check_in_place(names[i][1], out[i], strides[i][1], names[i][0], in[i], strides[i][0],
+                             true, tokens)) != LTX25_OK) {
       return rc;
     }
     a.in[i] = (const uint16_t*)in[i];

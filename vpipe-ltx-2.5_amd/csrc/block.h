@@ -23,21 +23,42 @@ struct Rotation {
 
 constexpr double kInv2Pi = 0.15915494309189533577;
 
-// A token's positions in turns (divided by 2 pi), in 64 bits. MANY: more than one axis.
-template <bool MANY>
-struct Turns {
-  double at[MANY ? kAxesMax : 1];
+// A token's positions as they lie in memory, the last one again past the axes; b, c and d with
+// MANY (more than one axis) alone: asked for before anything waits.
+struct Words {
+  uint32_t a = 0, b = 0, c = 0, d = 0;
 };
-
 template <bool MANY>
-__device__ __forceinline__ Turns<MANY> turns_of(const Rotation& r, long token)
+__device__ __forceinline__ Words words_of(const Rotation& r, long token)
 {
-  Turns<MANY> t;
-#pragma unroll
-  for (int a = 0; a < (MANY ? kAxesMax : 1); ++a) {
-    const long at = token * r.n_axes + min(a, r.n_axes - 1);
-    t.at[a] = (r.whole ? (double)((const int*)r.positions)[at]
-                       : (double)((const float*)r.positions)[at]) * kInv2Pi;
+  const uint32_t* const at = (const uint32_t*)r.positions + token * r.n_axes;
+  Words w;
+  w.a = at[0];
+  if constexpr (MANY) {
+    const int last = r.n_axes - 1;
+    w.b = at[min(1, last)];
+    w.c = at[min(2, last)];
+    w.d = at[min(3, last)];
+  }
+  return w;
+}
+
+// The same in turns (divided by 2 pi), in 64 bits
+struct Turns {
+  double a = 0.0, b = 0.0, c = 0.0, d = 0.0;
+};
+template <bool MANY>
+__device__ __forceinline__ Turns turns_of(const Rotation& r, const Words& w)
+{
+  auto turns = [&](uint32_t v) {
+    return (r.whole ? (double)(int)v : (double)__uint_as_float(v)) * kInv2Pi;
+  };
+  Turns t;
+  t.a = turns(w.a);
+  if constexpr (MANY) {
+    t.b = turns(w.b);
+    t.c = turns(w.c);
+    t.d = turns(w.d);
   }
   return t;
 }
@@ -46,14 +67,17 @@ __device__ __forceinline__ Turns<MANY> turns_of(const Rotation& r, long token)
 // bits: an angle of 2^20 radians has 2^-4 left of its own last bits in 32. What is left, at
 // most half a turn, goes to the hardware's sine and cosine, whose argument is in turns.
 template <bool MANY>
-__device__ __forceinline__ void sin_cos(const Turns<MANY>& t, double freq, int axis, float& sn,
+__device__ __forceinline__ void sin_cos(const Turns& t, double freq, int axis, float& sn,
                                         float& cs)
 {
-  double at = t.at[0];
+  double at = t.a;
   if constexpr (MANY) {
-    at = axis == 1 ? t.at[1] : at;
-    at = axis == 2 ? t.at[2] : at;
-    at = axis >= 3 ? t.at[3] : at;
+    // As values: of members the compiler selects the addresses and keeps them in LDS, or in
+    // scratch memory, and reads the workgroup's shape from the dispatch packet, which lies in the
+    // host's memory (128 tokens by three axes 13 us, so 3.1).
+    const double a = +t.a, b = +t.b, c = +t.c, d = +t.d;
+    const double low = axis == 1 ? +b : +a, high = axis == 2 ? +c : +d;
+    at = axis <= 1 ? +low : +high;
   }
   const double turns = at * freq;
   const float left = (float)(turns - rint(turns));
@@ -101,13 +125,13 @@ __device__ __forceinline__ float turned_b(float a, float b, float sn, float cs)
 
 // Eight channels of pairs side by side, turned by four frequencies
 template <bool MANY, int N>
-__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns<MANY>& t, const Pairs<N>& p)
+__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pairs<N>& p)
 {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float sn, cs;
-    sin_cos(t, p.freq[i], p.axis[i], sn, cs);
+    sin_cos<MANY>(t, p.freq[i], p.axis[i], sn, cs);
     const float a = low_f32(w[i]), b = high_f32(w[i]);
     w[i] = pack_bf16x2(turned_a(a, b, sn, cs), turned_b(a, b, sn, cs));
   }
@@ -116,15 +140,15 @@ __device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns<MANY>& t, cons
 
 // Eight pairs, their first channels in xa and their second in xb
 template <bool MANY>
-__device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns<MANY>& t,
+__device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns& t,
                                               const Pairs<8>& p)
 {
   uint32_t a[4] = {xa.x, xa.y, xa.z, xa.w}, b[4] = {xb.x, xb.y, xb.z, xb.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float s0, c0, s1, c1;
-    sin_cos(t, p.freq[2 * i], p.axis[2 * i], s0, c0);
-    sin_cos(t, p.freq[2 * i + 1], p.axis[2 * i + 1], s1, c1);
+    sin_cos<MANY>(t, p.freq[2 * i], p.axis[2 * i], s0, c0);
+    sin_cos<MANY>(t, p.freq[2 * i + 1], p.axis[2 * i + 1], s1, c1);
     const float a0 = low_f32(a[i]), a1 = high_f32(a[i]), b0 = low_f32(b[i]), b1 = high_f32(b[i]);
     a[i] = pack_bf16x2(turned_a(a0, b0, s0, c0), turned_a(a1, b1, s1, c1));
     b[i] = pack_bf16x2(turned_b(a0, b0, s0, c0), turned_b(a1, b1, s1, c1));
@@ -137,7 +161,7 @@ __device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns<
 // lane's own half of it, of its channels x and the other lane's.
 template <bool MANY>
 __device__ __forceinline__ uint4 rotate_half(uint4 x, uint4 other, bool second,
-                                             const Turns<MANY>& t, const Pairs<8>& p)
+                                             const Turns& t, const Pairs<8>& p)
 {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
   const uint32_t o[4] = {other.x, other.y, other.z, other.w};
@@ -147,7 +171,7 @@ __device__ __forceinline__ uint4 rotate_half(uint4 x, uint4 other, bool second,
     float sn[2], cs[2], v[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      sin_cos(t, p.freq[2 * i + h], p.axis[2 * i + h], sn[h], cs[h]);
+      sin_cos<MANY>(t, p.freq[2 * i + h], p.axis[2 * i + h], sn[h], cs[h]);
       const float mine = h ? high_f32(w[i]) : low_f32(w[i]);
       const float his = h ? high_f32(o[i]) : low_f32(o[i]);
       v[h] = fmaf(mine, cs[h], __uint_as_float(__float_as_uint(his * sn[h]) ^ sign));

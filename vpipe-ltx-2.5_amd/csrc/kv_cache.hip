@@ -248,8 +248,12 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
       pairs = pairs_of<kMany, 8>(rot, g, (piece - (second ? apart : 0)) * 8);
     }
   }
-  auto rotate = [&](uint4& w, int tok) {
-    const bool there = turning && tok >= sp.lo && tok < sp.hi;
+  const bool given = kMany || rot.positions != nullptr;
+  auto there = [&](int tok) { return turning && tok >= sp.lo && tok < sp.hi; };
+  auto words = [&](int tok) {
+    return given && there(tok) ? words_of<kMany>(rot, sp.first + tok) : Words();
+  };
+  auto rotate = [&](uint4& w, int tok, const Words& at) {
     const int from = (tid & 63) + (second ? -apart : apart);
     uint4 other = w;
     if (!rot.interleaved) {
@@ -258,26 +262,29 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
       other.z = __shfl((int)w.z, from);
       other.w = __shfl((int)w.w, from);
     }
-    if (there) {
-      Turns<kMany> t;
-      if (kMany || rot.positions != nullptr) {
-        t = turns_of<kMany>(rot, sp.first + tok);
+    if (there(tok)) {
+      Turns t;
+      if (given) {
+        t = turns_of<kMany>(rot, at);
       } else {
-        t.at[0] = (double)(sp.place + tok) * kInv2Pi;
+        t.a = (double)(sp.place + tok) * kInv2Pi;
       }
-      w = rot.interleaved ? rotate_side(w, t, pairs) : rotate_half(w, other, second, t, pairs);
+      w = rot.interleaved ? rotate_side<kMany>(w, t, pairs)
+                          : rotate_half<kMany>(w, other, second, t, pairs);
     }
   };
   uint4 held[kHeld][4];
+  Words at_words[ROPE ? kHeld : 1][4];
   uint32_t top = 0;
   bool odd = false;   // an infinity or a NaN among the lane's values
   if (few) {
     held[0][0] = make_uint4(0, 0, 0, 0);
+    if (ROPE && !values) { at_words[0][0] = words(sp.lo + tid / kPer); }
     if (tid < pieces) {
       held[0][0] = *(const uint4*)(x + (sp.first + sp.lo + tid / kPer) * stride + (tid % kPer) * 8);
     }
     if constexpr (ROPE) {
-      if (!values) { rotate(held[0][0], sp.lo + tid / kPer); }
+      if (!values) { rotate(held[0][0], sp.lo + tid / kPer, at_words[0][0]); }
     }
     const u16x2 tops = max_magnitudes(u16x2{0, 0}, held[0][0]);
     top = max((uint32_t)tops[0], (uint32_t)tops[1]);
@@ -295,6 +302,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
         if (at < pieces && tok >= sp.lo && tok < sp.hi) {
           held[i][j] = *(const uint4*)(x + (sp.first + tok) * stride + (at % kPer) * 8);
         }
+        if (ROPE && !values) { at_words[i][j] = words(tok); }
       }
     }
     if constexpr (ROPE) {
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
         for (int i = 0; i < kHeld; ++i) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            rotate(held[i][j], (quad0 + (tid + i * kThreads) / kPer) * 4 + j);
+            rotate(held[i][j], (quad0 + (tid + i * kThreads) / kPer) * 4 + j, at_words[i][j]);
           }
         }
       }

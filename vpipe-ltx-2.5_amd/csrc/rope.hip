@@ -2,7 +2,6 @@
 #include "block.h"
 
 #include <algorithm>
-#include <climits>
 
 namespace ltx25 {
 namespace {
@@ -19,79 +18,67 @@ struct RopeParams {
   long tokens;
   int chunks;        // a head's pieces of work
   int units;         // a token's
-  int blocks;        // workgroups over a token's
-  uint32_t by_chunks;   // ceil(2^32 / chunks)
+  uint32_t by_chunks, by_units;   // ceil(2^32 / them)
 };
 
 // n / d for n < 2^16, m = ceil(2^32 / d) (d = 1: m = 0)
 __device__ __forceinline__ uint32_t divide(uint32_t n, uint32_t m) { return m == 0 ? n : __umulhi(n, m); }
 
 // A thread turns eight channels (SIDE: pairs side by side) or twice eight, half of the rotated
-// channels apart, of TOKENS tokens one after another, for which it reads their frequencies and axes
-// once, and computes its pairs' sines itself.
+// channels apart, of one token, and computes its pairs' sines itself; threads are dealt out over
+// the tokens' pieces one after another, so that few heads fill waves too.
 //
-// Bound by memory.
-template <bool SIDE, bool MANY, int TOKENS>
+// Bound by memory: 8160 tokens of 32 + 32 heads of 128 by three axes, 267 MB, 50.5 us (5.3 TB/s),
+// 2048 of 32 + 8 by one 8.6. Two and four tokens a thread, which share their frequencies, are no
+// faster (50.0 and 52.4; 9.2 and 10.0).
+template <bool SIDE, bool MANY>
 __global__ void __launch_bounds__(kThreads) rope_kernel(RopeParams p, long first)
 {
-  const long group = first + (long)(blockIdx.x / (unsigned)p.blocks);
-  const uint32_t unit = blockIdx.x % (unsigned)p.blocks * kThreads + threadIdx.x;
-  if (unit >= (uint32_t)p.units) { return; }
+  // the workgroup's first token and unit, and the thread's
+  const uint32_t base = blockIdx.x * kThreads, units = (uint32_t)p.units;
+  const uint32_t token0 = base / units, at0 = base - token0 * units + threadIdx.x;
+  const uint32_t more = divide(at0, p.by_units);
+  const uint32_t unit = at0 - more * units;
+  const long token = first + token0 + more;
+  if (token >= p.tokens) { return; }
   int head = (int)divide(unit, p.by_chunks);
   const int chunk = (int)unit - head * p.chunks;
   const int which = head >= p.heads[0] ? 1 : 0;
   head -= which ? p.heads[0] : 0;
-  const uint16_t* const in = (which ? p.in[1] : p.in[0]) + head * p.dim;
-  uint16_t* const out = (which ? p.out[1] : p.out[0]) + head * p.dim;
-  const long in_stride = which ? p.in_stride[1] : p.in_stride[0];
-  const long out_stride = which ? p.out_stride[1] : p.out_stride[0];
   const bool turn = chunk * (SIDE ? 4 : 8) < p.r.pairs;
   // halves: chunks past the pairs' are those of the channels that are not rotated
-  const int at = SIDE || turn ? chunk * 8 : chunk * 8 + p.r.pairs;
-  const long token0 = group * TOKENS;
-  uint4 a[TOKENS], b[SIDE ? 1 : TOKENS];
-#pragma unroll
-  for (int t = 0; t < TOKENS; ++t) {
-    const long token = min(token0 + t, p.tokens - 1);
-    a[t] = *(const uint4*)(in + token * in_stride + at);
-    if constexpr (!SIDE) {
-      if (turn) { b[t] = *(const uint4*)(in + token * in_stride + at + p.r.pairs); }
-    }
-  }
+  const int at = head * p.dim + (SIDE || turn ? chunk * 8 : chunk * 8 + p.r.pairs);
+  const uint16_t* const in =
+      (which ? p.in[1] : p.in[0]) + token * (which ? p.in_stride[1] : p.in_stride[0]) + at;
+  uint16_t* const out =
+      (which ? p.out[1] : p.out[0]) + token * (which ? p.out_stride[1] : p.out_stride[0]) + at;
+  uint4 a = *(const uint4*)in, b;
   if (turn) {
+    if constexpr (!SIDE) { b = *(const uint4*)(in + p.r.pairs); }
+    const Words words = words_of<MANY>(p.r, token);
     const Pairs<SIDE ? 4 : 8> pairs = pairs_of<MANY, SIDE ? 4 : 8>(p.r, head, chunk * (SIDE ? 4 : 8));
-#pragma unroll
-    for (int t = 0; t < TOKENS; ++t) {
-      const Turns<MANY> turns = turns_of<MANY>(p.r, min(token0 + t, p.tokens - 1));
-      if constexpr (SIDE) {
-        a[t] = rotate_side<MANY>(a[t], turns, pairs);
-      } else {
-        rotate_halves<MANY>(a[t], b[t], turns, pairs);
-      }
+    const Turns turns = turns_of<MANY>(p.r, words);
+    if constexpr (SIDE) {
+      a = rotate_side<MANY>(a, turns, pairs);
+    } else {
+      rotate_halves<MANY>(a, b, turns, pairs);
+      *(uint4*)(out + p.r.pairs) = b;
     }
   }
-#pragma unroll
-  for (int t = 0; t < TOKENS; ++t) {
-    if (token0 + t >= p.tokens) { break; }
-    uint16_t* const to = out + (token0 + t) * out_stride + at;
-    *(uint4*)to = a[t];
-    if constexpr (!SIDE) {
-      if (turn) { *(uint4*)(to + p.r.pairs) = b[t]; }
-    }
-  }
+  *(uint4*)out = a;
 }
 
 uint32_t magic(int d) { return d <= 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / (unsigned)d); }
 
-template <bool SIDE, bool MANY, int TOKENS>
+template <bool SIDE, bool MANY>
 hipError_t run(const RopeParams& p, hipStream_t stream)
 {
   // a launch has fewer than 2^32 threads
-  const long groups = (p.tokens + TOKENS - 1) / TOKENS;
-  const long most = ((1L << 32) / kThreads - 1) / p.blocks;
-  for (long first = 0; first < groups; first += most) {
-    const long n = std::min(most, groups - first);
-    rope_kernel<SIDE, MANY, TOKENS><<<(unsigned)(n * p.blocks), kThreads, 0, stream>>>(p, first);
+  const long most = ((1L << 32) - 2 * kThreads) / p.units;
+  for (long first = 0; first < p.tokens; first += most) {
+    const long n = std::min(most, p.tokens - first);
+    const unsigned blocks = (unsigned)((n * p.units + kThreads - 1) / kThreads);
+    rope_kernel<SIDE, MANY><<<blocks, kThreads, 0, stream>>>(p, first);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) { return e; }
   }
@@ -115,16 +102,11 @@ hipError_t launch_rope(const RopeArgs& a, hipStream_t stream)
   p.tokens = a.tokens;
   p.chunks = a.r.interleaved ? a.head_dim / 8 : (a.head_dim - a.r.pairs) / 8;
   p.units = (a.heads[0] + a.heads[1]) * p.chunks;
-  p.blocks = (p.units + kThreads - 1) / kThreads;
   p.by_chunks = magic(p.chunks);
+  p.by_units = magic(p.units);
   const bool side = a.r.interleaved, many = a.r.n_axes > 1;
-  // Four tokens a thread where that leaves enough workgroups for the CUs
-  if ((long)a.tokens * p.blocks >= 8192) {
-    return side ? many ? run<true, true, 4>(p, stream) : run<true, false, 4>(p, stream)
-                : many ? run<false, true, 4>(p, stream) : run<false, false, 4>(p, stream);
-  }
-  return side ? many ? run<true, true, 1>(p, stream) : run<true, false, 1>(p, stream)
-              : many ? run<false, true, 1>(p, stream) : run<false, false, 1>(p, stream);
+  return side ? many ? run<true, true>(p, stream) : run<true, false>(p, stream)
+              : many ? run<false, true>(p, stream) : run<false, false>(p, stream);
 }
 
 }  // namespace ltx25

@@ -80,9 +80,9 @@ size_t ltx25_mx4_gemm_workspace(int M, int K, int N);
 /* The same with M rows of bf16 activations (x_stride elements from a row to the next,
  * a multiple of 8; x 16-byte aligned), which are coded as ltx25_mx4_quantize_rows
  * codes them on the way: the bits of the two calls.
- * workspace: at least ltx25_linear_mx4_workspace(M, K, N) bytes, the coded rows' (0 for
- * few rows, which are coded in the product's own kernel, and for sizes that the call
- * refuses). */
+ * workspace: at least ltx25_linear_mx4_workspace(M, K, N) bytes, the coded rows' (0 where
+ * up to 16 rows are coded in the product's own kernel, and for sizes that the call
+ * refuses); what the largest sizes of several calls need is enough for all. */
 int ltx25_linear_mx4(void* stream, const void* x, int64_t x_stride, int M, const ltx25_mx4* w,
                      const void* bias, int bias_dtype, void* y, int epilogue, void* workspace,
                      size_t workspace_bytes);

@@ -197,6 +197,28 @@ def test_few_rows_are_coded_alike(pkg, dev, m, k):
     assert torch.equal(torch.nan_to_num(one, nan=7.0), torch.nan_to_num(two, nan=7.0))
 
 
+@pytest.mark.parametrize("m,k,n,ahead", [(16, 4096, 4096, False), (17, 4096, 4096, True), (1, 4128, 4112, False),
+                                         (5, 4128, 4112, True), (16, 96, 8208, True), (9, 12320, 40, True),
+                                         (4, 12320, 40, False)])
+def test_few_rows_that_are_coded_ahead(pkg, dev, m, k, n, ahead):
+    """More coding than a launch costs goes into the workspace; the results are the two calls'."""
+    say(f"linear_mx4 coded ahead {m}x{k}->{n}")
+    need = pkg.linear_mx4_workspace(m, k, n)
+    assert (need > 0) == ahead and pkg.linear_mx4_workspace(m + 1, k, n) >= need
+    rng = np.random.default_rng(m * k)
+    x = _strided(_bits(rng, (m, k), False))
+    w = ref.upload(pkg, *ref.random_operand(rng, n, k, low=118))
+    q = pkg.MX4.empty(m, k)
+    pkg.mx4_quantize_rows(x, q)
+    one, two = (torch.empty((m, n), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ws = torch.full((need + 4096,), 0xAB, dtype=torch.uint8, device="cuda")
+    pkg.linear_mx4(x, w, None, one, workspace=ws[:need])
+    pkg.mx4_gemm(q, w, None, two)
+    assert bool((ws[need:] == 0xAB).all())
+    assert torch.equal(torch.isnan(one), torch.isnan(two))
+    assert torch.equal(torch.nan_to_num(one, nan=7.0), torch.nan_to_num(two, nan=7.0))
+
+
 # Outputs of enough tiles for each kind of workgroup in turn, the largest last, with rows, columns
 # and K that end inside a tile, spans of K fewer than and around the stages', and more tiles than
 # workgroups that walk them.

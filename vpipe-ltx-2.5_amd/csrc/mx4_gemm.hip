@@ -554,7 +554,11 @@ Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
     return (long)((M + rows - 1) / rows) * ((N + columns - 1) / columns);
   };
   Mx4Plan r;
-  r.codes_ahead = bf16 && M > 16;
+  // Rows that every workgroup of panels would code again cost 0.7 us for each time around the
+  // CUs, step of a wave's and four rows (1 x 15072 -> 15872, 16 of them: 37.5 us; 16 x 4096 ->
+  // 4096, 4: 6.8), a launch ahead 2.6 (26.1 + 2.6; 5.8 + 2.6).
+  const long coding = (groups(16, 16) + 255) / 256 * ((mx4_spans(K) + 7) / 8) * ((M + 3) / 4);
+  r.codes_ahead = bf16 && (M > 16 || coding > 4);
   // The largest tile that is half full and still gives three CUs of four a workgroup, wide ones
   // first (us; M x K -> N, replayed in a graph):
   //                         256 x 128  256 x 64  128 x 64  64 x 64  32 x 32  32 x 16 (8 waves)
@@ -566,8 +570,7 @@ Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
   //     64 x 4096 -> 4096                                      7.1      4.5      4.9
   //     32 x 4096 -> 4096                                      7.0      4.0      3.8
   //    128 x 16384 -> 64                                      19.1      6.7      5.6
-  // A panel of one block has the most workgroups (128 x 16384 -> 64: 4.6), and codes bf16
-  // activations itself.
+  // A panel of one block has the most workgroups (128 x 16384 -> 64: 4.6).
   constexpr long kEnough = 192;
   r.tile = M <= 16                                    ? kPanel11
            : M > 128 && groups(256, 128) >= kEnough ? kWide48

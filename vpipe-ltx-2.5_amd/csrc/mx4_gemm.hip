@@ -22,6 +22,7 @@ struct GemmParams {
   int M, N, K;
   int bias_type, epilogue;
   int tiles_m, tiles_n, group;
+  bool whole;   // rows of y lie in whole pieces of 64 bytes
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, size_t bytes)
@@ -32,24 +33,27 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, size_
 }
 
 // 2 W bf16 to columns n .. of a row of N, of which those past N are left alone. Rows of an
-// odd N begin anywhere: the store is one all the same.
+// odd N begin anywhere: the store is one all the same. `whole`: a wave's stores are whole
+// pieces of 64 aligned bytes, and pass the cache by (others go through it, which puts their
+// lines together: 5304 x 608 -> 11000 56 us, past it 118; 8160 x 512 -> 16376 122 and 261).
 template <int W>
 struct Words {
   uint32_t w[W];
 };
 template <int W>
-__device__ __forceinline__ void store_bf16(uint16_t* row, int n, int N, const Words<W>& v)
+__device__ __forceinline__ void store_bf16(uint16_t* row, int n, int N, bool whole,
+                                           const Words<W>& v)
 {
   typedef uint32_t words __attribute__((ext_vector_type(W), aligned(2)));
   if (n + 2 * W <= N) {
     words x;
 #pragma unroll
     for (int i = 0; i < W; ++i) { x[i] = v.w[i]; }
-    if (N % 8 == 0) {
+    if (whole) {
       __builtin_nontemporal_store(x, (words*)(row + n));
     } else {
-      // parts of lines, which the cache puts together. (The empty statement keeps the compiler
-      // from making one ordinary store of the two: 8160 x 4096 -> 16384 340 us for 267.)
+      // (The empty statement keeps the compiler from making one ordinary store of the two:
+      // 8160 x 4096 -> 16384 340 us for 267.)
       asm volatile("" ::: "memory");
       *(words*)(row + n) = x;
     }
@@ -333,7 +337,9 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
             if (i == 0) { __builtin_amdgcn_s_waitcnt(0x0f70); }
           }
           const int m = row0 + 16 * i + (lane & 15);
-          if (m < p.M) { store_bf16<4>(p.y + (size_t)m * p.N, n, p.N, {a[0], b[0], a[1], b[1]}); }
+          if (m < p.M) {
+            store_bf16<4>(p.y + (size_t)m * p.N, n, p.N, p.whole, {a[0], b[0], a[1], b[1]});
+          }
         }
       });
     };
@@ -523,7 +529,8 @@ mx4_panel_kernel(GemmParams p, const uint16_t* xb, long stride)
       v[r] += load_bias(p.bias, p.bias_type, min(n + r, p.N - 1));
       if (p.epilogue == kEpiGelu) { v[r] = gelu_tanh(v[r]); }
     }
-    store_bf16<2>(p.y + (size_t)m * p.N, n, p.N, {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+    store_bf16<2>(p.y + (size_t)m * p.N, n, p.N, false,
+                  {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
   }
 }
 
@@ -606,6 +613,7 @@ hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t st
     p.K = K;
     p.bias_type = g.bias_type;
     p.epilogue = g.epilogue;
+    p.whole = N % 32 == 0 && (uintptr_t)g.y % 64 == 0;
     hipError_t e = hipSuccess;
     switch (plan.tile) {
       case kWide48: e = run_wide<4, 8, 2, 4>(p, stream); break;

@@ -41,7 +41,8 @@ def _close(got, want, mag, kind, what):
     assert float(err.max()) <= 0, f"{what}: off by {float(err.max()):.3e}"
 
 
-WIDTHS = [8, 40, 504, 512, 520, 1024, 1032, 2048, 2056, 4096, 4104, 8192, 8200, 16384]
+WIDTHS = [8, 40, 64, 72, 128, 136, 256, 264, 504, 512, 520, 1024, 1032, 1536, 1544, 2048, 2056, 3080, 4096, 4104,
+          6144, 6152, 8192, 8200, 12288, 12296, 16384]
 FORMS = [  # kind of x, kind of the modulations, y, post, gate, weight, modulated, layer, alpha
     (BF16, BF16, True, False, True, False, True, False, 1.0),
     (F32, F32, True, True, True, True, True, True, 0.7),
@@ -124,7 +125,7 @@ def test_norm_rows_of_the_modulation(pkg, dev, tokens, rows):
 
 
 @pytest.mark.parametrize("layer", [False, True])
-@pytest.mark.parametrize("width", [32, 1024, 2048, 4096, 16384])
+@pytest.mark.parametrize("width", [32, 96, 160, 1024, 1280, 2048, 2400, 4096, 5120, 9600, 16384])
 def test_norm_of_values_at_both_ends(pkg, dev, width, layer):
     """Squares beyond f32's range and below it, constant rows, and values that are not finite, which
     stay in their rows."""
@@ -187,8 +188,8 @@ def test_norm_in_place(pkg, dev):
     assert torch.equal(y, want) and torch.equal(x, xo)
 
 
-@pytest.mark.parametrize("tokens,width", [(1, 32), (5, 544), (16, 512), (18, 1056), (33, 2048), (4, 4128),
-                                          (17, 8224), (2, 16384)])
+@pytest.mark.parametrize("tokens,width", [(1, 32), (5, 544), (16, 512), (18, 1056), (33, 2048), (40, 64),
+                                          (9, 2592), (4, 4128), (17, 8224), (2, 16384), (3, 12800)])
 def test_norm_coded(pkg, dev, tokens, width):
     """4-bit output: the codes of values within f32's roundings of the 64-bit ones, so that where no
     tie or largest value is that near they are the same."""

@@ -55,18 +55,23 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8])
 }
 
 // WAVES waves hold a token, CH chunks of eight values a lane: lane l of wave w has the
-// chunks w * 64 + l + i * 64 * WAVES. A single wave's tokens share a workgroup of four.
+// chunks w * 64 + l + i * 64 * WAVES. A single wave's tokens share a workgroup of four, and
+// of narrow ones, of LANES lanes each (a head's channels), several share a wave.
 //
 // Sums in f32, the mean taken off before the squares are added; where a sum leaves f32's
 // range the values are taken 2^-80 times as large, which leaves every square that counts
 // inside it.
 //
 // WIDE: x is f32. EARLY: what multiplies and shifts is bf16 and asked for before the sums.
-template <int WAVES, int CH, bool WIDE, bool EARLY>
+//
+// Bound by memory: 8192 tokens of 4096 with a branch, gate and modulation 48.9 us (268 MB, 5.5
+// TB/s), post-normed and with means 56.6, 4-bit output 47.8 (219 MB).
+template <int WAVES, int CH, bool WIDE, bool EARLY, int LANES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(NormArgs p, long first)
 {
+  static_assert(LANES == 64 || WAVES == 1, "lanes of a wave");
   __shared__ float part[4][WAVES];
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & (LANES - 1);
   const int wave = WAVES == 1 ? 0 : (int)(threadIdx.x >> 6);
   // Coded rows lie four to 64 bytes and 16 to a tile: 16 tokens go to workgroups of one XCD
   // (every eighth), whose cache puts their lines together.
@@ -74,12 +79,12 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
   if (p.q.codes != nullptr && (place | 127) < (long)gridDim.x) {
     place = (place & ~127L) + (place & 7) * 16 + ((place >> 3) & 15);
   }
-  const long token = first + (WAVES == 1 ? place * 4 + (threadIdx.x >> 6) : place);
+  const long token = first + (WAVES == 1 ? place * (256 / LANES) + threadIdx.x / LANES : place);
   if (token >= p.tokens) { return; }
   int turn = 0;
   auto total = [&](float v) {
 #pragma unroll
-    for (int i = 1; i < 64; i *= 2) { v += __shfl_xor(v, i); }
+    for (int i = 1; i < LANES; i *= 2) { v += __shfl_xor(v, i); }
     if constexpr (WAVES > 1) {
       // the next sum's slots are others: its writers do not meet this one's readers
       float* const at = part[turn & 3];
@@ -253,15 +258,15 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
   }
 }
 
-template <int WAVES, int CH, bool WIDE, bool EARLY>
+template <int WAVES, int CH, bool WIDE, bool EARLY, int LANES>
 hipError_t run(const NormArgs& a, hipStream_t stream)
 {
   // a launch has fewer than 2^32 threads; whole runs of 128 workgroups
-  constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES, kTokens = WAVES == 1 ? 4 : 1;
+  constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES, kTokens = WAVES == 1 ? 256 / LANES : 1;
   constexpr long kMost = (((1L << 32) / kThreads - 1) & ~127L) * kTokens;
   for (long first = 0; first < a.tokens; first += kMost) {
     const long n = std::min(kMost, a.tokens - first);
-    norm_kernel<WAVES, CH, WIDE, EARLY>
+    norm_kernel<WAVES, CH, WIDE, EARLY, LANES>
         <<<(unsigned)((n + kTokens - 1) / kTokens), kThreads, 0, stream>>>(a, first);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) { return e; }
@@ -269,27 +274,43 @@ hipError_t run(const NormArgs& a, hipStream_t stream)
   return hipSuccess;
 }
 
-template <int WAVES, int CH>
+template <int WAVES, int CH, int LANES = 64>
 hipError_t run(const NormArgs& a, hipStream_t stream)
 {
-  const bool narrow = !a.mod_wide && !a.weight_wide;
-  if (CH <= 2 && narrow) {
-    return a.wide ? run<WAVES, CH, true, CH <= 2>(a, stream) : run<WAVES, CH, false, CH <= 2>(a, stream);
+  constexpr bool kEarly = WAVES * CH < 24;   // wider ones: 10240 72.8 us, late 57.9
+  if (kEarly && !a.mod_wide && !a.weight_wide) {
+    return a.wide ? run<WAVES, CH, true, kEarly, LANES>(a, stream)
+                  : run<WAVES, CH, false, kEarly, LANES>(a, stream);
   }
-  return a.wide ? run<WAVES, CH, true, false>(a, stream) : run<WAVES, CH, false, false>(a, stream);
+  return a.wide ? run<WAVES, CH, true, false, LANES>(a, stream)
+                : run<WAVES, CH, false, false, LANES>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_norm(const NormArgs& a, hipStream_t stream)
 {
+  const bool coded = a.q.codes != nullptr;
   // the padded blocks of a 4-bit output's last span are the lanes' past the width, too
-  const int width = a.q.codes != nullptr ? (a.width + 511) / 512 * 512 : a.width;
-  if (width <= 512) { return run<1, 1>(a, stream); }
-  if (width <= 1024) { return run<1, 2>(a, stream); }
-  if (width <= 2048) { return run<4, 1>(a, stream); }
-  if (width <= 4096) { return run<4, 2>(a, stream); }
-  if (width <= 8192) { return run<8, 2>(a, stream); }
+  const int width = coded ? (a.width + 511) / 512 * 512 : a.width;
+  // Few idle lanes, then few waves to wait for (with a branch, gate and modulation, in the form
+  // taken and in the next larger: 65536 tokens of 128 13 us for 27, 30840 of 1088 50 for 57, 13107
+  // of 2560 52 for 57, 6553 of 5120 52 for 60).
+  auto fits = [&](int waves, int chunks, int lanes = 64) {
+    return width <= 8 * lanes * waves * chunks;
+  };
+  if (fits(1, 1, 8)) { return run<1, 1, 8>(a, stream); }
+  if (fits(1, 1, 16)) { return run<1, 1, 16>(a, stream); }
+  if (fits(1, 1, 32)) { return run<1, 1, 32>(a, stream); }
+  if (fits(1, 1)) { return run<1, 1>(a, stream); }
+  if (fits(1, 2)) { return run<1, 2>(a, stream); }
+  if (fits(3, 1)) { return run<3, 1>(a, stream); }
+  if (fits(4, 1)) { return run<4, 1>(a, stream); }
+  if (fits(3, 2)) { return run<3, 2>(a, stream); }
+  if (fits(4, 2)) { return run<4, 2>(a, stream); }
+  if (fits(4, 3)) { return run<4, 3>(a, stream); }
+  if (fits(8, 2)) { return run<8, 2>(a, stream); }
+  if (fits(8, 3)) { return run<8, 3>(a, stream); }
   return run<8, 4>(a, stream);
 }
 

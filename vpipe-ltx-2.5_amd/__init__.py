@@ -291,18 +291,22 @@ def _ptr(t) -> int | None:
 
 _torch = None
 _raw_stream = None
+_device_now = None
 
 
 def _import_torch():
     """torch, imported on first use, and how its current stream's handle is read: the accessor
     that returns the handle alone where torch has it (0.07 us; torch.cuda.current_stream() builds
     a Stream object, 2.7 of the 8.2 us that a call took on the host)."""
-    global _torch, _raw_stream
+    global _torch, _raw_stream, _device_now
     import torch
 
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     _raw_stream = raw if raw is not None else (
         lambda device: torch.cuda.current_stream(device).cuda_stream)
+    # where a tensor already lies on a GPU, and torch's CUDA state is there with it (0.14 us less
+    # than torch.cuda.current_device())
+    _device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
     _torch = torch
     return torch
 
@@ -647,7 +651,11 @@ def _on_device(stream, names: str, tensors) -> int:
             if t is not None and not t.is_cuda:
                 _reachable(names, *tensors)
         return stream
-    device = _device_of(names, tensors)
+    try:
+        device = _device_now()
+    except Exception:
+        _reachable(names, *tensors)   # without a GPU: a tensor in host memory is what is wrong
+        raise
     for t in tensors:
         if t is not None and t.get_device() != device:
             _reachable(names, *tensors)
@@ -657,14 +665,6 @@ def _on_device(stream, names: str, tensors) -> int:
                                      f"cuda:{device}")
             break
     return _raw_stream(device)
-
-
-def _device_of(names: str, tensors) -> int:
-    try:
-        return _torch.cuda.current_device()
-    except Exception:
-        _reachable(names, *tensors)   # without a GPU: a tensor in host memory is what is wrong
-        raise
 
 
 def _float_type(name: str, t) -> int:
@@ -908,12 +908,12 @@ def block_norm(x, out, *, y=None, x_out=None, gate=None, post_weight=None, weigh
         if out is not None:
             os_ = _alike("out", out, shape, _torch.bfloat16)
         held, fn, to = out, load().ltx25_block_norm, _ptr(out)
-    at = _on_device(stream, "x out y x_out gate post_weight weight scale shift rows",
-                    (x, held, y, x_out, gate, post_weight, weight, scale, shift, rows))
+    tensors = (x, y, x_out, post_weight, gate, weight, scale, shift, rows, held)
+    at = _on_device(stream, "x y x_out post_weight gate weight scale shift rows out", tensors)
     n = NormC(width, 1 if layer else 0, eps, residual_scale, kind, mod, weights, mod_rows, xs, xos,
               ys, ms, os_)
-    check(fn(at, ctypes.byref(n), x.data_ptr(), _ptr(y), _ptr(x_out), _ptr(post_weight), _ptr(gate),
-             _ptr(weight), _ptr(scale), _ptr(shift), _ptr(rows), to, tokens))
+    check(fn(at, ctypes.byref(n), *[t if t is None else t.data_ptr() for t in tensors[:9]], to,
+             tokens))
 
 
 def _rotation(head_dim: int, freqs, axes, positions, tokens: int, interleaved: bool) -> RotationC:

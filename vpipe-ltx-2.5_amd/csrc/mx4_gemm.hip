@@ -111,6 +111,10 @@ __device__ __forceinline__ void tile_at(int id, const GemmParams& p, int& tm, in
 // then carries 5 x 16 CB rows of K where both operands through LDS and 2 x 2 waves of the same
 // size carry 3 x (64 RB + 16 CB).
 //
+// 8160 x 4096 -> 16384 in 250 to 265 us, 4.1 to 4.4 PFLOP/s: address units are busy in 84% of the
+// cycles, matrix cores in 59, LDS in 18, at the clock that power leaves (1.76 GHz; on zeros 2.2
+// and as many cycles). The instructions alone reach 7.2 PFLOP/s on random operands.
+//
 // A span is 512 values: STAGES LDS stages of CB x 4 tiles of codes and all the workgroup's scales
 // take turns, filled STAGES - 1 spans ahead by loads that go straight into LDS, one barrier a
 // span. Tiles lie in LDS as in memory, and a fragment's read is the tile's 1 KB in the order of
@@ -373,7 +377,8 @@ hipError_t run_wide(GemmParams& p, hipStream_t stream)
 // operands go from memory straight to registers, a tile's 1 KB an instruction, with four slices
 // in flight (the next span's slice is asked for when this span's has been multiplied), no
 // barrier before the waves' sums meet in LDS. For outputs of few tiles, where a workgroup that
-// walks all of K is a chain of its loads' latencies.
+// walks all of K is a chain of its loads' latencies. 1 x 4096 -> 4096 5.0 us, latency; 16 x 15072
+// -> 15872, 127 MB, 27.9 us, memory.
 //
 // CODED false: bf16 activations, up to 16 rows. A wave codes what it multiplies: four lanes
 // have a block and find its largest value, and the codes change to the matrix instruction's

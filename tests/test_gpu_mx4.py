@@ -225,6 +225,7 @@ def test_few_rows_that_are_coded_ahead(pkg, dev, m, k, n, ahead):
 LARGE = [(20, 512, 3100, True), (100, 2080, 1800, False), (200, 544, 1300, True), (200, 32, 3100, False),
          (200, 1056, 3100, True), (250, 4608, 3101, False), (130, 32, 6151, True), (140, 1568, 6150, False),
          (130, 2592, 6152, False), (300, 64, 6200, False), (290, 1024, 6200, True), (300, 5120, 6199, False),
+         (1010, 1056, 6100, True), (600, 544, 12201, False), (2040, 32, 6104, True), (2810, 1568, 12792, True),
          (2100, 4096, 3000, True), (4097, 1056, 4104, False), (1500, 8192, 2049, False),
          (8160, 512, 4096, False), (8160, 96, 4095, True), (5000, 544, 4100, True)]
 

@@ -125,11 +125,13 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   static_assert(DEPTH == 4 || (DEPTH == 8 && STAGES > 2), "slices of x in flight: a span's or two");
   constexpr int kCodes = 4 * CB * kMx4CodeTile;
   constexpr int kScaleTiles = 4 * RB + CB, kScaleLoads = (kScaleTiles + 15) / 16;
-  constexpr int kStage = kCodes + kScaleTiles * kMx4Tile;
+  constexpr int kScaleRoom = (kScaleTiles + 3) / 4 * 4;   // four tiles a load
+  constexpr int kStage = kCodes + kScaleRoom * kMx4Tile;
   // behind the stages: where loads of no tile go, and a tile's bias, a copy a wave
   constexpr int kNowhere = STAGES * kStage, kBias = kNowhere + 4 * kMx4Tile;
-  constexpr int kLds = kBias + 4 * 64 * CB;
-  static_assert(kScaleTiles % 4 == 0 && kLds <= 80 * 1024, "two workgroups a CU");
+  constexpr int kBiases = (CB + 3) / 4;   // of 64 columns
+  constexpr int kLds = kBias + 4 * 256 * kBiases;
+  static_assert(kLds <= 80 * 1024, "two workgroups a CU");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -200,10 +202,11 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   // LDS at its start and a slice's of x behind the slice: 2.5 us a span of one workgroup a CU;
   // without those of x 1.9, without those to LDS 2.1): the k-th load to LDS at fragment 2 k,
   // and slice J - 1's registers are filled anew during slice J.
-  static_assert(2 * (kW - 1) < 4 * CB && CB % RB == 0, "a span has room for its loads");
-  constexpr int kXEvery = CB / RB;
-  // loads of x behind the last one to LDS
-  constexpr int kXBehind = (4 * CB - 1 - 2 * (kW - 1)) / kXEvery;
+  static_assert(2 * (kW - 1) < 4 * CB && CB >= RB, "a span has room for its loads");
+  // loads of x before the slice's fragment j, and those of a span behind its last one to LDS
+  constexpr auto x_before = [](int j) { return j * RB / CB; };
+  constexpr int kLast = 2 * (kW - 1);
+  constexpr int kXBehind = 4 * RB - (kLast / CB * RB + x_before(kLast % CB));
   f32x4 acc[RB][CB];
   int stage = 0;   // of the span
   auto step = [&](int span, auto parity) {
@@ -239,9 +242,9 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
       }
       // Unconditionally, so that the number of loads behind others is known.
       if constexpr (f % 2 == 0 && f / 2 < kW) { load_w(span + STAGES - 1, next, f / 2); }
-      if constexpr (j % kXEvery == kXEvery - 1) {
+      if constexpr (x_before(j + 1) > x_before(j)) {
         constexpr int kBuf = J > 0 ? B + J - 1 : DEPTH == 8 ? 7 - B : 3;
-        load_x(span + DEPTH / 4 - (J == 0 ? 1 : 0), (J + 3) % 4, kBuf, j / kXEvery);
+        load_x(span + DEPTH / 4 - (J == 0 ? 1 : 0), (J + 3) % 4, kBuf, x_before(j));
       }
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -289,9 +292,9 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
     int tm, tn;
     tile_at(tile, p, tm, tn);
     const int n0 = tn * 16 * CB, row0 = (tm * 4 + wave) * 16 * RB;   // the wave's rows
-    float bias[CB / 4];
+    float bias[kBiases];
 #pragma unroll
-    for (int i = 0; i < CB / 4; ++i) {
+    for (int i = 0; i < kBiases; ++i) {
       bias[i] = load_bias(p.bias, p.bias_type, min(n0 + 64 * i + lane, p.N - 1));
     }
     if constexpr (DEPTH == 8) {
@@ -309,9 +312,9 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
 
     // Block (i, j), lane l, register r: row 16 i + l % 16, column 16 j + 4 (l / 16) + r. The
     // loads of x that are in flight, the next tile's, have landed before anything is stored.
-    float* const biases = (float*)(lds + kBias) + wave * 16 * CB;
+    float* const biases = (float*)(lds + kBias) + wave * 64 * kBiases;
 #pragma unroll
-    for (int i = 0; i < CB / 4; ++i) { biases[64 * i + lane] = bias[i]; }
+    for (int i = 0; i < kBiases; ++i) { biases[64 * i + lane] = bias[i]; }
     // Two blocks side by side: the lanes' rows of 16 are exchanged so that each lane has eight
     // columns of one of them, 16 bytes.
     auto store = [&](auto gelu) {
@@ -558,7 +561,7 @@ constexpr size_t kSlabBytes = (size_t)1 << 30;
 }  // namespace
 
 // Tiles of a wide workgroup, 64 RB x 16 CB, and of a panel, 16 RB x 16 CB
-enum Tile : int { kWide48, kWide44, kWide24, kWide14, kPanel22, kPanel22x8, kPanel21, kPanel11 };
+enum Tile : int { kWide48, kWide46, kWide44, kWide24, kWide14, kPanel22, kPanel22x8, kPanel21, kPanel11 };
 
 Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
 {
@@ -593,6 +596,15 @@ Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
            : groups(32, 32) >= kEnough              ? kPanel22x8
            : groups(32, 16) >= kEnough              ? kPanel21
                                                     : kPanel11;
+  // Columns of blocks that a CU multiplies, in tiles of 256 x 128 and of 256 x 96 (a CU has one tile
+  // of up to 256, two of more): the narrower ones read more of x for each, and are taken for four
+  // fifths or less. 1024 x 4096 -> 12288 35.6 us and 33.3, 640 33.1 and 28.8, 1024 x 2048 -> 6144
+  // 13.8 and 12.1; of as many columns, 8160 x 4096 -> 12288, 209 and 220.
+  auto columns = [&](int cb) {
+    const long tiles = groups(256, 16 * cb);
+    return tiles <= 256 ? cb : (tiles + 511) / 512 * 2 * cb;
+  };
+  if (r.tile == kWide48 && 5 * columns(6) <= 4 * columns(8)) { r.tile = kWide46; }
   return r;
 }
 
@@ -622,6 +634,7 @@ hipError_t launch_mx4_gemm(const Mx4Gemm& g, const Mx4Plan& plan, hipStream_t st
     hipError_t e = hipSuccess;
     switch (plan.tile) {
       case kWide48: e = run_wide<4, 8, 2, 4>(p, stream); break;
+      case kWide46: e = run_wide<4, 6, 2, 4>(p, stream); break;
       case kWide44: e = run_wide<4, 4, 3, 4>(p, stream); break;
       case kWide24: e = run_wide<2, 4, 4, 8>(p, stream); break;
       case kWide14: e = run_wide<1, 4, 4, 8>(p, stream); break;

@@ -44,21 +44,16 @@ __device__ __forceinline__ uint32_t mx4_scale(uint32_t top)
   const uint32_t e = top >> 23;
   return e == 255 ? 255u : (uint32_t)max((int)e - 2, 0);
 }
-// 2^-exponent of a finite block: within 2^-125 .. 2^127
-__device__ __forceinline__ float mx4_factor(uint32_t scale)
-{
-  return __uint_as_float((254u - min(scale, 253u)) << 23);
-}
-
-// Eight values times 2^-exponent to codes, the first in the low bits: to the nearest,
-// ties to the even code, beyond 6 to 6 (the conversion's own rule).
-__device__ __forceinline__ uint32_t mx4_codes(const float (&v)[8], float f)
+// Eight values over 2^exponent to codes, the first in the low bits: to the nearest, ties to the
+// even code, beyond 6 to 6 (the conversion's own rule). It divides by 2^exponent, of which its
+// scale operand holds the bits: the exponent byte is f32's own, 0 for 2^-127 too.
+__device__ __forceinline__ uint32_t mx4_codes(const float (&v)[8], float unit)
 {
   uint32_t r = 0;
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0] * f, v[1] * f, 1.0f, 0);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2] * f, v[3] * f, 1.0f, 1);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4] * f, v[5] * f, 1.0f, 2);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6] * f, v[7] * f, 1.0f, 3);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], unit, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], unit, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], unit, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], unit, 3);
   return r;
 }
 
@@ -78,11 +73,10 @@ __device__ __forceinline__ uint32_t mx4_code_quad(const float (&v)[8], uint32_t&
 #pragma unroll
   for (int i = 0; i < 8; ++i) { top = max(top, __float_as_uint(v[i]) & 0x7fffffffu); }
   scale = mx4_scale(quad_max(top));
-  return scale == 255u ? 0u : mx4_codes(v, mx4_factor(scale));
+  return scale == 255u ? 0u : mx4_codes(v, __uint_as_float(scale << 23));
 }
 
-// The same of bf16 values as they lie in memory. The conversion divides by 2^exponent, of
-// which its scale operand holds the bits: the exponent byte is f32's own, 0 for 2^-127 too.
+// The same of bf16 values as they lie in memory
 __device__ __forceinline__ uint32_t mx4_code_bf16_quad(uint4 raw, uint32_t& scale)
 {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));

@@ -62,11 +62,13 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8])
 // range the values are taken 2^-80 times as large, which leaves every square that counts
 // inside it.
 //
-// WIDE: x is f32. EARLY: what multiplies and shifts is bf16 and asked for before the sums.
+// WIDE: x is f32. EARLY: what multiplies and shifts is bf16 and asked for before the sums. LONE:
+// there is no y, whose registers let more tokens be in flight (8160 x 4096 into 4 bits 22 us and, as
+// with one, 25; 4096 x 12288 45 and 51).
 //
 // Bound by memory: 8192 tokens of 4096 with a branch, gate and modulation 48.9 us (268 MB, 5.5
 // TB/s), post-normed and with means 53.7, 4-bit output 47.4 (219 MB).
-template <int WAVES, int CH, bool WIDE, bool EARLY, int LANES>
+template <int WAVES, int CH, bool WIDE, bool EARLY, int LANES, bool LONE>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(NormArgs p, long first)
 {
   static_assert(LANES == 64 || WAVES == 1, "lanes of a wave");
@@ -182,10 +184,12 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
     for (int i = 0; i < CH; ++i) { to[i] = fetch8<kWide>(t, at + from[i]); }
   };
   fetch(rx, p.x, token * p.xs);
-  fetch(ry, p.y, token * p.ys);
-  if constexpr (EARLY) {
+  if constexpr (!LONE) { fetch(ry, p.y, token * p.ys); }
+  if constexpr (EARLY && !LONE) {
     fetch(after, p.after, 0);
     fetch(gate, p.gate, row);
+  }
+  if constexpr (EARLY) {
     fetch(weight, p.weight, 0);
     fetch(scale, p.scale, row);
     fetch(shift, p.shift, row);
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
     for (int k = 0; k < 8; ++k) { x[i][k] = 0.0f; }
     if (in[i]) { values8(rx[i], x[i]); }
   }
-  if (p.y != nullptr) {
+  if (!LONE && p.y != nullptr) {
     float y[CH][8];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -280,7 +284,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) norm_kernel(Nor
   }
 }
 
-template <int WAVES, int CH, bool WIDE, bool EARLY, int LANES>
+template <int WAVES, int CH, bool WIDE, bool EARLY, int LANES, bool LONE>
 hipError_t run(const NormArgs& a, hipStream_t stream)
 {
   // a launch has fewer than 2^32 threads; whole runs of 128 workgroups
@@ -288,7 +292,7 @@ hipError_t run(const NormArgs& a, hipStream_t stream)
   constexpr long kMost = (((1L << 32) / kThreads - 1) & ~127L) * kTokens;
   for (long first = 0; first < a.tokens; first += kMost) {
     const long n = std::min(kMost, a.tokens - first);
-    norm_kernel<WAVES, CH, WIDE, EARLY, LANES>
+    norm_kernel<WAVES, CH, WIDE, EARLY, LANES, LONE>
         <<<(unsigned)((n + kTokens - 1) / kTokens), kThreads, 0, stream>>>(a, first);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) { return e; }
@@ -299,13 +303,18 @@ hipError_t run(const NormArgs& a, hipStream_t stream)
 template <int WAVES, int CH, int LANES = 64>
 hipError_t run(const NormArgs& a, hipStream_t stream)
 {
-  constexpr bool kEarly = WAVES * CH < 24;   // wider ones: 10240 72.8 us, late 57.9
-  if (kEarly && !a.mod_wide && !a.weight_wide) {
-    return a.wide ? run<WAVES, CH, true, kEarly, LANES>(a, stream)
-                  : run<WAVES, CH, false, kEarly, LANES>(a, stream);
+  constexpr bool kEarly = WAVES * CH < 24;   // wider ones with a y: 10240 72.8 us, late 57.9
+  const bool narrow = !a.mod_wide && !a.weight_wide;
+  if (narrow && a.y == nullptr) {
+    return a.wide ? run<WAVES, CH, true, true, LANES, true>(a, stream)
+                  : run<WAVES, CH, false, true, LANES, true>(a, stream);
   }
-  return a.wide ? run<WAVES, CH, true, false, LANES>(a, stream)
-                : run<WAVES, CH, false, false, LANES>(a, stream);
+  if (narrow && kEarly) {
+    return a.wide ? run<WAVES, CH, true, kEarly, LANES, false>(a, stream)
+                  : run<WAVES, CH, false, kEarly, LANES, false>(a, stream);
+  }
+  return a.wide ? run<WAVES, CH, true, false, LANES, false>(a, stream)
+                : run<WAVES, CH, false, false, LANES, false>(a, stream);
 }
 
 }  // namespace

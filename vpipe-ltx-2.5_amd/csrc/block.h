@@ -157,28 +157,43 @@ __device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns&
   xb = make_uint4(b[0], b[1], b[2], b[3]);
 }
 
-// The same where one lane has the pairs' first channels and another their second: the
-// lane's own half of it, of its channels x and the other lane's.
+// The same where one lane has eight pairs' first channels and another, `from`, their second (or
+// the other way round, `second`): the first takes four of the pairs and the second the other
+// four (`p`, theirs), and each gives the other what is its. Every lane takes part; `there`, which
+// both agree on: x is turned.
 template <bool MANY>
-__device__ __forceinline__ uint4 rotate_half(uint4 x, uint4 other, bool second,
-                                             const Turns& t, const Pairs<8>& p)
+__device__ __forceinline__ uint4 rotate_half(uint4 x, int from, bool second, bool there,
+                                             const Turns& t, const Pairs<4>& p)
 {
-  uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  const uint32_t o[4] = {other.x, other.y, other.z, other.w};
-  const uint32_t sign = second ? 0u : 0x80000000u;
+  const uint32_t given[2] = {second ? x.x : x.z, second ? x.y : x.w};
+  const uint32_t kept[2] = {second ? x.z : x.x, second ? x.w : x.y};
+  uint32_t first_w[2], second_w[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float sn[2], cs[2], v[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      sin_cos<MANY>(t, p.freq[2 * i + h], p.axis[2 * i + h], sn[h], cs[h]);
-      const float mine = h ? high_f32(w[i]) : low_f32(w[i]);
-      const float his = h ? high_f32(o[i]) : low_f32(o[i]);
-      v[h] = fmaf(mine, cs[h], __uint_as_float(__float_as_uint(his * sn[h]) ^ sign));
-    }
-    w[i] = pack_bf16x2(v[0], v[1]);
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t got = (uint32_t)__shfl((int)given[i], from);
+    first_w[i] = second ? got : kept[i];
+    second_w[i] = second ? kept[i] : got;
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  if (there) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float s0, c0, s1, c1;
+      sin_cos<MANY>(t, p.freq[2 * i], p.axis[2 * i], s0, c0);
+      sin_cos<MANY>(t, p.freq[2 * i + 1], p.axis[2 * i + 1], s1, c1);
+      const float a0 = low_f32(first_w[i]), a1 = high_f32(first_w[i]);
+      const float b0 = low_f32(second_w[i]), b1 = high_f32(second_w[i]);
+      first_w[i] = pack_bf16x2(turned_a(a0, b0, s0, c0), turned_a(a1, b1, s1, c1));
+      second_w[i] = pack_bf16x2(turned_b(a0, b0, s0, c0), turned_b(a1, b1, s1, c1));
+    }
+  }
+  uint32_t mine[2], his[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    mine[i] = second ? second_w[i] : first_w[i];
+    his[i] = (uint32_t)__shfl((int)(second ? first_w[i] : second_w[i]), from);
+  }
+  return second ? make_uint4(his[0], his[1], mine[0], mine[1])
+                : make_uint4(mine[0], mine[1], his[0], his[1]);
 }
 
 // ---- launchers --------------------------------------------------------------

@@ -201,9 +201,11 @@ __device__ __forceinline__ uint2 quantize8(uint4 x, float s, float rs)
 // and written, 14.9 us (3.4 TB/s; a page's first code waits for all its values).
 //
 // ROPE: the keys are turned in registers as they arrive and rounded to bf16, and from there on
-// are the keys of a plain append. Pairs half of the rotated channels apart meet by an exchange
-// of 16-byte pieces between lanes of one token. 8192 tokens of 8 heads of 128 19 us (pairs side
-// by side 17, by three axes 22): every head's workgroup computes its tokens' sines.
+// are the keys of a plain append. Pairs half of the rotated channels apart meet by exchanges
+// between two lanes of one token, each of which turns half of their pairs (all of them, its own
+// channels alone: half a microsecond more). 8192 tokens of 8 heads of 128 17.4 us (pairs side by
+// side 15.9, by three axes 19.1; not turned 13.1): every head's workgroup computes its tokens'
+// sines.
 // ROPE 2: positions of several axes.
 template <int D, int ROPE = 0>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotation rot)
@@ -236,18 +238,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
   const int apart = ROPE && !rot.interleaved ? rot.pairs / 8 : 0;   // pieces between a pair's two
   const bool second = apart > 0 && piece >= apart;
   const bool turning = ROPE && piece * 8 < 2 * rot.pairs;
-  Pairs<8> pairs;
+  // four of the pairs: those of the piece's channels, or half of those that it shares
+  Pairs<4> pairs;
   if (ROPE && !values && turning) {
-    if (rot.interleaved) {
-      const Pairs<4> four = pairs_of<kMany, 4>(rot, g, piece * 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pairs.freq[i] = four.freq[i];
-        pairs.axis[i] = four.axis[i];
-      }
-    } else {
-      pairs = pairs_of<kMany, 8>(rot, g, (piece - (second ? apart : 0)) * 8);
-    }
+    const int first = rot.interleaved ? piece * 4 : (piece - (second ? apart : 0)) * 8 + second * 4;
+    pairs = pairs_of<kMany, 4>(rot, g, first);
   }
   const bool given = kMany || rot.positions != nullptr;
   auto there = [&](int tok) { return turning && tok >= sp.lo && tok < sp.hi; };
@@ -255,23 +250,20 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
     return given && there(tok) ? words_of<kMany>(rot, sp.first + tok) : Words();
   };
   auto rotate = [&](uint4& w, int tok, const Words& at) {
-    const int from = (tid & 63) + (second ? -apart : apart);
-    uint4 other = w;
-    if (!rot.interleaved) {
-      other.x = __shfl((int)w.x, from);
-      other.y = __shfl((int)w.y, from);
-      other.z = __shfl((int)w.z, from);
-      other.w = __shfl((int)w.w, from);
+    const bool on = there(tok);
+    Turns t;
+    if (given) {
+      t = turns_of<kMany>(rot, at);
+    } else {
+      t.a = (double)(uint32_t)(sp.place + tok) * kInv2Pi;   // below 2^31 (find_span)
     }
-    if (there(tok)) {
-      Turns t;
-      if (given) {
-        t = turns_of<kMany>(rot, at);
-      } else {
-        t.a = (double)(sp.place + tok) * kInv2Pi;
-      }
-      w = rot.interleaved ? rotate_side<kMany>(w, t, pairs)
-                          : rotate_half<kMany>(w, other, second, t, pairs);
+    if (!rot.interleaved) {
+      const int from = (tid & 63) + (second ? -apart : apart);
+      // (of a channel that is not turned the partner may be any lane)
+      const uint4 r = rotate_half<kMany>(w, from & 63, second, on, t, pairs);
+      if (turning) { w = r; }
+    } else if (on) {
+      w = rotate_side<kMany>(w, t, pairs);
     }
   };
   uint4 held[kHeld][4];

@@ -254,6 +254,29 @@ def test_norm_and_rope_past_32_bits(pkg, dev):
 # ---- rotations ------------------------------------------------------------------------------
 
 
+def test_rope_of_more_threads_than_a_launch_has(pkg, dev):
+    """In place, where a token that two launches turned would be turned twice."""
+    say("rope past 2^32 threads")
+    tokens, heads, dim = (1 << 27) - 5, 17, 16
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 73 GB")
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    block = torch.randn((4096, heads, dim), device="cuda", generator=gen).to(BF16)
+    q = torch.empty((1 << 27, heads, dim), dtype=BF16, device="cuda")
+    q.view(-1, 4096, heads, dim).copy_(block)
+    positions = torch.arange(1 << 27, dtype=torch.int32, device="cuda").view(-1, 1)
+    freqs = torch.rand((1, dim // 2), device="cuda", generator=gen)
+    pkg.rope(q[:tokens], None, positions[:tokens], freqs, interleaved=True)
+    edge = ((1 << 32) - 512) // (heads * dim // 8) // 4096 * 4096
+    for lo in (0, edge - 4096, edge, edge + 4096, (1 << 27) - 4096):
+        n = min(4096, tokens - lo)
+        want = block.clone()
+        pkg.rope(want[:n], None, positions[lo:lo + n], freqs, interleaved=True)
+        assert torch.equal(q[lo:lo + 4096], want), lo
+    del q
+    torch.cuda.empty_cache()
+
+
 def _rope_case(rng, tokens, heads, kv, dim, rot, axes, per_head, whole, far=1000):
     proj = _t(rng, (tokens, (heads + 2 * kv) * dim), BF16)
     q, k, _ = (p.unflatten(1, (-1, dim)) for p in

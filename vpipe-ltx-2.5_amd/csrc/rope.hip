@@ -15,7 +15,7 @@ struct RopeParams {
   long in_stride[2], out_stride[2];
   int heads[2];
   int dim;
-  long tokens;
+  long tokens;       // the launch's end
   int chunks;        // a head's pieces of work
   int units;         // a token's
   uint32_t by_chunks, by_units;   // ceil(2^32 / them)
@@ -76,9 +76,11 @@ hipError_t run(const RopeParams& p, hipStream_t stream)
   // a launch has fewer than 2^32 threads
   const long most = ((1L << 32) - 2 * kThreads) / p.units;
   for (long first = 0; first < p.tokens; first += most) {
-    const long n = std::min(most, p.tokens - first);
+    RopeParams part = p;   // a launch's last workgroup ends with its tokens, not with all
+    part.tokens = std::min(p.tokens, first + most);
+    const long n = part.tokens - first;
     const unsigned blocks = (unsigned)((n * p.units + kThreads - 1) / kThreads);
-    rope_kernel<SIDE, MANY><<<blocks, kThreads, 0, stream>>>(p, first);
+    rope_kernel<SIDE, MANY><<<blocks, kThreads, 0, stream>>>(part, first);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) { return e; }
   }

@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
   };
   auto place_of = [&](int tile) {
     int tm, tn;
-    tile_at(tile, p, tm, tn);
     const bool in = tile < tiles;
+    tile_at(in ? tile : 0, p, tm, tn);
     Place at;
     at.w = in ? (uint32_t)(tn * CB) * pitch + lane * 16 : kPast;
     at.x = in ? (uint32_t)((tm * 4 + wave) * RB) * pitch + lane * 16 : kPast;

@@ -290,10 +290,15 @@ hipError_t run(const NormArgs& a, hipStream_t stream)
   // a launch has fewer than 2^32 threads; whole runs of 128 workgroups
   constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES, kTokens = WAVES == 1 ? 256 / LANES : 1;
   constexpr long kMost = (((1L << 32) / kThreads - 1) & ~127L) * kTokens;
+  // LDS that nothing uses, for four workgroups a CU and no fifth: with a y and one sum a token more
+  // of them at once take the memory longer (8160 x 4096 48.8 us, 50.3 of five and 51.7 of three;
+  // post-normed with means, four sums, 55.2, 53.9 of five; other widths equal or slower)
+  const bool four = WAVES == 4 && CH == 2 && !LONE && a.after == nullptr && !a.layer;
+  const size_t spare = four ? 36 << 10 : 0;
   for (long first = 0; first < a.tokens; first += kMost) {
     const long n = std::min(kMost, a.tokens - first);
     norm_kernel<WAVES, CH, WIDE, EARLY, LANES, LONE>
-        <<<(unsigned)((n + kTokens - 1) / kTokens), kThreads, 0, stream>>>(a, first);
+        <<<(unsigned)((n + kTokens - 1) / kTokens), kThreads, spare, stream>>>(a, first);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) { return e; }
   }

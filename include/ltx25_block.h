@@ -95,8 +95,10 @@ int ltx25_block_norm_mx4(void* stream, const ltx25_norm* n, const void* x, const
  *   freq_heads  1, or the number of heads (of the queries and of the keys): a head's
  *             own frequencies
  *   positions [tokens][n_axes], LTX25_DT_F32 or LTX25_DT_I32 (pos_dtype)
- * Angles are formed and reduced in 64 bits, whatever their size; sines and cosines
- * are good to 2^-20. Negated frequencies turn back. */
+ * Whole turns are taken off the product in 64 bits before it is rounded: angles lose
+ * nothing that counts below 2^52 radians (every int32 position at a frequency up to 2^21;
+ * larger ones turn by no particular angle). Sines and cosines are good to 2^-20. Negated
+ * frequencies turn back. */
 typedef struct ltx25_rotation {
   int head_dim;
   int rot_dim;

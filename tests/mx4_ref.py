@@ -161,6 +161,36 @@ def rotate(x, positions, freqs, axes, interleaved):
     return out, mag
 
 
+def _inverse_turn(bits):
+    """floor(2^bits / (2 pi)), by Machin's formula in whole numbers."""
+    one = 1 << (bits + 64)
+
+    def arctan(x):   # of 1 / x
+        term = total = one // x
+        n = 1
+        while term:
+            n, term = n + 2, -term // (x * x)
+            total += term // n
+        return total
+
+    return (one << bits) // (2 * 4 * (4 * arctan(5) - arctan(239)))
+
+
+def reduced_angles(positions, freqs):
+    """Whole or float32 positions [T] times float32 freqs [P], exactly, less whole turns: float64
+    [T][P] within half a turn, for products far past what 64 bits hold."""
+    bits = 400
+    inv = _inverse_turn(bits)
+    out = np.empty((len(positions), len(freqs)))
+    for i, p in enumerate(positions):
+        for j, f in enumerate(freqs):
+            (a, b), (c, d) = float(p).as_integer_ratio(), float(f).as_integer_ratio()
+            left = (a * c * inv // (b * d)) % (1 << bits)
+            left -= (1 << bits) if left >> (bits - 1) else 0
+            out[i, j] = 2 * math.pi * (left / (1 << bits))
+    return out
+
+
 def check_rotated(got, want, mag, what=""):
     """One rounding to bf16; sines and cosines to 2^-20, and the products' own roundings."""
     got = got.float().cpu().numpy().astype(np.float64)

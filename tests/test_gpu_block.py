@@ -341,6 +341,48 @@ def test_rope_far_positions(pkg, dev):
         ref.check_rotated(q, want, mag, "far")
 
 
+@pytest.mark.parametrize("side", [False, True])
+@pytest.mark.parametrize("axes", [1, 3])
+@pytest.mark.parametrize("top,whole", [(1 << 20, True), (1 << 24, True), ((1 << 31) - 1, True),
+                                       (1 << 24, False), (1 << 36, False)])
+def test_rope_angles_past_64_bits(pkg, dev, top, whole, axes, side):
+    """Positions and frequencies whose product's own bits go past what 64 bits hold: the angles come
+    from whole numbers. A channel pair (1, 0) gives the cosine and the sine themselves, and f32
+    products and sums of it have no error; the check's 2^-20 is the sine's."""
+    say(f"rope angles {top} {whole} {axes} {side}")
+    rng = np.random.default_rng(top % 1000 + axes)
+    tokens, pairs = 160, 8
+    at = rng.integers(top // 2, top, tokens, endpoint=True) * rng.choice([-1, 1], tokens)
+    at = at.astype(np.int32 if whole else np.float32)
+    freqs = (15708.0 * np.exp(rng.uniform(-3, 0, (1, pairs)))).astype(np.float32)
+    freqs[0, 0], freqs[0, 1] = 1.0, np.float32(np.pi)   # (a whole position is near half a turn)
+    ang = ref.reduced_angles(at, freqs[0])
+    x = np.zeros((tokens, 1, 16))
+    first, second = (slice(0, 16, 2), slice(1, 16, 2)) if side else (slice(0, 8), slice(8, 16))
+    x[:, :, first] = 1.0
+    want = np.zeros_like(x)
+    want[:, 0, first], want[:, 0, second] = np.cos(ang), np.sin(ang)
+    pos = np.zeros((tokens, axes), at.dtype)
+    pos[:, axes - 1] = at
+    which = np.full((1, pairs), axes - 1, np.int32)
+    up = [torch.from_numpy(a).cuda() for a in (pos, freqs, which)]
+    q = torch.from_numpy(x).to(BF16).cuda()
+    pkg.rope(q, None, *up, interleaved=side)
+    ref.check_rotated(q, want, np.ones_like(x), "far angles")
+    if not whole:
+        return
+    # the append's keys are turned alike (heads of 64, of which 16 channels turn)
+    parts, table, k, v, (cu, st) = _append_case(pkg, rng, ([3], [tokens], 2, 64, 32))
+    plain, one = (pkg.KVCache(*(t.clone() for t in parts)) for _ in range(2))
+    turned = torch.empty_like(k.contiguous())
+    pkg.rope(None, k, *up, k_out=turned, interleaved=side)
+    pkg.kv_append(plain, table, turned, v, cu, st)
+    pkg.kv_append_rope(one, table, k, v, cu, st, up[1], up[2], up[0], interleaved=side)
+    mask = _defined(([3], [tokens], 2, 64, 32), table.cpu().numpy(), one.k.shape, "k")
+    assert torch.equal(one.k.cpu()[mask], plain.k.cpu()[mask])
+    assert torch.equal(one.k_scale, plain.k_scale)
+
+
 def test_rope_axes_out_of_range_and_absent(pkg, dev):
     say("rope axes")
     rng = np.random.default_rng(2)

@@ -21,7 +21,9 @@ struct Rotation {
   bool interleaved = false;
 };
 
-constexpr double kInv2Pi = 0.15915494309189533577;
+// 1 / (2 pi), and what 64 bits leave of it
+constexpr double kInv2Pi = 0x1.45f306dc9c883p-3;
+constexpr double kInv2PiRest = -0x1.6b01ec5417056p-57;
 
 // A token's positions as they lie in memory, the last one again past the axes; b, c and d with
 // MANY (more than one axis) alone: asked for before anything waits.
@@ -43,31 +45,41 @@ __device__ __forceinline__ Words words_of(const Rotation& r, long token)
   return w;
 }
 
-// The same in turns (divided by 2 pi), in 64 bits
-struct Turns {
+// The same as numbers, which 64 bits hold exactly
+struct Places {
   double a = 0.0, b = 0.0, c = 0.0, d = 0.0;
 };
 template <bool MANY>
-__device__ __forceinline__ Turns turns_of(const Rotation& r, const Words& w)
+__device__ __forceinline__ Places places_of(const Rotation& r, const Words& w)
 {
-  auto turns = [&](uint32_t v) {
-    return (r.whole ? (double)(int)v : (double)__uint_as_float(v)) * kInv2Pi;
-  };
-  Turns t;
-  t.a = turns(w.a);
+  auto number = [&](uint32_t v) { return r.whole ? (double)(int)v : (double)__uint_as_float(v); };
+  Places t;
+  t.a = number(w.a);
   if constexpr (MANY) {
-    t.b = turns(w.b);
-    t.c = turns(w.c);
-    t.d = turns(w.d);
+    t.b = number(w.b);
+    t.c = number(w.c);
+    t.d = number(w.d);
   }
   return t;
 }
 
-// The sine and cosine of one pair's angle. The product and the removal of whole turns in 64
-// bits: an angle of 2^20 radians has 2^-4 left of its own last bits in 32. What is left, at
-// most half a turn, goes to the hardware's sine and cosine, whose argument is in turns.
+// A pair's frequency in turns (divided by 2 pi): a number of 64 bits and what that leaves. One
+// alone is off by 2^-53 of the turns: 2^-18 radians at position 2^20 of a frequency of 15708.
+struct Freq {
+  double turns, rest;
+};
+__device__ __forceinline__ Freq freq_of(float f)
+{
+  const double freq = (double)f, turns = freq * kInv2Pi;
+  return {turns, fma(freq, kInv2PiRest, fma(freq, kInv2Pi, -turns))};
+}
+
+// The sine and cosine of one pair's angle. Whole turns are taken off the product of position and
+// frequency in 64 bits before it is rounded: what is left is good to 2^-50 turns while the angle is
+// below 2^52 radians. It goes to the hardware's sine and cosine, whose argument is in turns (off by
+// at most 2^-22.9).
 template <bool MANY>
-__device__ __forceinline__ void sin_cos(const Turns& t, double freq, int axis, float& sn,
+__device__ __forceinline__ void sin_cos(const Places& t, const Freq& freq, int axis, float& sn,
                                         float& cs)
 {
   double at = t.a;
@@ -79,8 +91,8 @@ __device__ __forceinline__ void sin_cos(const Turns& t, double freq, int axis, f
     const double low = axis == 1 ? +b : +a, high = axis == 2 ? +c : +d;
     at = axis <= 1 ? +low : +high;
   }
-  const double turns = at * freq;
-  const float left = (float)(turns - rint(turns));
+  const double whole = rint(at * freq.turns);
+  const float left = (float)fma(at, freq.rest, fma(at, freq.turns, -whole));
   sn = __builtin_amdgcn_sinf(left);
   cs = __builtin_amdgcn_cosf(left);
 }
@@ -88,7 +100,7 @@ __device__ __forceinline__ void sin_cos(const Turns& t, double freq, int axis, f
 // N consecutive pairs' frequencies and axes (N 4 or 8, the first a multiple of 4)
 template <int N>
 struct Pairs {
-  double freq[N];
+  Freq freq[N];
   int axis[N];
 };
 template <bool MANY, int N>
@@ -102,7 +114,7 @@ __device__ __forceinline__ Pairs<N> pairs_of(const Rotation& r, int head, int fi
     const i32x4 a = MANY && r.axes != nullptr ? *(const i32x4*)(r.axes + at + i) : i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      p.freq[i + k] = (double)f[k];
+      p.freq[i + k] = freq_of(f[k]);
       p.axis[i + k] = min(a[k], r.n_axes - 1);
     }
   }
@@ -125,7 +137,7 @@ __device__ __forceinline__ float turned_b(float a, float b, float sn, float cs)
 
 // Eight channels of pairs side by side, turned by four frequencies
 template <bool MANY, int N>
-__device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pairs<N>& p)
+__device__ __forceinline__ uint4 rotate_side(uint4 x, const Places& t, const Pairs<N>& p)
 {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -140,7 +152,7 @@ __device__ __forceinline__ uint4 rotate_side(uint4 x, const Turns& t, const Pair
 
 // Eight pairs, their first channels in xa and their second in xb
 template <bool MANY>
-__device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns& t,
+__device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Places& t,
                                               const Pairs<8>& p)
 {
   uint32_t a[4] = {xa.x, xa.y, xa.z, xa.w}, b[4] = {xb.x, xb.y, xb.z, xb.w};
@@ -163,7 +175,7 @@ __device__ __forceinline__ void rotate_halves(uint4& xa, uint4& xb, const Turns&
 // both agree on: x is turned.
 template <bool MANY>
 __device__ __forceinline__ uint4 rotate_half(uint4 x, int from, bool second, bool there,
-                                             const Turns& t, const Pairs<4>& p)
+                                             const Places& t, const Pairs<4>& p)
 {
   const uint32_t given[2] = {second ? x.x : x.z, second ? x.y : x.w};
   const uint32_t kept[2] = {second ? x.z : x.x, second ? x.w : x.y};

@@ -251,11 +251,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotat
   };
   auto rotate = [&](uint4& w, int tok, const Words& at) {
     const bool on = there(tok);
-    Turns t;
+    Places t;
     if (given) {
-      t = turns_of<kMany>(rot, at);
+      t = places_of<kMany>(rot, at);
     } else {
-      t.a = (double)(uint32_t)(sp.place + tok) * kInv2Pi;   // below 2^31 (find_span)
+      t.a = (double)(uint32_t)(sp.place + tok);   // below 2^31 (find_span)
     }
     if (!rot.interleaved) {
       const int from = (tid & 63) + (second ? -apart : apart);

@@ -57,11 +57,11 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(RopeParams p, long first
     if constexpr (!SIDE) { b = *(const uint4*)(in + p.r.pairs); }
     const Words words = words_of<MANY>(p.r, token);
     const Pairs<SIDE ? 4 : 8> pairs = pairs_of<MANY, SIDE ? 4 : 8>(p.r, head, chunk * (SIDE ? 4 : 8));
-    const Turns turns = turns_of<MANY>(p.r, words);
+    const Places places = places_of<MANY>(p.r, words);
     if constexpr (SIDE) {
-      a = rotate_side<MANY>(a, turns, pairs);
+      a = rotate_side<MANY>(a, places, pairs);
     } else {
-      rotate_halves<MANY>(a, b, turns, pairs);
+      rotate_halves<MANY>(a, b, places, pairs);
       *(uint4*)(out + p.r.pairs) = b;
     }
   }

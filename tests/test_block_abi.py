@@ -372,3 +372,23 @@ def test_a_stream_of_the_callers_needs_its_workspace(pkg):
     w, x, y = _coded(pkg, 8), _gpu(40, 64), _gpu(40, 8)
     with pytest.raises(ValueError, match="workspace"):
         pkg.linear_mx4(x, w, None, y, stream=1)
+
+
+def test_a_stream_of_the_callers_needs_its_results(pkg):
+    """What packed() and unpacked() would allocate belongs to torch's current stream: work queued there
+    may still read memory that a kernel on another stream then writes."""
+    codes, scales = _gpu(4, 32, dtype=torch.uint8), _gpu(4, 2, dtype=torch.uint8)
+    q = _coded(pkg)
+    for call in (lambda: pkg.MX4.packed(codes, scales, stream=1), lambda: q.unpacked(stream=1),
+                 lambda: q.unpacked(stream=1, codes=codes), lambda: q.unpacked(1, scales=scales)):
+        with pytest.raises(ValueError, match="the caller's too"):
+            call()
+    for call in (lambda: pkg.MX4.packed(codes, scales, 1, _coded(pkg, 5)),
+                 lambda: pkg.MX4.packed(codes, scales, 1, _coded(pkg, 4, 96)),
+                 lambda: pkg.MX4.packed(codes, scales, 1, _coded(pkg, host=True)),
+                 lambda: q.unpacked(1, codes, codes), lambda: q.unpacked(1, scales, scales),
+                 lambda: q.unpacked(1, codes, scales.as_subclass(torch.Tensor)),
+                 lambda: q.unpacked(1, codes.as_subclass(torch.Tensor), scales)):
+        with pytest.raises((TypeError, ValueError)) as e:
+            call()
+        assert "too" not in str(e.value)

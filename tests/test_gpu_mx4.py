@@ -379,3 +379,19 @@ def test_captured_on_a_stream_and_repeated(pkg, dev, m, k, n):
             pkg.linear_mx4(a, w, bias, o)
     side.synchronize()
     assert all(torch.equal(o, t) for o, t in zip(outs, want))
+
+
+def test_orders_on_a_stream_of_the_callers(pkg, dev):
+    """Packing and unpacking into the caller's tensors on its stream."""
+    say("mx4 orders on a stream")
+    rng = np.random.default_rng(11)
+    codes, scales = ref.random_operand(rng, 37, 1056)
+    rows = [torch.from_numpy(t).cuda() for t in (ref.packed(codes), scales)]
+    q, back = pkg.MX4.empty(37, 1056), [torch.zeros_like(t) for t in rows]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    assert pkg.MX4.packed(*rows, stream=s.cuda_stream, out=q) is q
+    q.unpacked(s.cuda_stream, *back)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(rows, back))
+    assert all(torch.equal(a, b) for a, b in zip(pkg.MX4.packed(*rows).unpacked(), rows))

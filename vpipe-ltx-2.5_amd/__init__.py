@@ -667,6 +667,13 @@ def _on_device(stream, names: str, tensors) -> int:
     return _raw_stream(device)
 
 
+def _callers(stream, what: str) -> None:
+    """Refuse memory of the binding's own on a stream of the caller's: torch's allocator orders it
+    after the work of its own current stream alone, which may still read what lay there."""
+    if stream is not None:
+        raise ValueError(f"on a stream of the caller's, {what} must be the caller's too")
+
+
 def _float_type(name: str, t) -> int:
     if t.dtype is _torch.bfloat16:
         return DT_BF16
@@ -732,9 +739,10 @@ class MX4:
                    torch.empty(mx4_scale_bytes(rows, K), dtype=torch.uint8, device=device), rows, K)
 
     @classmethod
-    def packed(cls, codes, scales, stream=None):
+    def packed(cls, codes, scales, stream=None, out=None):
         """From uint8 codes [rows][K / 2], the earlier of a byte's two values in its low half, and
-        scales [rows][K / 32], as checkpoints hold them (ltx25_mx4_pack)."""
+        scales [rows][K / 32], as checkpoints hold them (ltx25_mx4_pack): into `out`, an MX4 of
+        their size, or on torch's current stream into a new one."""
         torch = _torch or _import_torch()
         rows, half = codes.shape
         if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or half % 16
@@ -743,18 +751,31 @@ class MX4:
             raise TypeError(f"codes and scales must be contiguous uint8 [rows][K / 2] and "
                             f"[rows][K / 32], got {codes.dtype} {tuple(codes.shape)}, "
                             f"{scales.dtype} {tuple(scales.shape)}")
-        at = _on_device(stream, "codes scales", (codes, scales))
-        q = cls.empty(rows, 2 * half, codes.device)
+        if out is None:
+            _callers(stream, "out")
+        elif out.rows != rows or out.K != 2 * half:
+            raise ValueError(f"out has {out.rows} rows of {out.K}, not {rows} of {2 * half}")
+        at = _on_device(stream, "codes scales out.codes",
+                        (codes, scales, None if out is None else out.codes))
+        q = cls.empty(rows, 2 * half, codes.device) if out is None else out
         check(load().ltx25_mx4_pack(at, _ptr(codes), _ptr(scales), ctypes.byref(q.c())))
         return q
 
-    def unpacked(self, stream=None):
-        """codes [rows][K / 2] and scales [rows][K / 32] as packed() takes them
-        (ltx25_mx4_unpack)."""
-        codes = self.codes.new_empty((self.rows, self.K // 2))
-        scales = self.codes.new_empty((self.rows, self.K // 32))
-        check(load().ltx25_mx4_unpack(_on_device(stream, "codes", (self.codes,)),
-                                      ctypes.byref(self.c()), _ptr(codes), _ptr(scales)))
+    def unpacked(self, stream=None, codes=None, scales=None):
+        """codes [rows][K / 2] and scales [rows][K / 32] as packed() takes them (ltx25_mx4_unpack):
+        into those given, or on torch's current stream into new ones."""
+        torch = _torch or _import_torch()
+        shapes = (self.rows, self.K // 2), (self.rows, self.K // 32)
+        for name, t, shape in zip(("codes", "scales"), (codes, scales), shapes):
+            if t is None:
+                _callers(stream, name)
+            elif t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise TypeError(f"{name} must be contiguous uint8 {list(shape)}, got {t.dtype} "
+                                f"{tuple(t.shape)}")
+        at = _on_device(stream, "q.codes codes scales", (self.codes, codes, scales))
+        codes, scales = (self.codes.new_empty(shape) if t is None else t
+                         for t, shape in zip((codes, scales), shapes))
+        check(load().ltx25_mx4_unpack(at, ctypes.byref(self.c()), _ptr(codes), _ptr(scales)))
         return codes, scales
 
     def c(self) -> Mx4C:
@@ -809,10 +830,8 @@ def _product(y, bias, M: int, K: int, N: int, workspace, need_of, stream):
         raise TypeError(f"bias must be contiguous [{N}], got {tuple(bias.shape)}")
     if workspace is None:
         need = need_of(M, K, N)
-        if need and stream is not None:
-            raise ValueError(f"on a stream of the caller's, {need} bytes of workspace are the "
-                             f"caller's too")
         if need:
+            _callers(stream, f"a workspace of {need} bytes")
             workspace = _torch.empty(need, dtype=_torch.uint8, device=y.device)
     return workspace
 

@@ -392,3 +392,44 @@ def test_a_stream_of_the_callers_needs_its_results(pkg):
         with pytest.raises((TypeError, ValueError)) as e:
             call()
         assert "too" not in str(e.value)
+
+
+class Pinned(torch.Tensor):
+    """A tensor that says that it lies in pinned host memory."""
+
+    def is_pinned(self, *args):
+        return True
+
+
+def test_memory_of_a_calls_own_beside_pinned_tensors_lies_on_the_gpu(pkg, monkeypatch):
+    """Beside a pinned tensor is pageable host memory, which a kernel may not touch."""
+    asked, empty = [], torch.empty
+
+    class Lib:
+        def __getattr__(self, name):
+            return getattr(lib, name) if name.endswith("_bytes") or "workspace" in name else (
+                lambda *args: pkg.OK)
+
+    def recorded(*shape, device=None, **kw):
+        asked.append(str(device))
+        return empty(*shape, **kw)
+
+    lib = pkg.load()
+    codes, scales, x, y = (torch.zeros(s, dtype=t).as_subclass(Pinned) for s, t in (
+        ((4, 32), torch.uint8), ((4, 2), torch.uint8), ((40, 64), torch.bfloat16),
+        ((40, 4), torch.bfloat16)))
+    held = pkg.MX4(*(torch.zeros(n, dtype=torch.uint8).as_subclass(Pinned)
+                     for n in (pkg.mx4_code_bytes(4, 64), pkg.mx4_scale_bytes(4, 64))), 4, 64)
+    q = torch.zeros((1, 8, 64), dtype=torch.bfloat16).as_subclass(Pinned)
+    k = torch.zeros((4096, 8, 64), dtype=torch.bfloat16).as_subclass(Pinned)
+    monkeypatch.setattr(torch, "empty", recorded)
+    monkeypatch.setattr(pkg, "load", Lib)
+    monkeypatch.setattr(pkg, "_on_device", lambda stream, names, tensors: 0)
+    monkeypatch.setattr(pkg, "_stream", lambda stream: 0)
+    monkeypatch.setattr(pkg, "_reachable", lambda names, *tensors: None)
+    for call, times in ((lambda: pkg.MX4.packed(codes, scales), 2), (held.unpacked, 2),
+                        (lambda: pkg.linear_mx4(x, held, None, y), 1),
+                        (lambda: pkg.attention(q, k, k, q.clone(), causal=False), 1)):
+        asked.clear()
+        call()
+        assert asked == ["cuda"] * times, asked

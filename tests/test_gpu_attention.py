@@ -453,3 +453,14 @@ def test_attention_in_parts_in_a_graph(pkg, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+
+
+def test_attention_in_parts_of_pinned_queries(pkg, dev):
+    """Queries in pinned host memory: the workspace of the call's own lies on the GPU."""
+    q, k, v = _randn(57, 3, 8, 128), _randn(58, 6000, 2, 128), _randn(59, 6000, 2, 128)
+    assert pkg.attention_workspace(8, 2, 128, 1, 3, 6000) > 0
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    say("attention in parts, pinned queries")
+    pkg.attention(q, k, v, want, causal=True)
+    pkg.attention(q.cpu().pin_memory(), k, v, got, causal=True)
+    assert torch.equal(got, want)

@@ -395,3 +395,23 @@ def test_orders_on_a_stream_of_the_callers(pkg, dev):
     s.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(rows, back))
     assert all(torch.equal(a, b) for a, b in zip(pkg.MX4.packed(*rows).unpacked(), rows))
+
+
+def test_results_beside_pinned_memory(pkg, dev):
+    """Inputs in pinned host memory: results and workspaces of the calls' own lie on the GPU."""
+    say("mx4 pinned")
+    rng = np.random.default_rng(12)
+    codes, scales = ref.random_operand(rng, 20, 1056)
+    rows = [torch.from_numpy(t).pin_memory() for t in (ref.packed(codes), scales)]
+    q = pkg.MX4.packed(*rows)
+    assert q.codes.is_cuda and q.scales.is_cuda
+    there = pkg.MX4(q.codes.cpu().pin_memory(), q.scales.cpu().pin_memory(), 20, 1056)
+    for held in (q, there):
+        back = held.unpacked()
+        assert all(b.is_cuda and torch.equal(b.cpu(), r) for b, r in zip(back, rows))
+    x = torch.from_numpy(rng.standard_normal((40, 1056))).bfloat16().cuda()
+    y, want = torch.zeros((40, 20), dtype=torch.bfloat16).pin_memory(), torch.empty((40, 20), dtype=torch.bfloat16, device="cuda")
+    pkg.linear_mx4(x, q, None, y)
+    pkg.linear_mx4(x, q, None, want)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want.cpu())

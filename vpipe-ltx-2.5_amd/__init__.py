@@ -458,6 +458,12 @@ def _reachable(names: str, *tensors) -> None:
                              f"{t.device}")
 
 
+def _gpu_of(t):
+    """Where memory of a call's own goes: beside t, or on the current GPU where t is pinned host
+    memory (beside it would be pageable host memory, which no kernel reaches)."""
+    return t.device if t.is_cuda else "cuda"
+
+
 def attention(q, k, v, out, cu_q=None, cu_k=None, *, causal: bool, scale: float = 0.0, lse=None,
               workspace=None, stream=None) -> None:
     """Attention of packed sequences (ltx25_attention): q, out [total_q][heads][head_dim], k, v
@@ -496,7 +502,7 @@ def attention(q, k, v, out, cu_q=None, cu_k=None, *, causal: bool, scale: float 
         need = load().ltx25_attention_workspace(ctypes.byref(a), batch, nq, nk)
         if need > 0:
             if workspace is None:
-                workspace = _torch.empty(need, dtype=_torch.uint8, device=q.device)
+                workspace = _torch.empty(need, dtype=_torch.uint8, device=_gpu_of(q))
             check(load().ltx25_attention_split(
                 _stream(stream), ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 out.data_ptr(), _ptr(lse), pq, pk, batch, nq, nk, workspace.data_ptr(),
@@ -757,7 +763,7 @@ class MX4:
             raise ValueError(f"out has {out.rows} rows of {out.K}, not {rows} of {2 * half}")
         at = _on_device(stream, "codes scales out.codes",
                         (codes, scales, None if out is None else out.codes))
-        q = cls.empty(rows, 2 * half, codes.device) if out is None else out
+        q = cls.empty(rows, 2 * half, _gpu_of(codes)) if out is None else out
         check(load().ltx25_mx4_pack(at, _ptr(codes), _ptr(scales), ctypes.byref(q.c())))
         return q
 
@@ -773,8 +779,8 @@ class MX4:
                 raise TypeError(f"{name} must be contiguous uint8 {list(shape)}, got {t.dtype} "
                                 f"{tuple(t.shape)}")
         at = _on_device(stream, "q.codes codes scales", (self.codes, codes, scales))
-        codes, scales = (self.codes.new_empty(shape) if t is None else t
-                         for t, shape in zip((codes, scales), shapes))
+        codes, scales = (torch.empty(shape, dtype=torch.uint8, device=_gpu_of(self.codes))
+                         if t is None else t for t, shape in zip((codes, scales), shapes))
         check(load().ltx25_mx4_unpack(at, ctypes.byref(self.c()), _ptr(codes), _ptr(scales)))
         return codes, scales
 
@@ -832,7 +838,7 @@ def _product(y, bias, M: int, K: int, N: int, workspace, need_of, stream):
         need = need_of(M, K, N)
         if need:
             _callers(stream, f"a workspace of {need} bytes")
-            workspace = _torch.empty(need, dtype=_torch.uint8, device=y.device)
+            workspace = _torch.empty(need, dtype=_torch.uint8, device=_gpu_of(y))
     return workspace
 
 

@@ -433,3 +433,14 @@ def test_memory_of_a_calls_own_beside_pinned_tensors_lies_on_the_gpu(pkg, monkey
         asked.clear()
         call()
         assert asked == ["cuda"] * times, asked
+
+
+def test_codes_and_scales_of_which_one_is_pinned(pkg):
+    """Calls look for pageable host memory among the codes; the scales lie there only with them."""
+    held = [torch.zeros(n, dtype=torch.uint8) for n in (pkg.mx4_code_bytes(4, 64), pkg.mx4_scale_bytes(4, 64))]
+    pinned = [t.as_subclass(Pinned) for t in held]
+    pkg.MX4(*held, 4, 64)
+    pkg.MX4(*pinned, 4, 64)
+    for pair in ((pinned[0], held[1]), (held[0], pinned[1])):
+        with pytest.raises(ValueError, match="pinned"):
+            pkg.MX4(*pair, 4, 64)

@@ -733,6 +733,9 @@ class MX4:
                                 f"{t.dtype} {tuple(t.shape)}")
         if codes.device != scales.device or codes.is_cuda != scales.is_cuda:
             raise ValueError(f"codes lie on {codes.device}, scales on {scales.device}")
+        # (calls look at the codes alone)
+        if not codes.is_cuda and codes.is_pinned() != scales.is_pinned():
+            raise ValueError("of codes and scales in host memory one is pinned and one is not")
         self._tensors = (codes, scales)
         self.rows, self.K = rows, K
         self._c = Mx4C(_ptr(codes), _ptr(scales), rows, K)

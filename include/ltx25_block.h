@@ -112,8 +112,9 @@ typedef struct ltx25_rotation {
 } ltx25_rotation;
 
 /* Rotates queries and keys, bf16 [tokens] of [heads][head_dim] at their strides (as in
- * ltx25_attn), into q_out and k_out, which may be q and k (at the same strides). q or
- * k may be NULL with 0 heads. One rounding to bf16. */
+ * ltx25_attn), into q_out and k_out, which may be q and k (q_out q, k_out k, at the same
+ * strides); else the outputs overlap nothing. q or k may be NULL with 0 heads. One
+ * rounding to bf16. */
 int ltx25_rope(void* stream, const ltx25_rotation* r, const void* q, void* q_out, int heads,
                int64_t q_stride, int64_t q_out_stride, const void* k, void* k_out, int kv_heads,
                int64_t k_stride, int64_t k_out_stride, int tokens);

@@ -444,3 +444,12 @@ def test_codes_and_scales_of_which_one_is_pinned(pkg):
     for pair in ((pinned[0], held[1]), (held[0], pinned[1])):
         with pytest.raises(ValueError, match="pinned"):
             pkg.MX4(*pair, 4, 64)
+
+
+@pytest.mark.parametrize("kw,what", [(dict(), "q_out is k_out"), (dict(q=2 * FAKE, k=3 * FAKE), "q_out is k_out"),
+                                     (dict(q_out=2 * FAKE, k=2 * FAKE, k_out=3 * FAKE), "q_out is k:"),
+                                     (dict(q_out=2 * FAKE, k=3 * FAKE), "k_out is q:")])
+def test_rope_of_one_tensor_as_queries_and_keys(pkg, lib, kw, what):
+    """Two threads would turn the same channels, or one read what the other writes."""
+    assert _rope(pkg, lib, kv=4, ks=256, kos=256, **kw) == pkg.E_INVAL
+    assert what in pkg.last_error()

@@ -296,6 +296,10 @@ int ltx25_rope(void* stream, const ltx25_rotation* r, const void* q, void* q_out
     a.heads[i] = counts[i];
   }
   if (tokens == 0) { return LTX25_OK; }
+  if (heads > 0 && kv_heads > 0 && (q_out == k_out || q_out == k || k_out == q)) {
+    return set_error(LTX25_E_INVAL, "%s: one tensor turned as queries and as keys",
+                     q_out == k_out ? "q_out is k_out" : q_out == k ? "q_out is k" : "k_out is q");
+  }
   if ((rc = ltx25::check_device()) != LTX25_OK) { return rc; }
   a.head_dim = r->head_dim;
   a.tokens = tokens;

@@ -240,8 +240,12 @@ __global__ void __launch_bounds__(256, 2) mx4_wide_kernel(GemmParams p)
       for (int i = 0; i < RB; ++i) {
         acc[i][j] = mfma_mx4<J>(w[f % 4], x[B + J][i], acc[i][j], ws[j], xs[i]);
       }
-      // Unconditionally, so that the number of loads behind others is known.
-      if constexpr (f % 2 == 0 && f / 2 < kW) { load_w(span + STAGES - 1, next, f / 2); }
+      // Unconditionally and in this order, so that the number of loads behind others is known: a
+      // load of x that came before the span's last one to LDS would let the wait end before that.
+      if constexpr (f % 2 == 0 && f / 2 < kW) {
+        load_w(span + STAGES - 1, next, f / 2);
+        if constexpr (f == kLast) { __builtin_amdgcn_sched_barrier(0); }
+      }
       if constexpr (x_before(j + 1) > x_before(j)) {
         constexpr int kBuf = J > 0 ? B + J - 1 : DEPTH == 8 ? 7 - B : 3;
         load_x(span + DEPTH / 4 - (J == 0 ? 1 : 0), (J + 3) % 4, kBuf, x_before(j));

@@ -220,6 +220,40 @@ def test_norm_coded(pkg, dev, tokens, width):
     assert torch.equal(xo, c["x_out"])
 
 
+CODED_FORMS = [  # the same, of coded outputs alone
+    (BF16, BF16, False, False, False, True, True, False, 1.0),
+    (BF16, F32, False, False, False, False, False, True, 1.0),
+    (F32, BF16, False, False, False, False, True, False, 1.0),
+    *FORMS]
+
+
+CODED_SIZES = [(515, 64), (1030, 512), (600, 544), (128, 1056), (129, 2048), (200, 2592), (140, 4128),
+               (131, 8224), (130, 16384)]
+
+
+@pytest.mark.parametrize("tokens,width,form", [(*size, (i + j) % len(CODED_FORMS))
+                                               for i, size in enumerate(CODED_SIZES) for j in (0, 3, 5)])
+def test_norm_coded_of_many_tokens(pkg, dev, tokens, width, form):
+    """From 128 workgroups on tokens change places, so that 16 rows are coded on one XCD: every row
+    its own, in every form, against the codes of 64 bits as in test_norm_coded."""
+    say(f"block_norm_mx4 {tokens}x{width} form {form}")
+    rng = np.random.default_rng(width + form)
+    c = _norm_case(rng, tokens, width, CODED_FORMS[form], tokens)
+    if "y" in c:
+        c["x_out"] = torch.empty_like(c["x"])
+    q = pkg.MX4.empty(tokens, width)
+    pkg.block_norm(out=q, **c)
+    h, x, mag, mag_x = _want(c, np.arange(tokens))
+    codes, scales = ref.download(q)
+    near = [ref.code(h + s * ref.F32_SHARE * mag) for s in (-1, 0, 1)]
+    sure = (near[0][1] == near[1][1]) & (near[1][1] == near[2][1])
+    assert sure.mean() > 0.98 and (scales == near[1][1])[sure].all()
+    firm = np.repeat(sure, 32, 1) & (near[0][0] == near[1][0]) & (near[1][0] == near[2][0])
+    assert firm.mean() > 0.95 and (codes == near[1][0])[firm].all()
+    if "y" in c:
+        _close(c["x_out"], x, mag_x, c["x"].dtype, "x_out")
+
+
 def test_norm_and_rope_past_32_bits(pkg, dev):
     """Tensors of more than 2^31 elements: their last rows against calls on those alone."""
     say("norm and rope past 32 bits")

@@ -415,3 +415,10 @@ def test_results_beside_pinned_memory(pkg, dev):
     pkg.linear_mx4(x, q, None, want)
     torch.cuda.synchronize()
     assert torch.equal(y, want.cpu())
+
+
+@pytest.mark.parametrize("m,k,n,gelu", [(8160, 1056, 4096, False), (8160, 1568, 4095, True)])
+def test_tiles_walked_over_several_spans(pkg, dev, m, k, n, gelu):
+    """1024 tiles of 256 x 128 for 512 workgroups: stages and rows of x change hands between a
+    workgroup's tiles after an odd and an even number of spans."""
+    test_large_products(pkg, dev, m, k, n, gelu)

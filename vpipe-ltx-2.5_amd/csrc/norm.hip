@@ -290,10 +290,16 @@ hipError_t run(const NormArgs& a, hipStream_t stream)
   // a launch has fewer than 2^32 threads; whole runs of 128 workgroups
   constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES, kTokens = WAVES == 1 ? 256 / LANES : 1;
   constexpr long kMost = (((1L << 32) / kThreads - 1) & ~127L) * kTokens;
-  // LDS that nothing uses, for four workgroups a CU and no fifth: with a y and one sum a token more
-  // of them at once take the memory longer (8160 x 4096 48.8 us, 50.3 of five and 51.7 of three;
-  // post-normed with means, four sums, 55.2, 53.9 of five; other widths equal or slower)
-  const bool four = WAVES == 4 && CH == 2 && !LONE && a.after == nullptr && !a.layer;
+  // LDS that nothing uses, for four workgroups a CU and no fifth: where a token has much to move and
+  // one sum, more of them at once take the memory longer. By the bytes of its x and y, 16 KB or more
+  // (with gate and modulation; in fours, and in fives): 8160 x 4096 48.2 us and 48.6, into 4 bits
+  // 46.4 and 46.5, 32768 tokens 178 and 182; of f32 x 72.1 and 73.4, 32768 tokens 273 and 280, 3080
+  // wide 57.1 and 60.9, into 4 bits 3584 wide 59.9 and 64.9 (2048 x 3080 18.1 and 16.0). Below:
+  // 3584 wide 45.1 and 44.2, into 4 bits 43.6 and 41.8, f32 modulations 53.4 and 51.2; 3840 wide
+  // 47.8 and 47.7, 45.6 and 45.0, 57.6 and 55.3. Post-normed with means, four sums, 8160 x 4096 55.2
+  // and 53.9.
+  const bool four = WAVES == 4 && CH == 2 && !LONE && a.after == nullptr && !a.layer &&
+                    (WIDE ? 6 : 4) * a.width >= 16 << 10;
   const size_t spare = four ? 36 << 10 : 0;
   for (long first = 0; first < a.tokens; first += kMost) {
     const long n = std::min(kMost, a.tokens - first);

@@ -66,18 +66,19 @@ __device__ __forceinline__ Places places_of(const Rotation& r, const Words& w)
 // A pair's frequency in turns (divided by 2 pi): a number of 64 bits and what that leaves. One
 // alone is off by 2^-53 of the turns: 2^-18 radians at position 2^20 of a frequency of 15708.
 struct Freq {
-  double turns, rest;
+  double turns;
+  float rest;
 };
 __device__ __forceinline__ Freq freq_of(float f)
 {
   const double freq = (double)f, turns = freq * kInv2Pi;
-  return {turns, fma(freq, kInv2PiRest, fma(freq, kInv2Pi, -turns))};
+  return {turns, (float)fma(freq, kInv2PiRest, fma(freq, kInv2Pi, -turns))};
 }
 
 // The sine and cosine of one pair's angle. Whole turns are taken off the product of position and
-// frequency in 64 bits before it is rounded: what is left is good to 2^-50 turns while the angle is
-// below 2^52 radians. It goes to the hardware's sine and cosine, whose argument is in turns (off by
-// at most 2^-22.9).
+// frequency in 64 bits before it is rounded; what is left, and the share of the frequency's rest (a
+// sixteenth of a turn at 2^52 radians), are good to 2^-25 turns in 32. They go to the hardware's sine
+// and cosine, whose argument is in turns (off by at most 2^-22.9).
 template <bool MANY>
 __device__ __forceinline__ void sin_cos(const Places& t, const Freq& freq, int axis, float& sn,
                                         float& cs)
@@ -92,7 +93,7 @@ __device__ __forceinline__ void sin_cos(const Places& t, const Freq& freq, int a
     at = axis <= 1 ? +low : +high;
   }
   const double whole = rint(at * freq.turns);
-  const float left = (float)fma(at, freq.rest, fma(at, freq.turns, -whole));
+  const float left = fmaf((float)at, freq.rest, (float)fma(at, freq.turns, -whole));
   sn = __builtin_amdgcn_sinf(left);
   cs = __builtin_amdgcn_cosf(left);
 }

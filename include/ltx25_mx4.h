@@ -74,7 +74,7 @@ int ltx25_mx4_unpack(void* stream, const ltx25_mx4* q, void* codes, void* scales
  * workspace: at least ltx25_mx4_gemm_workspace(M, K, N) bytes. */
 int ltx25_mx4_gemm(void* stream, const ltx25_mx4* x, const ltx25_mx4* w, const void* bias,
                    int bias_dtype, void* y, int epilogue, void* workspace, size_t workspace_bytes);
-/* 0 where none is needed (every size, at present) and for sizes that the call refuses. */
+/* 0: no size needs any at present, and none is looked at. */
 size_t ltx25_mx4_gemm_workspace(int M, int K, int N);
 
 /* The same with M rows of bf16 activations (x_stride elements from a row to the next,

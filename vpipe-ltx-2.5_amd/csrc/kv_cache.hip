@@ -198,14 +198,15 @@ __device__ __forceinline__ uint2 quantize8(uint4 x, float s, float rs)
 // 128: 5.7 us, 8.4 by fours).
 //
 // Bound by memory where there is much to do: 8192 tokens of 8 heads of 128, 50 MB read
-// and written, 14.9 us (3.4 TB/s; a page's first code waits for all its values).
+// and written, 17.0 us on changing tensors (3.0 TB/s; a page's first code waits for all its
+// values), 13.4 on the same ones again.
 //
 // ROPE: the keys are turned in registers as they arrive and rounded to bf16, and from there on
 // are the keys of a plain append. Pairs half of the rotated channels apart meet by exchanges
 // between two lanes of one token, each of which turns half of their pairs (all of them, its own
-// channels alone: half a microsecond more). 8192 tokens of 8 heads of 128 17.4 us (pairs side by
-// side 15.9, by three axes 19.1; not turned 13.1): every head's workgroup computes its tokens'
-// sines.
+// channels alone: half a microsecond more). 8192 tokens of 8 heads of 128 19.3 us on changing
+// tensors (pairs side by side 18.1, by three axes 21.0), 17.5 on the same ones again (15.6, 18.2):
+// every head's workgroup computes its tokens' sines.
 // ROPE 2: positions of several axes.
 template <int D, int ROPE = 0>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(MoveParams p, Rotation rot)

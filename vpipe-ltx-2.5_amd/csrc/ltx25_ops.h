@@ -184,7 +184,8 @@ public:
   }
 
   // The microscaled 4-bit tier: rows to codes and back, the product of two coded
-  // operands, and a linear that codes its activations on the way.
+  // operands, and a linear that codes its activations on the way. Biases are bf16, as
+  // in every linear here (ltx25_mx4_gemm and ltx25_linear_mx4 take f32 ones too).
   void mx4_quantize_rows(hipStream_t enc, const void* x, int x_dtype, int64_t x_stride,
                          const ltx25_mx4& q) const
   {

@@ -111,9 +111,10 @@ __device__ __forceinline__ void tile_at(int id, const GemmParams& p, int& tm, in
 // then carries 5 x 16 CB rows of K where both operands through LDS and 2 x 2 waves of the same
 // size carry 3 x (64 RB + 16 CB).
 //
-// 8160 x 4096 -> 16384 in 250 to 265 us, 4.1 to 4.4 PFLOP/s: address units are busy in 84% of the
-// cycles, matrix cores in 59, LDS in 18, at the clock that power leaves (1.76 GHz; on zeros 2.2
-// and as many cycles). The instructions alone reach 7.2 PFLOP/s on random operands.
+// 8160 x 4096 -> 16384 in 272 us one after another, 4.0 PFLOP/s (250 to 305 one at a time, as power
+// allows: 4.45e5 cycles, at 1.76 GHz 250 us): address units are busy in 84% of the cycles, matrix
+// cores in 59, LDS in 18; on zeros as many cycles at 2.2 GHz. The instructions alone reach 7.2
+// PFLOP/s on random operands.
 //
 // A span is 512 values: STAGES LDS stages of CB x 4 tiles of codes and all the workgroup's scales
 // take turns, filled STAGES - 1 spans ahead by loads that go straight into LDS, one barrier a
@@ -578,8 +579,10 @@ Mx4Plan plan_mx4(int M, int K, int N, bool bf16)
   // 4096, 4: 6.8), a launch ahead 2.6 (26.1 + 2.6; 5.8 + 2.6).
   const long coding = (groups(16, 16) + 255) / 256 * ((mx4_spans(K) + 7) / 8) * ((M + 3) / 4);
   r.codes_ahead = bf16 && (M > 16 || coding > 4);
-  // The largest tile that is half full and still gives three CUs of four a workgroup, wide ones
-  // first (us; M x K -> N, replayed in a graph):
+  // The largest tile whose rows are half there and that still gives three CUs of four a workgroup,
+  // wide ones first (us; M x K -> N, replayed in a graph). Columns are not asked for: with few of
+  // them many rows take tiles that are mostly empty (16384 x 4096 -> 8 9.2 us, by panels 7.4; 50000
+  // 21.9 and 21.3, 200000 87 and 78; at 32 columns 9.2 and 7.8, 21.4 and 21.7).
   //                         256 x 128  256 x 64  128 x 64  64 x 64  32 x 32  32 x 16 (8 waves)
   //   8160 x 4096 -> 4096        64        81        92      128      173
   //   1024 x 4096 -> 4096        17.4      12.8      13.7     18.9     26.3

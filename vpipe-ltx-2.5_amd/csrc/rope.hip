@@ -28,9 +28,9 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, uint32_t m) { return m ==
 // channels apart, of one token, and computes its pairs' sines itself; threads are dealt out over
 // the tokens' pieces one after another, so that few heads fill waves too.
 //
-// Bound by memory: 8160 tokens of 32 + 32 heads of 128 by three axes, 267 MB, 50.5 us (5.3 TB/s),
-// 2048 of 32 + 8 by one 8.6. Two and four tokens a thread, which share their frequencies, are no
-// faster (50.0 and 52.4; 9.2 and 10.0).
+// Bound by memory: 8160 tokens of 32 + 32 heads of 128 by three axes, 267 MB, 54.5 us (4.9 TB/s),
+// 2048 of 32 + 8 by one 8.8, changing tensors. Two and four tokens a thread, which share their
+// frequencies, were no faster (50.0 and 52.4 us where one token's were 50.5; 9.2 and 10.0 for 8.6).
 template <bool SIDE, bool MANY>
 __global__ void __launch_bounds__(kThreads) rope_kernel(RopeParams p, long first)
 {

@@ -10,7 +10,7 @@
  * no scratch of the library's own: what a call needs beyond its tensors is the
  * caller's `workspace` (device memory, 16-byte aligned, any contents, in use until
  * the call has run), so calls on different streams may overlap and a call may be
- * captured into a HIP graph.
+ * captured into a HIP graph. Outputs and the workspace overlap nothing else of the call.
  */
 #ifndef LTX25_MX4_H
 #define LTX25_MX4_H

@@ -453,3 +453,22 @@ def test_rope_of_one_tensor_as_queries_and_keys(pkg, lib, kw, what):
     """Two threads would turn the same channels, or one read what the other writes."""
     assert _rope(pkg, lib, kv=4, ks=256, kos=256, **kw) == pkg.E_INVAL
     assert what in pkg.last_error()
+
+
+def test_4_bit_outputs_in_an_inputs_place(pkg, lib):
+    """What is written where the call still reads: K is N, or the rows and the order have one size."""
+    a, b = 4 * FAKE, 5 * FAKE
+    q = _mx4(pkg, 16, 128, a, b)
+    for codes, scales in ((a, FAKE), (FAKE, b), (b, FAKE), (FAKE, a)):
+        assert lib.ltx25_mx4_pack(None, codes, scales, ctypes.byref(q)) == pkg.E_INVAL
+        assert "not in place" in pkg.last_error()
+        assert lib.ltx25_mx4_unpack(None, ctypes.byref(q), codes, scales) == pkg.E_INVAL
+        assert "not in place" in pkg.last_error()
+    x, w = _mx4(pkg, 4, 64, 6 * FAKE, 7 * FAKE), _mx4(pkg, 64, 64, a, b)
+    for y in (a, b, 6 * FAKE, 7 * FAKE, 8 * FAKE):
+        assert _gemm(pkg, lib, x, w, 8 * FAKE, BF16, y) == pkg.E_INVAL
+        assert "y is " in pkg.last_error()
+    for m in (4, 40):
+        for y in (a, b, 6 * FAKE, 7 * FAKE, 8 * FAKE):
+            assert _linear(pkg, lib, 6 * FAKE, 64, m, w, 8 * FAKE, BF16, y, ws=7 * FAKE) == pkg.E_INVAL
+            assert "y is " in pkg.last_error()

@@ -6,6 +6,8 @@
 #include "checks.h"
 #include "mx4.h"
 
+#include <initializer_list>
+
 namespace {
 
 using namespace ltx25::checks;
@@ -85,6 +87,33 @@ int check_product(const ltx25::Mx4Args& w, int M, const void* bias, int bias_dty
   return need > 0 ? check_workspace(workspace, workspace_bytes, need) : LTX25_OK;
 }
 
+// An output that begins where another tensor of the call does would be written while that is
+// still read.
+struct Named {
+  const char* name;
+  const void* at;
+};
+int check_apart(Named out, std::initializer_list<Named> others)
+{
+  for (const Named& o : others) {
+    if (o.at == out.at) {
+      return set_error(LTX25_E_INVAL, "%s is %s: not in place", out.name, o.name);
+    }
+  }
+  return LTX25_OK;
+}
+
+// Rows and the library's order of them
+int check_orders(const void* codes, const void* scales, const ltx25_mx4* q)
+{
+  int rc = check_pointer("codes", codes, 16);
+  if (rc != LTX25_OK || (rc = check_pointer("scales", scales, 16)) != LTX25_OK) { return rc; }
+  rc = check_apart({"codes", codes}, {{"q's codes", q->codes}, {"q's scales", q->scales}});
+  return rc != LTX25_OK
+             ? rc
+             : check_apart({"scales", scales}, {{"q's codes", q->codes}, {"q's scales", q->scales}});
+}
+
 int check_source(const char* name, const void* x, int64_t stride, int K, bool wide)
 {
   const int rc = check_row_stride(name, stride, K, wide ? 4 : 8);
@@ -160,8 +189,7 @@ int ltx25_mx4_pack(void* stream, const void* codes, const void* scales, const lt
   ltx25::Mx4Args a;
   int rc = check_operand("q", q, &a);
   if (rc != LTX25_OK || a.rows == 0) { return rc; }
-  if ((rc = check_pointer("codes", codes, 16)) != LTX25_OK ||
-      (rc = check_pointer("scales", scales, 16)) != LTX25_OK ||
+  if ((rc = check_orders(codes, scales, q)) != LTX25_OK ||
       (rc = ltx25::check_device()) != LTX25_OK) {
     return rc;
   }
@@ -175,8 +203,7 @@ int ltx25_mx4_unpack(void* stream, const ltx25_mx4* q, void* codes, void* scales
   ltx25::Mx4Args a;
   int rc = check_operand("q", q, &a);
   if (rc != LTX25_OK || a.rows == 0) { return rc; }
-  if ((rc = check_pointer("codes", codes, 16)) != LTX25_OK ||
-      (rc = check_pointer("scales", scales, 16)) != LTX25_OK ||
+  if ((rc = check_orders(codes, scales, q)) != LTX25_OK ||
       (rc = ltx25::check_device()) != LTX25_OK) {
     return rc;
   }
@@ -200,6 +227,9 @@ int ltx25_mx4_gemm(void* stream, const ltx25_mx4* x, const ltx25_mx4* w, const v
   const size_t need = ltx25_mx4_gemm_workspace(g.x.rows, g.x.K, g.w.rows);
   rc = check_product(g.w, g.x.rows, bias, bias_dtype, y, epilogue, workspace, workspace_bytes, need);
   if (rc != LTX25_OK || g.x.rows == 0 || g.w.rows == 0) { return rc; }
+  rc = check_apart({"y", y}, {{"x's codes", x->codes}, {"x's scales", x->scales},
+                              {"w's codes", w->codes}, {"w's scales", w->scales}, {"bias", bias}});
+  if (rc != LTX25_OK) { return rc; }
   return run(stream, g, ltx25::plan_mx4(g.x.rows, g.x.K, g.w.rows, false), bias, bias_dtype, y,
              epilogue);
 }
@@ -221,7 +251,11 @@ int ltx25_linear_mx4(void* stream, const void* x, int64_t x_stride, int M, const
   const size_t need = ltx25_linear_mx4_workspace(M, g.w.K, g.w.rows);
   rc = check_product(g.w, M, bias, bias_dtype, y, epilogue, workspace, workspace_bytes, need);
   if (rc != LTX25_OK || M == 0 || g.w.rows == 0) { return rc; }
-  if ((rc = check_source("x_stride", x, x_stride, g.w.K, false)) != LTX25_OK) { return rc; }
+  if ((rc = check_source("x_stride", x, x_stride, g.w.K, false)) != LTX25_OK ||
+      (rc = check_apart({"y", y}, {{"x", x}, {"w's codes", w->codes}, {"w's scales", w->scales},
+                                   {"bias", bias}, {"the workspace", workspace}})) != LTX25_OK) {
+    return rc;
+  }
   const ltx25::Mx4Plan plan = ltx25::plan_mx4(M, g.w.K, g.w.rows, true);
   g.x.codes = (uint8_t*)workspace;
   g.x.scales = (uint8_t*)workspace + scales_at(M, g.w.K);

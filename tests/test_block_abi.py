@@ -472,3 +472,44 @@ def test_4_bit_outputs_in_an_inputs_place(pkg, lib):
         for y in (a, b, 6 * FAKE, 7 * FAKE, 8 * FAKE):
             assert _linear(pkg, lib, 6 * FAKE, 64, m, w, 8 * FAKE, BF16, y, ws=7 * FAKE) == pkg.E_INVAL
             assert "y is " in pkg.last_error()
+
+
+class OnSecond(OnGpu):
+    """A tensor of the second GPU."""
+
+    def get_device(self):
+        return 1
+
+    @property
+    def device(self):
+        return torch.device("cuda", 1)
+
+
+class OnFirst(OnGpu):
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("name", ["freqs", "axes", "positions", "k", "v", "table", "cu", "start", "cache.k",
+                                  "cache.v", "cache.k_scale", "cache.v_scale"])
+def test_append_takes_no_other_gpus_memory(pkg, monkeypatch, name):
+    """Every tensor must lie on the GPU whose stream the call goes to."""
+    int8, f32, i32, bf16 = torch.int8, torch.float32, torch.int32, torch.bfloat16
+    shapes = dict(freqs=((1, 32), f32), axes=((1, 32), i32), positions=((4, 1), i32), k=((4, 2, 64), bf16),
+                  v=((4, 2, 64), bf16), table=((1, 3), i32), cu=((2,), i32), start=((1,), i32))
+    shapes.update({"cache.k": ((4, 2, 64, 64), int8), "cache.v": ((4, 2, 64, 64), int8),
+                   "cache.k_scale": ((4, 2), f32), "cache.v_scale": ((4, 2), f32)})
+    t = {n: torch.zeros(s, dtype=d).as_subclass(OnSecond if n == name else OnFirst)
+         for n, (s, d) in shapes.items()}
+    monkeypatch.setattr(pkg, "_device_now", lambda: 0)
+    cache = pkg.KVCache(*(t["cache." + n] for n in ("k", "v", "k_scale", "v_scale")))
+    # (a cache of two GPUs is refused by itself, at its tensor of the lower one)
+    with pytest.raises(ValueError, match="^cache.* lies on" if "cache" in name else f"^{name} lies on"):
+        pkg.kv_append_rope(cache, *(t[n] for n in ("table", "k", "v", "cu", "start", "freqs", "axes",
+                                                   "positions")))
+    if "cache" not in name:
+        return
+    cache = pkg.KVCache(*(t["cache." + n].as_subclass(OnSecond) for n in ("k", "v", "k_scale", "v_scale")))
+    with pytest.raises(ValueError, match="^cache.k lies on"):
+        pkg.kv_append_rope(cache, *(t[n] for n in ("table", "k", "v", "cu", "start", "freqs", "axes",
+                                                   "positions")))

@@ -567,12 +567,20 @@ class KVCache:
         return self._c
 
     def check(self) -> None:
-        """Refuse a cache in host memory, which may be made but not given to a kernel."""
-        _reachable("cache.k cache.v cache.k_scale cache.v_scale", *self._tensors)
+        """Refuse a cache in host memory or of several GPUs, which may be made but not given to a
+        kernel."""
+        names = "cache.k cache.v cache.k_scale cache.v_scale"
+        _reachable(names, *self._tensors)
+        on = [t.get_device() for t in self._tensors]
+        for name, t, at in zip(names.split(), self._tensors, on):
+            if t.is_cuda and at != max(on):
+                raise ValueError(f"{name} lies on {t.device}, others of the cache on cuda:{max(on)}")
         self.checked = True
 
 
-def _moved(cache: KVCache, table, k, v, cu, start):
+def _moved(cache: KVCache, table, k, v, cu, start, looked: bool = False):
+    """The arguments that appending and reading share; `looked`: the caller looks at where the
+    tensors lie."""
     shape = k.shape
     ks, vs = _tokens("k", k, shape), _tokens("v", v, v.shape)
     total, heads, dim = shape
@@ -585,7 +593,7 @@ def _moved(cache: KVCache, table, k, v, cu, start):
     _int32("start", start, batch)
     if not cache.checked:
         cache.check()
-    if not (table.is_cuda and k.is_cuda and v.is_cuda and cu.is_cuda and start.is_cuda):
+    if not (looked or table.is_cuda and k.is_cuda and v.is_cuda and cu.is_cuda and start.is_cuda):
         _reachable("table k v cu start", table, k, v, cu, start)
     return (ctypes.byref(cache.c()), table.data_ptr(), stride, k.data_ptr(), v.data_ptr(), ks, vs,
             cu.data_ptr(), start.data_ptr(), batch, total)
@@ -1011,9 +1019,10 @@ def kv_append_rope(cache: KVCache, table, k, v, cu, start, freqs, axes=None, pos
     """kv_append with the keys rotated on the way (ltx25_kv_append_rope): the bits of rope on k and
     kv_append. positions [total][axes] as for rope, or None: a token's place in its sequence on
     every axis."""
-    args = _moved(cache, table, k, v, cu, start)
+    args = _moved(cache, table, k, v, cu, start, True)
     r = _rotation(cache.head_dim, freqs, axes, positions, k.shape[0], interleaved)
-    at = _on_device(stream, "freqs axes positions k", (freqs, axes, positions, k))
+    at = _on_device(stream, "freqs axes positions k v table cu start cache.k",
+                    (freqs, axes, positions, k, v, table, cu, start, cache.k))
     check(load().ltx25_kv_append_rope(at, *args[:9], ctypes.byref(r), *args[9:]))
 
 
